@@ -23,6 +23,9 @@ HIPCC_FLAGS = [
     f"--offload-arch={ARCH}", "-O3", "-std=c++17", "-fPIC",
     # every f32/f64 operation must round where the reference rounds
     "-ffp-contract=off", "-fhip-fp32-correctly-rounded-divide-sqrt",
+    # no packed f32 arithmetic (v_pk_add / mul / fma_f32): some of its forms have given wrong
+    # results on this hardware.  The host pass does not know the feature and says so: harmless
+    "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",
     "-Wall", "-Wno-unused-function",
 ]
 # per-source extra flags.  rtenv.hip: machine LICM hoists the f64 series
