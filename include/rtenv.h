@@ -19,6 +19,7 @@
  *   rollout loop              train.py:138-161  | rt_env_rollout_policy (persistent)
  *   PPO minibatch step        train.py:197-246  | rt_ppo_grad + rt_adam_step / rt_ppo_update
  *   FeaturesExtractor3D.cnn   networks.py:8-45  | rt_conv_relu_pool_fwd (+ backward kernels)
+ *   (not in the reference: categorical policies) | rt_cat_sample, rt_cat_ppo, rt_cat_distill
  *
  * Conventions
  *  - Plain pointers and sizes only; `*_d` arguments are DEVICE pointers
@@ -518,6 +519,129 @@ int64_t rt_conv_mfma_count(const rt_conv_layer* layer, int32_t batch, int32_t pa
 /* Gradient w.r.t. the stage input (cin 16 stages): dx [B][16][D][H][W]. */
 int rt_conv_relu_pool_dgrad(const rt_conv_layer* layer, int32_t batch, const float* w_d, const float* dy_d,
                             const uint8_t* argmax_d, float* dx_d, void* stream);
+
+/* ---- categorical policies -------------------------------------------------
+ * The rollout and update steps of a policy that acts by picking one of `vocab`
+ * entries (a discretised beam action, a token) from a row of logits; the
+ * Gaussian agent's are rt_policy_sample and rt_ppo_grad.  Logits are rows of
+ * f32, bf16 or f16 (RT_DT_*), element stride 1, rows row_stride elements apart
+ * (any alignment; 0 or overlapping rows are fine where they are only read).
+ * -inf marks an entry that cannot be taken.  All sums over a row are held in
+ * f64 or in whole numbers, or in f32 partial sums of a few terms. */
+#define RT_DT_F32 0
+#define RT_DT_BF16 1
+#define RT_DT_F16 2
+#define RT_CAT_MAX_VOCAB (1 << 20)
+#define RT_CAT_MAX_TOP 1024   /* most teacher entries per row (rt_cat_distill) */
+#define RT_CAT_ROW_STATE 5    /* f64 per row that a backward call needs */
+
+typedef struct rt_cat_logits {
+    const void* x;         /* device, aligned to its element */
+    int64_t rows;          /* >= 1 */
+    int64_t row_stride;    /* elements */
+    int32_t vocab;         /* 1 .. RT_CAT_MAX_VOCAB */
+    int32_t dtype;         /* RT_DT_* */
+} rt_cat_logits;
+
+/* Per-row parameters of rt_cat_sample: a device array [rows], or NULL and one
+ * value for all rows. */
+typedef struct rt_cat_sampling {
+    const float* u;                /* [rows] uniform numbers in [0, 1) (clamped into it; NaN: 0) */
+    const float* temperature;      /* <= 0 or NaN: greedy */
+    const int32_t* top_k;          /* <= 0 or >= vocab: off */
+    const float* top_p;            /* >= 1 or NaN: off; <= 0: the first entry alone */
+    const float* min_p;            /* <= 0 or NaN: off; > 1 acts as 1 */
+    float temperature_all;
+    int32_t top_k_all;
+    float top_p_all;
+    float min_p_all;
+} rt_cat_sampling;
+
+/* One action per row from given random numbers.  With m the row's maximum,
+ * entry i weighs w_i = 2^40 exp((x_i - m) / T), rounded to a whole number, so
+ * sums do not depend on their order.  In the order of falling logits, equal
+ * ones by index, three prefixes: the first top_k; the entries before which
+ * less than top_p of the first prefix's weight lies (at least one); those with
+ * x_i - m >= T log(min_p).  The shortest is kept, M its weight, and the action
+ * is the first kept entry, by index, where the running weight exceeds
+ * floor(u M).  logprob: log softmax(x / T) at the action over the whole row
+ * (what the PPO loss compares with); kept_logprob: over the kept entries.
+ * Greedy rows: the first maximum, both 0.  A row with a NaN or +inf, or
+ * nothing but -inf: action -1, both NaN.
+ * workspace_d: rt_cat_sample_workspace_bytes bytes (may be 0: then NULL),
+ * 16-B aligned, not shared with another call in flight; its contents need no
+ * preparation.  -1 on a bad argument. */
+int64_t rt_cat_sample_workspace_bytes(int64_t rows, int32_t vocab, int32_t dtype);
+int rt_cat_sample(const rt_cat_logits* logits, const rt_cat_sampling* params, int64_t* action_d, float* logprob_d,
+                  float* kept_logprob_d, void* workspace_d, int64_t workspace_bytes, void* stream);
+
+typedef struct rt_cat_ppo_batch {
+    const int64_t* actions;        /* [rows]; outside [0, vocab): the row is ignored */
+    const float* old_logprobs;     /* [rows] */
+    const float* advantages;       /* [rows] */
+    const float* weights;          /* [rows] or NULL (1 / rows each); 0: the row is ignored */
+    const float* ref_logprobs;     /* [rows] or NULL (no KL term) */
+} rt_cat_ppo_batch;
+
+typedef struct rt_cat_ppo_hparams {
+    float temperature;             /* > 0 */
+    float clip_low, clip_high;     /* ratio clipped to [1 - clip_low, 1 + clip_high]; train.py:221-225 */
+    float ent_coef, kl_coef;
+} rt_cat_ppo_hparams;
+
+typedef struct rt_cat_ppo_out {
+    float* loss;                   /* [1] */
+    float* logprob;                /* [rows] new log-probability of the action, ignored rows 0 */
+    float* entropy;                /* [rows] of softmax(x / T), ignored rows 0 */
+    float* stats;                  /* [6] weighted sums: pg_loss, kl, entropy, old_approx_kl, approx_kl, clipfrac */
+    void* grad;                    /* d loss / d logits in the logits' type, or NULL (loss alone).
+                                      May be the logits themselves (same address and stride) */
+    int64_t grad_stride;           /* elements, >= vocab */
+    double* row_state;             /* [rows][RT_CAT_ROW_STATE] for rt_cat_ppo_backward, or NULL */
+} rt_cat_ppo_out;
+
+/* The clipped PPO loss of a categorical policy (train.py:200-226, 243):
+ *   sum_n w_n (max(-A r, -A clamp(r)) + kl_coef KL - ent_coef H),
+ * r = exp(lp - old), lp = log softmax(x / T)[action], H the row's entropy,
+ * KL = exp(ref - lp) - (ref - lp) - 1; with its gradient in the same call where
+ * out->grad is given.  A row that is ignored, or has no finite logit, adds
+ * nothing and gets a zero gradient, whatever its numbers are.
+ * workspace_d: rt_cat_loss_workspace_bytes, rules as rt_cat_sample. */
+int64_t rt_cat_loss_workspace_bytes(int64_t rows, int32_t vocab, int32_t dtype);
+int rt_cat_ppo(const rt_cat_logits* logits, const rt_cat_ppo_batch* batch, const rt_cat_ppo_hparams* hp,
+               const rt_cat_ppo_out* out, void* workspace_d, int64_t workspace_bytes, void* stream);
+/* The gradient from the row_state of an earlier rt_cat_ppo on the same logits,
+ * actions and temperature, times grad_loss_d[0] (NULL: 1). */
+int rt_cat_ppo_backward(const rt_cat_logits* logits, const int64_t* actions_d, float temperature,
+                        const double* row_state_d, const float* grad_loss_d, void* grad_d, int64_t grad_stride,
+                        void* stream);
+
+typedef struct rt_cat_teacher {
+    const int64_t* idx;            /* [rows][k] entries the teacher names; outside [0, vocab): unused */
+    const float* logits;           /* [rows][k] the teacher's logits (any constant off per row) */
+    const float* lse;              /* [rows] the teacher's log sum exp(logits / T) over its whole vocabulary,
+                                      or NULL: its probabilities are normalised over the k */
+    const float* weights;          /* [rows] or NULL (1 / rows each); 0: the row is ignored */
+    int32_t k;                     /* 1 .. RT_CAT_MAX_TOP */
+    float temperature;             /* > 0, of both sides */
+} rt_cat_teacher;
+
+typedef struct rt_cat_distill_out {
+    float* loss;                   /* [1] sum_n w_n kl_n */
+    float* kl;                     /* [rows], ignored rows 0 */
+    void* grad;                    /* as rt_cat_ppo_out.grad */
+    int64_t grad_stride;
+    double* row_state;             /* [rows][RT_CAT_ROW_STATE] for rt_cat_distill_backward, or NULL */
+} rt_cat_distill_out;
+
+/* Distillation from a teacher's top logits: kl_n = sum_j q_j (log q_j -
+ * log softmax(x / T)[idx_j]), q_j = exp(t_j / T - lse); entries that name the
+ * same idx count one by one.  Gradient w / T (p_v sum_j q_j - sum_j q_j
+ * [idx_j = v]).  Ignored rows and rows without a finite logit as rt_cat_ppo. */
+int rt_cat_distill(const rt_cat_logits* logits, const rt_cat_teacher* teacher, const rt_cat_distill_out* out,
+                   void* workspace_d, int64_t workspace_bytes, void* stream);
+int rt_cat_distill_backward(const rt_cat_logits* logits, const rt_cat_teacher* teacher, const double* row_state_d,
+                            const float* grad_loss_d, void* grad_d, int64_t grad_stride, void* stream);
 
 const char* rt_last_error(void);
 int rt_abi_version(void);

@@ -26,6 +26,8 @@ STEP_DENSE, STEP_INCREMENTAL = 0, 1
 DP_ID_BYTES, DP_F32, DP_F64 = 128, 0, 1  # RT_DP_ID_BYTES, RT_DP_F32, RT_DP_F64
 PPO_PREC = {"f32": 0, "bf16x3": 1}  # RT_PPO_PREC_* (rt_ppo_hparams.precision)
 CONV_PREC = {"f32": 0, "bf16x3": 1}  # RT_CONV_PREC_* (rt_conv_layer.precision)
+DT_F32, DT_BF16, DT_F16 = 0, 1, 2  # RT_DT_* (rt_cat_logits.dtype)
+CAT_MAX_VOCAB, CAT_MAX_TOP, CAT_ROW_STATE = 1 << 20, 1024, 5  # RT_CAT_*
 
 RT_ELIMIT = -5
 RT_ERRORS = {0: "RT_OK", -1: "RT_EINVAL", -2: "RT_ENOMEM", -3: "RT_EDEVICE", -4: "RT_ELAUNCH", -5: "RT_ELIMIT"}
@@ -43,6 +45,8 @@ EXPORTS = [
     "rt_ppo_shuffle", "rt_ppo_shuffle_epochs", "rt_ppo_shuffle_adv", "rt_ppo_adv_stats", "rt_ppo_adv_sums", "rt_ppo_adv_finalize",
     "rt_conv_out_dims", "rt_conv_relu_pool_fwd", "rt_conv_wgrad_workspace_floats", "rt_conv_relu_pool_wgrad", "rt_conv_mfma_count",
     "rt_conv_relu_pool_dgrad",
+    "rt_cat_sample_workspace_bytes", "rt_cat_sample", "rt_cat_loss_workspace_bytes", "rt_cat_ppo", "rt_cat_ppo_backward",
+    "rt_cat_distill", "rt_cat_distill_backward",
     "rt_last_error", "rt_abi_version",
 ]
 
@@ -122,6 +126,40 @@ class RtPolicyRollout(ctypes.Structure):
 class RtConvLayer(ctypes.Structure):
     _fields_ = [("cin", ctypes.c_int32), ("groups", ctypes.c_int32), ("in_dims", ctypes.c_int32 * 3),
                 ("pool_pad", ctypes.c_int32 * 3), ("precision", ctypes.c_int32)]
+
+
+class RtCatLogits(ctypes.Structure):
+    _fields_ = [("x", ctypes.c_void_p), ("rows", ctypes.c_int64), ("row_stride", ctypes.c_int64),
+                ("vocab", ctypes.c_int32), ("dtype", ctypes.c_int32)]
+
+
+class RtCatSampling(ctypes.Structure):
+    _fields_ = [(k, ctypes.c_void_p) for k in ("u", "temperature", "top_k", "top_p", "min_p")] + [
+        ("temperature_all", ctypes.c_float), ("top_k_all", ctypes.c_int32), ("top_p_all", ctypes.c_float),
+        ("min_p_all", ctypes.c_float)]
+
+
+class RtCatPpoBatch(ctypes.Structure):
+    _fields_ = [(k, ctypes.c_void_p) for k in ("actions", "old_logprobs", "advantages", "weights", "ref_logprobs")]
+
+
+class RtCatPpoHparams(ctypes.Structure):
+    _fields_ = [(k, ctypes.c_float) for k in ("temperature", "clip_low", "clip_high", "ent_coef", "kl_coef")]
+
+
+class RtCatPpoOut(ctypes.Structure):
+    _fields_ = [(k, ctypes.c_void_p) for k in ("loss", "logprob", "entropy", "stats", "grad")] + [
+        ("grad_stride", ctypes.c_int64), ("row_state", ctypes.c_void_p)]
+
+
+class RtCatTeacher(ctypes.Structure):
+    _fields_ = [(k, ctypes.c_void_p) for k in ("idx", "logits", "lse", "weights")] + [
+        ("k", ctypes.c_int32), ("temperature", ctypes.c_float)]
+
+
+class RtCatDistillOut(ctypes.Structure):
+    _fields_ = [(k, ctypes.c_void_p) for k in ("loss", "kl", "grad")] + [
+        ("grad_stride", ctypes.c_int64), ("row_state", ctypes.c_void_p)]
 
 
 _lib = None
@@ -206,6 +244,17 @@ def load(build_if_missing: bool = True):
         "rt_conv_relu_pool_wgrad": ([ctypes.POINTER(RtConvLayer), i32, vp, vp, vp, vp, vp, vp, vp, i64, vp],
                                     ctypes.c_int),
         "rt_conv_relu_pool_dgrad": ([ctypes.POINTER(RtConvLayer), i32, vp, vp, vp, vp, vp], ctypes.c_int),
+        "rt_cat_sample_workspace_bytes": ([i64, i32, i32], i64),
+        "rt_cat_sample": ([ctypes.POINTER(RtCatLogits), ctypes.POINTER(RtCatSampling), vp, vp, vp, vp, i64, vp],
+                          ctypes.c_int),
+        "rt_cat_loss_workspace_bytes": ([i64, i32, i32], i64),
+        "rt_cat_ppo": ([ctypes.POINTER(RtCatLogits), ctypes.POINTER(RtCatPpoBatch), ctypes.POINTER(RtCatPpoHparams),
+                        ctypes.POINTER(RtCatPpoOut), vp, i64, vp], ctypes.c_int),
+        "rt_cat_ppo_backward": ([ctypes.POINTER(RtCatLogits), vp, ctypes.c_float, vp, vp, vp, i64, vp], ctypes.c_int),
+        "rt_cat_distill": ([ctypes.POINTER(RtCatLogits), ctypes.POINTER(RtCatTeacher),
+                            ctypes.POINTER(RtCatDistillOut), vp, i64, vp], ctypes.c_int),
+        "rt_cat_distill_backward": ([ctypes.POINTER(RtCatLogits), ctypes.POINTER(RtCatTeacher), vp, vp, vp, i64, vp],
+                                    ctypes.c_int),
         "rt_last_error": ([], ctypes.c_char_p),
         "rt_abi_version": ([], ctypes.c_int),
     }

@@ -14,7 +14,8 @@ PKG = os.path.dirname(os.path.abspath(__file__))
 REPO = os.path.dirname(PKG)
 SRC = os.path.join(PKG, "csrc", "rtenv.hip")
 SRCS = [SRC, os.path.join(PKG, "csrc", "policy.hip"), os.path.join(PKG, "csrc", "ppo_update.hip"),
-        os.path.join(PKG, "csrc", "c3d.hip")]
+        os.path.join(PKG, "csrc", "c3d.hip"), os.path.join(PKG, "csrc", "cat_sample.hip"),
+        os.path.join(PKG, "csrc", "cat_loss.hip")]
 HDR = os.path.join(REPO, "include", "rtenv.h")
 OUT = os.path.join(PKG, "librtenv.so")
 ARCH = os.environ.get("RT_OFFLOAD_ARCH", "gfx950")
@@ -52,7 +53,8 @@ def needs_build() -> bool:
     if not os.path.exists(OUT):
         return True
     t = os.path.getmtime(OUT)
-    deps = (*SRCS, HDR, *(os.path.join(PKG, "csrc", h) for h in ("rt_ddmath.h", "rt_trace.h", "policy_core.h")),
+    deps = (*SRCS, HDR, *(os.path.join(PKG, "csrc", h) for h in ("rt_ddmath.h", "rt_trace.h", "policy_core.h",
+                                                            "cat_rows.h")),
             __file__)
     return any(os.path.getmtime(p) > t for p in deps)
 

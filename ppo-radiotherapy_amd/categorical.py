@@ -1,0 +1,346 @@
+"""Operators of categorical policies: sampling, the PPO loss, distillation.
+
+The Gaussian agent's rollout and update steps (rt_policy_sample, rt_ppo_grad;
+train.py:143-149, 197-246) for a policy that picks one entry of a row of
+logits: a discretised beam action ([..., bins]) or a token ([..., vocab]).
+
+    a = sample(logits, u, temperature=0.8, top_k=50, top_p=0.9)    # rollout
+    out = ppo_loss(logits, a.action, a.logprob, adv)               # update, autograd
+    out.loss.backward()
+    out, grad = ppo_loss_grad(logits, a.action, a.logprob, adv)    # the same in one pass over the logits
+    out = distill_loss(logits, idx, top_logits, temperature=2.0)   # from a teacher's top logits
+
+Logits are float32, bfloat16 or float16 on the GPU, entries of a row adjacent
+(stride 1), leading dimensions any that collapse to evenly spaced rows; -inf
+marks an entry that cannot be taken.  Everything is enqueued on the current
+stream of the logits' device, nothing synchronises, and all of it can be
+captured in a graph (in a training graph prefer the `_grad` forms: they need no
+autograd).  The definitions stand in include/rtenv.h; wrong arguments raise
+ValueError or TypeError before anything is launched.
+"""
+from __future__ import annotations
+
+import ctypes
+import math
+from typing import NamedTuple
+
+import torch
+
+from . import _lib
+
+_DTYPES = {torch.float32: _lib.DT_F32, torch.bfloat16: _lib.DT_BF16, torch.float16: _lib.DT_F16}
+
+
+class Sample(NamedTuple):
+    action: torch.Tensor        # int64 [...], -1 where a row has no distribution
+    logprob: torch.Tensor       # f32 [...]: log softmax(logits / T) of the action
+    kept_logprob: torch.Tensor  # f32 [...]: the same over the kept entries alone
+
+
+class PpoLoss(NamedTuple):
+    loss: torch.Tensor     # f32 scalar
+    logprob: torch.Tensor  # f32 [...]
+    entropy: torch.Tensor  # f32 [...]
+    stats: torch.Tensor    # f32 [6]: pg_loss, kl, entropy, old_approx_kl, approx_kl, clipfrac
+
+
+class DistillLoss(NamedTuple):
+    loss: torch.Tensor  # f32 scalar
+    kl: torch.Tensor    # f32 [...]
+
+
+class _Rows:
+    """Logits as evenly spaced rows, and the checks every operator makes."""
+
+    def __init__(self, logits: torch.Tensor):
+        if not isinstance(logits, torch.Tensor):
+            raise TypeError("logits: expected a tensor")
+        if logits.dtype not in _DTYPES:
+            raise TypeError(f"logits: {logits.dtype} is not one of float32, bfloat16, float16")
+        if logits.dim() < 1 or logits.shape[-1] < 1:
+            raise ValueError(f"logits: shape {tuple(logits.shape)} has no entries in a row")
+        if logits.device.type != "cuda":
+            raise ValueError("logits: expected a tensor on the GPU")
+        self.x = logits.detach()
+        self.lead, self.vocab = tuple(logits.shape[:-1]), logits.shape[-1]
+        self.n = math.prod(self.lead)
+        self.device = logits.device
+        if self.vocab > _lib.CAT_MAX_VOCAB:
+            raise ValueError(f"logits: {self.vocab} entries in a row, at most {_lib.CAT_MAX_VOCAB}")
+        if self.n > 2**31 - 1:
+            raise ValueError(f"logits: {self.n} rows, at most 2^31 - 1")
+        if self.vocab > 1 and logits.stride(-1) != 1:
+            raise ValueError("logits: the entries of a row are not adjacent (stride 1)")
+        self.stride = self.vocab
+        if self.n > 0:
+            try:
+                self.stride = self.x.view(self.n, self.vocab).stride(0) if self.n > 1 else self.vocab
+            except RuntimeError:
+                raise ValueError("logits: the leading dimensions do not collapse to evenly spaced rows") from None
+
+    def arg(self):
+        return _lib.RtCatLogits(self.x.data_ptr(), self.n, self.stride, self.vocab, _DTYPES[self.x.dtype])
+
+    def per_row(self, t, name: str, dtype=torch.float32, tail=()):
+        """`t` ([...] or [..., k]) as the kernels read it, or None."""
+        if t is None:
+            return None
+        if not isinstance(t, torch.Tensor):
+            raise TypeError(f"{name}: expected a tensor")
+        if tuple(t.shape) != self.lead + tuple(tail):
+            raise ValueError(f"{name}: shape {tuple(t.shape)}, expected {self.lead + tuple(tail)}")
+        if t.device != self.device:
+            raise ValueError(f"{name}: on {t.device}, the logits on {self.device}")
+        if dtype.is_floating_point != t.dtype.is_floating_point or t.dtype in (torch.bool,) or t.is_complex():
+            raise TypeError(f"{name}: {t.dtype}")
+        return t.detach().to(dtype).contiguous()
+
+    def empty(self, dtype=torch.float32):
+        return torch.empty(self.lead, dtype=dtype, device=self.device)
+
+    def grad_buffer(self, out):
+        """(tensor of the logits' shape, row stride) that a gradient is written to."""
+        if out is None:
+            # rows placed like the logits' modulo 16 bytes, so that both sides take wide accesses
+            per = 16 // self.x.element_size()
+            lead = self.x.data_ptr() // self.x.element_size() % per
+            stride = self.vocab + (self.stride - self.vocab) % per
+            flat = torch.empty(lead + max(self.n, 1) * stride, dtype=self.x.dtype, device=self.device)
+            return flat.as_strided((self.n, self.vocab), (stride, 1), lead).view(self.x.shape), stride
+        if not isinstance(out, torch.Tensor) or out.shape != self.x.shape or out.dtype != self.x.dtype or out.device != self.device:
+            raise ValueError("out: expected a tensor of the logits' shape, type and device")
+        if out.requires_grad:
+            raise ValueError("out: requires grad")
+        o = _Rows(out)
+        if self.n > 1 and o.stride < self.vocab:
+            raise ValueError("out: rows overlap")
+        return out, max(o.stride, self.vocab)
+
+
+def _workspace(fn, r: _Rows):
+    n = int(fn(r.n, r.vocab, _DTYPES[r.x.dtype]))
+    return torch.empty(n, dtype=torch.uint8, device=r.device) if n else None, n
+
+
+def _coef(v, name: str, low=None, positive=False) -> float:
+    v = float(v)
+    if not math.isfinite(v) or (low is not None and v < low) or (positive and v <= 0):
+        raise ValueError(f"{name}: {v}")
+    return v
+
+
+def sample(logits, u, *, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0) -> Sample:
+    """One action per row from uniform numbers u in [0, 1) (rt_cat_sample).
+
+    temperature, top_k, top_p and min_p are numbers or tensors of one value per
+    row; temperature 0 takes the largest logit.  Equal logits rank by index.
+    Rows without a distribution (a NaN, +inf, nothing but -inf) get action -1
+    and NaN."""
+    r = _Rows(logits)
+    p = _lib.RtCatSampling()
+    hold = [r.per_row(u, "u")]
+    if hold[0] is None:
+        raise TypeError("u: expected a tensor")
+    p.u = hold[0].data_ptr()
+    for name, v, dtype in (("temperature", temperature, torch.float32), ("top_k", top_k, torch.int32),
+                           ("top_p", top_p, torch.float32), ("min_p", min_p, torch.float32)):
+        if isinstance(v, torch.Tensor):
+            if dtype == torch.int32 and v.dtype == torch.int64:
+                v = v.clamp(0, 2**31 - 1)
+            hold.append(r.per_row(v, name, dtype))
+            setattr(p, name, hold[-1].data_ptr())
+        elif dtype == torch.int32:
+            if int(v) != v or not 0 <= v < 2**31:
+                raise ValueError(f"top_k: {v}")
+            p.top_k_all = int(v)
+        else:
+            setattr(p, name + "_all", _coef(v, name, low=0.0))
+    out = Sample(r.empty(torch.int64), r.empty(), r.empty())
+    if r.n == 0:
+        return out
+    L = _lib.load()
+    with torch.cuda.device(r.device):
+        ws, n = _workspace(L.rt_cat_sample_workspace_bytes, r)
+        _lib.check(L.rt_cat_sample(ctypes.byref(r.arg()), ctypes.byref(p), out.action.data_ptr(),
+                                   out.logprob.data_ptr(), out.kept_logprob.data_ptr(), _lib.ptr(ws), n,
+                                   _lib.stream_handle()), "rt_cat_sample")
+    return out
+
+
+class _Ppo:
+    """The arguments of a PPO loss, checked and laid out."""
+
+    def __init__(self, logits, actions, old_logprobs, advantages, weights, ref_logprobs, temperature, clip_coef,
+                 clip_coef_high, ent_coef, kl_coef):
+        r = self.r = _Rows(logits)
+        need = {"actions": (actions, torch.int64), "old_logprobs": (old_logprobs, torch.float32),
+                "advantages": (advantages, torch.float32)}
+        self.t = {}
+        for name, (t, dtype) in need.items():
+            self.t[name] = r.per_row(t, name, dtype)
+            if t is None:
+                raise TypeError(f"{name}: expected a tensor")
+        self.t["weights"] = r.per_row(weights, "weights")
+        self.t["ref_logprobs"] = r.per_row(ref_logprobs, "ref_logprobs")
+        low = _coef(clip_coef, "clip_coef", low=0.0)
+        high = low if clip_coef_high is None else _coef(clip_coef_high, "clip_coef_high", low=0.0)
+        self.hp = _lib.RtCatPpoHparams(_coef(temperature, "temperature", positive=True), low, high,
+                                       _coef(ent_coef, "ent_coef"), _coef(kl_coef, "kl_coef"))
+        if self.hp.kl_coef != 0.0 and ref_logprobs is None:
+            raise ValueError("kl_coef without ref_logprobs")
+
+    def run(self, grad=None, stride=0, keep=False):
+        """(PpoLoss, row state or None); the gradient into `grad`."""
+        r = self.r
+        f32 = dict(dtype=torch.float32, device=r.device)
+        res = PpoLoss(torch.empty((), **f32), r.empty(), r.empty(), torch.empty(6, **f32))
+        state = torch.empty((r.n, _lib.CAT_ROW_STATE), dtype=torch.float64, device=r.device) if keep else None
+        if r.n == 0:
+            res.loss.zero_()
+            res.stats.zero_()
+            return res, state
+        L = _lib.load()
+        with torch.cuda.device(r.device):
+            ws, n = _workspace(L.rt_cat_loss_workspace_bytes, r)
+            batch = _lib.RtCatPpoBatch(**{k: _lib.ptr(t) for k, t in self.t.items()})
+            out = _lib.RtCatPpoOut(res.loss.data_ptr(), res.logprob.data_ptr(), res.entropy.data_ptr(),
+                                   res.stats.data_ptr(), _lib.ptr(grad), stride, _lib.ptr(state))
+            _lib.check(L.rt_cat_ppo(ctypes.byref(r.arg()), ctypes.byref(batch), ctypes.byref(self.hp),
+                                    ctypes.byref(out), _lib.ptr(ws), n, _lib.stream_handle()), "rt_cat_ppo")
+        return res, state
+
+
+class _PpoFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, op):
+        res, state = op.run(keep=True)
+        ctx.op = op
+        ctx.save_for_backward(logits, op.t["actions"], state)
+        ctx.mark_non_differentiable(*res[1:])
+        return tuple(res)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, gloss, *_):
+        logits, actions, state = ctx.saved_tensors
+        r = _Rows(logits)
+        grad, stride = r.grad_buffer(None)
+        if r.n == 0:
+            return grad, None
+        gloss = gloss.to(torch.float32).contiguous()
+        L = _lib.load()
+        with torch.cuda.device(r.device):
+            _lib.check(L.rt_cat_ppo_backward(ctypes.byref(r.arg()), actions.data_ptr(), ctx.op.hp.temperature,
+                                             state.data_ptr(), gloss.data_ptr(), grad.data_ptr(), stride,
+                                             _lib.stream_handle()), "rt_cat_ppo_backward")
+        return grad, None
+
+
+def ppo_loss(logits, actions, old_logprobs, advantages, *, weights=None, ref_logprobs=None, temperature=1.0,
+             clip_coef=0.2, clip_coef_high=None, ent_coef=0.0, kl_coef=0.0) -> PpoLoss:
+    """The clipped PPO loss of a categorical policy (rt_cat_ppo): the weighted
+    sum over rows of the surrogate, - ent_coef * entropy, + kl_coef * the KL
+    estimate against ref_logprobs.
+
+    weights: one per row, None: 1 / rows each.  A row with weight 0 or an
+    action outside the vocabulary is ignored.  Only `loss` is differentiable,
+    and only with respect to the logits."""
+    op = _Ppo(logits, actions, old_logprobs, advantages, weights, ref_logprobs, temperature, clip_coef,
+              clip_coef_high, ent_coef, kl_coef)
+    if torch.is_grad_enabled() and logits.requires_grad:
+        return PpoLoss(*_PpoFn.apply(logits, op))
+    return op.run()[0]
+
+
+def ppo_loss_grad(logits, actions, old_logprobs, advantages, *, weights=None, ref_logprobs=None, temperature=1.0,
+                  clip_coef=0.2, clip_coef_high=None, ent_coef=0.0, kl_coef=0.0, out=None):
+    """(ppo_loss, its gradient by the logits) in one call, outside autograd.
+
+    out: where the gradient goes; the logits themselves may be given."""
+    op = _Ppo(logits, actions, old_logprobs, advantages, weights, ref_logprobs, temperature, clip_coef,
+              clip_coef_high, ent_coef, kl_coef)
+    grad, stride = op.r.grad_buffer(out)
+    return op.run(grad, stride)[0], grad
+
+
+class _Distill:
+    def __init__(self, logits, idx, top, weights, teacher_lse, temperature):
+        r = self.r = _Rows(logits)
+        if not isinstance(idx, torch.Tensor) or idx.dim() != len(r.lead) + 1:
+            raise ValueError("teacher_idx: expected a tensor [..., k]")
+        self.k = k = idx.shape[-1]
+        if not 1 <= k <= _lib.CAT_MAX_TOP:
+            raise ValueError(f"teacher_idx: {k} entries in a row, expected 1 to {_lib.CAT_MAX_TOP}")
+        if top is None:
+            raise TypeError("teacher_logits: expected a tensor")
+        self.idx = r.per_row(idx, "teacher_idx", torch.int64, (k,))
+        self.top = r.per_row(top, "teacher_logits", torch.float32, (k,))
+        self.lse = r.per_row(teacher_lse, "teacher_lse")
+        self.weights = r.per_row(weights, "weights")
+        self.temperature = _coef(temperature, "temperature", positive=True)
+
+    def arg(self):
+        return _lib.RtCatTeacher(self.idx.data_ptr(), self.top.data_ptr(), _lib.ptr(self.lse),
+                                 _lib.ptr(self.weights), self.k, self.temperature)
+
+    def run(self, grad=None, stride=0, keep=False):
+        r = self.r
+        res = DistillLoss(torch.empty((), dtype=torch.float32, device=r.device), r.empty())
+        state = torch.empty((r.n, _lib.CAT_ROW_STATE), dtype=torch.float64, device=r.device) if keep else None
+        if r.n == 0:
+            res.loss.zero_()
+            return res, state
+        L = _lib.load()
+        with torch.cuda.device(r.device):
+            ws, n = _workspace(L.rt_cat_loss_workspace_bytes, r)
+            out = _lib.RtCatDistillOut(res.loss.data_ptr(), res.kl.data_ptr(), _lib.ptr(grad), stride, _lib.ptr(state))
+            _lib.check(L.rt_cat_distill(ctypes.byref(r.arg()), ctypes.byref(self.arg()), ctypes.byref(out),
+                                        _lib.ptr(ws), n, _lib.stream_handle()), "rt_cat_distill")
+        return res, state
+
+
+class _DistillFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, op):
+        res, state = op.run(keep=True)
+        ctx.op = op
+        ctx.save_for_backward(logits, op.idx, op.top, *(t for t in (op.lse, op.weights) if t is not None), state)
+        ctx.mark_non_differentiable(res.kl)
+        return tuple(res)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, gloss, *_):
+        logits, *_, state = ctx.saved_tensors  # raises where one of them was changed in place
+        r = _Rows(logits)
+        grad, stride = r.grad_buffer(None)
+        if r.n == 0:
+            return grad, None
+        gloss = gloss.to(torch.float32).contiguous()
+        L = _lib.load()
+        with torch.cuda.device(r.device):
+            _lib.check(L.rt_cat_distill_backward(ctypes.byref(r.arg()), ctypes.byref(ctx.op.arg()), state.data_ptr(),
+                                                 gloss.data_ptr(), grad.data_ptr(), stride, _lib.stream_handle()),
+                       "rt_cat_distill_backward")
+        return grad, None
+
+
+def distill_loss(logits, teacher_idx, teacher_logits, *, weights=None, teacher_lse=None, temperature=1.0) -> DistillLoss:
+    """KL from a teacher's top logits (rt_cat_distill), both sides at
+    `temperature`: sum_n w_n sum_j q_j (log q_j - log softmax(x / T)[idx_j]).
+
+    teacher_idx, teacher_logits [..., k]: entries outside the vocabulary (-1)
+    are unused.  teacher_lse: the teacher's logsumexp(logits / T) over its whole
+    vocabulary; without it its probabilities are normalised over the k.
+    weights: as ppo_loss.  Only `loss` is differentiable, by the logits."""
+    op = _Distill(logits, teacher_idx, teacher_logits, weights, teacher_lse, temperature)
+    if torch.is_grad_enabled() and logits.requires_grad:
+        return DistillLoss(*_DistillFn.apply(logits, op))
+    return op.run()[0]
+
+
+def distill_loss_grad(logits, teacher_idx, teacher_logits, *, weights=None, teacher_lse=None, temperature=1.0, out=None):
+    """(distill_loss, its gradient by the logits) in one call, outside autograd; `out` as ppo_loss_grad."""
+    op = _Distill(logits, teacher_idx, teacher_logits, weights, teacher_lse, temperature)
+    grad, stride = op.r.grad_buffer(out)
+    return op.run(grad, stride)[0], grad

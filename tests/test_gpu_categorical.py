@@ -1,0 +1,550 @@
+"""Categorical-policy operators (ppo_radiotherapy_amd.categorical) on the GPU
+against their definitions in 64 bits (tests/cat_plain.py): sampling, the PPO
+loss and distillation, with their gradients, over row lengths, types, strides
+and special rows."""
+import math
+
+import numpy as np
+import pytest
+
+pytestmark = pytest.mark.gpu
+torch = pytest.importorskip("torch")
+
+import cat_plain as P  # noqa: E402
+
+INF, NAN = math.inf, math.nan
+DTYPES = [torch.float32, torch.bfloat16, torch.float16]
+# one entry, one lane's worth, around a wave, around a block's tile, odd and large
+VOCABS = [1, 2, 3, 11, 16, 17, 63, 64, 65, 127, 300, 1000, 1024, 1025, 4096, 4097, 8191, 20011, 50021]
+
+
+@pytest.fixture(scope="module")
+def C():
+    import _rtpkg  # noqa: F401
+    from ppo_radiotherapy_amd import categorical
+
+    return categorical
+
+
+def gen(seed):
+    return torch.Generator(device="cuda").manual_seed(seed)
+
+
+def rows(n, v, dtype, seed, pad=0, off=0, kind="normal"):
+    """[n, v] logits inside a wider buffer whose other places hold NaN."""
+    g = gen(seed)
+    flat = torch.full((off + n * (v + pad),), NAN, dtype=dtype, device="cuda")
+    x = flat.as_strided((n, v), (v + pad, 1), off)
+    if kind == "ties":       # few distinct values: every cut falls among equals
+        x.copy_(torch.randint(-3, 4, (n, v), generator=g, device="cuda"))
+    elif kind == "flat":
+        x.fill_(1.5)
+    elif kind == "peaked":
+        x.copy_(torch.randn(n, v, generator=g, device="cuda") * 8)
+    else:
+        x.copy_(torch.randn(n, v, generator=g, device="cuda") * 2)
+    return x
+
+
+def check_sample(C, x, u, par):
+    n = x.shape[0]
+    got = C.sample(x, u, **par)
+    full = {k: (t.cpu().numpy() if torch.is_tensor(t) else np.full(n, t)) for k, t in
+            ({"temperature": 1.0, "top_k": 0, "top_p": 1.0, "min_p": 0.0} | par).items()}
+    a, lp, kp = P.sample(x.double().cpu().numpy(), u.double().cpu().numpy(), full["temperature"].astype(np.float32),
+                         full["top_k"], full["top_p"].astype(np.float32), full["min_p"].astype(np.float32))
+    assert got.action.dtype == torch.int64 and got.logprob.dtype == torch.float32
+    np.testing.assert_array_equal(got.action.cpu().numpy(), a)
+    # whole-number sums: what is left is the rounding of the result, and of exp and log (2^-50)
+    for mine, want in ((got.logprob, lp), (got.kept_logprob, kp)):
+        mine = mine.double().cpu().numpy()
+        np.testing.assert_array_equal(np.isnan(mine), np.isnan(want))
+        ok = ~np.isnan(want)
+        assert (np.abs(mine - want)[ok] <= 2.0 ** -24 * np.abs(want[ok]) + 2.0 ** -40).all()
+    return got
+
+
+FILTERS = {
+    "none": {}, "k": {"top_k": 7}, "k1": {"top_k": 1}, "p": {"top_p": 0.8}, "p0": {"top_p": 0.0},
+    "min_p": {"min_p": 0.1}, "min_p1": {"min_p": 1.0}, "k+p": {"top_k": 20, "top_p": 0.7, "temperature": 0.7},
+    "all": {"top_k": 300, "top_p": 0.95, "min_p": 0.01, "temperature": 1.7}, "greedy": {"temperature": 0.0},
+    "big k": {"top_k": 3000, "top_p": 0.97},
+}
+
+
+@pytest.mark.parametrize("v", VOCABS)
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_sample_lengths(C, v, dtype):
+    for i, (name, par) in enumerate(FILTERS.items()):
+        x = rows(5, v, dtype, 100 * v + i, pad=(0, 3, 8)[i % 3], off=i % 2)
+        u = torch.rand(5, generator=gen(v + i), device="cuda")
+        check_sample(C, x, u, par)
+
+
+@pytest.mark.parametrize("kind", ["ties", "flat", "peaked"])
+@pytest.mark.parametrize("v", [5, 64, 700, 5000, 33000])
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_sample_ties_and_peaks(C, kind, v, dtype):
+    for i, par in enumerate(FILTERS.values()):
+        x = rows(4, v, dtype, v + i, kind=kind)
+        check_sample(C, x, torch.rand(4, generator=gen(i), device="cuda"), par)
+
+
+@pytest.mark.parametrize("v", [11, 1000, 9000])
+def test_sample_extreme_numbers(C, v):
+    """u at and beyond its ends; per-row parameters at and beyond theirs."""
+    u = torch.tensor([0.0, 2.0 ** -24, 0.5, 1 - 2.0 ** -24, 1.0, 3.0, -1.0, NAN, INF], device="cuda")
+    n = len(u)
+    x = rows(n, v, torch.float32, 3)
+    check_sample(C, x, u, {})
+    check_sample(C, x, u, {"top_k": 3, "top_p": 0.5})
+    t = torch.tensor([1e-38, 1e-45, 1e30, INF, NAN, -1.0, 0.0, 1.0, 3.0], device="cuda")
+    k = torch.tensor([0, -5, v, v + 1, 2 ** 31 - 1, 1, 2, v - 1, 5], dtype=torch.int32, device="cuda")
+    p = torch.tensor([NAN, 1.0, 1e-30, -1.0, 2.0, 1 - 2.0 ** -24, 0.3, 0.5, 0.9], device="cuda")
+    q = torch.tensor([NAN, -1.0, 0.0, 2.0, 1.0, 1e-30, 0.5, 0.01, 0.1], device="cuda")
+    u = torch.rand(n, generator=gen(1), device="cuda")
+    for par in ({"temperature": t}, {"top_k": k}, {"top_p": p}, {"min_p": q},
+                {"temperature": t, "top_k": k, "top_p": p, "min_p": q}):
+        check_sample(C, x, u, par)
+    check_sample(C, x, u, {"top_k": k.long() * 4})
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("v", [3, 70, 1500, 20000])
+def test_sample_special_rows(C, dtype, v):
+    low = torch.finfo(dtype).min
+    x = rows(12, v, dtype, 9)
+    x[0] = -INF
+    x[1, 1:] = -INF
+    x[2, :-1] = -INF
+    x[3, v // 2] = NAN
+    x[4, -1] = INF
+    x[5] = NAN
+    x[6] = low
+    x[7, 1:] = low
+    x[8, ::2] = -INF
+    x[9] = torch.finfo(dtype).max
+    x[10] = 0.0
+    x[10, ::2] = -0.0
+    x[11] = -INF
+    x[11, v // 2] = low
+    u = torch.rand(12, generator=gen(2), device="cuda")
+    for par in FILTERS.values():
+        check_sample(C, x, u, par)
+
+
+def test_sample_large_batches(C):
+    """More rows than a grid holds at once, wide rows of every filter side by side, and one long row."""
+    g = gen(4)
+    x = torch.randn(30001, 11, generator=g, device="cuda")
+    check_sample(C, x, torch.rand(30001, generator=g, device="cuda"), {})
+    n, v = 40, 131072
+    x = (torch.randn(n, v, generator=g, device="cuda") * 2).bfloat16()
+    pick = lambda *s: torch.tensor(s, device="cuda")[torch.randint(len(s), (n,), generator=g, device="cuda")]  # noqa: E731
+    par = {"temperature": pick(0.0, 0.5, 1.0, 2.0), "top_k": pick(0, 1, 50, 5000).int(),
+           "top_p": pick(1.0, 0.95, 0.5), "min_p": pick(0.0, 0.05)}
+    check_sample(C, x, torch.rand(n, generator=g, device="cuda"), par)
+    x = torch.randn(1, 2 ** 20, generator=g, device="cuda")
+    for par in ({}, {"top_p": 0.9}, {"top_k": 100}, {"top_k": 100000, "top_p": 0.5}):
+        check_sample(C, x, torch.rand(1, generator=g, device="cuda"), par)
+
+
+def test_sample_frequencies(C):
+    """Equal steps of u meet each kept entry as often as its probability says (within one step)."""
+    n = 4096
+    x = torch.randn(1, 37, generator=gen(5), device="cuda")
+    u = (torch.arange(n, device="cuda") + 0.5) / n
+    a = C.sample(x.expand(n, 37), u, top_k=10, temperature=1.3).action
+    top = x[0].topk(10)
+    p = torch.softmax(top.values.double() / 1.3, 0)
+    count = torch.bincount(a, minlength=37)
+    assert int(count.sum()) == int(count[top.indices].sum()) == n
+    assert ((count[top.indices] - p * n).abs() <= 1.0).all()
+
+
+# ---- losses ---------------------------------------------------------------
+def ppo_inputs(n, v, seed, logits):
+    g = gen(seed)
+    a = torch.randint(0, v, (n,), generator=g, device="cuda")
+    lp = torch.log_softmax(logits.double().nan_to_num(0, 0, -30), 1).gather(1, a[:, None])[:, 0]
+    old = (lp + 0.3 * torch.randn(n, generator=g, device="cuda")).float()
+    ref = (lp + 0.2 * torch.randn(n, generator=g, device="cuda")).float()
+    adv = torch.randn(n, generator=g, device="cuda")
+    w = torch.rand(n, generator=g, device="cuda")
+    return a, old, adv, w, ref
+
+
+def teacher_inputs(n, v, k, seed):
+    g = gen(seed)
+    idx = torch.randint(0, v, (n, k), generator=g, device="cuda")
+    return idx, torch.randn(n, k, generator=g, device="cuda") * 3, torch.rand(n, generator=g, device="cuda")
+
+
+def near(got, want, names):
+    for k in names:
+        value, tol = want[k]
+        d = (got[k].double() - value).abs()
+        same = (got[k].double() == value) | (got[k].isnan() & value.isnan())
+        bad = ~(same | (d <= tol))
+        assert not bad.any(), f"{k}: {int(bad.sum())} of {bad.numel()} off, the worst by {float((d / tol.clamp(min=1e-300))[bad].max()):.3g} of its tolerance"
+
+
+def run_ppo(C, x, a, old, adv, grad=True, **kw):
+    r, g = C.ppo_loss_grad(x, a, old, adv, **kw)
+    return r._asdict() | {"grad": g}
+
+
+@pytest.mark.parametrize("v", VOCABS)
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_ppo_lengths(C, v, dtype):
+    for i, (n, pad, off) in enumerate([(1, 0, 0), (6, 0, 1), (70, 5, 0), (9, 8, 3)]):
+        x = rows(n, v, dtype, v + i, pad, off, kind=("normal", "peaked", "normal", "flat")[i])
+        a, old, adv, w, ref = ppo_inputs(n, v, v + i, x)
+        want = P.ppo(x, a, old, adv, w, ref, 0.9, 0.2, 0.3, 0.01, 0.1)
+        got = run_ppo(C, x, a, old, adv, weights=w, ref_logprobs=ref, temperature=0.9, clip_coef=0.2,
+                      clip_coef_high=0.3, ent_coef=0.01, kl_coef=0.1)
+        near(got, want, ("loss", "stats", "logprob", "entropy", "grad"))
+        # the loss alone, and the gradient through autograd with a factor behind it
+        alone = C.ppo_loss(x, a, old, adv, weights=w, ref_logprobs=ref, temperature=0.9, clip_coef=0.2,
+                           clip_coef_high=0.3, ent_coef=0.01, kl_coef=0.1)
+        near(alone._asdict(), want, ("loss", "stats", "logprob", "entropy"))
+        want = P.ppo(x, a, old, adv, None, None, 1.0, 0.2, 0.2, 0.0, 0.0, scale=-2.5)
+        leaf = x.detach().requires_grad_()
+        r = C.ppo_loss(leaf, a, old, adv)
+        near(r._asdict(), want, ("loss", "stats", "logprob", "entropy"))
+        g, = torch.autograd.grad(-2.5 * r.loss, leaf)
+        near({"grad": g}, want, ("grad",))
+
+
+@pytest.mark.parametrize("v,k", [(1, 1), (2, 3), (11, 4), (17, 16), (64, 8), (65, 65), (300, 256), (1000, 33), (1025, 7),
+                                 (4097, 64), (20011, 1024), (50021, 33)])
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_distill_lengths(C, v, k, dtype):
+    for i, (n, pad, off) in enumerate([(1, 0, 0), (6, 0, 1), (70, 5, 0), (9, 8, 3)]):
+        x = rows(n, v, dtype, v + i, pad, off, kind=("normal", "peaked", "normal", "flat")[i])
+        idx, top, w = teacher_inputs(n, v, k, v + i)
+        lse = torch.logsumexp(top / 2.0, 1) + 0.3 if i % 2 else None
+        if i > 1:
+            idx[0] = -1                # a teacher without entries
+            idx[1, k // 2:] = v + 5    # ... with fewer
+            top[1, k // 2:] = NAN
+            idx[2] = int(idx[2, 0])         # the same index throughout
+            top[3, 0] = -INF
+        want = P.distill(x, idx, top, w, lse, 2.0)
+        r, g = C.distill_loss_grad(x, idx, top, weights=w, teacher_lse=lse, temperature=2.0)
+        near(r._asdict() | {"grad": g}, want, ("loss", "kl", "grad"))
+        want = P.distill(x, idx, top, None, lse, 2.0, scale=3.0)
+        leaf = x.detach().requires_grad_()
+        r = C.distill_loss(leaf, idx, top, teacher_lse=lse, temperature=2.0)
+        g, = torch.autograd.grad(3.0 * r.loss, leaf)
+        near(r._asdict() | {"grad": g}, want, ("loss", "kl", "grad"))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("v", [5, 100, 3000, 40000])
+def test_losses_special_rows(C, dtype, v):
+    """Masked entries, rows of nothing, ignored rows whose numbers are NaN, a NaN that counts."""
+    n = 10
+    x = rows(n, v, dtype, 21)
+    low = torch.finfo(dtype).min
+    a, old, adv, w, ref = ppo_inputs(n, v, 21, x)
+    x[0] = -INF
+    x[1, 1:] = -INF
+    a[1] = 0
+    x[2, ::2] = -INF
+    a[2] = 1
+    x[3] = NAN
+    w[3] = 0.0
+    x[4] = INF
+    a[4] = -1
+    a[5] = v
+    x[6] = low
+    x[7, 1:] = low
+    a[7] = 0
+    x[8] = torch.finfo(dtype).max
+    kw = dict(weights=w, ref_logprobs=ref, ent_coef=0.02, kl_coef=0.1)
+    want = P.ppo(x, a, old, adv, w, ref, ent=0.02, klc=0.1)
+    near(run_ppo(C, x, a, old, adv, **kw), want, ("loss", "stats", "logprob", "entropy", "grad"))
+    leaf = x.detach().requires_grad_()
+    g, = torch.autograd.grad(C.ppo_loss(leaf, a, old, adv, **kw).loss, leaf)
+    near({"grad": g}, want, ("grad",))
+    assert not g[[0, 3, 4, 5]].any()
+
+    x[4] = 1.0
+    idx, top, w = teacher_inputs(n, v, 3, 22)
+    w[3] = 0.0
+    idx[1] = 0
+    idx[2] = torch.tensor([1, 3, 1])
+    want = P.distill(x, idx, top, w)
+    r, g = C.distill_loss_grad(x, idx, top, weights=w)
+    near(r._asdict() | {"grad": g}, want, ("loss", "kl", "grad"))
+    leaf = x.detach().requires_grad_()
+    g, = torch.autograd.grad(C.distill_loss(leaf, idx, top, weights=w).loss, leaf)
+    near({"grad": g}, want, ("grad",))
+
+    # a NaN in a row that counts, and all of one: the loss and that row say so, the others do not notice
+    for fill in (slice(1, 2), slice(None)):
+        y = rows(3, v, dtype, 23)
+        y[1, fill] = NAN
+        a, old, adv, w, _ = ppo_inputs(3, v, 23, y)
+        r, g = C.ppo_loss_grad(y, a, old, adv)
+        assert r.loss.isnan() and r.logprob.isnan().tolist() == [False, True, False]
+        assert g.isnan().any(1).tolist() == [False, True, False]
+        idx, top, _ = teacher_inputs(3, v, 2, 24)
+        r, g = C.distill_loss_grad(y, idx, top)
+        assert r.loss.isnan() and r.kl.isnan().tolist() == [False, True, False]
+        assert g.isnan().any(1).tolist() == [False, True, False]
+
+
+def test_distill_impossible_entry(C):
+    """A student that rules out what the teacher names: infinite, with a finite gradient."""
+    x = torch.zeros(2, 4, device="cuda")
+    x[0, 2] = -INF
+    idx = torch.tensor([[2, 0], [2, 0]], device="cuda")
+    r, g = C.distill_loss_grad(x, idx, torch.zeros(2, 2, device="cuda"))
+    assert r.loss == INF and r.kl[0] == INF and r.kl[1].isfinite()
+    assert torch.allclose(g[0].double(), torch.tensor([1 / 6 - 1 / 4, 1 / 6, -1 / 4, 1 / 6], device="cuda", dtype=torch.float64), atol=2.0 ** -20)
+
+
+def test_ppo_clip_sides(C):
+    """The clipped side has no gradient, the other has; both signs of the advantage."""
+    x = torch.randn(4, 9, generator=gen(6), device="cuda")
+    a = torch.tensor([0, 1, 2, 3], device="cuda")
+    lp = torch.log_softmax(x.double(), 1).gather(1, a[:, None])[:, 0]
+    old = (lp - torch.tensor([0.5, 0.5, -0.5, -0.5], device="cuda")).float()
+    adv = torch.tensor([1.0, -1.0, 1.0, -1.0], device="cuda")
+    r, g = C.ppo_loss_grad(x, a, old, adv, clip_coef=0.2)
+    assert g.any(1).tolist() == [False, True, True, False] and r.stats[5] == 1.0
+
+
+def test_gradients_against_differences(C):
+    """Along random directions, the oracle's loss in 64 bits changes by what the kernels' gradients say."""
+    n, v = 7, 53
+    x = torch.randn(n, v, generator=gen(7), device="cuda")
+    a, old, adv, w, ref = ppo_inputs(n, v, 7, x)
+    idx, top, _ = teacher_inputs(n, v, 5, 7)
+    g1 = C.ppo_loss_grad(x, a, old, adv, weights=w, ref_logprobs=ref, temperature=1.3, ent_coef=0.1, kl_coef=0.2)[1]
+    g2 = C.distill_loss_grad(x, idx, top, weights=w, temperature=1.7)[1]
+    f1 = lambda y: P.ppo(y, a, old, adv, w, ref, 1.3, 0.2, 0.2, 0.1, 0.2)["loss"][0]  # noqa: E731
+    f2 = lambda y: P.distill(y, idx, top, w, None, 1.7)["loss"][0]  # noqa: E731
+    for s in range(5):
+        d = torch.randn(n, v, generator=gen(70 + s), device="cuda", dtype=torch.float64)
+        for f, g in ((f1, g1), (f2, g2)):
+            h = 1e-5  # truncation h^2, cancellation 2^-52 / h
+            slope = (f(x.double() + h * d) - f(x.double() - h * d)) / (2 * h)
+            size = (g.double() * d).abs().sum()
+            assert abs(float(slope - (g.double() * d).sum())) <= 1e-6 * float(size) + 1e-8
+
+
+@pytest.mark.parametrize("v", [11, 300, 5000, 60000])
+def test_shapes_strides_and_places(C, v):
+    """Leading dimensions, broadcast rows, one row, no rows, gradients into given memory and in place."""
+    g = gen(8)
+    x = torch.randn(4, 3, v + 2, generator=g, device="cuda")[..., 1:-1]
+    u = torch.rand(4, 3, generator=g, device="cuda")
+    flat = x.reshape(12, v)
+    s, t = C.sample(x, u, top_k=5), C.sample(flat, u.reshape(12), top_k=5)
+    assert s.action.shape == (4, 3) and torch.equal(s.action.reshape(12), t.action)
+    a, old, adv, w, _ = ppo_inputs(12, v, 8, flat)
+    shape = lambda q: q.reshape(4, 3)  # noqa: E731
+    r1, g1 = C.ppo_loss_grad(x, shape(a), shape(old), shape(adv))
+    r2, g2 = C.ppo_loss_grad(flat, a, old, adv)
+    assert g1.shape == x.shape and torch.equal(g1.reshape(12, v), g2) and torch.equal(r1.loss, r2.loss)
+    one = C.ppo_loss_grad(flat[0], a[0], old[0], adv[0])[1]
+    two = C.ppo_loss_grad(flat[:1], a[:1], old[:1], adv[:1])[1]
+    assert one.shape == (v,) and torch.equal(one, two[0])
+    # broadcast rows: the gradient of the row they come from is the sum
+    base = flat[:1].clone().requires_grad_()
+    C.ppo_loss(base.expand(12, v), a, old, adv).loss.backward()
+    many = C.ppo_loss_grad(flat[:1].repeat(12, 1), a, old, adv)[1]
+    assert torch.allclose(base.grad[0].double(), many.double().sum(0), rtol=0, atol=12 * 2.0 ** -22 * float(many.abs().max()))
+    # given memory: what lies between the rows stays
+    for dtype in DTYPES:
+        y = flat.to(dtype)
+        ref = C.ppo_loss_grad(y, a, old, adv)[1]
+        wide = torch.full((12, v + 7), 5.0, dtype=dtype, device="cuda")
+        got = C.ppo_loss_grad(y, a, old, adv, out=wide[:, 2:v + 2])[1]
+        assert torch.equal(got, ref) and (wide[:, :2] == 5).all() and (wide[:, v + 2:] == 5).all()
+        idx, top, w = teacher_inputs(12, v, 4, 8)
+        idx[0] = 0
+        want = C.distill_loss_grad(y, idx, top)[1]
+        z = y.clone()
+        assert torch.equal(C.distill_loss_grad(z, idx, top, out=z)[1], want) and torch.equal(z, want)
+        z = torch.nn.functional.pad(y, (1, 2))[:, 1:-2]
+        C.ppo_loss_grad(z, a, old, adv, out=z)
+        assert torch.equal(z, ref)
+    none = torch.empty(0, v, device="cuda", requires_grad=True)
+    e = torch.empty(0, device="cuda")
+    assert C.sample(none, e).action.shape == (0,)
+    r = C.ppo_loss(none, e.long(), e, e)
+    r.loss.backward()
+    assert r.loss == 0 and none.grad.shape == (0, v)
+    r, gr = C.distill_loss_grad(none, torch.empty(0, 3, dtype=torch.int64, device="cuda"), torch.empty(0, 3, device="cuda"))
+    assert r.loss == 0 and gr.shape == (0, v)
+
+
+def test_rows_past_32_bits(C):
+    """Rows that start more than 2^32 bytes and 2^31 elements into their buffer."""
+    v, n = 131072, 16500
+    x = torch.zeros(n, v, dtype=torch.bfloat16, device="cuda")
+    tail = rows(4, v, torch.bfloat16, 31)
+    x[-4:] = tail
+    a, old, adv, w, _ = ppo_inputs(4, v, 31, tail)
+    pad = lambda t, fill: torch.cat([torch.full((n - 4,), fill, dtype=t.dtype, device="cuda"), t])  # noqa: E731
+    want = P.ppo(tail, a, old, adv, w)
+    r, g = C.ppo_loss_grad(x, pad(a, -1), pad(old, 0.0), pad(adv, 0.0), weights=pad(w, 1.0), out=x)
+    near({"loss": r.loss, "logprob": r.logprob[-4:], "grad": g[-4:]}, want, ("loss", "logprob", "grad"))
+    assert not g[:-4].any()
+
+
+def test_repeated_runs_are_bitwise_equal(C):
+    for v in (11, 500, 50021):
+        x = rows(33, v, torch.bfloat16, 41)
+        a, old, adv, w, ref = ppo_inputs(33, v, 41, x)
+        first = run_ppo(C, x, a, old, adv, weights=w, ent_coef=0.1)
+        idx, top, _ = teacher_inputs(33, v, 9, 41)
+        second, grad = C.distill_loss_grad(x, idx, top)
+        u = torch.rand(33, generator=gen(1), device="cuda")
+        third = C.sample(x, u, top_p=0.9)
+        for _ in range(5):
+            again = run_ppo(C, x, a, old, adv, weights=w, ent_coef=0.1)
+            assert all(torch.equal(again[k], first[k]) for k in first)
+            r, g = C.distill_loss_grad(x, idx, top)
+            assert torch.equal(g, grad) and torch.equal(r.loss, second.loss)
+            assert all(torch.equal(p, q) for p, q in zip(C.sample(x, u, top_p=0.9), third))
+
+
+@pytest.mark.parametrize("v", [11, 2000, 60000])
+def test_graph_and_stream(C, v):
+    """Captured on a stream of its own, replayed on changing inputs with eager work between, two graphs side by side."""
+    n = 13
+    x = torch.empty(n, v, dtype=torch.bfloat16, device="cuda")
+    u = torch.empty(n, device="cuda")
+    a, old, adv, w, _ = ppo_inputs(n, v, 51, rows(n, v, torch.bfloat16, 51))
+    idx, top, _ = teacher_inputs(n, v, 6, 51)
+
+    def step():
+        s = C.sample(x, u, top_k=40, top_p=0.9)
+        r, g = C.ppo_loss_grad(x, s.action, s.logprob, adv, weights=w, ent_coef=0.01)
+        d, h = C.distill_loss_grad(x, idx, top, temperature=1.5)
+        return [*s, *r, g, *d, h]
+
+    def fill(seed):
+        x.copy_(rows(n, v, torch.bfloat16, seed))
+        u.copy_(torch.rand(n, generator=gen(seed), device="cuda"))
+
+    fill(0)
+    step()
+    torch.cuda.synchronize()
+    graphs = []
+    for _ in range(2):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            out = step()
+        graphs.append((g, out))
+    for seed in range(1, 5):
+        fill(seed)
+        want = step()
+        for g, _ in graphs:
+            g.replay()
+        torch.cuda.synchronize()
+        for _, out in graphs:
+            for p, q in zip(out, want):
+                assert torch.equal(p, q)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = step()
+    side.synchronize()
+    assert all(torch.equal(p, q) for p, q in zip(got, want))
+
+
+def test_changed_inputs_are_noticed(C):
+    """Autograd's own check: logits or actions changed in place between the loss and its gradient."""
+    x = torch.randn(3, 20, device="cuda", requires_grad=True)
+    y = x * 1.0
+    a, old, adv, _, _ = ppo_inputs(3, 20, 61, x.detach())
+    r = C.ppo_loss(y, a, old, adv)
+    with torch.no_grad():
+        y.add_(1.0)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        r.loss.backward()
+
+
+def test_refusals(C):
+    x = torch.randn(4, 10, device="cuda")
+    v = torch.zeros(4, device="cuda")
+    i = torch.zeros(4, dtype=torch.int64, device="cuda")
+    bad = [
+        (lambda: C.sample(x.double(), v), TypeError), (lambda: C.sample(x.cpu(), v), ValueError),
+        (lambda: C.sample(x, v.cpu()), ValueError), (lambda: C.sample(x, v[:3]), ValueError),
+        (lambda: C.sample(x, None), TypeError), (lambda: C.sample(x.t(), torch.zeros(10, device="cuda")), ValueError),
+        (lambda: C.sample(x, v, temperature=-1.0), ValueError), (lambda: C.sample(x, v, temperature=NAN), ValueError),
+        (lambda: C.sample(x, v, top_k=-1), ValueError), (lambda: C.sample(x, v, top_k=1.5), ValueError),
+        (lambda: C.sample(x, v, top_p=NAN), ValueError), (lambda: C.sample(x, v, min_p=-0.1), ValueError),
+        (lambda: C.sample(x, v, top_k=v), TypeError), (lambda: C.sample(x[:, :0], v), ValueError),
+        (lambda: C.sample(torch.randn(4, 3, 10, device="cuda")[:, :2], torch.zeros(4, 2, device="cuda")), ValueError),
+        (lambda: C.ppo_loss(x, i, v, v, temperature=0.0), ValueError), (lambda: C.ppo_loss(x, i, v, v, clip_coef=-1), ValueError),
+        (lambda: C.ppo_loss(x, i, v, v, ent_coef=INF), ValueError), (lambda: C.ppo_loss(x, i, v, v, kl_coef=0.1), ValueError),
+        (lambda: C.ppo_loss(x, v, v, v), TypeError), (lambda: C.ppo_loss(x, i, v, None), TypeError),
+        (lambda: C.ppo_loss_grad(x, i, v, v, out=x.half()), ValueError),
+        (lambda: C.ppo_loss_grad(x, i, v, v, out=x[:1].expand(4, 10)), ValueError),
+        (lambda: C.distill_loss(x, i, v), ValueError),
+        (lambda: C.distill_loss(x, i[:, None], v[:, None], temperature=INF), ValueError),
+        (lambda: C.distill_loss(x, i[:, None].expand(4, 1025), v[:, None].expand(4, 1025)), ValueError),
+        (lambda: C.distill_loss(x, i[:, None][:, :0], v[:, None][:, :0]), ValueError),
+        (lambda: C.distill_loss(x, i[:, None], v[:, None], teacher_lse=i), TypeError),
+    ]
+    for k, (call, kind) in enumerate(bad):
+        with pytest.raises(kind):
+            call()
+            pytest.fail(f"call {k} was not refused")
+    import _rtpkg  # noqa: F401
+    from ppo_radiotherapy_amd._lib import RtError
+
+    wide = torch.randn(4, 20, device="cuda")
+    with pytest.raises(RtError, match="overlaps"):
+        C.ppo_loss_grad(wide[:, :10], i, v, v, out=wide[:, 5:15])
+
+
+def test_policy_iteration_together(C):
+    """The operators as one iteration uses them: sample a rollout, GAE, a PPO update of a linear policy through
+    autograd, then its distillation into another; each step against the definitions in 64 bits."""
+    import _rtpkg  # noqa: F401
+    from ppo_radiotherapy_amd import _lib
+
+    L = _lib.load()
+    T, N, D, V = 8, 32, 12, 44
+    g = gen(77)
+    W = (0.3 * torch.randn(D, V, generator=g, device="cuda")).requires_grad_()
+    obs = torch.randn(T, N, D, generator=g, device="cuda")
+    u = torch.rand(T, N, generator=g, device="cuda")
+    with torch.no_grad():
+        logits = obs.reshape(T * N, D).mm(W).reshape(T, N, V)
+        s = C.sample(logits, u, temperature=1.1)
+    reward = (s.action % 5 == 0).float()
+    values, zero = torch.zeros(T, N, device="cuda"), torch.zeros(T, N, device="cuda")
+    last = torch.zeros(N, device="cuda")
+    adv, ret = torch.empty_like(values), torch.empty_like(values)
+    _lib.check(L.rt_gae(T, N, reward.data_ptr(), values.data_ptr(), zero.data_ptr(), last.data_ptr(), last.data_ptr(),
+                        0.99, 0.95, adv.data_ptr(), ret.data_ptr(), _lib.stream_handle()), "rt_gae")
+    x = obs.reshape(T * N, D).mm(W)
+    out = C.ppo_loss(x, s.action.reshape(-1), s.logprob.reshape(-1), adv.reshape(-1), temperature=1.1, ent_coef=0.01)
+    # the policy has not moved: its log-probabilities are the rollout's, the ratio is 1
+    assert float((out.logprob - s.logprob.reshape(-1)).abs().max()) <= 2.0 ** -19
+    assert out.stats[5] == 0 and abs(float(out.stats[4])) <= 2.0 ** -30
+    out.loss.backward()
+    want = P.ppo(x.detach(), s.action.reshape(-1), s.logprob.reshape(-1), adv.reshape(-1), T=1.1, ent=0.01)
+    gW = obs.reshape(T * N, D).double().t() @ want["grad"][0]
+    room = obs.reshape(T * N, D).double().abs().t() @ (want["grad"][1] + want["grad"][0].abs() * 2.0 ** -20)
+    assert ((W.grad.double() - gW).abs() <= room).all()
+    before = float(want["loss"][0])
+    with torch.no_grad():
+        W -= 0.5 * W.grad
+        x = obs.reshape(T * N, D).mm(W)
+        after = float(C.ppo_loss(x, s.action.reshape(-1), s.logprob.reshape(-1), adv.reshape(-1), temperature=1.1, ent_coef=0.01).loss)
+    assert after < before
+    top, idx = x.topk(6, dim=1)
+    student = torch.zeros(T * N, V, device="cuda")
+    r, grad = C.distill_loss_grad(student, idx, top, temperature=1.0)
+    near(r._asdict() | {"grad": grad}, P.distill(student, idx, top), ("loss", "kl", "grad"))
