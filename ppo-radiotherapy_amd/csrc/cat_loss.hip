@@ -8,15 +8,15 @@
 // plus something at a few named entries: C at the action (PPO), or -C q_j at
 // each of the teacher's (distillation, where E = 0).  A row's state is
 // therefore five numbers: m, log S, E, F, C.
+#include <algorithm>
 #include <string>
+#include <type_traits>
 
 #include "cat_rows.h"
 
 namespace {
 
 using namespace rtcat;
-
-constexpr int kThreads = 256;
 
 // (m and log S apart: their sum would lose log S beside a lowest-value m)
 struct RowState {
@@ -90,140 +90,343 @@ struct Distill {
     }
 };
 
-// What a block holds of a row's teacher: the entries inside the vocabulary
-// (others idx -1, q 0).
-struct Teacher {
-    int32_t idx[RT_CAT_MAX_TOP];
-    double q[RT_CAT_MAX_TOP];   // first log q, then q
-};
-
 template <class D>
 __device__ __forceinline__ const typename D::raw* row_of(const Logits& l, int64_t n) {
     return static_cast<const typename D::raw*>(l.x) + n * l.stride;
 }
 
-// The teacher's entries and their log-probabilities into LDS.
+// A row as 16-byte pieces that are aligned wherever the row starts, and the
+// few entries before and after them ("edges", at most 2 (PER - 1) <= 14: one
+// per thread).
+template <class D>
+struct Span {
+    static constexpr int kPer = 16 / (int)sizeof(typename D::raw);
+    const typename D::raw* x;
+    int32_t head, pieces, edges;
+
+    __device__ Span(const typename D::raw* row, int32_t V) : x(row) {
+        head = min(V, (int32_t)((0 - (uintptr_t)row) % 16 / sizeof(typename D::raw)));
+        pieces = (V - head) / kPer;
+        edges = V - pieces * kPer;
+    }
+    __device__ __forceinline__ int32_t edge(int t) const { return t < head ? t : pieces * kPer + t; }
+    __device__ __forceinline__ uint4 piece(int32_t i) const {
+        return *reinterpret_cast<const uint4*>(x + head + (int64_t)i * kPer);
+    }
+};
+
+template <class D>
+struct Unpack {
+    static constexpr int kPer = 16 / (int)sizeof(typename D::raw);
+    float v[kPer];
+    __device__ __forceinline__ explicit Unpack(const uint4& r) {
+        const uint32_t w[4] = {r.x, r.y, r.z, r.w};
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) {
+            if constexpr (kPer == 4) v[i] = __uint_as_float(w[i]);
+            else v[i] = D::get((typename D::raw)(i & 1 ? w[i / 2] >> 16 : w[i / 2] & 0xffff));
+        }
+    }
+    __device__ __forceinline__ float max() const {
+        float m = v[0];
+#pragma unroll
+        for (int i = 1; i < kPer; ++i) m = fmaxf(m, v[i]);
+        return m;
+    }
+};
+
+template <class D>
+__device__ __forceinline__ uint4 pack(const float* v) {
+    uint32_t w[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        if constexpr (sizeof(typename D::raw) == 4) w[i] = __float_as_uint(v[i]);
+        else w[i] = (uint32_t)D::put(v[2 * i]) | (uint32_t)D::put(v[2 * i + 1]) << 16;
+    }
+    return make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+// 16 bytes of entries that add nothing
+template <class D>
+__device__ __forceinline__ uint4 nothing() {
+    if constexpr (sizeof(typename D::raw) == 4) return make_uint4(0xff800000u, 0xff800000u, 0xff800000u, 0xff800000u);
+    const uint32_t two = (uint32_t)D::put(-INFINITY) * 0x10001u;
+    return make_uint4(two, two, two, two);
+}
+
+// ---- a row's sums ----------------------------------------------------------
+// In units of log 2: t = (x - m) c, c = log2(e) / T.  exp2 is the hardware's
+// (within one unit of the last place); up to eight terms are added in f32,
+// those sums in f64.  c is rounded to f32 (2^-25 of t) and so is t (2^-24):
+// together they move log S by less than 2^-23 of the row's entropy, less than
+// the f32 outputs resolve.
+struct Sums {
+    double s, u;  // sum 2^t and sum t 2^t
+};
+
+__device__ __forceinline__ float scale_of(double t) { return (float)fmin(1.4426950408889634 / t, 3.0e38); }
+
+// t for a factor beside 2^t: where 2^t is 0 anyway it must stay finite.  2^t
+// itself is taken of the plain t, so that a NaN reaches the sums.
+__device__ __forceinline__ float finite_t(float t) { return fmaxf(t, -200.0f); }
+
+template <class D, bool U>
+__device__ __forceinline__ void add_piece(const uint4& r, float m, float c, Sums& a) {
+    const Unpack<D> x(r);
+    float s = 0.0f, u = 0.0f;
+#pragma unroll
+    for (int i = 0; i < Unpack<D>::kPer; ++i) {
+        const float t = (x.v[i] - m) * c, e = __builtin_amdgcn_exp2f(t);
+        s += e;
+        if (U) u = fmaf(e, finite_t(t), u);
+    }
+    a.s += (double)s;
+    if (U) a.u += (double)u;
+}
+
+template <bool U>
+__device__ __forceinline__ void move_to(Sums& a, double by) {  // by = (old m - new m) c <= 0
+    const double f = exp2(by);
+    if (U) a.u = f == 0.0 ? 0.0 : f * (a.u + by * a.s);
+    a.s *= f;
+}
+
+constexpr int kBatch = 4;  // pieces a thread has in flight where a row is streamed
+
+// The maximum and sums of pieces [from, to) of a row, and of its edges where
+// `edges` is set.  The first THREADS * HELD pieces stay in `held`; what is left
+// is streamed, each thread with a maximum of its own.  The result is the same
+// in every thread.  A part of nothing but -inf: m = -inf and sums 0, or NaN
+// where it has one.
+template <class D, int THREADS, int HELD, bool U>
+__device__ void row_sums(const Span<D>& row, int32_t from, int32_t to, bool edges, float c, uint4* held, float* fs,
+                         double* ds, float* m_out, Sums* out) {
+    const int tid = threadIdx.x;
+    float top = -INFINITY, mine = -INFINITY;  // of what is held; of what is streamed
+    Sums a{0.0, 0.0};
+    float xe = -INFINITY;
+    if (edges && tid < row.edges) xe = D::get(row.x[row.edge(tid)]);
+#pragma unroll
+    for (int k = 0; k < HELD; ++k) {
+        const int32_t i = from + k * THREADS + tid;
+        held[k] = i < to ? row.piece(i) : nothing<D>();
+    }
+    for (int32_t i = from + HELD * THREADS + tid; i < to; i += kBatch * THREADS) {
+        uint4 r[kBatch];
+#pragma unroll
+        for (int k = 0; k < kBatch; ++k) r[k] = i + k * THREADS < to ? row.piece(i + k * THREADS) : nothing<D>();
+        float bm = mine;
+#pragma unroll
+        for (int k = 0; k < kBatch; ++k) bm = fmaxf(bm, Unpack<D>(r[k]).max());
+        if (bm > mine) {
+            if (mine > -INFINITY) move_to<U>(a, ((double)mine - (double)bm) * (double)c);
+            mine = bm;
+        }
+        if (mine > -INFINITY) {
+#pragma unroll
+            for (int k = 0; k < kBatch; ++k) add_piece<D, U>(r[k], mine, c, a);
+        } else {  // only -inf so far, or a NaN
+            float bad = 0.0f;
+#pragma unroll
+            for (int k = 0; k < kBatch; ++k) {
+                const Unpack<D> x(r[k]);
+#pragma unroll
+                for (int j = 0; j < Unpack<D>::kPer; ++j) bad = x.v[j] != x.v[j] ? x.v[j] : bad;
+            }
+            a.s += (double)bad;
+        }
+    }
+    top = fmaxf(xe, mine);
+#pragma unroll
+    for (int k = 0; k < HELD; ++k) top = fmaxf(top, Unpack<D>(held[k]).max());
+    const float m = block_max<THREADS>(top, fs);
+    if (m == -INFINITY) {
+        float bad = xe != xe ? xe : 0.0f;
+#pragma unroll
+        for (int k = 0; k < HELD; ++k) {
+            const Unpack<D> x(held[k]);
+#pragma unroll
+            for (int j = 0; j < Unpack<D>::kPer; ++j) bad = x.v[j] != x.v[j] ? x.v[j] : bad;
+        }
+        a.s += (double)bad;
+    } else {
+        if (mine > -INFINITY && mine != m) move_to<U>(a, ((double)mine - (double)m) * (double)c);
+#pragma unroll
+        for (int k = 0; k < HELD; ++k) add_piece<D, U>(held[k], m, c, a);
+        const float t = (xe - m) * c, e = __builtin_amdgcn_exp2f(t);
+        if (edges && tid < row.edges) {
+            a.s += (double)e;
+            if (U) a.u += (double)(e * finite_t(t));
+        }
+    }
+    out->s = block_sum<THREADS>(a.s, ds);
+    out->u = U ? block_sum<THREADS>(a.u, ds) : 0.0;
+    *m_out = m;
+}
+
+// ---- a row's gradient ------------------------------------------------------
+// scale p (E lp + F) = 2^t (a t + b), f32; rounded once to the logits' type.
+struct Slope {
+    float m, c, a, b;
+};
+
+__device__ __forceinline__ Slope slope_of(const RowState& s, double t, double scale) {
+    const double inv = scale * exp(-s.logs);
+    return Slope{(float)s.m, scale_of(t), (float)(inv * s.e * 0.6931471805599453), (float)(inv * (s.f - s.e * s.logs))};
+}
+
+template <bool E>
+__device__ __forceinline__ float slope_at(const Slope& g, float x) {
+    const float t = (x - g.m) * g.c, e = __builtin_amdgcn_exp2f(t);
+    return E ? e * fmaf(finite_t(t), g.a, g.b) : e * g.b;
+}
+
+template <class D, bool E>
+__device__ __forceinline__ void put_piece(typename D::raw* g, const Span<D>& row, int32_t i, bool aligned, const uint4& r,
+                                          const Slope& sl, bool skip) {
+    const Unpack<D> x(r);
+    float v[Unpack<D>::kPer];
+#pragma unroll
+    for (int k = 0; k < Unpack<D>::kPer; ++k) v[k] = skip ? 0.0f : slope_at<E>(sl, x.v[k]);
+    typename D::raw* at = g + row.head + (int64_t)i * Span<D>::kPer;
+    if (aligned) {
+        *reinterpret_cast<uint4*>(at) = pack<D>(v);
+    } else {
+#pragma unroll
+        for (int k = 0; k < Span<D>::kPer; ++k) at[k] = D::put(v[k]);
+    }
+}
+
+// The same numbers at one entry, in f64.
+template <class Op, class D>
+__device__ double dense_at(const Op& op, const RowState& s, const typename D::raw* x, int64_t i) {
+    const double lp = ((double)D::get(x[i]) - s.m) / op.t - s.logs, p = exp(lp);
+    return p == 0.0 ? 0.0 : p * ((Op::ppo ? s.e : 0.0) * lp + s.f);
+}
+
+// What a block holds of a row's teacher: the entries inside the vocabulary
+// (others idx -1, q 0).
+struct Teacher {
+    int32_t idx[RT_CAT_MAX_TOP];
+    double q[RT_CAT_MAX_TOP];  // log q, then q
+};
+struct NoTeacher {};
+
+// log of the teacher's normaliser
 template <int THREADS>
-__device__ void teacher_load(const Distill& op, int64_t n, int32_t V, Teacher& te, float* fs, double* ds) {
+__device__ double teacher_lse(const Distill& op, int64_t n, int32_t V, float* fs, double* ds) {
+    if (op.b.lse) return op.b.lse[n];
     const int64_t at = n * op.b.k;
     float m = -INFINITY;
     for (int j = threadIdx.x; j < op.b.k; j += THREADS) {
         const int64_t i = op.b.idx[at + j];
+        if (i >= 0 && i < V) m = fmaxf(m, op.b.logits[at + j]);
+    }
+    m = block_max<THREADS>(m, fs);
+    if (m == -INFINITY) m = 0.0f;
+    double s = 0.0;
+    for (int j = threadIdx.x; j < op.b.k; j += THREADS) {
+        const int64_t i = op.b.idx[at + j];
+        if (i >= 0 && i < V) s += exp(((double)op.b.logits[at + j] - (double)m) / op.t);
+    }
+    s = block_sum<THREADS>(s, ds);
+    return s == 0.0 ? 0.0 : (double)m / op.t + log(s);
+}
+
+// The teacher's entries and their log-probabilities into LDS.
+template <int THREADS>
+__device__ void teacher_load(const Distill& op, int64_t n, int32_t V, double lse, Teacher& te) {
+    const int64_t at = n * op.b.k;
+    for (int j = threadIdx.x; j < op.b.k; j += THREADS) {
+        const int64_t i = op.b.idx[at + j];
         const bool in = i >= 0 && i < V;
         te.idx[j] = in ? (int32_t)i : -1;
-        te.q[j] = in ? (double)op.b.logits[at + j] : -INFINITY;
-        if (in) m = fmaxf(m, op.b.logits[at + j]);
+        te.q[j] = in ? (double)op.b.logits[at + j] / op.t - lse : -INFINITY;
     }
-    double lse;
-    if (op.b.lse) {
-        lse = op.b.lse[n];
-    } else {
-        m = block_max<THREADS>(m, fs);
-        if (m == -INFINITY) m = 0.0f;
-        double s = 0.0;
-        for (int j = threadIdx.x; j < op.b.k; j += THREADS) s += exp((te.q[j] - (double)m) / op.t);
-        s = block_sum<THREADS>(s, ds);
-        lse = s == 0.0 ? 0.0 : (double)m / op.t + log(s);
-    }
-    for (int j = threadIdx.x; j < op.b.k; j += THREADS) te.q[j] = te.idx[j] < 0 ? -INFINITY : te.q[j] / op.t - lse;
     __syncthreads();
 }
 
-// ---- one block per row -----------------------------------------------------
-// d loss / d x at the entries that are named, on top of the dense part: each
-// value is computed whole before any is written (the gradient may lie in the
-// logits' own memory) and rounded once.
-constexpr int kNamed = RT_CAT_MAX_TOP / kThreads;
+// What the named entries' gradient is on top of the dense part: each is
+// computed whole, before anything is written (the gradient may lie in the
+// logits' own memory), and stored over the dense value.
+template <int THREADS>
+struct Named {
+    static constexpr int kMost = (RT_CAT_MAX_TOP + THREADS - 1) / THREADS;
+    int32_t at[kMost];
+    float v[kMost];
+};
 
-template <class D, class Op, int THREADS>
-__device__ void write_grad(const Logits& l, const Op& op, int64_t n, const RowState& s, double scale, bool skip,
-                           const Teacher* te, typename D::raw* g) {
-    const auto* x = row_of<D>(l, n);
-    const int32_t V = l.vocab;
+// first, last: the entries that this block writes
+template <class D, class Op, int THREADS, class Te>
+__device__ void named_find(const Op& op, int64_t n, const RowState& s, double scale, bool skip, const Te& te,
+                           const typename D::raw* x, Named<THREADS>& e, int32_t first, int32_t last) {
     const int tid = threadIdx.x;
-    const auto dense = [&](int32_t i) {
-        const double lp = ((double)D::get(x[i]) - s.m) / op.t - s.logs, p = exp(lp);
-        return p == 0.0 ? 0.0 : p * (s.e * lp + s.f);
-    };
-    int32_t at[kNamed];
-    float v[kNamed];
     if constexpr (Op::ppo) {
-        at[0] = -1;
+        e.at[0] = -1;
         if (!skip && tid == 0) {
-            at[0] = (int32_t)op.b.actions[n];
-            v[0] = (float)(scale * (dense(at[0]) + s.c));
+            const int64_t a = op.b.actions[n];
+            if (a >= first && a < last) {
+                e.at[0] = (int32_t)a;
+                e.v[0] = (float)(scale * (dense_at<Op, D>(op, s, x, a) + s.c));
+            }
         }
     } else {
 #pragma unroll
-        for (int k = 0; k < kNamed; ++k) {
+        for (int k = 0; k < Named<THREADS>::kMost; ++k) {
             const int j = tid + k * THREADS;
-            at[k] = !skip && j < op.b.k ? te->idx[j] : -1;
-            if (at[k] < 0) continue;
+            e.at[k] = !skip && j < op.b.k ? te.idx[j] : -1;
+            if (e.at[k] < first || e.at[k] >= last) e.at[k] = -1;
+            if (e.at[k] < 0) continue;
             double q = 0.0;
             for (int i = 0; i < op.b.k; ++i)
-                if (te->idx[i] == at[k]) q += te->q[i];
-            v[k] = (float)(scale * (dense(at[k]) - s.c * q));
+                if (te.idx[i] == e.at[k]) q += te.q[i];
+            e.v[k] = (float)(scale * (dense_at<Op, D>(op, s, x, e.at[k]) - s.c * q));
         }
     }
-    __syncthreads();
-    for (int i = tid; i < V; i += THREADS) g[i] = D::put(skip ? 0.0f : (float)(scale * dense(i)));
-    __syncthreads();
-#pragma unroll
-    for (int k = 0; k < (Op::ppo ? 1 : kNamed); ++k)
-        if (at[k] >= 0) g[at[k]] = D::put(v[k]);
 }
 
 template <class D, class Op, int THREADS>
-__global__ __launch_bounds__(THREADS) void k_cat_row(Logits l, Op op, Out o, double* terms) {
-    __shared__ float fs[THREADS / 64];
-    __shared__ double ds[THREADS / 64];
-    __shared__ Teacher te;
-    const int64_t n = blockIdx.x;
-    const int32_t V = l.vocab;
-    const int tid = threadIdx.x;
-    const auto* x = row_of<D>(l, n);
+__device__ void named_put(const Named<THREADS>& e, typename D::raw* g) {
+#pragma unroll
+    for (int k = 0; k < (Op::ppo ? 1 : Named<THREADS>::kMost); ++k)
+        if (e.at[k] >= 0) g[e.at[k]] = D::put(e.v[k]);
+}
 
-    bool skip = op.ignored(n, V);
-    float m = -INFINITY;
-    double S = 0.0, U = 0.0;
-    if (!skip) {
-        float nan = 0.0f;
-        for (int i = tid; i < V; i += THREADS) {
-            const float v = D::get(x[i]);
-            m = fmaxf(m, v);
-            nan += v != v ? 1.0f : 0.0f;
-        }
-        m = block_max<THREADS>(m, fs);
-        nan = block_sum<THREADS>(nan, fs);
-        skip = m == -INFINITY && nan == 0.0f;
-    }
-    if (!skip) {
-        for (int i = tid; i < V; i += THREADS) {
-            const double z = ((double)D::get(x[i]) - (double)m) / op.t, e = exp(z);
-            S += e;
-            if (Op::ppo && e != 0.0) U += e * z;
-        }
-        S = block_sum<THREADS>(S, ds);
-        if (Op::ppo) U = block_sum<THREADS>(U, ds);
-    }
-    double term[Op::terms] = {};
+// ---- from the sums to the loss ---------------------------------------------
+// The row's outputs, its terms of the sums over rows, and its state.  Every
+// thread of the block calls it; every thread gets the state.
+template <class D, class Op, int THREADS, class Te>
+__device__ RowState finish_row(const Logits& l, const Op& op, const Out& o, int64_t n, bool skip, float m,
+                               const Sums& sums, const typename D::raw* x, Te& te, double* terms, bool write, float* fs,
+                               double* ds, RowState* share) {
+    const int tid = threadIdx.x;
     RowState st{0.0, INFINITY, 0.0, 0.0, 0.0};  // log S +inf: a row that adds nothing
-    const double logs = log(S);
     if constexpr (Op::ppo) {
-        double lp = 0.0, h = 0.0;
-        if (!skip) {
-            lp = ((double)D::get(x[op.b.actions[n]]) - (double)m) / op.t - logs;
-            h = logs - U / S;
-            st = op.finish(n, l.rows, m, logs, lp, h, term);
+        if (tid < 64) {
+            double term[Op::terms] = {}, lp = 0.0, h = 0.0;
+            if (!skip) {
+                const double logs = log(sums.s);
+                lp = ((double)D::get(x[op.b.actions[n]]) - (double)m) / op.t - logs;
+                h = logs - 0.6931471805599453 * (sums.u / sums.s);
+                st = op.finish(n, l.rows, m, logs, lp, h, term);
+            }
+            if (tid == 0) {
+                *share = st;
+                if (write) {
+                    o.logprob[n] = (float)lp;
+                    o.entropy[n] = (float)h;
+                    for (int k = 0; k < Op::terms; ++k) terms[n * Op::terms + k] = term[k];
+                }
+            }
         }
-        if (tid == 0) {
-            o.logprob[n] = (float)lp;
-            o.entropy[n] = (float)h;
-        }
+        __syncthreads();
+        st = *share;
     } else {
-        double kl = 0.0, Q = 0.0;
+        double kl = 0.0;
         if (!skip) {
-            teacher_load<THREADS>(op, n, V, te, fs, ds);
+            const double logs = log(sums.s), lse = teacher_lse<THREADS>(op, n, l.vocab, fs, ds);
+            teacher_load<THREADS>(op, n, l.vocab, lse, te);
+            double Q = 0.0;
             for (int j = tid; j < op.b.k; j += THREADS) {
                 const double lq = te.q[j], q = exp(lq);
                 if (te.idx[j] >= 0 && q != 0.0) kl += q * (lq - (((double)D::get(x[te.idx[j]]) - (double)m) / op.t - logs));
@@ -233,45 +436,107 @@ __global__ __launch_bounds__(THREADS) void k_cat_row(Logits l, Op op, Out o, dou
             Q = block_sum<THREADS>(Q, ds);
             kl = block_sum<THREADS>(kl, ds);
             const double w = op.weight(n, l.rows);
-            st = RowState{m, logs, 0.0, w * Q / op.t, w / op.t};
-            term[0] = w * kl;
+            // E is 0 throughout: its place keeps the teacher's normaliser for the backward pass
+            st = RowState{m, logs, lse, w * Q / op.t, w / op.t};
+            if (tid == 0 && write) terms[n] = w * kl;
+        } else if (tid == 0 && write) {
+            terms[n] = 0.0;
         }
-        if (tid == 0) o.kl[n] = (float)kl;
+        if (tid == 0 && write) o.kl[n] = (float)kl;
     }
-    if (tid == 0) {
-        for (int k = 0; k < Op::terms; ++k) terms[n * Op::terms + k] = term[k];
-        if (o.state) {
-            double* s = o.state + n * RT_CAT_ROW_STATE;
-            s[0] = st.m;
-            s[1] = st.logs;
-            s[2] = st.e;
-            s[3] = st.f;
-            s[4] = st.c;
-        }
-    }
-    if (o.grad)
-        write_grad<D, Op, THREADS>(l, op, n, st, 1.0, skip, &te, static_cast<typename D::raw*>(o.grad) + n * o.grad_stride);
+    if (tid == 0 && write && o.state) *reinterpret_cast<RowState*>(o.state + n * RT_CAT_ROW_STATE) = st;
+    return st;
 }
 
-template <class D, class Op, int THREADS>
-__global__ __launch_bounds__(THREADS) void k_cat_backward(Logits l, Op op, const double* state, const float* gout,
-                                                          void* grad, int64_t grad_stride) {
+template <class Op>
+__device__ __forceinline__ Slope op_slope(const Op& op, RowState s, double scale) {
+    if (!Op::ppo) s.e = 0.0;
+    return slope_of(s, op.t, scale);
+}
+
+// ---- one block per row -----------------------------------------------------
+// The row is read once: HELD pieces of every thread stay in registers between
+// the sums and the gradient, which longer rows read again.
+template <class D, class Op, int THREADS, int HELD>
+__global__ __launch_bounds__(THREADS) void k_cat_row(Logits l, Op op, Out o, double* terms) {
     __shared__ float fs[THREADS / 64];
     __shared__ double ds[THREADS / 64];
-    __shared__ Teacher te;
+    __shared__ RowState share;
+    __shared__ std::conditional_t<Op::ppo, NoTeacher, Teacher> te;
     const int64_t n = blockIdx.x;
-    const double* s = state + n * RT_CAT_ROW_STATE;
-    const RowState st{s[0], s[1], s[2], s[3], s[4]};
+    const int tid = threadIdx.x;
+    const auto* x = row_of<D>(l, n);
+    const Span<D> row(x, l.vocab);
+    uint4 held[HELD ? HELD : 1];
+    float m = -INFINITY;
+    Sums sums{0.0, 0.0};
+    bool skip = op.ignored(n, l.vocab);
+    if (!skip) {
+        row_sums<D, THREADS, HELD, Op::ppo>(row, 0, row.pieces, true, scale_of(op.t), held, fs, ds, &m, &sums);
+        skip = m == -INFINITY && sums.s == 0.0;
+    }
+    const RowState st = finish_row<D, Op, THREADS>(l, op, o, n, skip, m, sums, x, te, terms, true, fs, ds, &share);
+    if (!o.grad) return;
+    auto* g = static_cast<typename D::raw*>(o.grad) + n * o.grad_stride;
+    Named<THREADS> named;
+    named_find<D, Op, THREADS>(op, n, st, 1.0, skip, te, x, named, 0, l.vocab);
+    const Slope sl = op_slope(op, st, 1.0);
+    const bool aligned = (((uintptr_t)g ^ (uintptr_t)x) & 15) == 0;
+    float xe = 0.0f;
+    if (tid < row.edges) xe = D::get(x[row.edge(tid)]);
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < HELD; ++k) {
+        const int32_t i = k * THREADS + tid;
+        if (i < row.pieces) put_piece<D, Op::ppo>(g, row, i, aligned, held[k], sl, skip);
+    }
+    for (int32_t i = HELD * THREADS + tid; i < row.pieces; i += THREADS)
+        put_piece<D, Op::ppo>(g, row, i, aligned, row.piece(i), sl, skip);
+    if (tid < row.edges) g[row.edge(tid)] = D::put(skip ? 0.0f : slope_at<Op::ppo>(sl, xe));
+    __syncthreads();
+    named_put<D, Op, THREADS>(named, g);
+}
+
+// ---- a row's gradient from its state, by parts -----------------------------
+template <class D, class Op, int THREADS>
+__global__ __launch_bounds__(THREADS) void k_cat_backward(Logits l, Op op, const RowState* state, const float* gout,
+                                                          void* grad, int64_t grad_stride, int32_t parts) {
+    __shared__ std::conditional_t<Op::ppo, NoTeacher, Teacher> te;
+    const int64_t n = blockIdx.x / parts;
+    const int32_t part = blockIdx.x % parts;
+    const int tid = threadIdx.x;
+    const auto* x = row_of<D>(l, n);
+    auto* g = static_cast<typename D::raw*>(grad) + n * grad_stride;
+    const Span<D> row(x, l.vocab);
+    const RowState st = state[n];
     const bool skip = st.logs == INFINITY;
+    const double scale = gout ? (double)*gout : 1.0;
+    const int32_t per = (row.pieces + parts - 1) / parts;
+    const int32_t from = min(part * per, row.pieces), to = min(from + per, row.pieces);
+    // the first part also has the entries before the pieces, the last those behind
+    const int32_t first = part == 0 ? 0 : row.head + from * Span<D>::kPer;
+    const int32_t last = part == parts - 1 ? l.vocab : row.head + to * Span<D>::kPer;
     if constexpr (!Op::ppo) {
         if (!skip) {
-            teacher_load<THREADS>(op, n, l.vocab, te, fs, ds);
-            for (int j = threadIdx.x; j < op.b.k; j += THREADS) te.q[j] = exp(te.q[j]);
+            teacher_load<THREADS>(op, n, l.vocab, st.e, te);
+            for (int j = tid; j < op.b.k; j += THREADS) te.q[j] = exp(te.q[j]);
             __syncthreads();
         }
     }
-    write_grad<D, Op, THREADS>(l, op, n, st, gout ? (double)*gout : 1.0, skip, &te,
-                               static_cast<typename D::raw*>(grad) + n * grad_stride);
+    Named<THREADS> named;
+    named_find<D, Op, THREADS>(op, n, st, scale, skip, te, x, named, first, last);
+    const Slope sl = op_slope(op, st, scale);
+    const bool aligned = (((uintptr_t)g ^ (uintptr_t)x) & 15) == 0;
+    const int32_t e = tid < row.edges ? row.edge(tid) : -1;
+    const bool mine = e >= first && e < last;
+    float xe = 0.0f;
+    if (mine) xe = D::get(x[e]);
+    __syncthreads();
+    for (int32_t i = from + tid; i < to; i += THREADS)
+        put_piece<D, Op::ppo>(g, row, i, aligned, skip ? nothing<D>() : row.piece(i), sl, skip);
+    if (mine) g[e] = D::put(skip ? 0.0f : slope_at<Op::ppo>(sl, xe));
+    __syncthreads();
+    named_put<D, Op, THREADS>(named, g);
 }
 
 // ---- sums over the rows ----------------------------------------------------
@@ -295,9 +560,19 @@ __global__ __launch_bounds__(1024) void k_cat_total(const double* terms, int64_t
 // per-row terms of the sums over rows: the loss and up to six statistics
 int64_t terms_bytes(int64_t rows) { return rows * Ppo::terms * (int64_t)sizeof(double); }
 
+template <class D, class Op, int THREADS, int HELD>
+void launch_row(const Logits& l, const Op& op, const Out& o, double* ws, hipStream_t st) {
+    hipLaunchKernelGGL((k_cat_row<D, Op, THREADS, HELD>), dim3((unsigned)l.rows), dim3(THREADS), 0, st, l, op, o, ws);
+}
+
 template <class D, class Op>
 int run_loss(const Logits& l, const Op& op, const Out& o, double* ws, hipStream_t st) {
-    hipLaunchKernelGGL((k_cat_row<D, Op, kThreads>), dim3((unsigned)l.rows), dim3(kThreads), 0, st, l, op, o, ws);
+    const int32_t pieces = l.vocab / Span<D>::kPer;
+    if (!o.grad) launch_row<D, Op, 256, 0>(l, op, o, ws, st);
+    else if (pieces <= 256 * 4) launch_row<D, Op, 256, 4>(l, op, o, ws, st);
+    else if (pieces <= 256 * 16) launch_row<D, Op, 256, 16>(l, op, o, ws, st);
+    else if (pieces <= 512 * 16) launch_row<D, Op, 512, 16>(l, op, o, ws, st);
+    else launch_row<D, Op, 1024, 16>(l, op, o, ws, st);
     hipLaunchKernelGGL((k_cat_total<Op::terms>), dim3(1), dim3(1024), 0, st, ws, l.rows, o.loss, o.stats);
     return launched();
 }
@@ -312,8 +587,10 @@ int pick_loss(int dtype, const Logits& l, const Op& op, const Out& o, double* ws
 template <class D, class Op>
 int run_backward(const Logits& l, const Op& op, const double* state, const float* gout, void* grad, int64_t stride,
                  hipStream_t st) {
-    hipLaunchKernelGGL((k_cat_backward<D, Op, kThreads>), dim3((unsigned)l.rows), dim3(kThreads), 0, st, l, op, state,
-                       gout, grad, stride);
+    // 256 threads, eight pieces each
+    const int64_t parts = std::max<int64_t>(1, std::min<int64_t>(l.vocab / (2048 * Span<D>::kPer), INT32_MAX / l.rows));
+    hipLaunchKernelGGL((k_cat_backward<D, Op, 256>), dim3((unsigned)(l.rows * parts)), dim3(256), 0, st, l, op,
+                       reinterpret_cast<const RowState*>(state), gout, grad, stride, (int32_t)parts);
     return launched();
 }
 
