@@ -21,6 +21,7 @@ ValueError or TypeError before anything is launched.
 from __future__ import annotations
 
 import ctypes
+import functools
 import math
 from typing import NamedTuple
 
@@ -52,34 +53,42 @@ class DistillLoss(NamedTuple):
 class _Rows:
     """Logits as evenly spaced rows, and the checks every operator makes."""
 
+    __slots__ = ("x", "lead", "n", "vocab", "stride", "device", "dtype")
+
     def __init__(self, logits: torch.Tensor):
         if not isinstance(logits, torch.Tensor):
             raise TypeError("logits: expected a tensor")
-        if logits.dtype not in _DTYPES:
+        self.dtype = _DTYPES.get(logits.dtype, -1)
+        if self.dtype < 0:
             raise TypeError(f"logits: {logits.dtype} is not one of float32, bfloat16, float16")
-        if logits.dim() < 1 or logits.shape[-1] < 1:
-            raise ValueError(f"logits: shape {tuple(logits.shape)} has no entries in a row")
-        if logits.device.type != "cuda":
+        shape = logits.shape
+        if not shape or shape[-1] < 1:
+            raise ValueError(f"logits: shape {tuple(shape)} has no entries in a row")
+        if not logits.is_cuda:
             raise ValueError("logits: expected a tensor on the GPU")
-        self.x = logits.detach()
-        self.lead, self.vocab = tuple(logits.shape[:-1]), logits.shape[-1]
+        self.x, self.device = logits, logits.device
+        self.lead, self.vocab = shape[:-1], shape[-1]
         self.n = math.prod(self.lead)
-        self.device = logits.device
         if self.vocab > _lib.CAT_MAX_VOCAB:
             raise ValueError(f"logits: {self.vocab} entries in a row, at most {_lib.CAT_MAX_VOCAB}")
         if self.n > 2**31 - 1:
             raise ValueError(f"logits: {self.n} rows, at most 2^31 - 1")
-        if self.vocab > 1 and logits.stride(-1) != 1:
+        strides = logits.stride()
+        if self.vocab > 1 and strides[-1] != 1:
             raise ValueError("logits: the entries of a row are not adjacent (stride 1)")
-        self.stride = self.vocab
-        if self.n > 0:
-            try:
-                self.stride = self.x.view(self.n, self.vocab).stride(0) if self.n > 1 else self.vocab
-            except RuntimeError:
-                raise ValueError("logits: the leading dimensions do not collapse to evenly spaced rows") from None
+        # the leading dimensions, from the last: each as far apart as all rows before it together
+        self.stride, rows = self.vocab, 1
+        for size, step in zip(reversed(self.lead), reversed(strides[:-1])):
+            if size == 1 or self.n == 0:
+                continue
+            if rows == 1:
+                self.stride = step
+            elif step != self.stride * rows:
+                raise ValueError("logits: the leading dimensions do not collapse to evenly spaced rows")
+            rows *= size
 
     def arg(self):
-        return _lib.RtCatLogits(self.x.data_ptr(), self.n, self.stride, self.vocab, _DTYPES[self.x.dtype])
+        return _lib.RtCatLogits(self.x.data_ptr(), self.n, self.stride, self.vocab, self.dtype)
 
     def per_row(self, t, name: str, dtype=torch.float32, tail=()):
         """`t` ([...] or [..., k]) as the kernels read it, or None."""
@@ -87,11 +96,13 @@ class _Rows:
             return None
         if not isinstance(t, torch.Tensor):
             raise TypeError(f"{name}: expected a tensor")
-        if tuple(t.shape) != self.lead + tuple(tail):
-            raise ValueError(f"{name}: shape {tuple(t.shape)}, expected {self.lead + tuple(tail)}")
+        if t.shape != self.lead + tail:
+            raise ValueError(f"{name}: shape {tuple(t.shape)}, expected {tuple(self.lead + tail)}")
         if t.device != self.device:
             raise ValueError(f"{name}: on {t.device}, the logits on {self.device}")
-        if dtype.is_floating_point != t.dtype.is_floating_point or t.dtype in (torch.bool,) or t.is_complex():
+        if t.dtype == dtype and t.is_contiguous():
+            return t
+        if dtype.is_floating_point != t.dtype.is_floating_point or t.dtype == torch.bool or t.is_complex():
             raise TypeError(f"{name}: {t.dtype}")
         return t.detach().to(dtype).contiguous()
 
@@ -102,9 +113,11 @@ class _Rows:
         """(tensor of the logits' shape, row stride) that a gradient is written to."""
         if out is None:
             # rows placed like the logits' modulo 16 bytes, so that both sides take wide accesses
-            per = 16 // self.x.element_size()
-            lead = self.x.data_ptr() // self.x.element_size() % per
-            stride = self.vocab + (self.stride - self.vocab) % per
+            size = self.x.element_size()
+            lead, extra = self.x.data_ptr() % 16 // size, (self.stride - self.vocab) % (16 // size)
+            if not lead and not extra:
+                return torch.empty(self.x.shape, dtype=self.x.dtype, device=self.device), self.vocab
+            stride = self.vocab + extra
             flat = torch.empty(lead + max(self.n, 1) * stride, dtype=self.x.dtype, device=self.device)
             return flat.as_strided((self.n, self.vocab), (stride, 1), lead).view(self.x.shape), stride
         if not isinstance(out, torch.Tensor) or out.shape != self.x.shape or out.dtype != self.x.dtype or out.device != self.device:
@@ -116,9 +129,28 @@ class _Rows:
             raise ValueError("out: rows overlap")
         return out, max(o.stride, self.vocab)
 
+    def call(self, fn, what: str, *args):
+        """fn(*args, stream) on the logits' device and its current stream."""
+        here = torch.cuda.current_device()
+        if here == self.device.index:
+            _lib.check(fn(*args, _raw_stream(here) or None), what)
+        else:
+            with torch.cuda.device(self.device):
+                _lib.check(fn(*args, _raw_stream(self.device.index) or None), what)
 
-def _workspace(fn, r: _Rows):
-    n = int(fn(r.n, r.vocab, _DTYPES[r.x.dtype]))
+
+# the handle alone: building torch's Stream object costs more than a launch
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
+    lambda index: torch.cuda.current_stream(index).cuda_stream)
+
+
+@functools.lru_cache(maxsize=256)
+def _workspace_bytes(name: str, rows: int, vocab: int, dtype: int) -> int:
+    return int(getattr(_lib.load(), name)(rows, vocab, dtype))
+
+
+def _workspace(name: str, r: _Rows):
+    n = _workspace_bytes(name, r.n, r.vocab, r.dtype)
     return torch.empty(n, dtype=torch.uint8, device=r.device) if n else None, n
 
 
@@ -158,12 +190,9 @@ def sample(logits, u, *, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0) -> Samp
     out = Sample(r.empty(torch.int64), r.empty(), r.empty())
     if r.n == 0:
         return out
-    L = _lib.load()
-    with torch.cuda.device(r.device):
-        ws, n = _workspace(L.rt_cat_sample_workspace_bytes, r)
-        _lib.check(L.rt_cat_sample(ctypes.byref(r.arg()), ctypes.byref(p), out.action.data_ptr(),
-                                   out.logprob.data_ptr(), out.kept_logprob.data_ptr(), _lib.ptr(ws), n,
-                                   _lib.stream_handle()), "rt_cat_sample")
+    ws, n = _workspace("rt_cat_sample_workspace_bytes", r)
+    r.call(_lib.load().rt_cat_sample, "rt_cat_sample", ctypes.byref(r.arg()), ctypes.byref(p), out.action.data_ptr(),
+           out.logprob.data_ptr(), out.kept_logprob.data_ptr(), _lib.ptr(ws), n)
     return out
 
 
@@ -199,14 +228,14 @@ class _Ppo:
             res.loss.zero_()
             res.stats.zero_()
             return res, state
-        L = _lib.load()
-        with torch.cuda.device(r.device):
-            ws, n = _workspace(L.rt_cat_loss_workspace_bytes, r)
-            batch = _lib.RtCatPpoBatch(**{k: _lib.ptr(t) for k, t in self.t.items()})
-            out = _lib.RtCatPpoOut(res.loss.data_ptr(), res.logprob.data_ptr(), res.entropy.data_ptr(),
-                                   res.stats.data_ptr(), _lib.ptr(grad), stride, _lib.ptr(state))
-            _lib.check(L.rt_cat_ppo(ctypes.byref(r.arg()), ctypes.byref(batch), ctypes.byref(self.hp),
-                                    ctypes.byref(out), _lib.ptr(ws), n, _lib.stream_handle()), "rt_cat_ppo")
+        ws, n = _workspace("rt_cat_loss_workspace_bytes", r)
+        t = self.t
+        batch = _lib.RtCatPpoBatch(t["actions"].data_ptr(), t["old_logprobs"].data_ptr(), t["advantages"].data_ptr(),
+                                   _lib.ptr(t["weights"]), _lib.ptr(t["ref_logprobs"]))
+        out = _lib.RtCatPpoOut(res.loss.data_ptr(), res.logprob.data_ptr(), res.entropy.data_ptr(),
+                               res.stats.data_ptr(), _lib.ptr(grad), stride, _lib.ptr(state))
+        r.call(_lib.load().rt_cat_ppo, "rt_cat_ppo", ctypes.byref(r.arg()), ctypes.byref(batch), ctypes.byref(self.hp),
+               ctypes.byref(out), _lib.ptr(ws), n)
         return res, state
 
 
@@ -228,11 +257,8 @@ class _PpoFn(torch.autograd.Function):
         if r.n == 0:
             return grad, None
         gloss = gloss.to(torch.float32).contiguous()
-        L = _lib.load()
-        with torch.cuda.device(r.device):
-            _lib.check(L.rt_cat_ppo_backward(ctypes.byref(r.arg()), actions.data_ptr(), ctx.op.hp.temperature,
-                                             state.data_ptr(), gloss.data_ptr(), grad.data_ptr(), stride,
-                                             _lib.stream_handle()), "rt_cat_ppo_backward")
+        r.call(_lib.load().rt_cat_ppo_backward, "rt_cat_ppo_backward", ctypes.byref(r.arg()), actions.data_ptr(),
+               ctx.op.hp.temperature, state.data_ptr(), gloss.data_ptr(), grad.data_ptr(), stride)
         return grad, None
 
 
@@ -290,12 +316,10 @@ class _Distill:
         if r.n == 0:
             res.loss.zero_()
             return res, state
-        L = _lib.load()
-        with torch.cuda.device(r.device):
-            ws, n = _workspace(L.rt_cat_loss_workspace_bytes, r)
-            out = _lib.RtCatDistillOut(res.loss.data_ptr(), res.kl.data_ptr(), _lib.ptr(grad), stride, _lib.ptr(state))
-            _lib.check(L.rt_cat_distill(ctypes.byref(r.arg()), ctypes.byref(self.arg()), ctypes.byref(out),
-                                        _lib.ptr(ws), n, _lib.stream_handle()), "rt_cat_distill")
+        ws, n = _workspace("rt_cat_loss_workspace_bytes", r)
+        out = _lib.RtCatDistillOut(res.loss.data_ptr(), res.kl.data_ptr(), _lib.ptr(grad), stride, _lib.ptr(state))
+        r.call(_lib.load().rt_cat_distill, "rt_cat_distill", ctypes.byref(r.arg()), ctypes.byref(self.arg()),
+               ctypes.byref(out), _lib.ptr(ws), n)
         return res, state
 
 
@@ -317,11 +341,8 @@ class _DistillFn(torch.autograd.Function):
         if r.n == 0:
             return grad, None
         gloss = gloss.to(torch.float32).contiguous()
-        L = _lib.load()
-        with torch.cuda.device(r.device):
-            _lib.check(L.rt_cat_distill_backward(ctypes.byref(r.arg()), ctypes.byref(ctx.op.arg()), state.data_ptr(),
-                                                 gloss.data_ptr(), grad.data_ptr(), stride, _lib.stream_handle()),
-                       "rt_cat_distill_backward")
+        r.call(_lib.load().rt_cat_distill_backward, "rt_cat_distill_backward", ctypes.byref(r.arg()),
+               ctypes.byref(ctx.op.arg()), state.data_ptr(), gloss.data_ptr(), grad.data_ptr(), stride)
         return grad, None
 
 

@@ -539,6 +539,311 @@ __global__ __launch_bounds__(THREADS) void k_cat_backward(Logits l, Op op, const
     named_put<D, Op, THREADS>(named, g);
 }
 
+// ---- short rows ------------------------------------------------------------
+// Up to 1024 entries: many rows, so more of them lie next to the border of the
+// clip, and the memory they need is small beside the arithmetic of a row: the
+// sums are in f64 throughout.
+
+// From the state, or from a row's sums, to the state and the terms; what the
+// two kernels below share.  Every lane of the G that have the row calls it.
+__device__ __forceinline__ RowState ppo_row(const Ppo& op, const Out& o, int64_t n, int64_t rows, float m, double S,
+                                            double U, float xa, bool write, double* term) {
+    const double logs = log(S), lp = ((double)xa - (double)m) / op.t - logs;
+    const double h = logs - 0.6931471805599453 * (U / S);
+    const RowState st = op.finish(n, rows, m, logs, lp, h, term);
+    if (write) {
+        o.logprob[n] = (float)lp;
+        o.entropy[n] = (float)h;
+    }
+    return st;
+}
+
+// The sums of a block's rows, in a fixed order.
+template <int TERMS>
+__device__ __forceinline__ void block_terms(const double* term, double* ds, double* to) {
+#pragma unroll
+    for (int k = 0; k < TERMS; ++k) {
+        const double r = block_sum<256>(term[k], ds);
+        if (threadIdx.x == 0) to[(int64_t)blockIdx.x * TERMS + k] = r;
+    }
+}
+
+// G lanes per row, E entries each, in registers.  GIVEN: the backward pass,
+// from the state.
+template <class D, class Op, int G, int E, bool GIVEN>
+__global__ __launch_bounds__(256) void k_cat_short(Logits l, Op op, Out o, double* terms, const RowState* state,
+                                                   const float* gout) {
+    __shared__ double ds[4];
+    const int t = threadIdx.x % G;
+    const int64_t n = (int64_t)blockIdx.x * (256 / G) + threadIdx.x / G;
+    const bool in = n < l.rows;
+    const int32_t V = l.vocab;
+    const auto* x = row_of<D>(l, in ? n : 0);
+    double term[Op::terms] = {};
+    RowState st{0.0, INFINITY, 0.0, 0.0, 0.0};
+    bool skip = !in || (GIVEN ? false : op.ignored(n, V));
+    if (GIVEN && in) {
+        st = state[n];
+        skip = st.logs == INFINITY;
+    }
+    float v[E], m = -INFINITY;
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+        const int32_t i = t + G * e;
+        v[e] = !skip && i < V ? D::get(x[i]) : -INFINITY;
+        m = fmaxf(m, v[e]);
+    }
+    if constexpr (!GIVEN) {
+        const double c = 1.4426950408889634 / op.t;
+#pragma unroll
+        for (int d = G / 2; d; d >>= 1) m = fmaxf(m, __shfl_xor(m, d));
+        const float mf = m == -INFINITY ? 0.0f : m;
+        double S = 0.0, U = 0.0;
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+            const double z = ((double)v[e] - (double)mf) * c, p = exp2_64(z);
+            S += p;
+            if (Op::ppo) U = fma(p, z < -1100.0 ? -1100.0 : z, U);
+        }
+#pragma unroll
+        for (int d = G / 2; d; d >>= 1) {
+            S += __shfl_xor(S, d);
+            if (Op::ppo) U += __shfl_xor(U, d);
+        }
+        skip = skip || S == 0.0;
+        if constexpr (Op::ppo) {
+            if (!skip) {
+                st = ppo_row(op, o, n, l.rows, m, S, U, D::get(x[op.b.actions[n]]), t == 0, term);
+            } else if (in && t == 0) {
+                o.logprob[n] = o.entropy[n] = 0.0f;
+            }
+        } else {
+            double kl = 0.0, Q = 0.0, lse = 0.0;
+            const double logs = log(S), w = skip ? 0.0 : op.weight(n, l.rows);
+            const int64_t at = in ? n * op.b.k : 0;
+            if (op.b.lse) {
+                if (!skip) lse = op.b.lse[n];
+            } else {
+                float tm = -INFINITY;
+                for (int j = t; j < op.b.k; j += G) {
+                    const int64_t i = op.b.idx[at + j];
+                    if (i >= 0 && i < V) tm = fmaxf(tm, op.b.logits[at + j]);
+                }
+#pragma unroll
+                for (int d = G / 2; d; d >>= 1) tm = fmaxf(tm, __shfl_xor(tm, d));
+                if (tm == -INFINITY) tm = 0.0f;
+                for (int j = t; j < op.b.k; j += G) {
+                    const int64_t i = op.b.idx[at + j];
+                    if (i >= 0 && i < V) lse += exp2_64(((double)op.b.logits[at + j] - (double)tm) * c);
+                }
+#pragma unroll
+                for (int d = G / 2; d; d >>= 1) lse += __shfl_xor(lse, d);
+                lse = lse == 0.0 ? 0.0 : (double)tm / op.t + log(lse);
+            }
+            if (!skip) {
+                for (int j = t; j < op.b.k; j += G) {
+                    const int64_t i = op.b.idx[at + j];
+                    if (i < 0 || i >= V) continue;
+                    const double lq = (double)op.b.logits[at + j] / op.t - lse, q = exp(lq);
+                    if (q != 0.0) kl += q * (lq - (((double)D::get(x[i]) - (double)m) / op.t - logs));
+                    Q += q;
+                }
+            }
+#pragma unroll
+            for (int d = G / 2; d; d >>= 1) {
+                kl += __shfl_xor(kl, d);
+                Q += __shfl_xor(Q, d);
+            }
+            if (!skip) {
+                st = RowState{m, logs, lse, w * Q / op.t, w / op.t};
+                term[0] = w * kl;
+            }
+            if (in && t == 0) o.kl[n] = (float)kl;
+        }
+        if (in && t == 0 && o.state) *reinterpret_cast<RowState*>(o.state + n * RT_CAT_ROW_STATE) = st;
+        if (t) {
+#pragma unroll
+            for (int k = 0; k < Op::terms; ++k) term[k] = 0.0;
+        }
+        block_terms<Op::terms>(term, ds, terms);
+    }
+    if (!o.grad || !in) return;
+    auto* g = static_cast<typename D::raw*>(o.grad) + n * o.grad_stride;
+    const double scale = gout ? (double)*gout : 1.0;
+    float named[E] = {};
+    if constexpr (!Op::ppo) {
+        // the teacher's entries in turn, each met by the lane that has its place
+        const int64_t at = n * op.b.k;
+        for (int j0 = 0; j0 < op.b.k; j0 += G) {
+            int32_t idx = -1;
+            float q = 0.0f;
+            if (!skip && j0 + t < op.b.k) {
+                const int64_t i = op.b.idx[at + j0 + t];
+                if (i >= 0 && i < V) {
+                    idx = (int32_t)i;
+                    q = (float)exp((double)op.b.logits[at + j0 + t] / op.t - st.e);
+                }
+            }
+            const int many = min(G, op.b.k - j0);
+            for (int j = 0; j < many; ++j) {
+                const int32_t bi = __shfl(idx, j, G);
+                const float bq = __shfl(q, j, G);
+#pragma unroll
+                for (int e = 0; e < E; ++e) named[e] += bi == t + G * e ? bq : 0.0f;
+            }
+        }
+    } else if (!skip) {
+        const int64_t a = op.b.actions[n];
+#pragma unroll
+        for (int e = 0; e < E; ++e) named[e] = a == t + G * e ? 1.0f : 0.0f;
+    }
+    const Slope sl = op_slope(op, st, scale);
+    const float each = (float)(Op::ppo ? scale * st.c : -scale * st.c);
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+        const int32_t i = t + G * e;
+        if (i < V) g[i] = D::put(skip ? 0.0f : slope_at<Op::ppo>(sl, v[e]) + (named[e] != 0.0f ? each * named[e] : 0.0f));
+    }
+}
+
+// Up to 32 entries: one lane per row, so that the arithmetic of a row (log,
+// exp, divisions) is done once and not by every lane that has a part of it.
+// The block's rows pass through LDS (rows an odd number of words apart: no two
+// lanes on one bank), where the accesses to memory are those of one long row.
+constexpr int kTiny = 32;
+
+template <class D, class Op, bool GIVEN>
+__global__ __launch_bounds__(256) void k_cat_tiny(Logits l, Op op, Out o, double* terms, const RowState* state,
+                                                  const float* gout) {
+    __shared__ double ds[4];
+    __shared__ float tile[256 * (kTiny + 1)];
+    const int tid = threadIdx.x;
+    const int32_t V = l.vocab, pitch = V | 1;
+    const int64_t n0 = (int64_t)blockIdx.x * 256, n = n0 + tid;
+    const int32_t here = (int32_t)min((int64_t)256, l.rows - n0);
+    const float per = 1.0f / (float)V;  // (i + 1/2) / V is 1/64 or more away from a whole number
+    for (int32_t i = tid; i < here * V; i += 256) {
+        const int32_t r = (int32_t)(((float)i + 0.5f) * per), c = i - r * V;
+        tile[r * pitch + c] = D::get(row_of<D>(l, n0 + r)[c]);
+    }
+    __syncthreads();
+    const bool in = tid < here;
+    float* x = tile + tid * pitch;
+    double term[Op::terms] = {};
+    RowState st{0.0, INFINITY, 0.0, 0.0, 0.0};
+    bool skip = !in || (GIVEN ? false : op.ignored(n, V));
+    if (GIVEN && in) {
+        st = state[n];
+        skip = st.logs == INFINITY;
+    }
+    if constexpr (!GIVEN) {
+        if (!skip) {
+            const double c = 1.4426950408889634 / op.t;
+            float m = x[0];
+            for (int i = 1; i < V; ++i) m = fmaxf(m, x[i]);
+            const float mf = m == -INFINITY ? 0.0f : m;
+            double S = 0.0, U = 0.0;
+            for (int i = 0; i < V; ++i) {
+                const double z = ((double)x[i] - (double)mf) * c, p = exp2_64(z);
+                S += p;
+                if (Op::ppo) U = fma(p, z < -1100.0 ? -1100.0 : z, U);
+            }
+            skip = S == 0.0;
+            if (!skip) {
+                if constexpr (Op::ppo) {
+                    st = ppo_row(op, o, n, l.rows, m, S, U, x[op.b.actions[n]], true, term);
+                } else {
+                    const double logs = log(S), w = op.weight(n, l.rows);
+                    const int64_t at = n * op.b.k;
+                    double lse = 0.0, kl = 0.0, Q = 0.0;
+                    if (op.b.lse) {
+                        lse = op.b.lse[n];
+                    } else {
+                        float tm = -INFINITY;
+                        for (int j = 0; j < op.b.k; ++j) {
+                            const int64_t i = op.b.idx[at + j];
+                            if (i >= 0 && i < V) tm = fmaxf(tm, op.b.logits[at + j]);
+                        }
+                        if (tm == -INFINITY) tm = 0.0f;
+                        for (int j = 0; j < op.b.k; ++j) {
+                            const int64_t i = op.b.idx[at + j];
+                            if (i >= 0 && i < V) lse += exp2_64(((double)op.b.logits[at + j] - (double)tm) * c);
+                        }
+                        lse = lse == 0.0 ? 0.0 : (double)tm / op.t + log(lse);
+                    }
+                    for (int j = 0; j < op.b.k; ++j) {
+                        const int64_t i = op.b.idx[at + j];
+                        if (i < 0 || i >= V) continue;
+                        const double lq = (double)op.b.logits[at + j] / op.t - lse, q = exp(lq);
+                        if (q != 0.0) kl += q * (lq - (((double)x[i] - (double)m) / op.t - logs));
+                        Q += q;
+                    }
+                    st = RowState{m, logs, lse, w * Q / op.t, w / op.t};
+                    term[0] = w * kl;
+                    o.kl[n] = (float)kl;
+                }
+            }
+        }
+        if (in && skip) {
+            if constexpr (Op::ppo) o.logprob[n] = o.entropy[n] = 0.0f;
+            else o.kl[n] = 0.0f;
+        }
+        if (in && o.state) *reinterpret_cast<RowState*>(o.state + n * RT_CAT_ROW_STATE) = st;
+        block_terms<Op::terms>(term, ds, terms);
+    }
+    if (!o.grad) return;
+    if (in) {
+        const double scale = gout ? (double)*gout : 1.0;
+        const Slope sl = op_slope(op, st, scale);
+        const float each = (float)(scale * st.c);
+        for (int i = 0; i < V; ++i) x[i] = skip ? 0.0f : slope_at<Op::ppo>(sl, x[i]);
+        if (!skip) {
+            if constexpr (Op::ppo) {
+                const int64_t a = op.b.actions[n];
+                if (a >= 0 && a < V) x[a] += each;
+            } else {
+                const int64_t at = n * op.b.k;
+                for (int j = 0; j < op.b.k; ++j) {
+                    const int64_t i = op.b.idx[at + j];
+                    const float q = (float)exp((double)op.b.logits[at + j] / op.t - st.e);
+                    if (i >= 0 && i < V && q != 0.0f) x[i] -= each * q;
+                }
+            }
+        }
+    }
+    __syncthreads();
+    for (int32_t i = tid; i < here * V; i += 256) {
+        const int32_t r = (int32_t)(((float)i + 0.5f) * per), c = i - r * V;
+        static_cast<typename D::raw*>(o.grad)[(n0 + r) * o.grad_stride + c] = D::put(tile[r * pitch + c]);
+    }
+}
+
+constexpr int kShort = 1024;
+
+template <class Op>
+bool tiny(const Op& op, int32_t V) {
+    if constexpr (Op::ppo) return V <= kTiny;
+    else return V <= kTiny && op.b.k <= kTiny;
+}
+
+// Launches the kernel for short rows; how many blocks it had.
+template <class D, class Op, bool GIVEN>
+int64_t launch_short(const Logits& l, const Op& op, const Out& o, double* ws, const RowState* state, const float* gout,
+                     hipStream_t st) {
+    const auto go = [&](auto kernel, int per_block) {
+        const int64_t blocks = (l.rows + per_block - 1) / per_block;
+        hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(256), 0, st, l, op, o, ws, state, gout);
+        return blocks;
+    };
+    const int32_t V = l.vocab;
+    if (tiny(op, V)) return go(k_cat_tiny<D, Op, GIVEN>, 256);
+    if (V <= 64) return go(k_cat_short<D, Op, 16, 4, GIVEN>, 16);
+    if (V <= 128) return go(k_cat_short<D, Op, 16, 8, GIVEN>, 16);
+    if (V <= 256) return go(k_cat_short<D, Op, 64, 4, GIVEN>, 4);
+    if (V <= 512) return go(k_cat_short<D, Op, 64, 8, GIVEN>, 4);
+    return go(k_cat_short<D, Op, 64, 16, GIVEN>, 4);
+}
+
 // ---- sums over the rows ----------------------------------------------------
 // One block; every thread a fixed set of rows, then a fixed tree: the same
 // bits every time.
@@ -568,12 +873,14 @@ void launch_row(const Logits& l, const Op& op, const Out& o, double* ws, hipStre
 template <class D, class Op>
 int run_loss(const Logits& l, const Op& op, const Out& o, double* ws, hipStream_t st) {
     const int32_t pieces = l.vocab / Span<D>::kPer;
-    if (!o.grad) launch_row<D, Op, 256, 0>(l, op, o, ws, st);
+    int64_t parts = l.rows;
+    if (l.vocab <= kShort) parts = launch_short<D, Op, false>(l, op, o, ws, nullptr, nullptr, st);
+    else if (!o.grad) launch_row<D, Op, 256, 0>(l, op, o, ws, st);
     else if (pieces <= 256 * 4) launch_row<D, Op, 256, 4>(l, op, o, ws, st);
     else if (pieces <= 256 * 16) launch_row<D, Op, 256, 16>(l, op, o, ws, st);
     else if (pieces <= 512 * 16) launch_row<D, Op, 512, 16>(l, op, o, ws, st);
     else launch_row<D, Op, 1024, 16>(l, op, o, ws, st);
-    hipLaunchKernelGGL((k_cat_total<Op::terms>), dim3(1), dim3(1024), 0, st, ws, l.rows, o.loss, o.stats);
+    hipLaunchKernelGGL((k_cat_total<Op::terms>), dim3(1), dim3(1024), 0, st, ws, parts, o.loss, o.stats);
     return launched();
 }
 
@@ -587,6 +894,13 @@ int pick_loss(int dtype, const Logits& l, const Op& op, const Out& o, double* ws
 template <class D, class Op>
 int run_backward(const Logits& l, const Op& op, const double* state, const float* gout, void* grad, int64_t stride,
                  hipStream_t st) {
+    if (l.vocab <= kShort) {
+        Out o{};
+        o.grad = grad;
+        o.grad_stride = stride;
+        launch_short<D, Op, true>(l, op, o, nullptr, reinterpret_cast<const RowState*>(state), gout, st);
+        return launched();
+    }
     // 256 threads, eight pieces each
     const int64_t parts = std::max<int64_t>(1, std::min<int64_t>(l.vocab / (2048 * Span<D>::kPer), INT32_MAX / l.rows));
     hipLaunchKernelGGL((k_cat_backward<D, Op, 256>), dim3((unsigned)(l.rows * parts)), dim3(256), 0, st, l, op,

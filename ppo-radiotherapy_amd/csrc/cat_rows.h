@@ -34,6 +34,27 @@ struct F16 {
     static __device__ __forceinline__ raw put(float f) { return __builtin_bit_cast(raw, (_Float16)f); }
 };
 
+// ---- 2^t in 64 bits --------------------------------------------------------
+// t <= 0 or NaN.  t = n + f, |f| <= 1/2; the Taylor sum of exp(f ln 2) up to
+// f^11 leaves (ln 2 / 2)^12 / 12! < 7e-15.
+__device__ __forceinline__ double exp2_64(double t) {
+    t = t < -1100.0 ? -1100.0 : t;
+    const double n = rint(t), f = t - n;
+    double p = 4.44553827187081e-10;  // (ln 2)^11 / 11!, and so on down
+    p = fma(p, f, 7.054911620801121e-09);
+    p = fma(p, f, 1.0178086009239696e-07);
+    p = fma(p, f, 1.3215486790144305e-06);
+    p = fma(p, f, 1.5252733804059838e-05);
+    p = fma(p, f, 0.00015403530393381606);
+    p = fma(p, f, 0.0013333558146428441);
+    p = fma(p, f, 0.009618129107628477);
+    p = fma(p, f, 0.055504108664821576);
+    p = fma(p, f, 0.2402265069591007);
+    p = fma(p, f, 0.6931471805599453);
+    p = fma(p, f, 1.0);
+    return ldexp(p, (int)n);
+}
+
 // ---- reductions ------------------------------------------------------------
 template <class T>
 __device__ __forceinline__ T wave_sum(T v) {
