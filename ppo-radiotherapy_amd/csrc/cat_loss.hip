@@ -95,46 +95,6 @@ __device__ __forceinline__ const typename D::raw* row_of(const Logits& l, int64_
     return static_cast<const typename D::raw*>(l.x) + n * l.stride;
 }
 
-// A row as 16-byte pieces that are aligned wherever the row starts, and the
-// few entries before and after them ("edges", at most 2 (PER - 1) <= 14: one
-// per thread).
-template <class D>
-struct Span {
-    static constexpr int kPer = 16 / (int)sizeof(typename D::raw);
-    const typename D::raw* x;
-    int32_t head, pieces, edges;
-
-    __device__ Span(const typename D::raw* row, int32_t V) : x(row) {
-        head = min(V, (int32_t)((0 - (uintptr_t)row) % 16 / sizeof(typename D::raw)));
-        pieces = (V - head) / kPer;
-        edges = V - pieces * kPer;
-    }
-    __device__ __forceinline__ int32_t edge(int t) const { return t < head ? t : pieces * kPer + t; }
-    __device__ __forceinline__ uint4 piece(int32_t i) const {
-        return *reinterpret_cast<const uint4*>(x + head + (int64_t)i * kPer);
-    }
-};
-
-template <class D>
-struct Unpack {
-    static constexpr int kPer = 16 / (int)sizeof(typename D::raw);
-    float v[kPer];
-    __device__ __forceinline__ explicit Unpack(const uint4& r) {
-        const uint32_t w[4] = {r.x, r.y, r.z, r.w};
-#pragma unroll
-        for (int i = 0; i < kPer; ++i) {
-            if constexpr (kPer == 4) v[i] = __uint_as_float(w[i]);
-            else v[i] = D::get((typename D::raw)(i & 1 ? w[i / 2] >> 16 : w[i / 2] & 0xffff));
-        }
-    }
-    __device__ __forceinline__ float max() const {
-        float m = v[0];
-#pragma unroll
-        for (int i = 1; i < kPer; ++i) m = fmaxf(m, v[i]);
-        return m;
-    }
-};
-
 template <class D>
 __device__ __forceinline__ uint4 pack(const float* v) {
     uint32_t w[4];

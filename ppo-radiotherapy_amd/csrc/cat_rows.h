@@ -55,6 +55,28 @@ __device__ __forceinline__ double exp2_64(double t) {
     return ldexp(p, (int)n);
 }
 
+// Weights of a sampled row: 2^40 2^t as a whole number, t <= 0 (half to even,
+// by the rounding of the sum with 2^52, whose bits then hold it).
+constexpr double kUnit = 1099511627776.0;  // 2^40
+constexpr uint64_t kMagic = 0x4330000000000000ull;  // 2^52
+__device__ __forceinline__ uint64_t whole_bits(double t) {  // kMagic + the weight
+    t = fmax(t, -1100.0);
+    const double n = rint(t), f = t - n;
+    double p = 4.44553827187081e-10;
+    p = fma(p, f, 7.054911620801121e-09);
+    p = fma(p, f, 1.0178086009239696e-07);
+    p = fma(p, f, 1.3215486790144305e-06);
+    p = fma(p, f, 1.5252733804059838e-05);
+    p = fma(p, f, 0.00015403530393381606);
+    p = fma(p, f, 0.0013333558146428441);
+    p = fma(p, f, 0.009618129107628477);
+    p = fma(p, f, 0.055504108664821576);
+    p = fma(p, f, 0.2402265069591007);
+    p = fma(p, f, 0.6931471805599453);
+    p = fma(p, f, 1.0);
+    return __builtin_bit_cast(uint64_t, ldexp(p, (int)n + 40) + 4503599627370496.0);
+}
+
 // ---- reductions ------------------------------------------------------------
 template <class T>
 __device__ __forceinline__ T wave_sum(T v) {
@@ -94,6 +116,47 @@ __device__ __forceinline__ float block_max(float v, float* slots) {
     __syncthreads();
     return r;
 }
+
+// ---- rows as 16-byte pieces ------------------------------------------------
+// A row as 16-byte pieces that are aligned wherever the row starts, and the
+// few entries before and after them ("edges", at most 2 (PER - 1) <= 14: one
+// per thread).
+template <class D>
+struct Span {
+    static constexpr int kPer = 16 / (int)sizeof(typename D::raw);
+    const typename D::raw* x;
+    int32_t head, pieces, edges;
+
+    __device__ Span(const typename D::raw* row, int32_t V) : x(row) {
+        head = min(V, (int32_t)((0 - (uintptr_t)row) % 16 / sizeof(typename D::raw)));
+        pieces = (V - head) / kPer;
+        edges = V - pieces * kPer;
+    }
+    __device__ __forceinline__ int32_t edge(int t) const { return t < head ? t : pieces * kPer + t; }
+    __device__ __forceinline__ uint4 piece(int32_t i) const {
+        return *reinterpret_cast<const uint4*>(x + head + (int64_t)i * kPer);
+    }
+};
+
+template <class D>
+struct Unpack {
+    static constexpr int kPer = 16 / (int)sizeof(typename D::raw);
+    float v[kPer];
+    __device__ __forceinline__ explicit Unpack(const uint4& r) {
+        const uint32_t w[4] = {r.x, r.y, r.z, r.w};
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) {
+            if constexpr (kPer == 4) v[i] = __uint_as_float(w[i]);
+            else v[i] = D::get((typename D::raw)(i & 1 ? w[i / 2] >> 16 : w[i / 2] & 0xffff));
+        }
+    }
+    __device__ __forceinline__ float max() const {
+        float m = v[0];
+#pragma unroll
+        for (int i = 1; i < kPer; ++i) m = fmaxf(m, v[i]);
+        return m;
+    }
+};
 
 // ---- argument checks -------------------------------------------------------
 inline int elem_size(int32_t dtype) { return dtype == RT_DT_F32 ? 4 : 2; }

@@ -20,8 +20,8 @@ namespace {
 
 using namespace rtcat;
 
-constexpr double kUnit = 1099511627776.0;  // 2^40
-constexpr int kBins = 2048;                // of one digit: 11 bits
+constexpr int kBins = 2048;  // of a histogram; 11 bits of a key
+constexpr int kList = 2048;  // entries that a block can sort
 
 struct Args {
     const void* x;
@@ -42,30 +42,31 @@ __device__ __forceinline__ float of_key(uint32_t k) {
 }
 
 struct Weigher {
-    double m, inv_t;
-    __device__ __forceinline__ uint64_t operator()(float x) const {
-        return x == -INFINITY ? 0 : (uint64_t)rint(exp(((double)x - m) * inv_t) * kUnit);
-    }
+    double m, c;  // c = log2(e) / T
+    __device__ __forceinline__ uint64_t operator()(float x) const { return whole_bits(((double)x - m) * c) - kMagic; }
 };
 
 template <int THREADS>
 struct Shared {
-    uint64_t hist[kBins];
+    uint64_t hist[kBins];  // also the list's second half of a sort by index
+    uint64_t list[kList];
     uint64_t slots[THREADS / 64];
     float fslots[THREADS / 64];
     uint64_t found[2];
-    int32_t where;
+    int32_t where, many;
 };
 
-// The bin, from the highest down, in which a running sum reaches `want`
-// (want >= 1 and <= the sum of all bins): the bin, and the sum above it.
-template <int THREADS>
+// The bin in which a running sum, from the highest bin down or (UP) from the
+// lowest up, reaches `want` (want >= 1 and <= the sum of all bins): the bin,
+// and the sum before it.
+template <int THREADS, bool UP = false>
 __device__ int find_bin(Shared<THREADS>& s, uint64_t want, uint64_t* above) {
+    const auto place = [](int i) { return UP ? i : kBins - 1 - i; };
     constexpr int kPer = kBins / THREADS;
     const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
-    uint64_t mine = 0;  // thread 0 has the highest bins
+    uint64_t mine = 0;
 #pragma unroll
-    for (int i = 0; i < kPer; ++i) mine += s.hist[kBins - 1 - (tid * kPer + i)];
+    for (int i = 0; i < kPer; ++i) mine += s.hist[place(tid * kPer + i)];
     uint64_t run = mine;
 #pragma unroll
     for (int o = 1; o < 64; o <<= 1) {
@@ -78,7 +79,7 @@ __device__ int find_bin(Shared<THREADS>& s, uint64_t want, uint64_t* above) {
     for (int i = 0; i < w; ++i) before += s.slots[i];
     if (before < want && want <= before + mine) {
         for (int i = 0; i < kPer; ++i) {
-            const int b = kBins - 1 - (tid * kPer + i);
+            const int b = place(tid * kPer + i);
             const uint64_t h = s.hist[b];
             if (want <= before + h) {
                 s.where = b;
@@ -129,10 +130,9 @@ __device__ uint32_t find_key(Shared<THREADS>& s, int32_t V, Get get, Weight weig
 // `target` (target < the sum of all): the block halves its way down, each wave
 // summing a part of the segment that holds it.
 template <int THREADS, class Weight>
-__device__ int32_t find_index(Shared<THREADS>& s, int32_t V, Weight weight, uint64_t target) {
+__device__ int32_t find_index(Shared<THREADS>& s, int32_t lo, int32_t len, Weight weight, uint64_t target) {
     constexpr int kWaves = THREADS / 64;
     const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-    int32_t lo = 0, len = V;
     while (len > 64) {
         const int32_t part = (len + kWaves - 1) / kWaves;
         const int32_t a = min(lo + w * part, lo + len), b = min(a + part, lo + len);
@@ -164,45 +164,46 @@ __device__ int32_t find_index(Shared<THREADS>& s, int32_t V, Weight weight, uint
     return lo + (over ? __ffsll((long long)over) - 1 : len - 1);
 }
 
+// What a row is asked for.
+struct Ask {
+    float T, P, Q, u;
+    int32_t K;
+    __device__ Ask(const rt_cat_sampling& p, int64_t n, int32_t V)
+        : T(p.temperature ? p.temperature[n] : p.temperature_all), P(p.top_p ? p.top_p[n] : p.top_p_all),
+          Q(p.min_p ? p.min_p[n] : p.min_p_all), u(p.u[n]), K(p.top_k ? p.top_k[n] : p.top_k_all) {
+        if (K >= V) K = 0;
+    }
+    __device__ double least() const {  // of x - m
+        return Q >= 1.0f ? 0.0 : Q > 0.0f ? (double)T * log((double)Q) : -INFINITY;
+    }
+    __device__ uint64_t limit(uint64_t mass) const {  // of the weight before the last that top-p keeps
+        const double part = ceil((double)P * (double)mass);
+        return part >= 1.0 ? (uint64_t)part : 1;
+    }
+    __device__ uint64_t target(uint64_t left) const {
+        const double hit = floor((u > 0.0f ? (double)u : 0.0) * (double)left);
+        const uint64_t t = hit < (double)left ? (uint64_t)hit : left - 1;
+        return t < left ? t : left - 1;
+    }
+};
+
+__device__ __forceinline__ void answer(const Args& A, int64_t n, int32_t a, double z, uint64_t all, uint64_t left) {
+    A.action[n] = a;
+    A.logprob[n] = (float)(z - log((double)all / kUnit));
+    A.kept[n] = (float)(z - log((double)left / kUnit));
+}
+
+// ---- any row, slowly -------------------------------------------------------
+// Digit by digit over the whole row: for rows whose cut falls among more
+// entries than a list holds (many equal logits, a very large k) and for
+// temperatures past the histogram's range.
 template <class D, int THREADS>
-__global__ __launch_bounds__(THREADS) void k_cat_sample(Args A) {
-    __shared__ Shared<THREADS> s;
+__device__ void slow_row(const Args& A, int64_t n, const Ask& ask, float m, Shared<THREADS>& s) {
     constexpr bool kShort = sizeof(typename D::raw) == 2;
-    const int64_t n = blockIdx.x;
     const int32_t V = A.vocab;
     const auto* row = static_cast<const typename D::raw*>(A.x) + n * A.stride;
     const auto get = [&](int32_t i) { return D::get(row[i]); };
-    const float T = A.p.temperature ? A.p.temperature[n] : A.p.temperature_all;
-    const int32_t K = A.p.top_k ? A.p.top_k[n] : A.p.top_k_all;
-    const float P = A.p.top_p ? A.p.top_p[n] : A.p.top_p_all;
-    const float Q = A.p.min_p ? A.p.min_p[n] : A.p.min_p_all;
-
-    float m = -INFINITY;
-    uint32_t odd = 0;
-    for (int i = threadIdx.x; i < V; i += THREADS) {
-        const float v = get(i);
-        m = fmaxf(m, v);
-        odd |= v != v || v == INFINITY;
-    }
-    m = block_max<THREADS>(m, s.fslots);
-    odd = (uint32_t)__syncthreads_or((int)odd);
-    if (odd || m == -INFINITY) {
-        if (threadIdx.x == 0) {
-            A.action[n] = -1;
-            A.logprob[n] = A.kept[n] = NAN;
-        }
-        return;
-    }
-    if (!(T > 0.0f)) {
-        const uint32_t top = key_of(m);
-        const int32_t a = find_index<THREADS>(s, V, [&](int32_t i) { return (uint64_t)(key_of(get(i)) == top); }, 0);
-        if (threadIdx.x == 0) {
-            A.action[n] = a;
-            A.logprob[n] = A.kept[n] = 0.0f;
-        }
-        return;
-    }
-    const Weigher weigh{(double)m, 1.0 / (double)T};
+    const Weigher weigh{(double)m, fmax(1.4426950408889634 / (double)ask.T, 1e-300)};
     uint64_t all = 0;
     for (int i = threadIdx.x; i < V; i += THREADS) all += weigh(get(i));
     all = block_sum<THREADS>(all, s.slots);
@@ -210,20 +211,19 @@ __global__ __launch_bounds__(THREADS) void k_cat_sample(Args A) {
     // the least key that is kept, and how many of the entries equal to it
     uint32_t cut = 0;
     uint64_t ties = UINT64_MAX, mass = all;
-    if (K > 0 && K < V) {
+    if (ask.K > 0) {
         uint64_t above;
-        cut = find_key<THREADS, kShort>(s, V, get, [](float, uint32_t) { return (uint64_t)1; }, (uint64_t)K, &above);
-        ties = (uint64_t)K - above;
+        cut = find_key<THREADS, kShort>(s, V, get, [](float, uint32_t) { return (uint64_t)1; }, (uint64_t)ask.K, &above);
+        ties = (uint64_t)ask.K - above;
         mass = 0;
-        if (P < 1.0f) {
+        if (ask.P < 1.0f) {
             for (int i = threadIdx.x; i < V; i += THREADS)
                 if (key_of(get(i)) > cut) mass += weigh(get(i));
             mass = block_sum<THREADS>(mass, s.slots) + ties * weigh(of_key(cut));
         }
     }
-    if (P < 1.0f) {
-        const double part = ceil((double)P * (double)mass);
-        const uint64_t want = part >= 1.0 ? (uint64_t)part : 1;
+    if (ask.P < 1.0f) {
+        const uint64_t want = ask.limit(mass);
         const uint32_t from = cut;
         uint64_t above;
         const uint32_t k = find_key<THREADS, kShort>(
@@ -233,7 +233,7 @@ __global__ __launch_bounds__(THREADS) void k_cat_sample(Args A) {
         if (k > cut || need < ties) ties = need;
         cut = k;
     }
-    const double theta = Q >= 1.0f ? 0.0 : Q > 0.0f ? (double)T * log((double)Q) : -INFINITY;
+    const double theta = ask.least();
     // entries equal to the cut: the last index that is kept
     int32_t last = V;
     if (ties != UINT64_MAX) {
@@ -241,7 +241,7 @@ __global__ __launch_bounds__(THREADS) void k_cat_sample(Args A) {
         for (int i = threadIdx.x; i < V; i += THREADS) equal += key_of(get(i)) == cut;
         equal = block_sum<THREADS>(equal, s.slots);
         if (ties < equal)
-            last = find_index<THREADS>(s, V, [&](int32_t i) { return (uint64_t)(key_of(get(i)) == cut); }, ties - 1);
+            last = find_index<THREADS>(s, 0, V, [&](int32_t i) { return (uint64_t)(key_of(get(i)) == cut); }, ties - 1);
     }
     const auto kept = [&](int32_t i) -> uint64_t {
         const float x = get(i);
@@ -252,21 +252,365 @@ __global__ __launch_bounds__(THREADS) void k_cat_sample(Args A) {
     uint64_t left = 0;
     for (int i = threadIdx.x; i < V; i += THREADS) left += kept(i);
     left = block_sum<THREADS>(left, s.slots);
-    const float u = A.p.u[n];
-    const double hit = floor((u > 0.0f ? (double)u : 0.0) * (double)left);
-    const uint64_t target = hit < (double)left ? (uint64_t)hit : left - 1;
-    const int32_t a = find_index<THREADS>(s, V, kept, target < left ? target : left - 1);
-    if (threadIdx.x == 0) {
-        const double z = ((double)get(a) - (double)m) / (double)T;
-        A.action[n] = a;
-        A.logprob[n] = (float)(z - log((double)all / kUnit));
-        A.kept[n] = (float)(z - log((double)left / kUnit));
+    const int32_t a = find_index<THREADS>(s, 0, V, kept, ask.target(left));
+    if (threadIdx.x == 0) answer(A, n, a, ((double)get(a) - (double)m) / (double)ask.T, all, left);
+}
+
+// ---- one block per row -----------------------------------------------------
+// An entry's place in the order, larger first: key, then index from below.
+__device__ __forceinline__ uint64_t rank_of(float x, int32_t i) { return (uint64_t)key_of(x) << 32 | (uint32_t)~i; }
+
+// Sorts list[0, n), n <= kList, largest first; what lies behind it is filled
+// with 0.  Returns after a barrier.
+template <int THREADS>
+__device__ void sort_list(uint64_t* list, int n) {
+    int size = 2;
+    while (size < n) size <<= 1;
+    for (int i = n + threadIdx.x; i < size; i += THREADS) list[i] = 0;
+    __syncthreads();
+    for (int k = 2; k <= size; k <<= 1) {
+        for (int j = k >> 1; j; j >>= 1) {
+            for (int p = threadIdx.x; p < size / 2; p += THREADS) {
+                const int i = 2 * p - (p & (j - 1)), o = i + j;
+                const uint64_t a = list[i], b = list[o];
+                if ((a < b) == ((i & k) == 0)) {
+                    list[i] = b;
+                    list[o] = a;
+                }
+            }
+            __syncthreads();
+        }
     }
+}
+
+// Where the running sum of value(i), i < n <= kList, first exceeds `target`,
+// n if it never does; and the sum before that place.
+template <int THREADS, class Value>
+__device__ int scan_to(Shared<THREADS>& s, int n, Value value, uint64_t target, uint64_t* before) {
+    constexpr int kPer = kList / THREADS;
+    const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
+    uint64_t v[kPer], mine = 0;
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+        v[i] = tid * kPer + i < n ? value(tid * kPer + i) : 0;
+        mine += v[i];
+    }
+    uint64_t run = mine;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+        const uint64_t q = __shfl_up(run, o);
+        if (lane >= o) run += q;
+    }
+    if (lane == 63) s.slots[w] = run;
+    if (tid == 0) s.where = n;
+    __syncthreads();
+    uint64_t at = run - mine, total = 0;
+    for (int i = 0; i < THREADS / 64; ++i) {
+        if (i < w) at += s.slots[i];
+        total += s.slots[i];
+    }
+    if (tid == 0) s.found[0] = total;
+    __syncthreads();
+    if (at <= target && target < at + mine) {
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) {
+            if (at <= target && target < at + v[i]) {
+                s.where = tid * kPer + i;
+                s.found[0] = at;
+            }
+            at += v[i];
+        }
+    }
+    __syncthreads();
+    const int r = s.where;
+    *before = s.found[0];
+    __syncthreads();
+    return r;
+}
+
+// A wave's part of a row, in the order of the index: whole pieces, the first
+// wave also what lies before them, the last what lies behind.
+template <class D>
+struct Part {
+    int32_t from, to, first, last;  // pieces; entries
+    __device__ Part(const Span<D>& row, int32_t V, int w, int waves) {
+        const int32_t per = (row.pieces + waves - 1) / waves;
+        from = min(w * per, row.pieces);
+        to = min(from + per, row.pieces);
+        first = w == 0 ? 0 : row.head + from * Span<D>::kPer;
+        last = w == waves - 1 ? V : row.head + to * Span<D>::kPer;
+    }
+};
+
+// f(x, i) for every entry of a part; the lanes of one wave together.
+template <class D, class F>
+__device__ __forceinline__ void walk(const Span<D>& row, const Part<D>& p, F f) {
+    const int lane = threadIdx.x & 63;
+    constexpr int kPer = Span<D>::kPer, kBatch = 4;
+    const int32_t a = row.head + p.from * kPer, b = row.head + p.to * kPer;
+    if (p.first + lane < a) f(D::get(row.x[p.first + lane]), p.first + lane);
+    if (b + lane < p.last) f(D::get(row.x[b + lane]), b + lane);
+    for (int32_t i = p.from + lane; i < p.to; i += 64 * kBatch) {
+        uint4 r[kBatch];
+#pragma unroll
+        for (int k = 0; k < kBatch; ++k)
+            if (i + 64 * k < p.to) r[k] = row.piece(i + 64 * k);
+#pragma unroll
+        for (int k = 0; k < kBatch; ++k) {
+            if (i + 64 * k >= p.to) break;
+            const Unpack<D> x(r[k]);
+#pragma unroll
+            for (int j = 0; j < kPer; ++j) f(x.v[j], row.head + (i + 64 * k) * kPer + j);
+        }
+    }
+}
+
+// Bins of falling logits, by t = (m - x) / (T ln 2): the last holds what weighs
+// nothing (2^(40 - 41.5) < 1/2).  Each step of the arithmetic keeps the order,
+// so a bin's entries come before those of the next.
+struct Binner {
+    float m, scale;
+    __device__ __forceinline__ int operator()(float x) const { return (int)fminf((m - x) * scale, (float)(kBins - 1)); }
+};
+
+template <class D, int THREADS>
+__global__ __launch_bounds__(THREADS) void k_cat_sample(Args A) {
+    __shared__ Shared<THREADS> s;
+    constexpr int kWaves = THREADS / 64;
+    const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
+    const int64_t n = blockIdx.x;
+    const int32_t V = A.vocab;
+    const Span<D> row(static_cast<const typename D::raw*>(A.x) + n * A.stride, V);
+    const Part<D> part(row, V, w, kWaves);
+    const auto get = [&](int32_t i) { return D::get(row.x[i]); };
+    const Ask ask(A.p, n, V);
+
+    float m = -INFINITY;
+    int odd = 0;
+    walk(row, part, [&](float x, int32_t) {
+        m = fmaxf(m, x);
+        odd |= !(x < INFINITY);
+    });
+    m = block_max<THREADS>(m, s.fslots);
+    odd = __syncthreads_or(odd);
+    if (odd || m == -INFINITY) {
+        if (tid == 0) {
+            A.action[n] = -1;
+            A.logprob[n] = A.kept[n] = NAN;
+        }
+        return;
+    }
+    if (!(ask.T > 0.0f)) {
+        const uint32_t top = key_of(m);
+        const int32_t a = find_index<THREADS>(s, 0, V, [&](int32_t i) { return (uint64_t)(key_of(get(i)) == top); }, 0);
+        if (tid == 0) {
+            A.action[n] = a;
+            A.logprob[n] = A.kept[n] = 0.0f;
+        }
+        return;
+    }
+    const bool some = ask.K > 0 || ask.P < 1.0f;
+    if (some && ask.T > 1e30f) return slow_row<D, THREADS>(A, n, ask, m, s);
+
+    const double c = fmax(1.4426950408889634 / (double)ask.T, 1e-300), theta = ask.least();
+    const Weigher weigh{(double)m, c};
+    const Binner bin{m, (float)fmin(fmax(c * (kBins - 1) / 41.5, 1e-30), 3e38)};
+    // the weight of all, and what is needed to find the cut: how many entries, or how much weight, each bin has
+    uint64_t sum = 0;
+    if (some) {
+        for (int i = tid; i < kBins; i += THREADS) s.hist[i] = 0;
+        __syncthreads();
+        const bool count = ask.K > 0;
+        walk(row, part, [&](float x, int32_t) {
+            const uint64_t v = weigh(x), add = count ? 1 : v;
+            sum += v;
+            if (v) atomicAdd(reinterpret_cast<unsigned long long*>(&s.hist[bin(x)]), (unsigned long long)add);
+        });
+    } else {
+        walk(row, part, [&](float x, int32_t) { sum += weigh(x); });
+    }
+    sum = wave_sum(sum);
+    if (lane == 0) s.slots[w] = sum;
+    __syncthreads();
+    uint64_t all = 0;
+    for (int i = 0; i < kWaves; ++i) all += s.slots[i];
+    __syncthreads();
+
+    // Entries that weigh nothing are not in the histogram: they stand behind all others, and keeping them
+    // or not changes nothing.
+    uint64_t cut = 0;  // least rank that is kept
+    bool done = !some;
+    if (ask.K > 0) {
+        uint64_t total = 0;
+        for (int i = tid; i < kBins; i += THREADS) total += s.hist[i];
+        total = block_sum<THREADS>(total, s.slots);
+        const uint64_t want = min((uint64_t)ask.K, total);
+        uint64_t before;
+        const int b = find_bin<THREADS, true>(s, want, &before);
+        const uint64_t many = before + s.hist[b];
+        if (many > kList) return slow_row<D, THREADS>(A, n, ask, m, s);
+        // the first `many` of the order, sorted: all that is left is in the list
+        if (tid == 0) s.many = 0;
+        __syncthreads();
+        walk(row, part, [&](float x, int32_t i) {
+            if (bin(x) <= b && weigh(x)) {
+                const int at = atomicAdd(&s.many, 1);
+                if (at < kList) s.list[at] = rank_of(x, i);  // always: there are `many`
+            }
+        });
+        __syncthreads();
+        sort_list<THREADS>(s.list, (int)many);
+        const auto value = [&](int i) { return weigh(of_key((uint32_t)(s.list[i] >> 32))); };
+        int keep = (int)want;
+        uint64_t left, skipped;
+        scan_to<THREADS>(s, keep, value, UINT64_MAX, &left);
+        if (ask.P < 1.0f) {
+            // kept: those before which less than the limit lies
+            const int at = scan_to<THREADS>(s, keep, value, ask.limit(left) - 1, &skipped);
+            keep = min(keep, at + 1);
+        }
+        cut = s.list[keep - 1];
+        done = false;
+    } else if (ask.P < 1.0f) {
+        const uint64_t want = ask.limit(all);
+        uint64_t before, skipped;
+        const int b = find_bin<THREADS, true>(s, want, &before);
+        if (tid == 0) s.many = 0;
+        __syncthreads();
+        walk(row, part, [&](float x, int32_t i) {
+            if (bin(x) == b && weigh(x)) {
+                const int at = atomicAdd(&s.many, 1);
+                if (at < kList) s.list[at] = rank_of(x, i);
+            }
+        });
+        __syncthreads();
+        const int held = s.many;
+        if (held > kList) return slow_row<D, THREADS>(A, n, ask, m, s);
+        sort_list<THREADS>(s.list, held);
+        const int at = scan_to<THREADS>(
+            s, held, [&](int i) { return weigh(of_key((uint32_t)(s.list[i] >> 32))); }, want - before - 1, &skipped);
+        cut = s.list[min(at, held - 1)];
+        done = false;
+    }
+    __syncthreads();
+    const auto kept = [&](float x, int32_t i) -> uint64_t {
+        if (rank_of(x, i) < cut || (double)x - (double)m < theta) return 0;
+        return weigh(x);
+    };
+    // the weight of what is kept, by waves: the first step of the search
+    if (!done || ask.Q > 0.0f) {
+        sum = 0;
+        walk(row, part, [&](float x, int32_t i) { sum += kept(x, i); });
+        sum = wave_sum(sum);
+    }
+    if (lane == 0) s.slots[w] = sum;
+    __syncthreads();
+    uint64_t left = 0;
+    for (int i = 0; i < kWaves; ++i) left += s.slots[i];
+    uint64_t target = ask.target(left);
+    int at = 0;
+    for (; at < kWaves - 1 && target >= s.slots[at]; ++at) target -= s.slots[at];
+    __syncthreads();
+    const Part<D> seg(row, V, at, kWaves);
+    const int32_t a = find_index<THREADS>(s, seg.first, seg.last - seg.first,
+                                          [&](int32_t i) { return kept(get(i), i); }, target);
+    if (tid == 0) answer(A, n, a, ((double)get(a) - (double)m) / (double)ask.T, all, left);
+}
+
+// ---- short rows ------------------------------------------------------------
+// Up to 32 entries: one lane per row, the block's rows in LDS (an odd number of
+// words apart: no two lanes on one bank).  The order is not sorted: an entry's
+// place in it is how many stand before it, and what is kept is a 32-bit mask.
+constexpr int kTiny = 32;
+
+template <class D>
+__global__ __launch_bounds__(64) void k_cat_sample_tiny(Args A, int64_t rows) {
+    __shared__ float tile[64 * (kTiny + 1)];
+    __shared__ uint64_t weight[64 * (kTiny + 1)];
+    const int tid = threadIdx.x;
+    const int32_t V = A.vocab, pitch = V | 1;
+    const int64_t n0 = (int64_t)blockIdx.x * 64, n = n0 + tid;
+    const int32_t here = (int32_t)min((int64_t)64, rows - n0);
+    const float per = 1.0f / (float)V;  // (i + 1/2) / V is 1/64 or more away from a whole number
+    for (int32_t i = tid; i < here * V; i += 64) {
+        const int32_t r = (int32_t)(((float)i + 0.5f) * per), c = i - r * V;
+        tile[r * pitch + c] = D::get(static_cast<const typename D::raw*>(A.x)[(n0 + r) * A.stride + c]);
+    }
+    __syncthreads();
+    if (tid >= here) return;
+    const float* x = tile + tid * pitch;
+    uint64_t* wt = weight + tid * pitch;
+    const Ask ask(A.p, n, V);
+    float m = x[0];
+    int32_t first = 0;
+    bool odd = !(x[0] < INFINITY);
+    for (int i = 1; i < V; ++i) {
+        odd |= !(x[i] < INFINITY);
+        if (x[i] > m) {
+            m = x[i];
+            first = i;
+        }
+    }
+    if (odd || m == -INFINITY) {
+        A.action[n] = -1;
+        A.logprob[n] = A.kept[n] = NAN;
+        return;
+    }
+    if (!(ask.T > 0.0f)) {
+        A.action[n] = first;
+        A.logprob[n] = A.kept[n] = 0.0f;
+        return;
+    }
+    const Weigher weigh{(double)m, fmax(1.4426950408889634 / (double)ask.T, 1e-300)};
+    uint64_t all = 0;
+    for (int i = 0; i < V; ++i) {
+        wt[i] = weigh(x[i]);
+        all += wt[i];
+    }
+    uint32_t keep = 0xffffffffu >> (32 - V);
+    uint64_t mass = all;
+    if (ask.K > 0) {
+        mass = 0;
+        for (int i = 0; i < V; ++i) {
+            int ahead = 0;
+            for (int j = 0; j < V; ++j) ahead += x[j] > x[i] || (x[j] == x[i] && j < i);
+            if (ahead >= ask.K) keep &= ~(1u << i);
+            else mass += wt[i];
+        }
+    }
+    if (ask.P < 1.0f) {
+        const uint64_t limit = ask.limit(mass);
+        for (int i = 0; i < V; ++i) {
+            uint64_t before = 0;
+            for (int j = 0; j < V; ++j) before += x[j] > x[i] || (x[j] == x[i] && j < i) ? wt[j] : 0;
+            if (before >= limit) keep &= ~(1u << i);
+        }
+    }
+    const double theta = ask.least();
+    uint64_t left = 0;
+    for (int i = 0; i < V; ++i) {
+        if ((double)x[i] - (double)m < theta) keep &= ~(1u << i);
+        if (keep >> i & 1) left += wt[i];
+    }
+    const uint64_t target = ask.target(left);
+    uint64_t run = 0;
+    int32_t a = 0;
+    for (int i = V - 1; i >= 0; --i) {  // from the end: the last that passes is the first that exceeds
+        if (!(keep >> i & 1)) continue;
+        run += wt[i];
+        if (left - run <= target) {
+            a = i;
+            break;
+        }
+    }
+    answer(A, n, a, ((double)x[a] - (double)m) / (double)ask.T, all, left);
 }
 
 template <class D>
 int run_sample(const Args& a, int64_t rows, hipStream_t st) {
-    if (a.vocab > 4096)
+    if (a.vocab <= kTiny)
+        hipLaunchKernelGGL(k_cat_sample_tiny<D>, dim3((unsigned)((rows + 63) / 64)), dim3(64), 0, st, a, rows);
+    else if (a.vocab > 4096)
         hipLaunchKernelGGL((k_cat_sample<D, 1024>), dim3((unsigned)rows), dim3(1024), 0, st, a);
     else
         hipLaunchKernelGGL((k_cat_sample<D, 256>), dim3((unsigned)rows), dim3(256), 0, st, a);
