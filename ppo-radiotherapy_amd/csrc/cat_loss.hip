@@ -39,10 +39,11 @@ struct Logits {
 // ---- the two losses --------------------------------------------------------
 struct Ppo {
     rt_cat_ppo_batch b;
-    double t, low, high, ent, klc;
+    double t, inv, low, high, ent, klc;  // inv = 1 / t
     static constexpr int terms = 7;
     static constexpr bool ppo = true;
 
+    __device__ int32_t k() const { return 0; }
     __device__ bool ignored(int64_t n, int32_t V) const {
         const int64_t a = b.actions[n];
         return a < 0 || a >= V || (b.weights && b.weights[n] == 0.0f);
@@ -50,14 +51,14 @@ struct Ppo {
     // From the row's log-probability of its action and its entropy: the state, and the weighted terms.
     __device__ RowState finish(int64_t n, int64_t rows, double m, double logs, double lp, double h, double* term) const {
         const double w = b.weights ? (double)b.weights[n] : 1.0 / (double)rows;
-        const double A = b.advantages[n], lr = lp - (double)b.old_logprobs[n], r = exp(lr);
+        const double A = b.advantages[n], lr = lp - (double)b.old_logprobs[n], r = exp_64(lr);
         const double lo = 1.0 - low, hi = 1.0 + high;
         const double rc = r < lo ? lo : r > hi ? hi : r;
         const double one = -A * r, two = -A * rc;
         const double pg = one >= two ? one : two > one ? two : one + two;  // the larger, NaN if one is
         double c = one >= two ? one : two > one ? 0.0 : pg, kl = 0.0;
         if (b.ref_logprobs) {
-            const double away = (double)b.ref_logprobs[n] - lp, q = exp(away);
+            const double away = (double)b.ref_logprobs[n] - lp, q = exp_64(away);
             kl = q - away - 1.0;
             if (klc != 0.0) c += klc * (1.0 - q);
         }
@@ -71,8 +72,8 @@ struct Ppo {
         RowState s;
         s.m = m;
         s.logs = logs;
-        s.c = w * c / t;
-        s.e = w * ent / t;
+        s.c = w * c * inv;
+        s.e = w * ent * inv;
         s.f = s.e * h - s.c;
         return s;
     }
@@ -80,11 +81,12 @@ struct Ppo {
 
 struct Distill {
     rt_cat_teacher b;
-    double t;
+    double t, inv;  // inv = 1 / t
     static constexpr int terms = 1;
     static constexpr bool ppo = false;
 
     __device__ bool ignored(int64_t n, int32_t) const { return b.weights && b.weights[n] == 0.0f; }
+    __device__ int32_t k() const { return b.k; }
     __device__ double weight(int64_t n, int64_t rows) const {
         return b.weights ? (double)b.weights[n] : 1.0 / (double)rows;
     }
@@ -101,7 +103,7 @@ __device__ __forceinline__ uint4 pack(const float* v) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
         if constexpr (sizeof(typename D::raw) == 4) w[i] = __float_as_uint(v[i]);
-        else w[i] = (uint32_t)D::put(v[2 * i]) | (uint32_t)D::put(v[2 * i + 1]) << 16;
+        else w[i] = D::put2(v[2 * i], v[2 * i + 1]);
     }
     return make_uint4(w[0], w[1], w[2], w[3]);
 }
@@ -124,11 +126,24 @@ struct Sums {
     double s, u;  // sum 2^t and sum t 2^t
 };
 
-__device__ __forceinline__ float scale_of(double t) { return (float)fmin(1.4426950408889634 / t, 3.0e38); }
+// What a block's waves tell each other about a row, each place written once.
+template <int THREADS>
+struct Slots {
+    float top[THREADS / 64];
+    Sums sums[THREADS / 64];
+    RowState state;
+};
+
+__device__ __forceinline__ float scale_of(double inv) { return (float)fmin(1.4426950408889634 * inv, 3.0e38); }
 
 // t for a factor beside 2^t: where 2^t is 0 anyway it must stay finite.  2^t
 // itself is taken of the plain t, so that a NaN reaches the sums.
 __device__ __forceinline__ float finite_t(float t) { return fmaxf(t, -200.0f); }
+
+// The compiler is to unpack a held piece again each time it is used, not to
+// keep its entries as f32 (at 16 pieces of bf16 that is 128 more registers, and
+// spills).
+__device__ __forceinline__ void keep_packed(uint4& r) { asm volatile("" : "+v"(r.x), "+v"(r.y), "+v"(r.z), "+v"(r.w)); }
 
 template <class D, bool U>
 __device__ __forceinline__ void add_piece(const uint4& r, float m, float c, Sums& a) {
@@ -155,22 +170,17 @@ constexpr int kBatch = 4;  // pieces a thread has in flight where a row is strea
 
 // The maximum and sums of pieces [from, to) of a row, and of its edges where
 // `edges` is set.  The first THREADS * HELD pieces stay in `held`; what is left
-// is streamed, each thread with a maximum of its own.  The result is the same
+// is streamed before, each thread with a maximum of its own.  The result is the same
 // in every thread.  A part of nothing but -inf: m = -inf and sums 0, or NaN
 // where it has one.
 template <class D, int THREADS, int HELD, bool U>
-__device__ void row_sums(const Span<D>& row, int32_t from, int32_t to, bool edges, float c, uint4* held, float* fs,
-                         double* ds, float* m_out, Sums* out) {
+__device__ __forceinline__ void row_sums(const Span<D>& row, int32_t from, int32_t to, bool edges, float c, uint4* held,
+                                         Slots<THREADS>& slots, float* m_out, Sums* out) {
     const int tid = threadIdx.x;
     float top = -INFINITY, mine = -INFINITY;  // of what is held; of what is streamed
     Sums a{0.0, 0.0};
     float xe = -INFINITY;
     if (edges && tid < row.edges) xe = D::get(row.x[row.edge(tid)]);
-#pragma unroll
-    for (int k = 0; k < HELD; ++k) {
-        const int32_t i = from + k * THREADS + tid;
-        held[k] = i < to ? row.piece(i) : nothing<D>();
-    }
     for (int32_t i = from + HELD * THREADS + tid; i < to; i += kBatch * THREADS) {
         uint4 r[kBatch];
 #pragma unroll
@@ -184,7 +194,10 @@ __device__ void row_sums(const Span<D>& row, int32_t from, int32_t to, bool edge
         }
         if (mine > -INFINITY) {
 #pragma unroll
-            for (int k = 0; k < kBatch; ++k) add_piece<D, U>(r[k], mine, c, a);
+            for (int k = 0; k < kBatch; ++k) {
+                keep_packed(r[k]);
+                add_piece<D, U>(r[k], mine, c, a);
+            }
         } else {  // only -inf so far, or a NaN
             float bad = 0.0f;
 #pragma unroll
@@ -196,14 +209,27 @@ __device__ void row_sums(const Span<D>& row, int32_t from, int32_t to, bool edge
             a.s += (double)bad;
         }
     }
+#pragma unroll
+    for (int k = 0; k < HELD; ++k) {
+        const int32_t i = from + k * THREADS + tid;
+        held[k] = i < to ? row.piece(i) : nothing<D>();
+    }
     top = fmaxf(xe, mine);
 #pragma unroll
     for (int k = 0; k < HELD; ++k) top = fmaxf(top, Unpack<D>(held[k]).max());
-    const float m = block_max<THREADS>(top, fs);
+    top = wave_max(top);
+    if constexpr (THREADS > 64) {
+        if ((tid & 63) == 0) slots.top[tid >> 6] = top;
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < THREADS / 64; ++i) top = fmaxf(top, slots.top[i]);
+    }
+    const float m = top;
     if (m == -INFINITY) {
         float bad = xe != xe ? xe : 0.0f;
 #pragma unroll
         for (int k = 0; k < HELD; ++k) {
+            keep_packed(held[k]);
             const Unpack<D> x(held[k]);
 #pragma unroll
             for (int j = 0; j < Unpack<D>::kPer; ++j) bad = x.v[j] != x.v[j] ? x.v[j] : bad;
@@ -212,15 +238,29 @@ __device__ void row_sums(const Span<D>& row, int32_t from, int32_t to, bool edge
     } else {
         if (mine > -INFINITY && mine != m) move_to<U>(a, ((double)mine - (double)m) * (double)c);
 #pragma unroll
-        for (int k = 0; k < HELD; ++k) add_piece<D, U>(held[k], m, c, a);
+        for (int k = 0; k < HELD; ++k) {
+            keep_packed(held[k]);
+            add_piece<D, U>(held[k], m, c, a);
+        }
         const float t = (xe - m) * c, e = __builtin_amdgcn_exp2f(t);
         if (edges && tid < row.edges) {
             a.s += (double)e;
             if (U) a.u += (double)(e * finite_t(t));
         }
     }
-    out->s = block_sum<THREADS>(a.s, ds);
-    out->u = U ? block_sum<THREADS>(a.u, ds) : 0.0;
+    a.s = wave_sum(a.s);
+    if (U) a.u = wave_sum(a.u);
+    if constexpr (THREADS > 64) {
+        if ((tid & 63) == 0) slots.sums[tid >> 6] = a;
+        __syncthreads();
+        a = slots.sums[0];
+#pragma unroll
+        for (int i = 1; i < THREADS / 64; ++i) {
+            a.s += slots.sums[i].s;
+            a.u += slots.sums[i].u;
+        }
+    }
+    *out = a;
     *m_out = m;
 }
 
@@ -230,9 +270,9 @@ struct Slope {
     float m, c, a, b;
 };
 
-__device__ __forceinline__ Slope slope_of(const RowState& s, double t, double scale) {
-    const double inv = scale * exp(-s.logs);
-    return Slope{(float)s.m, scale_of(t), (float)(inv * s.e * 0.6931471805599453), (float)(inv * (s.f - s.e * s.logs))};
+__device__ __forceinline__ Slope slope_of(const RowState& s, double t_inv, double scale) {
+    const double inv = scale * exp_64(-s.logs);
+    return Slope{(float)s.m, scale_of(t_inv), (float)(inv * s.e * 0.6931471805599453), (float)(inv * (s.f - s.e * s.logs))};
 }
 
 template <bool E>
@@ -241,227 +281,241 @@ __device__ __forceinline__ float slope_at(const Slope& g, float x) {
     return E ? e * fmaf(finite_t(t), g.a, g.b) : e * g.b;
 }
 
+// How a gradient's pieces are stored.
+enum { kPlain, kStream, kSingle };
+
+// Rows of logits and gradient that start alike within 16 bytes take whole
+// pieces.  A gradient that is larger than half the 256 MB behind the L2 goes
+// past it: the logits that are read twice stay there (4096 x 131072 bf16, PPO:
+// 441 us, plain stores 476); a smaller one is likely read from there next.
+__device__ __forceinline__ int store_mode(const void* g, const void* x, int64_t bytes) {
+    return (((uintptr_t)g ^ (uintptr_t)x) & 15) ? kSingle : bytes > (128ll << 20) ? kStream : kPlain;
+}
+
+template <class D>
+__device__ __forceinline__ void store_piece(typename D::raw* g, const Span<D>& row, int32_t i, int mode, const uint4& r) {
+    typename D::raw* at = g + row.head + (int64_t)i * Span<D>::kPer;
+    if (mode == kStream) {
+        typedef uint32_t u4 __attribute__((ext_vector_type(4)));
+        __builtin_nontemporal_store(u4{r.x, r.y, r.z, r.w}, reinterpret_cast<u4*>(at));
+    } else if (mode == kPlain) {
+        *reinterpret_cast<uint4*>(at) = r;
+    } else {
+        const typename D::raw* v = reinterpret_cast<const typename D::raw*>(&r);
+#pragma unroll
+        for (int k = 0; k < Span<D>::kPer; ++k) at[k] = v[k];
+    }
+}
+
 template <class D, bool E>
-__device__ __forceinline__ void put_piece(typename D::raw* g, const Span<D>& row, int32_t i, bool aligned, const uint4& r,
-                                          const Slope& sl, bool skip) {
+__device__ __forceinline__ uint4 slope_piece(const uint4& r, const Slope& sl) {
     const Unpack<D> x(r);
     float v[Unpack<D>::kPer];
 #pragma unroll
-    for (int k = 0; k < Unpack<D>::kPer; ++k) v[k] = skip ? 0.0f : slope_at<E>(sl, x.v[k]);
-    typename D::raw* at = g + row.head + (int64_t)i * Span<D>::kPer;
-    if (aligned) {
-        *reinterpret_cast<uint4*>(at) = pack<D>(v);
-    } else {
+    for (int k = 0; k < Unpack<D>::kPer; ++k) v[k] = slope_at<E>(sl, x.v[k]);
+    return pack<D>(v);
+}
+
+// The dense gradient of pieces [from, to) of a row that are not held; a row
+// that is ignored gets zeros and is not read.
+template <class D, bool E, int THREADS>
+__device__ __forceinline__ void put_pieces(typename D::raw* g, const Span<D>& row, int32_t from, int32_t to, int mode,
+                                           const Slope& sl, bool skip) {
+    if (skip) {
+        for (int32_t i = from + (int)threadIdx.x; i < to; i += THREADS) store_piece<D>(g, row, i, mode, make_uint4(0, 0, 0, 0));
+        return;
+    }
+    for (int32_t i = from + (int)threadIdx.x; i < to; i += kBatch * THREADS) {
+        uint4 r[kBatch];
 #pragma unroll
-        for (int k = 0; k < Span<D>::kPer; ++k) at[k] = D::put(v[k]);
+        for (int k = 0; k < kBatch; ++k)
+            if (i + k * THREADS < to) r[k] = row.piece(i + k * THREADS);
+#pragma unroll
+        for (int k = 0; k < kBatch; ++k)
+            if (i + k * THREADS < to) store_piece<D>(g, row, i + k * THREADS, mode, slope_piece<D, E>(r[k], sl));
     }
 }
 
-// The same numbers at one entry, in f64.
-template <class Op, class D>
-__device__ double dense_at(const Op& op, const RowState& s, const typename D::raw* x, int64_t i) {
-    const double lp = ((double)D::get(x[i]) - s.m) / op.t - s.logs, p = exp(lp);
-    return p == 0.0 ? 0.0 : p * ((Op::ppo ? s.e : 0.0) * lp + s.f);
-}
-
-// What a block holds of a row's teacher: the entries inside the vocabulary
-// (others idx -1, q 0).
+// What a block holds of a row's teacher, k entries of each (dynamic LDS):
+// those outside the vocabulary have idx -1 and q 0.
 struct Teacher {
-    int32_t idx[RT_CAT_MAX_TOP];
-    double q[RT_CAT_MAX_TOP];  // log q, then q
+    double *lq, *q;
+    float* v;      // the logits at idx, then the gradient there
+    int32_t* idx;
+    __device__ Teacher(char* lds, int32_t k)
+        : lq(reinterpret_cast<double*>(lds)), q(lq + k), v(reinterpret_cast<float*>(q + k)),
+          idx(reinterpret_cast<int32_t*>(v + k)) {}
+    static size_t bytes(int32_t k) { return (size_t)k * 24; }
 };
-struct NoTeacher {};
 
-// log of the teacher's normaliser
-template <int THREADS>
-__device__ double teacher_lse(const Distill& op, int64_t n, int32_t V, float* fs, double* ds) {
-    if (op.b.lse) return op.b.lse[n];
+// By one wave: the entries, their probabilities q, and sum q.  lse: the
+// teacher's normaliser, NaN for one that is still to be found.
+template <class D>
+__device__ double teacher_load(const Distill& op, int64_t n, int32_t V, const typename D::raw* x, Teacher& te,
+                               double* lse) {
+    const int lane = threadIdx.x & 63;
     const int64_t at = n * op.b.k;
+    const double inv = op.inv;
     float m = -INFINITY;
-    for (int j = threadIdx.x; j < op.b.k; j += THREADS) {
-        const int64_t i = op.b.idx[at + j];
-        if (i >= 0 && i < V) m = fmaxf(m, op.b.logits[at + j]);
-    }
-    m = block_max<THREADS>(m, fs);
-    if (m == -INFINITY) m = 0.0f;
-    double s = 0.0;
-    for (int j = threadIdx.x; j < op.b.k; j += THREADS) {
-        const int64_t i = op.b.idx[at + j];
-        if (i >= 0 && i < V) s += exp(((double)op.b.logits[at + j] - (double)m) / op.t);
-    }
-    s = block_sum<THREADS>(s, ds);
-    return s == 0.0 ? 0.0 : (double)m / op.t + log(s);
-}
-
-// The teacher's entries and their log-probabilities into LDS.
-template <int THREADS>
-__device__ void teacher_load(const Distill& op, int64_t n, int32_t V, double lse, Teacher& te) {
-    const int64_t at = n * op.b.k;
-    for (int j = threadIdx.x; j < op.b.k; j += THREADS) {
+    for (int j = lane; j < op.b.k; j += 64) {
         const int64_t i = op.b.idx[at + j];
         const bool in = i >= 0 && i < V;
+        const float t = in ? op.b.logits[at + j] : -INFINITY;
         te.idx[j] = in ? (int32_t)i : -1;
-        te.q[j] = in ? (double)op.b.logits[at + j] / op.t - lse : -INFINITY;
+        te.lq[j] = t;
+        te.v[j] = in ? D::get(x[i]) : 0.0f;
+        m = fmaxf(m, t);
     }
-    __syncthreads();
-}
-
-// What the named entries' gradient is on top of the dense part: each is
-// computed whole, before anything is written (the gradient may lie in the
-// logits' own memory), and stored over the dense value.
-template <int THREADS>
-struct Named {
-    static constexpr int kMost = (RT_CAT_MAX_TOP + THREADS - 1) / THREADS;
-    int32_t at[kMost];
-    float v[kMost];
-};
-
-// first, last: the entries that this block writes
-template <class D, class Op, int THREADS, class Te>
-__device__ void named_find(const Op& op, int64_t n, const RowState& s, double scale, bool skip, const Te& te,
-                           const typename D::raw* x, Named<THREADS>& e, int32_t first, int32_t last) {
-    const int tid = threadIdx.x;
-    if constexpr (Op::ppo) {
-        e.at[0] = -1;
-        if (!skip && tid == 0) {
-            const int64_t a = op.b.actions[n];
-            if (a >= first && a < last) {
-                e.at[0] = (int32_t)a;
-                e.v[0] = (float)(scale * (dense_at<Op, D>(op, s, x, a) + s.c));
-            }
-        }
+    if (op.b.lse) {
+        *lse = op.b.lse[n];
     } else {
-#pragma unroll
-        for (int k = 0; k < Named<THREADS>::kMost; ++k) {
-            const int j = tid + k * THREADS;
-            e.at[k] = !skip && j < op.b.k ? te.idx[j] : -1;
-            if (e.at[k] < first || e.at[k] >= last) e.at[k] = -1;
-            if (e.at[k] < 0) continue;
-            double q = 0.0;
-            for (int i = 0; i < op.b.k; ++i)
-                if (te.idx[i] == e.at[k]) q += te.q[i];
-            e.v[k] = (float)(scale * (dense_at<Op, D>(op, s, x, e.at[k]) - s.c * q));
-        }
+        m = wave_max(m);
+        if (m == -INFINITY) m = 0.0f;
+        double s = 0.0;
+        for (int j = lane; j < op.b.k; j += 64) s += exp2_64((te.lq[j] - (double)m) * (1.4426950408889634 * inv));
+        s = wave_sum(s);
+        *lse = s == 0.0 ? 0.0 : (double)m * inv + log_64(s);
     }
-}
-
-template <class D, class Op, int THREADS>
-__device__ void named_put(const Named<THREADS>& e, typename D::raw* g) {
-#pragma unroll
-    for (int k = 0; k < (Op::ppo ? 1 : Named<THREADS>::kMost); ++k)
-        if (e.at[k] >= 0) g[e.at[k]] = D::put(e.v[k]);
+    double Q = 0.0;
+    for (int j = lane; j < op.b.k; j += 64) {
+        const double lq = te.idx[j] < 0 ? -INFINITY : te.lq[j] * inv - *lse, q = exp2_64(lq * 1.4426950408889634);
+        te.lq[j] = lq;
+        te.q[j] = q;
+        Q += q;
+    }
+    return wave_sum(Q);
 }
 
 // ---- from the sums to the loss ---------------------------------------------
-// The row's outputs, its terms of the sums over rows, and its state.  Every
-// thread of the block calls it; every thread gets the state.
-template <class D, class Op, int THREADS, class Te>
-__device__ RowState finish_row(const Logits& l, const Op& op, const Out& o, int64_t n, bool skip, float m,
-                               const Sums& sums, const typename D::raw* x, Te& te, double* terms, bool write, float* fs,
-                               double* ds, RowState* share) {
-    const int tid = threadIdx.x;
-    RowState st{0.0, INFINITY, 0.0, 0.0, 0.0};  // log S +inf: a row that adds nothing
-    if constexpr (Op::ppo) {
-        if (tid < 64) {
-            double term[Op::terms] = {}, lp = 0.0, h = 0.0;
-            if (!skip) {
-                const double logs = log(sums.s);
-                lp = ((double)D::get(x[op.b.actions[n]]) - (double)m) / op.t - logs;
-                h = logs - 0.6931471805599453 * (sums.u / sums.s);
-                st = op.finish(n, l.rows, m, logs, lp, h, term);
-            }
-            if (tid == 0) {
-                *share = st;
-                if (write) {
-                    o.logprob[n] = (float)lp;
-                    o.entropy[n] = (float)h;
-                    for (int k = 0; k < Op::terms; ++k) terms[n * Op::terms + k] = term[k];
-                }
-            }
-        }
-        __syncthreads();
-        st = *share;
-    } else {
-        double kl = 0.0;
-        if (!skip) {
-            const double logs = log(sums.s), lse = teacher_lse<THREADS>(op, n, l.vocab, fs, ds);
-            teacher_load<THREADS>(op, n, l.vocab, lse, te);
-            double Q = 0.0;
-            for (int j = tid; j < op.b.k; j += THREADS) {
-                const double lq = te.q[j], q = exp(lq);
-                if (te.idx[j] >= 0 && q != 0.0) kl += q * (lq - (((double)D::get(x[te.idx[j]]) - (double)m) / op.t - logs));
-                Q += q;
-                te.q[j] = q;
-            }
-            Q = block_sum<THREADS>(Q, ds);
-            kl = block_sum<THREADS>(kl, ds);
-            const double w = op.weight(n, l.rows);
-            // E is 0 throughout: its place keeps the teacher's normaliser for the backward pass
-            st = RowState{m, logs, lse, w * Q / op.t, w / op.t};
-            if (tid == 0 && write) terms[n] = w * kl;
-        } else if (tid == 0 && write) {
-            terms[n] = 0.0;
-        }
-        if (tid == 0 && write) o.kl[n] = (float)kl;
+// By one wave: the row's state, its outputs, its terms of the sums over rows.
+__device__ __forceinline__ RowState ppo_row(const Ppo& op, const Out& o, int64_t n, int64_t rows, float m, double S,
+                                            double U, float xa, bool write, double* term) {
+    const double logs = log_64(S), lp = ((double)xa - (double)m) * op.inv - logs;
+    const double h = logs - 0.6931471805599453 * (U / S);
+    const RowState st = op.finish(n, rows, m, logs, lp, h, term);
+    if (write) {
+        o.logprob[n] = (float)lp;
+        o.entropy[n] = (float)h;
     }
-    if (tid == 0 && write && o.state) *reinterpret_cast<RowState*>(o.state + n * RT_CAT_ROW_STATE) = st;
     return st;
+}
+
+__device__ __forceinline__ RowState distill_row(const Distill& op, const Out& o, int64_t n, int64_t rows, float m, double S,
+                                                const Teacher& te, double lse, double Q, double* term) {
+    const int lane = threadIdx.x & 63;
+    const double logs = log_64(S), inv = op.inv;
+    double kl = 0.0;
+    for (int j = lane; j < op.b.k; j += 64) {
+        const double q = te.q[j];
+        if (te.idx[j] >= 0 && q != 0.0) kl += q * (te.lq[j] - (((double)te.v[j] - (double)m) * inv - logs));
+    }
+    kl = wave_sum(kl);
+    const double w = op.weight(n, rows);
+    if (lane == 0) o.kl[n] = (float)kl;
+    term[0] = w * kl;
+    // E is 0 throughout: its place keeps the teacher's normaliser for the backward pass
+    return RowState{m, logs, lse, w * Q * inv, w * inv};
 }
 
 template <class Op>
 __device__ __forceinline__ Slope op_slope(const Op& op, RowState s, double scale) {
     if (!Op::ppo) s.e = 0.0;
-    return slope_of(s, op.t, scale);
+    return slope_of(s, op.inv, scale);
 }
 
+// The gradient at the teacher's entries, in the place of their logits: the
+// dense part and all that names the same entry, in the entries' order.
+template <int THREADS>
+__device__ __forceinline__ void named_slopes(const Teacher& te, int32_t k, const Slope& sl, float each) {
+    for (int j = threadIdx.x; j < k; j += THREADS) {
+        const int32_t at = te.idx[j];
+        if (at < 0) continue;
+        double q = 0.0;
+        for (int i = 0; i < k; ++i) q += te.idx[i] == at ? te.q[i] : 0.0;
+        te.v[j] = slope_at<false>(sl, te.v[j]) - each * (float)q;
+    }
+}
+
+extern __shared__ __align__(16) char teacher_lds[];
+
 // ---- one block per row -----------------------------------------------------
-// The row is read once: HELD pieces of every thread stay in registers between
-// the sums and the gradient, which longer rows read again.
+// HELD pieces of every thread stay in registers between the sums and the
+// gradient; longer rows are read again for the rest.
 template <class D, class Op, int THREADS, int HELD>
 __global__ __launch_bounds__(THREADS) void k_cat_row(Logits l, Op op, Out o, double* terms) {
-    __shared__ float fs[THREADS / 64];
-    __shared__ double ds[THREADS / 64];
-    __shared__ RowState share;
-    __shared__ std::conditional_t<Op::ppo, NoTeacher, Teacher> te;
+    __shared__ Slots<THREADS> slots;
+    Teacher te(teacher_lds, Op::ppo ? 0 : op.k());
     const int64_t n = blockIdx.x;
     const int tid = threadIdx.x;
     const auto* x = row_of<D>(l, n);
     const Span<D> row(x, l.vocab);
     uint4 held[HELD ? HELD : 1];
-    float m = -INFINITY;
+    float m = -INFINITY, xa = 0.0f;
     Sums sums{0.0, 0.0};
     bool skip = op.ignored(n, l.vocab);
+    double lse = 0.0, Q = 0.0;
     if (!skip) {
-        row_sums<D, THREADS, HELD, Op::ppo>(row, 0, row.pieces, true, scale_of(op.t), held, fs, ds, &m, &sums);
+        if constexpr (Op::ppo) xa = D::get(x[op.b.actions[n]]);
+        else if (tid < 64) Q = teacher_load<D>(op, n, l.vocab, x, te, &lse);
+        row_sums<D, THREADS, HELD, Op::ppo>(row, 0, row.pieces, true, scale_of(op.inv), held, slots, &m, &sums);
         skip = m == -INFINITY && sums.s == 0.0;
     }
-    const RowState st = finish_row<D, Op, THREADS>(l, op, o, n, skip, m, sums, x, te, terms, true, fs, ds, &share);
+    if (tid < 64) {
+        RowState st{0.0, INFINITY, 0.0, 0.0, 0.0};  // log S +inf: a row that adds nothing
+        double term[Op::terms] = {};
+        if constexpr (Op::ppo) {
+            if (!skip) st = ppo_row(op, o, n, l.rows, m, sums.s, sums.u, xa, tid == 0, term);
+            else if (tid == 0) o.logprob[n] = o.entropy[n] = 0.0f;
+        } else {
+            if (!skip) st = distill_row(op, o, n, l.rows, m, sums.s, te, lse, Q, term);
+            else if (tid == 0) o.kl[n] = 0.0f;
+        }
+        if (tid == 0) {
+#pragma unroll
+            for (int k = 0; k < Op::terms; ++k) terms[n * Op::terms + k] = term[k];
+            if (o.state) *reinterpret_cast<RowState*>(o.state + n * RT_CAT_ROW_STATE) = st;
+            slots.state = st;
+        }
+    }
     if (!o.grad) return;
     auto* g = static_cast<typename D::raw*>(o.grad) + n * o.grad_stride;
-    Named<THREADS> named;
-    named_find<D, Op, THREADS>(op, n, st, 1.0, skip, te, x, named, 0, l.vocab);
-    const Slope sl = op_slope(op, st, 1.0);
-    const bool aligned = (((uintptr_t)g ^ (uintptr_t)x) & 15) == 0;
     float xe = 0.0f;
     if (tid < row.edges) xe = D::get(x[row.edge(tid)]);
     __syncthreads();
-#pragma unroll
-    for (int k = 0; k < HELD; ++k) {
-        const int32_t i = k * THREADS + tid;
-        if (i < row.pieces) put_piece<D, Op::ppo>(g, row, i, aligned, held[k], sl, skip);
+    const RowState st = slots.state;
+    const Slope sl = op_slope(op, st, 1.0);
+    if constexpr (!Op::ppo) {
+        if (!skip) named_slopes<THREADS>(te, op.b.k, sl, (float)st.c);
+        __syncthreads();
     }
-    for (int32_t i = HELD * THREADS + tid; i < row.pieces; i += THREADS)
-        put_piece<D, Op::ppo>(g, row, i, aligned, row.piece(i), sl, skip);
+    // the gradient may lie in the logits' own memory: from here on only what is not held is read, each
+    // entry by the thread that writes it
+    const int mode = store_mode(g, x, l.rows * l.vocab * (int64_t)sizeof(typename D::raw));
+    if (!skip) {
+#pragma unroll
+        for (int k = 0; k < HELD; ++k) {
+            const int32_t i = k * THREADS + tid;
+            keep_packed(held[k]);
+            if (i < row.pieces) store_piece<D>(g, row, i, mode, slope_piece<D, Op::ppo>(held[k], sl));
+        }
+    }
+    put_pieces<D, Op::ppo, THREADS>(g, row, skip ? 0 : HELD * THREADS, row.pieces, mode, sl, skip);
     if (tid < row.edges) g[row.edge(tid)] = D::put(skip ? 0.0f : slope_at<Op::ppo>(sl, xe));
+    if (skip) return;
     __syncthreads();
-    named_put<D, Op, THREADS>(named, g);
+    if constexpr (Op::ppo) {
+        if (tid == 0) g[op.b.actions[n]] = D::put(slope_at<true>(sl, xa) + (float)st.c);
+    } else {
+        for (int j = tid; j < op.b.k; j += THREADS)
+            if (te.idx[j] >= 0) g[te.idx[j]] = D::put(te.v[j]);
+    }
 }
 
 // ---- a row's gradient from its state, by parts -----------------------------
 template <class D, class Op, int THREADS>
 __global__ __launch_bounds__(THREADS) void k_cat_backward(Logits l, Op op, const RowState* state, const float* gout,
                                                           void* grad, int64_t grad_stride, int32_t parts) {
-    __shared__ std::conditional_t<Op::ppo, NoTeacher, Teacher> te;
+    Teacher te(teacher_lds, Op::ppo ? 0 : op.k());
     const int64_t n = blockIdx.x / parts;
     const int32_t part = blockIdx.x % parts;
     const int tid = threadIdx.x;
@@ -476,47 +530,49 @@ __global__ __launch_bounds__(THREADS) void k_cat_backward(Logits l, Op op, const
     // the first part also has the entries before the pieces, the last those behind
     const int32_t first = part == 0 ? 0 : row.head + from * Span<D>::kPer;
     const int32_t last = part == parts - 1 ? l.vocab : row.head + to * Span<D>::kPer;
-    if constexpr (!Op::ppo) {
-        if (!skip) {
-            teacher_load<THREADS>(op, n, l.vocab, st.e, te);
-            for (int j = tid; j < op.b.k; j += THREADS) te.q[j] = exp(te.q[j]);
-            __syncthreads();
-        }
-    }
-    Named<THREADS> named;
-    named_find<D, Op, THREADS>(op, n, st, scale, skip, te, x, named, first, last);
     const Slope sl = op_slope(op, st, scale);
-    const bool aligned = (((uintptr_t)g ^ (uintptr_t)x) & 15) == 0;
+    const float each = (float)(scale * st.c);
+    int64_t a = -1;
+    float va = 0.0f;
+    if constexpr (Op::ppo) {
+        if (!skip && tid == 0) {
+            a = op.b.actions[n];
+            if (a >= first && a < last) va = slope_at<true>(sl, D::get(x[a])) + each;
+            else a = -1;
+        }
+    } else if (!skip) {
+        for (int j = tid; j < op.b.k; j += THREADS) {
+            const int64_t i = op.b.idx[n * op.b.k + j];
+            const bool in = i >= first && i < last;
+            te.idx[j] = in ? (int32_t)i : -1;
+            te.q[j] = in ? exp_64((double)op.b.logits[n * op.b.k + j] * op.inv - st.e) : 0.0;
+            te.v[j] = in ? D::get(x[i]) : 0.0f;
+        }
+        __syncthreads();
+        named_slopes<THREADS>(te, op.b.k, sl, each);
+    }
+    const int mode = store_mode(g, x, l.rows * l.vocab * (int64_t)sizeof(typename D::raw));
     const int32_t e = tid < row.edges ? row.edge(tid) : -1;
     const bool mine = e >= first && e < last;
     float xe = 0.0f;
     if (mine) xe = D::get(x[e]);
     __syncthreads();
-    for (int32_t i = from + tid; i < to; i += THREADS)
-        put_piece<D, Op::ppo>(g, row, i, aligned, skip ? nothing<D>() : row.piece(i), sl, skip);
+    put_pieces<D, Op::ppo, THREADS>(g, row, from, to, mode, sl, skip);
     if (mine) g[e] = D::put(skip ? 0.0f : slope_at<Op::ppo>(sl, xe));
+    if (skip) return;
     __syncthreads();
-    named_put<D, Op, THREADS>(named, g);
+    if constexpr (Op::ppo) {
+        if (a >= 0) g[a] = D::put(va);
+    } else {
+        for (int j = tid; j < op.b.k; j += THREADS)
+            if (te.idx[j] >= 0) g[te.idx[j]] = D::put(te.v[j]);
+    }
 }
 
 // ---- short rows ------------------------------------------------------------
 // Up to 1024 entries: many rows, so more of them lie next to the border of the
 // clip, and the memory they need is small beside the arithmetic of a row: the
 // sums are in f64 throughout.
-
-// From the state, or from a row's sums, to the state and the terms; what the
-// two kernels below share.  Every lane of the G that have the row calls it.
-__device__ __forceinline__ RowState ppo_row(const Ppo& op, const Out& o, int64_t n, int64_t rows, float m, double S,
-                                            double U, float xa, bool write, double* term) {
-    const double logs = log(S), lp = ((double)xa - (double)m) / op.t - logs;
-    const double h = logs - 0.6931471805599453 * (U / S);
-    const RowState st = op.finish(n, rows, m, logs, lp, h, term);
-    if (write) {
-        o.logprob[n] = (float)lp;
-        o.entropy[n] = (float)h;
-    }
-    return st;
-}
 
 // The sums of a block's rows, in a fixed order.
 template <int TERMS>
@@ -554,9 +610,8 @@ __global__ __launch_bounds__(256) void k_cat_short(Logits l, Op op, Out o, doubl
         m = fmaxf(m, v[e]);
     }
     if constexpr (!GIVEN) {
-        const double c = 1.4426950408889634 / op.t;
-#pragma unroll
-        for (int d = G / 2; d; d >>= 1) m = fmaxf(m, __shfl_xor(m, d));
+        const double c = 1.4426950408889634 * op.inv;
+        m = lanes_max<G>(m);
         const float mf = m == -INFINITY ? 0.0f : m;
         double S = 0.0, U = 0.0;
 #pragma unroll
@@ -565,11 +620,8 @@ __global__ __launch_bounds__(256) void k_cat_short(Logits l, Op op, Out o, doubl
             S += p;
             if (Op::ppo) U = fma(p, z < -1100.0 ? -1100.0 : z, U);
         }
-#pragma unroll
-        for (int d = G / 2; d; d >>= 1) {
-            S += __shfl_xor(S, d);
-            if (Op::ppo) U += __shfl_xor(U, d);
-        }
+        S = lanes_sum<G>(S);
+        if (Op::ppo) U = lanes_sum<G>(U);
         skip = skip || S == 0.0;
         if constexpr (Op::ppo) {
             if (!skip) {
@@ -579,7 +631,7 @@ __global__ __launch_bounds__(256) void k_cat_short(Logits l, Op op, Out o, doubl
             }
         } else {
             double kl = 0.0, Q = 0.0, lse = 0.0;
-            const double logs = log(S), w = skip ? 0.0 : op.weight(n, l.rows);
+            const double logs = log_64(S), w = skip ? 0.0 : op.weight(n, l.rows);
             const int64_t at = in ? n * op.b.k : 0;
             if (op.b.lse) {
                 if (!skip) lse = op.b.lse[n];
@@ -589,33 +641,28 @@ __global__ __launch_bounds__(256) void k_cat_short(Logits l, Op op, Out o, doubl
                     const int64_t i = op.b.idx[at + j];
                     if (i >= 0 && i < V) tm = fmaxf(tm, op.b.logits[at + j]);
                 }
-#pragma unroll
-                for (int d = G / 2; d; d >>= 1) tm = fmaxf(tm, __shfl_xor(tm, d));
+                tm = lanes_max<G>(tm);
                 if (tm == -INFINITY) tm = 0.0f;
                 for (int j = t; j < op.b.k; j += G) {
                     const int64_t i = op.b.idx[at + j];
                     if (i >= 0 && i < V) lse += exp2_64(((double)op.b.logits[at + j] - (double)tm) * c);
                 }
-#pragma unroll
-                for (int d = G / 2; d; d >>= 1) lse += __shfl_xor(lse, d);
-                lse = lse == 0.0 ? 0.0 : (double)tm / op.t + log(lse);
+                lse = lanes_sum<G>(lse);
+                lse = lse == 0.0 ? 0.0 : (double)tm * op.inv + log_64(lse);
             }
             if (!skip) {
                 for (int j = t; j < op.b.k; j += G) {
                     const int64_t i = op.b.idx[at + j];
                     if (i < 0 || i >= V) continue;
-                    const double lq = (double)op.b.logits[at + j] / op.t - lse, q = exp(lq);
-                    if (q != 0.0) kl += q * (lq - (((double)D::get(x[i]) - (double)m) / op.t - logs));
+                    const double lq = (double)op.b.logits[at + j] * op.inv - lse, q = exp_64(lq);
+                    if (q != 0.0) kl += q * (lq - (((double)D::get(x[i]) - (double)m) * op.inv - logs));
                     Q += q;
                 }
             }
-#pragma unroll
-            for (int d = G / 2; d; d >>= 1) {
-                kl += __shfl_xor(kl, d);
-                Q += __shfl_xor(Q, d);
-            }
+            kl = lanes_sum<G>(kl);
+            Q = lanes_sum<G>(Q);
             if (!skip) {
-                st = RowState{m, logs, lse, w * Q / op.t, w / op.t};
+                st = RowState{m, logs, lse, w * Q * op.inv, w * op.inv};
                 term[0] = w * kl;
             }
             if (in && t == 0) o.kl[n] = (float)kl;
@@ -641,7 +688,7 @@ __global__ __launch_bounds__(256) void k_cat_short(Logits l, Op op, Out o, doubl
                 const int64_t i = op.b.idx[at + j0 + t];
                 if (i >= 0 && i < V) {
                     idx = (int32_t)i;
-                    q = (float)exp((double)op.b.logits[at + j0 + t] / op.t - st.e);
+                    q = (float)exp_64((double)op.b.logits[at + j0 + t] * op.inv - st.e);
                 }
             }
             const int many = min(G, op.b.k - j0);
@@ -698,7 +745,7 @@ __global__ __launch_bounds__(256) void k_cat_tiny(Logits l, Op op, Out o, double
     }
     if constexpr (!GIVEN) {
         if (!skip) {
-            const double c = 1.4426950408889634 / op.t;
+            const double c = 1.4426950408889634 * op.inv;
             float m = x[0];
             for (int i = 1; i < V; ++i) m = fmaxf(m, x[i]);
             const float mf = m == -INFINITY ? 0.0f : m;
@@ -713,7 +760,7 @@ __global__ __launch_bounds__(256) void k_cat_tiny(Logits l, Op op, Out o, double
                 if constexpr (Op::ppo) {
                     st = ppo_row(op, o, n, l.rows, m, S, U, x[op.b.actions[n]], true, term);
                 } else {
-                    const double logs = log(S), w = op.weight(n, l.rows);
+                    const double logs = log_64(S), w = op.weight(n, l.rows);
                     const int64_t at = n * op.b.k;
                     double lse = 0.0, kl = 0.0, Q = 0.0;
                     if (op.b.lse) {
@@ -729,16 +776,16 @@ __global__ __launch_bounds__(256) void k_cat_tiny(Logits l, Op op, Out o, double
                             const int64_t i = op.b.idx[at + j];
                             if (i >= 0 && i < V) lse += exp2_64(((double)op.b.logits[at + j] - (double)tm) * c);
                         }
-                        lse = lse == 0.0 ? 0.0 : (double)tm / op.t + log(lse);
+                        lse = lse == 0.0 ? 0.0 : (double)tm * op.inv + log_64(lse);
                     }
                     for (int j = 0; j < op.b.k; ++j) {
                         const int64_t i = op.b.idx[at + j];
                         if (i < 0 || i >= V) continue;
-                        const double lq = (double)op.b.logits[at + j] / op.t - lse, q = exp(lq);
-                        if (q != 0.0) kl += q * (lq - (((double)x[i] - (double)m) / op.t - logs));
+                        const double lq = (double)op.b.logits[at + j] * op.inv - lse, q = exp_64(lq);
+                        if (q != 0.0) kl += q * (lq - (((double)x[i] - (double)m) * op.inv - logs));
                         Q += q;
                     }
-                    st = RowState{m, logs, lse, w * Q / op.t, w / op.t};
+                    st = RowState{m, logs, lse, w * Q * op.inv, w * op.inv};
                     term[0] = w * kl;
                     o.kl[n] = (float)kl;
                 }
@@ -765,7 +812,7 @@ __global__ __launch_bounds__(256) void k_cat_tiny(Logits l, Op op, Out o, double
                 const int64_t at = n * op.b.k;
                 for (int j = 0; j < op.b.k; ++j) {
                     const int64_t i = op.b.idx[at + j];
-                    const float q = (float)exp((double)op.b.logits[at + j] / op.t - st.e);
+                    const float q = (float)exp_64((double)op.b.logits[at + j] * op.inv - st.e);
                     if (i >= 0 && i < V && q != 0.0f) x[i] -= each * q;
                 }
             }
@@ -805,29 +852,60 @@ int64_t launch_short(const Logits& l, const Op& op, const Out& o, double* ws, co
 }
 
 // ---- sums over the rows ----------------------------------------------------
-// One block; every thread a fixed set of rows, then a fixed tree: the same
-// bits every time.
+// Every thread a fixed set of rows, then a fixed tree: the same bits every
+// time.  One block, or, past 4096 rows (one block takes 50 us for 65536), one
+// for each 1024 rows that leave their sums for it.
+constexpr int64_t kFold = 1024;
+
 template <int TERMS>
-__global__ __launch_bounds__(1024) void k_cat_total(const double* terms, int64_t n, float* loss, float* stats) {
-    __shared__ double ds[16];
+__global__ __launch_bounds__(1024) void k_cat_total(const double* terms, int64_t n, int64_t per, double* sums, float* loss,
+                                                    float* stats) {
+    __shared__ double part[16][TERMS];
+    const int64_t from = blockIdx.x * per, to = min(from + per, n);
     double s[TERMS] = {};
-    for (int64_t i = threadIdx.x; i < n; i += 1024)
+    for (int64_t i = from + threadIdx.x; i < to; i += 1024)
+#pragma unroll
         for (int k = 0; k < TERMS; ++k) s[k] += terms[i * TERMS + k];
+#pragma unroll
     for (int k = 0; k < TERMS; ++k) {
-        const double r = block_sum<1024>(s[k], ds);
-        if (threadIdx.x == 0) {
-            if (k == 0) *loss = (float)r;
-            else stats[k - 1] = (float)r;
-        }
+        const double r = wave_sum(s[k]);
+        if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6][k] = r;
     }
+    __syncthreads();
+    const int k = threadIdx.x;
+    if (k >= TERMS) return;
+    double r = part[0][k];
+#pragma unroll
+    for (int i = 1; i < 16; ++i) r += part[i][k];
+    if (sums) sums[blockIdx.x * TERMS + k] = r;
+    else if (k == 0) *loss = (float)r;
+    else stats[k - 1] = (float)r;
 }
 
-// per-row terms of the sums over rows: the loss and up to six statistics
-int64_t terms_bytes(int64_t rows) { return rows * Ppo::terms * (int64_t)sizeof(double); }
+// per-row terms of the sums over rows: the loss and up to six statistics; and of each kFold rows
+int64_t terms_bytes(int64_t rows) { return (rows + (rows + kFold - 1) / kFold) * Ppo::terms * (int64_t)sizeof(double); }
+
+template <int TERMS>
+void launch_total(const double* terms, int64_t n, double* sums, const Out& o, hipStream_t st) {
+    const auto go = [&](const double* from, int64_t n, int64_t blocks, int64_t per, double* to) {
+        hipLaunchKernelGGL((k_cat_total<TERMS>), dim3((unsigned)blocks), dim3(1024), 0, st, from, n, per, to, o.loss, o.stats);
+    };
+    if (n > 4 * kFold) {
+        const int64_t blocks = (n + kFold - 1) / kFold;
+        go(terms, n, blocks, kFold, sums);
+        terms = sums;
+        n = blocks;
+    }
+    go(terms, n, 1, n, nullptr);
+}
+
+size_t teacher_bytes(const Ppo&) { return 0; }
+size_t teacher_bytes(const Distill& op) { return Teacher::bytes(op.b.k); }
 
 template <class D, class Op, int THREADS, int HELD>
 void launch_row(const Logits& l, const Op& op, const Out& o, double* ws, hipStream_t st) {
-    hipLaunchKernelGGL((k_cat_row<D, Op, THREADS, HELD>), dim3((unsigned)l.rows), dim3(THREADS), 0, st, l, op, o, ws);
+    hipLaunchKernelGGL((k_cat_row<D, Op, THREADS, HELD>), dim3((unsigned)l.rows), dim3(THREADS), teacher_bytes(op), st, l,
+                       op, o, ws);
 }
 
 template <class D, class Op>
@@ -835,12 +913,19 @@ int run_loss(const Logits& l, const Op& op, const Out& o, double* ws, hipStream_
     const int32_t pieces = l.vocab / Span<D>::kPer;
     int64_t parts = l.rows;
     if (l.vocab <= kShort) parts = launch_short<D, Op, false>(l, op, o, ws, nullptr, nullptr, st);
+    // Short rows leave most of a block idle between its barriers, long ones need many threads to be in
+    // flight; what is held beyond a row's length is computed for nothing.  Measured, PPO with gradient, us:
+    //   2048 x 65536 bf16:   64 threads x 4 pieces 178, 128 x 4 243, 256 x 8 477, 512 x 8 996
+    //   8192 x 16384 bf16:   64 x 8 133, 128 x 8 130, 256 x 8 163, 512 x 8 306
+    //   32000 x 8000 bf16:   64 x 8 285, 128 x 8 239, 256 x 8 218, 512 x 8 258
+    //   131072 x 2048 bf16:  64 x 8 338, 128 x 8 313, 256 x 8 284, 512 x 8 258, 1024 x 8 286
+    else if (pieces <= 64 * 4) launch_row<D, Op, 64, 4>(l, op, o, ws, st);
+    else if (pieces <= 64 * 8) launch_row<D, Op, 64, 8>(l, op, o, ws, st);
     else if (!o.grad) launch_row<D, Op, 256, 0>(l, op, o, ws, st);
-    else if (pieces <= 256 * 4) launch_row<D, Op, 256, 4>(l, op, o, ws, st);
-    else if (pieces <= 256 * 16) launch_row<D, Op, 256, 16>(l, op, o, ws, st);
-    else if (pieces <= 512 * 16) launch_row<D, Op, 512, 16>(l, op, o, ws, st);
-    else launch_row<D, Op, 1024, 16>(l, op, o, ws, st);
-    hipLaunchKernelGGL((k_cat_total<Op::terms>), dim3(1), dim3(1024), 0, st, ws, parts, o.loss, o.stats);
+    else if (pieces <= 128 * 8) launch_row<D, Op, 128, 8>(l, op, o, ws, st);
+    else if (pieces <= 256 * 16) launch_row<D, Op, 256, 8>(l, op, o, ws, st);
+    else launch_row<D, Op, 512, 8>(l, op, o, ws, st);
+    launch_total<Op::terms>(ws, parts, ws + l.rows * Op::terms, o, st);
     return launched();
 }
 
@@ -863,7 +948,7 @@ int run_backward(const Logits& l, const Op& op, const double* state, const float
     }
     // 256 threads, eight pieces each
     const int64_t parts = std::max<int64_t>(1, std::min<int64_t>(l.vocab / (2048 * Span<D>::kPer), INT32_MAX / l.rows));
-    hipLaunchKernelGGL((k_cat_backward<D, Op, 256>), dim3((unsigned)(l.rows * parts)), dim3(256), 0, st, l, op,
+    hipLaunchKernelGGL((k_cat_backward<D, Op, 256>), dim3((unsigned)(l.rows * parts)), dim3(256), teacher_bytes(op), st, l, op,
                        reinterpret_cast<const RowState*>(state), gout, grad, stride, (int32_t)parts);
     return launched();
 }
@@ -924,7 +1009,7 @@ extern "C" int rt_cat_ppo(const rt_cat_logits* logits, const rt_cat_ppo_batch* b
         if (const char* f = grad_fault(logits, out->grad, out->grad_stride)) return bad(me, f);
     if (const char* f = workspace_fault(logits, workspace_d, workspace_bytes)) return bad(me, f);
     const Logits l{logits->x, logits->rows, logits->row_stride, logits->vocab};
-    const Ppo op{*batch, hp->temperature, hp->clip_low, hp->clip_high, hp->ent_coef, hp->kl_coef};
+    const Ppo op{*batch, hp->temperature, 1.0 / hp->temperature, hp->clip_low, hp->clip_high, hp->ent_coef, hp->kl_coef};
     const Out o{out->loss, out->logprob, out->entropy, out->stats, nullptr, out->grad, out->grad_stride, out->row_state};
     return pick_loss(logits->dtype, l, op, o, static_cast<double*>(workspace_d), reinterpret_cast<hipStream_t>(stream));
 }
@@ -941,6 +1026,7 @@ extern "C" int rt_cat_ppo_backward(const rt_cat_logits* logits, const int64_t* a
     Ppo op{};
     op.b.actions = actions_d;
     op.t = temperature;
+    op.inv = 1.0 / op.t;
     return pick_backward(logits->dtype, l, op, row_state_d, grad_loss_d, grad_d, grad_stride,
                          reinterpret_cast<hipStream_t>(stream));
 }
@@ -956,7 +1042,7 @@ extern "C" int rt_cat_distill(const rt_cat_logits* logits, const rt_cat_teacher*
         if (const char* f = grad_fault(logits, out->grad, out->grad_stride)) return bad(me, f);
     if (const char* f = workspace_fault(logits, workspace_d, workspace_bytes)) return bad(me, f);
     const Logits l{logits->x, logits->rows, logits->row_stride, logits->vocab};
-    const Distill op{*teacher, teacher->temperature};
+    const Distill op{*teacher, teacher->temperature, 1.0 / teacher->temperature};
     const Out o{out->loss, nullptr, nullptr, nullptr, out->kl, out->grad, out->grad_stride, out->row_state};
     return pick_loss(logits->dtype, l, op, o, static_cast<double*>(workspace_d), reinterpret_cast<hipStream_t>(stream));
 }
@@ -970,6 +1056,6 @@ extern "C" int rt_cat_distill_backward(const rt_cat_logits* logits, const rt_cat
     if (!row_state_d || !grad_d) return bad(me, "NULL argument");
     if (const char* f = grad_fault(logits, grad_d, grad_stride)) return bad(me, f);
     const Logits l{logits->x, logits->rows, logits->row_stride, logits->vocab};
-    return pick_backward(logits->dtype, l, Distill{*teacher, teacher->temperature}, row_state_d, grad_loss_d, grad_d,
+    return pick_backward(logits->dtype, l, Distill{*teacher, teacher->temperature, 1.0 / teacher->temperature}, row_state_d, grad_loss_d, grad_d,
                          grad_stride, reinterpret_cast<hipStream_t>(stream));
 }

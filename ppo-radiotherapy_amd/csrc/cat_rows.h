@@ -21,17 +21,18 @@ struct F32 {
 struct BF16 {
     using raw = uint16_t;
     static __device__ __forceinline__ float get(raw r) { return __uint_as_float((uint32_t)r << 16); }
-    // round to nearest even, NaN kept a (quiet) NaN
-    static __device__ __forceinline__ raw put(float f) {
-        const uint32_t b = __float_as_uint(f);
-        if (f != f) return (raw)((b >> 16) | 0x40);
-        return (raw)((b + 0x7fff + ((b >> 16) & 1)) >> 16);
+    static __device__ __forceinline__ raw put(float f) { return __builtin_bit_cast(raw, (__bf16)f); }
+    static __device__ __forceinline__ uint32_t put2(float lo, float hi) {  // one instruction for both
+        typedef float f2 __attribute__((ext_vector_type(2)));
+        typedef __bf16 b2 __attribute__((ext_vector_type(2)));
+        return __builtin_bit_cast(uint32_t, __builtin_convertvector((f2{lo, hi}), b2));
     }
 };
 struct F16 {
     using raw = uint16_t;
     static __device__ __forceinline__ float get(raw r) { return (float)__builtin_bit_cast(_Float16, r); }
     static __device__ __forceinline__ raw put(float f) { return __builtin_bit_cast(raw, (_Float16)f); }
+    static __device__ __forceinline__ uint32_t put2(float lo, float hi) { return put(lo) | (uint32_t)put(hi) << 16; }
 };
 
 // ---- 2^t in 64 bits --------------------------------------------------------
@@ -53,6 +54,16 @@ __device__ __forceinline__ double exp2_64(double t) {
     p = fma(p, f, 0.6931471805599453);
     p = fma(p, f, 1.0);
     return ldexp(p, (int)n);
+}
+
+__device__ __forceinline__ double exp_64(double x) { return exp2_64(x * 1.4426950408889634); }
+
+// log s, s >= 1 or NaN: the hardware's log2 (within 2^-22), corrected by what
+// it leaves, d < 2^-20: log(1 + d) up to d^3 is exact to 2^-80.
+__device__ __forceinline__ double log_64(double s) {
+    const double y = (double)__builtin_amdgcn_logf((float)s);
+    const double d = s * exp2_64(-y) - 1.0;
+    return y * 0.6931471805599453 + d * (1.0 - d * (0.5 - d * 0.3333333333333333));
 }
 
 // Weights of a sampled row: 2^40 2^t as a whole number, t <= 0 (half to even,
@@ -78,17 +89,39 @@ __device__ __forceinline__ uint64_t whole_bits(double t) {  // kMagic + the weig
 }
 
 // ---- reductions ------------------------------------------------------------
+// A value from the lane that the DPP control names: within 16 lanes an exchange
+// costs one VALU move and no trip through LDS.
+template <int CTRL, class T>
+__device__ __forceinline__ T dpp(T v) {
+    constexpr int kWords = sizeof(T) / 4;
+    struct Words { int w[kWords]; } x = __builtin_bit_cast(Words, v);
+#pragma unroll
+    for (int i = 0; i < kWords; ++i) x.w[i] = __builtin_amdgcn_update_dpp(0, x.w[i], CTRL, 0xf, 0xf, true);
+    return __builtin_bit_cast(T, x);
+}
+// op over G lanes (a power of two), every lane gets the result: the two swaps
+// within four lanes, the mirrors of 8 and 16, then LDS permutes.
+template <int G, class T, class Op>
+__device__ __forceinline__ T lanes(T v, Op op) {
+    if constexpr (G >= 2) v = op(v, dpp<0xb1>(v));
+    if constexpr (G >= 4) v = op(v, dpp<0x4e>(v));
+    if constexpr (G >= 8) v = op(v, dpp<0x141>(v));
+    if constexpr (G >= 16) v = op(v, dpp<0x140>(v));
+    if constexpr (G >= 32) v = op(v, __shfl_xor(v, 16));
+    if constexpr (G >= 64) v = op(v, __shfl_xor(v, 32));
+    return v;
+}
+template <int G, class T>
+__device__ __forceinline__ T lanes_sum(T v) {
+    return lanes<G>(v, [](T a, T b) { return a + b; });
+}
+template <int G>
+__device__ __forceinline__ float lanes_max(float v) {  // NaN loses; the sums keep it
+    return lanes<G>(v, [](float a, float b) { return fmaxf(a, b); });
+}
 template <class T>
-__device__ __forceinline__ T wave_sum(T v) {
-#pragma unroll
-    for (int o = 32; o; o >>= 1) v += __shfl_xor(v, o);
-    return v;
-}
-__device__ __forceinline__ float wave_max(float v) {
-#pragma unroll
-    for (int o = 32; o; o >>= 1) v = fmaxf(v, __shfl_xor(v, o));  // NaN loses; the sums keep it
-    return v;
-}
+__device__ __forceinline__ T wave_sum(T v) { return lanes_sum<64>(v); }
+__device__ __forceinline__ float wave_max(float v) { return lanes_max<64>(v); }
 
 // Whole-block reductions through one LDS slot per wave; every thread gets the
 // result, and the slots may be used again at once.

@@ -373,6 +373,157 @@ struct Binner {
     __device__ __forceinline__ int operator()(float x) const { return (int)fminf((m - x) * scale, (float)(kBins - 1)); }
 };
 
+// What is known of a row when its maximum is.
+struct Head {
+    float m;
+    double c, theta;
+    Weigher weigh;
+    __device__ Head(const Ask& ask, float m)
+        : m(m), c(fmax(1.4426950408889634 / (double)ask.T, 1e-300)), theta(ask.least()), weigh{(double)m, c} {}
+    __device__ __forceinline__ bool likely(float x) const { return !((double)x - (double)m < theta); }  // min-p keeps it
+};
+
+// A row with top-k or top-p whose kept entries are too many for a list: the
+// cut from a histogram, by number or by weight, of the whole row; the entries
+// of the bin where it falls (top-k: up to there) are sorted.
+template <class D, int THREADS>
+__device__ void wide_row(const Args& A, int64_t n, const Ask& ask, const Head& h, Shared<THREADS>& s) {
+    if (ask.T > 1e30f) return slow_row<D, THREADS>(A, n, ask, h.m, s);
+    constexpr int kWaves = THREADS / 64;
+    const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
+    const int32_t V = A.vocab;
+    const Span<D> row(static_cast<const typename D::raw*>(A.x) + n * A.stride, V);
+    const Part<D> part(row, V, w, kWaves);
+    const Weigher weigh = h.weigh;
+    const Binner bin{h.m, (float)fmin(fmax(h.c * (kBins - 1) / 41.5, 1e-30), 3e38)};
+    uint64_t all = 0;
+    for (int i = tid; i < kBins; i += THREADS) s.hist[i] = 0;
+    __syncthreads();
+    walk(row, part, [&](float x, int32_t) {
+        const uint64_t v = weigh(x);
+        all += v;
+        if (v) atomicAdd(reinterpret_cast<unsigned long long*>(&s.hist[bin(x)]), (unsigned long long)(ask.K > 0 ? 1 : v));
+    });
+    all = block_sum<THREADS>(all, s.slots);
+
+    // Entries that weigh nothing are not in the histogram: they stand behind all others, and keeping them
+    // or not changes nothing.
+    uint64_t total = all, before, skipped;
+    if (ask.K > 0) {
+        total = 0;
+        for (int i = tid; i < kBins; i += THREADS) total += s.hist[i];
+        total = block_sum<THREADS>(total, s.slots);
+    }
+    const uint64_t want = ask.K > 0 ? min((uint64_t)ask.K, total) : ask.limit(all);
+    const int b = find_bin<THREADS, true>(s, want, &before);
+    if (tid == 0) s.many = 0;
+    __syncthreads();
+    walk(row, part, [&](float x, int32_t i) {
+        const int at = bin(x);
+        if ((at == b || (ask.K > 0 && at < b)) && weigh(x)) {
+            const int to = atomicAdd(&s.many, 1);
+            if (to < kList) s.list[to] = rank_of(x, i);
+        }
+    });
+    __syncthreads();
+    const int held = s.many;
+    if (held > kList) return slow_row<D, THREADS>(A, n, ask, h.m, s);
+    sort_list<THREADS>(s.list, held);
+    const auto value = [&](int i) { return weigh(of_key((uint32_t)(s.list[i] >> 32))); };
+    int keep;
+    if (ask.K > 0) {
+        uint64_t mass;
+        keep = (int)want;
+        scan_to<THREADS>(s, keep, value, UINT64_MAX, &mass);
+        if (ask.P < 1.0f) keep = min(keep, scan_to<THREADS>(s, keep, value, ask.limit(mass) - 1, &skipped) + 1);
+    } else {
+        keep = min(held, scan_to<THREADS>(s, held, value, want - before - 1, &skipped) + 1);
+    }
+    const uint64_t cut = s.list[keep - 1];  // the least rank that is kept
+    __syncthreads();
+    const auto kept = [&](float x, int32_t i) -> uint64_t {
+        return rank_of(x, i) < cut || !h.likely(x) ? 0 : weigh(x);
+    };
+    // the weight of what is kept, by waves: the first step of the search
+    uint64_t sum = 0, left = 0;
+    walk(row, part, [&](float x, int32_t i) { sum += kept(x, i); });
+    sum = wave_sum(sum);
+    if (lane == 0) s.slots[w] = sum;
+    __syncthreads();
+    for (int i = 0; i < kWaves; ++i) left += s.slots[i];
+    uint64_t target = ask.target(left);
+    int at = 0;
+    for (; at < kWaves - 1 && target >= s.slots[at]; ++at) target -= s.slots[at];
+    __syncthreads();
+    const Part<D> seg(row, V, at, kWaves);
+    const int32_t a = find_index<THREADS>(s, seg.first, seg.last - seg.first,
+                                          [&](int32_t i) { return kept(D::get(row.x[i]), i); }, target);
+    if (tid == 0) answer(A, n, a, ((double)D::get(row.x[a]) - (double)h.m) / (double)ask.T, all, left);
+}
+
+// The answer from a list of `held` entries that has all of the kept ones; false
+// where it has not (top-p needs more than the list weighs).
+template <int THREADS>
+__device__ bool from_list(const Args& A, int64_t n, const Ask& ask, const Head& h, int held, uint64_t all,
+                          Shared<THREADS>& s) {
+    sort_list<THREADS>(s.list, held);
+    uint64_t mass, skipped;
+    const auto high = [&](int i) { return of_key((uint32_t)(s.list[i] >> 32)); };
+    const auto value = [&](int i) { return h.weigh(high(i)); };
+    int keep = ask.K > 0 ? min(ask.K, held) : held;
+    scan_to<THREADS>(s, keep, value, UINT64_MAX, &mass);
+    if (ask.P < 1.0f) {
+        const uint64_t limit = ask.limit(ask.K > 0 ? mass : all);
+        if (limit > mass) return false;
+        // kept: those before which less than the limit lies
+        keep = min(keep, scan_to<THREADS>(s, keep, value, limit - 1, &skipped) + 1);
+    }
+    if (ask.Q > 0.0f)
+        keep = max(1, scan_to<THREADS>(s, keep, [&](int i) { return (uint64_t)!h.likely(high(i)); }, 0, &skipped));
+    scan_to<THREADS>(s, keep, value, UINT64_MAX, &mass);
+    // by index: a rank with its halves exchanged sorts that way
+    for (int i = threadIdx.x; i < keep; i += THREADS) s.list[i] = s.list[i] << 32 | s.list[i] >> 32;
+    __syncthreads();
+    sort_list<THREADS>(s.list, keep);
+    const int at = scan_to<THREADS>(s, keep, [&](int i) { return h.weigh(of_key((uint32_t)s.list[i])); }, ask.target(mass), &skipped);
+    if (threadIdx.x == 0) {
+        const uint64_t e = s.list[min(at, keep - 1)];
+        answer(A, n, (int32_t)~(uint32_t)(e >> 32), ((double)of_key((uint32_t)e) - (double)h.m) / (double)ask.T, all, mass);
+    }
+    return true;
+}
+
+// A value that surely has what is kept at or above it, if the kept are few: of
+// the maxima of `sets` disjoint parts of the row (as ranks, in s.list) the
+// K-th, since as many entries are not below it; without top-k the middle one.
+// 0: none.
+template <int THREADS>
+__device__ uint32_t floor_key(const Ask& ask, int sets, Shared<THREADS>& s) {
+    const int place = ask.K > 0 ? ask.K : sets / 2;
+    if (place > sets - sets / 4) return 0;  // the list would be too long
+    sort_list<THREADS>(s.list, sets);
+    const uint32_t key = (uint32_t)(s.list[place - 1] >> 32);
+    __syncthreads();
+    return key;
+}
+
+__device__ __forceinline__ void no_answer(const Args& A, int64_t n) {
+    A.action[n] = -1;
+    A.logprob[n] = A.kept[n] = NAN;
+}
+
+template <class D, int THREADS>
+__device__ void greedy(const Args& A, int64_t n, float m, int32_t lo, int32_t len, const Span<D>& row, Shared<THREADS>& s) {
+    const uint32_t top = key_of(m);
+    const int32_t a = find_index<THREADS>(s, lo, len, [&](int32_t i) { return (uint64_t)(key_of(D::get(row.x[i])) == top); }, 0);
+    if (threadIdx.x == 0) {
+        A.action[n] = a;
+        A.logprob[n] = A.kept[n] = 0.0f;
+    }
+}
+
+// One block per row, two passes over it: the maxima, then the weight of all
+// and a list of the entries that may be kept.
 template <class D, int THREADS>
 __global__ __launch_bounds__(THREADS) void k_cat_sample(Args A) {
     __shared__ Shared<THREADS> s;
@@ -382,7 +533,6 @@ __global__ __launch_bounds__(THREADS) void k_cat_sample(Args A) {
     const int32_t V = A.vocab;
     const Span<D> row(static_cast<const typename D::raw*>(A.x) + n * A.stride, V);
     const Part<D> part(row, V, w, kWaves);
-    const auto get = [&](int32_t i) { return D::get(row.x[i]); };
     const Ask ask(A.p, n, V);
 
     float m = -INFINITY;
@@ -391,118 +541,41 @@ __global__ __launch_bounds__(THREADS) void k_cat_sample(Args A) {
         m = fmaxf(m, x);
         odd |= !(x < INFINITY);
     });
+    s.list[tid] = (uint64_t)key_of(m) << 32;
     m = block_max<THREADS>(m, s.fslots);
-    odd = __syncthreads_or(odd);
-    if (odd || m == -INFINITY) {
-        if (tid == 0) {
-            A.action[n] = -1;
-            A.logprob[n] = A.kept[n] = NAN;
-        }
+    if (__syncthreads_or(odd) || m == -INFINITY) {
+        if (tid == 0) no_answer(A, n);
         return;
     }
-    if (!(ask.T > 0.0f)) {
-        const uint32_t top = key_of(m);
-        const int32_t a = find_index<THREADS>(s, 0, V, [&](int32_t i) { return (uint64_t)(key_of(get(i)) == top); }, 0);
-        if (tid == 0) {
-            A.action[n] = a;
-            A.logprob[n] = A.kept[n] = 0.0f;
-        }
-        return;
-    }
+    if (!(ask.T > 0.0f)) return greedy<D, THREADS>(A, n, m, 0, V, row, s);
+
+    const Head h(ask, m);
     const bool some = ask.K > 0 || ask.P < 1.0f;
-    if (some && ask.T > 1e30f) return slow_row<D, THREADS>(A, n, ask, m, s);
-
-    const double c = fmax(1.4426950408889634 / (double)ask.T, 1e-300), theta = ask.least();
-    const Weigher weigh{(double)m, c};
-    const Binner bin{m, (float)fmin(fmax(c * (kBins - 1) / 41.5, 1e-30), 3e38)};
-    // the weight of all, and what is needed to find the cut: how many entries, or how much weight, each bin has
-    uint64_t sum = 0;
+    const uint32_t least = !some ? 0 : V <= kList ? 1 : floor_key<THREADS>(ask, THREADS, s);
+    if (some && !least) return wide_row<D, THREADS>(A, n, ask, h, s);
+    if (tid == 0) s.many = 0;
+    __syncthreads();
+    uint64_t all = 0, sum = 0;
     if (some) {
-        for (int i = tid; i < kBins; i += THREADS) s.hist[i] = 0;
-        __syncthreads();
-        const bool count = ask.K > 0;
-        walk(row, part, [&](float x, int32_t) {
-            const uint64_t v = weigh(x), add = count ? 1 : v;
-            sum += v;
-            if (v) atomicAdd(reinterpret_cast<unsigned long long*>(&s.hist[bin(x)]), (unsigned long long)add);
-        });
-    } else {
-        walk(row, part, [&](float x, int32_t) { sum += weigh(x); });
-    }
-    sum = wave_sum(sum);
-    if (lane == 0) s.slots[w] = sum;
-    __syncthreads();
-    uint64_t all = 0;
-    for (int i = 0; i < kWaves; ++i) all += s.slots[i];
-    __syncthreads();
-
-    // Entries that weigh nothing are not in the histogram: they stand behind all others, and keeping them
-    // or not changes nothing.
-    uint64_t cut = 0;  // least rank that is kept
-    bool done = !some;
-    if (ask.K > 0) {
-        uint64_t total = 0;
-        for (int i = tid; i < kBins; i += THREADS) total += s.hist[i];
-        total = block_sum<THREADS>(total, s.slots);
-        const uint64_t want = min((uint64_t)ask.K, total);
-        uint64_t before;
-        const int b = find_bin<THREADS, true>(s, want, &before);
-        const uint64_t many = before + s.hist[b];
-        if (many > kList) return slow_row<D, THREADS>(A, n, ask, m, s);
-        // the first `many` of the order, sorted: all that is left is in the list
-        if (tid == 0) s.many = 0;
-        __syncthreads();
+        const float floor = least > 1 ? of_key(least) : -INFINITY;
         walk(row, part, [&](float x, int32_t i) {
-            if (bin(x) <= b && weigh(x)) {
-                const int at = atomicAdd(&s.many, 1);
-                if (at < kList) s.list[at] = rank_of(x, i);  // always: there are `many`
-            }
-        });
-        __syncthreads();
-        sort_list<THREADS>(s.list, (int)many);
-        const auto value = [&](int i) { return weigh(of_key((uint32_t)(s.list[i] >> 32))); };
-        int keep = (int)want;
-        uint64_t left, skipped;
-        scan_to<THREADS>(s, keep, value, UINT64_MAX, &left);
-        if (ask.P < 1.0f) {
-            // kept: those before which less than the limit lies
-            const int at = scan_to<THREADS>(s, keep, value, ask.limit(left) - 1, &skipped);
-            keep = min(keep, at + 1);
-        }
-        cut = s.list[keep - 1];
-        done = false;
-    } else if (ask.P < 1.0f) {
-        const uint64_t want = ask.limit(all);
-        uint64_t before, skipped;
-        const int b = find_bin<THREADS, true>(s, want, &before);
-        if (tid == 0) s.many = 0;
-        __syncthreads();
-        walk(row, part, [&](float x, int32_t i) {
-            if (bin(x) == b && weigh(x)) {
+            all += h.weigh(x);
+            if (x >= floor) {
                 const int at = atomicAdd(&s.many, 1);
                 if (at < kList) s.list[at] = rank_of(x, i);
             }
         });
-        __syncthreads();
-        const int held = s.many;
-        if (held > kList) return slow_row<D, THREADS>(A, n, ask, m, s);
-        sort_list<THREADS>(s.list, held);
-        const int at = scan_to<THREADS>(
-            s, held, [&](int i) { return weigh(of_key((uint32_t)(s.list[i] >> 32))); }, want - before - 1, &skipped);
-        cut = s.list[min(at, held - 1)];
-        done = false;
+        all = block_sum<THREADS>(all, s.slots);
+        if (s.many > kList || !from_list<THREADS>(A, n, ask, h, s.many, all, s)) wide_row<D, THREADS>(A, n, ask, h, s);
+        return;
     }
-    __syncthreads();
-    const auto kept = [&](float x, int32_t i) -> uint64_t {
-        if (rank_of(x, i) < cut || (double)x - (double)m < theta) return 0;
-        return weigh(x);
-    };
-    // the weight of what is kept, by waves: the first step of the search
-    if (!done || ask.Q > 0.0f) {
-        sum = 0;
-        walk(row, part, [&](float x, int32_t i) { sum += kept(x, i); });
-        sum = wave_sum(sum);
-    }
+    walk(row, part, [&](float x, int32_t) {
+        const uint64_t v = h.weigh(x);
+        all += v;
+        sum += h.likely(x) ? v : 0;
+    });
+    all = block_sum<THREADS>(all, s.slots);
+    sum = wave_sum(sum);
     if (lane == 0) s.slots[w] = sum;
     __syncthreads();
     uint64_t left = 0;
@@ -512,9 +585,14 @@ __global__ __launch_bounds__(THREADS) void k_cat_sample(Args A) {
     for (; at < kWaves - 1 && target >= s.slots[at]; ++at) target -= s.slots[at];
     __syncthreads();
     const Part<D> seg(row, V, at, kWaves);
-    const int32_t a = find_index<THREADS>(s, seg.first, seg.last - seg.first,
-                                          [&](int32_t i) { return kept(get(i), i); }, target);
-    if (tid == 0) answer(A, n, a, ((double)get(a) - (double)m) / (double)ask.T, all, left);
+    const int32_t a = find_index<THREADS>(
+        s, seg.first, seg.last - seg.first,
+        [&](int32_t i) {
+            const float x = D::get(row.x[i]);
+            return h.likely(x) ? h.weigh(x) : 0;
+        },
+        target);
+    if (tid == 0) answer(A, n, a, ((double)D::get(row.x[a]) - (double)m) / (double)ask.T, all, left);
 }
 
 // ---- short rows ------------------------------------------------------------
@@ -595,13 +673,9 @@ __global__ __launch_bounds__(64) void k_cat_sample_tiny(Args A, int64_t rows) {
     const uint64_t target = ask.target(left);
     uint64_t run = 0;
     int32_t a = 0;
-    for (int i = V - 1; i >= 0; --i) {  // from the end: the last that passes is the first that exceeds
-        if (!(keep >> i & 1)) continue;
-        run += wt[i];
-        if (left - run <= target) {
-            a = i;
-            break;
-        }
+    for (; a < V - 1; ++a) {
+        if (keep >> a & 1) run += wt[a];
+        if (run > target) break;
     }
     answer(A, n, a, ((double)x[a] - (double)m) / (double)ask.T, all, left);
 }
