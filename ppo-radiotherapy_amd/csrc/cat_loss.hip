@@ -401,7 +401,7 @@ __device__ __forceinline__ RowState ppo_row(const Ppo& op, const Out& o, int64_t
 }
 
 __device__ __forceinline__ RowState distill_row(const Distill& op, const Out& o, int64_t n, int64_t rows, float m, double S,
-                                                const Teacher& te, double lse, double Q, double* term) {
+                                                const Teacher& te, double lse, double Q, bool write, double* term) {
     const int lane = threadIdx.x & 63;
     const double logs = log_64(S), inv = op.inv;
     double kl = 0.0;
@@ -411,10 +411,33 @@ __device__ __forceinline__ RowState distill_row(const Distill& op, const Out& o,
     }
     kl = wave_sum(kl);
     const double w = op.weight(n, rows);
-    if (lane == 0) o.kl[n] = (float)kl;
+    if (write) o.kl[n] = (float)kl;
     term[0] = w * kl;
     // E is 0 throughout: its place keeps the teacher's normaliser for the backward pass
     return RowState{m, logs, lse, w * Q * inv, w * inv};
+}
+
+template <class Op>
+__device__ __forceinline__ RowState finish_row(const Op& op, const Out& o, int64_t n, int64_t rows, bool skip, float m,
+                                               const Sums& sums, float xa, const Teacher& te, double lse, double Q,
+                                               bool write, double* terms) {
+    const int tid = threadIdx.x;
+    RowState st{0.0, INFINITY, 0.0, 0.0, 0.0};  // log S +inf: a row that adds nothing
+    double term[Op::terms] = {};
+    write = write && tid == 0;
+    if constexpr (Op::ppo) {
+        if (!skip) st = ppo_row(op, o, n, rows, m, sums.s, sums.u, xa, write, term);
+        else if (write) o.logprob[n] = o.entropy[n] = 0.0f;
+    } else {
+        if (!skip) st = distill_row(op, o, n, rows, m, sums.s, te, lse, Q, write, term);
+        else if (write) o.kl[n] = 0.0f;
+    }
+    if (write) {
+#pragma unroll
+        for (int k = 0; k < Op::terms; ++k) terms[n * Op::terms + k] = term[k];
+        if (o.state) *reinterpret_cast<RowState*>(o.state + n * RT_CAT_ROW_STATE) = st;
+    }
+    return st;
 }
 
 template <class Op>
@@ -426,10 +449,11 @@ __device__ __forceinline__ Slope op_slope(const Op& op, RowState s, double scale
 // The gradient at the teacher's entries, in the place of their logits: the
 // dense part and all that names the same entry, in the entries' order.
 template <int THREADS>
-__device__ __forceinline__ void named_slopes(const Teacher& te, int32_t k, const Slope& sl, float each) {
+__device__ __forceinline__ void named_slopes(const Teacher& te, int32_t k, int32_t first, int32_t last, const Slope& sl,
+                                             float each) {
     for (int j = threadIdx.x; j < k; j += THREADS) {
         const int32_t at = te.idx[j];
-        if (at < 0) continue;
+        if (at < first || at >= last) continue;
         double q = 0.0;
         for (int i = 0; i < k; ++i) q += te.idx[i] == at ? te.q[i] : 0.0;
         te.v[j] = slope_at<false>(sl, te.v[j]) - each * (float)q;
@@ -461,21 +485,8 @@ __global__ __launch_bounds__(THREADS) void k_cat_row(Logits l, Op op, Out o, dou
         skip = m == -INFINITY && sums.s == 0.0;
     }
     if (tid < 64) {
-        RowState st{0.0, INFINITY, 0.0, 0.0, 0.0};  // log S +inf: a row that adds nothing
-        double term[Op::terms] = {};
-        if constexpr (Op::ppo) {
-            if (!skip) st = ppo_row(op, o, n, l.rows, m, sums.s, sums.u, xa, tid == 0, term);
-            else if (tid == 0) o.logprob[n] = o.entropy[n] = 0.0f;
-        } else {
-            if (!skip) st = distill_row(op, o, n, l.rows, m, sums.s, te, lse, Q, term);
-            else if (tid == 0) o.kl[n] = 0.0f;
-        }
-        if (tid == 0) {
-#pragma unroll
-            for (int k = 0; k < Op::terms; ++k) terms[n * Op::terms + k] = term[k];
-            if (o.state) *reinterpret_cast<RowState*>(o.state + n * RT_CAT_ROW_STATE) = st;
-            slots.state = st;
-        }
+        const RowState st = finish_row(op, o, n, l.rows, skip, m, sums, xa, te, lse, Q, true, terms);
+        if (tid == 0) slots.state = st;
     }
     if (!o.grad) return;
     auto* g = static_cast<typename D::raw*>(o.grad) + n * o.grad_stride;
@@ -485,7 +496,7 @@ __global__ __launch_bounds__(THREADS) void k_cat_row(Logits l, Op op, Out o, dou
     const RowState st = slots.state;
     const Slope sl = op_slope(op, st, 1.0);
     if constexpr (!Op::ppo) {
-        if (!skip) named_slopes<THREADS>(te, op.b.k, sl, (float)st.c);
+        if (!skip) named_slopes<THREADS>(te, op.b.k, 0, l.vocab, sl, (float)st.c);
         __syncthreads();
     }
     // the gradient may lie in the logits' own memory: from here on only what is not held is read, each
@@ -511,25 +522,95 @@ __global__ __launch_bounds__(THREADS) void k_cat_row(Logits l, Op op, Out o, dou
     }
 }
 
-// ---- a row's gradient from its state, by parts -----------------------------
-template <class D, class Op, int THREADS>
-__global__ __launch_bounds__(THREADS) void k_cat_backward(Logits l, Op op, const RowState* state, const float* gout,
-                                                          void* grad, int64_t grad_stride, int32_t parts) {
-    Teacher te(teacher_lds, Op::ppo ? 0 : op.k());
+// ---- a row by parts --------------------------------------------------------
+// Few long rows leave most of the card idle at one block each, so several have
+// a part of a row: its sums first, then, each block from all parts' sums, the
+// part's gradient.  The backward pass is the second step alone, from the state.
+struct PartSums {
+    double m;
+    Sums sums;
+};
+
+struct Piece {  // [from, to) of the pieces, [first, last) of the entries
+    int32_t from, to, first, last;
+    template <class D>
+    __device__ Piece(const Span<D>& row, int32_t V, int32_t part, int32_t parts) {
+        const int32_t per = (row.pieces + parts - 1) / parts;
+        from = min(part * per, row.pieces);
+        to = min(from + per, row.pieces);
+        // the first part also has the entries before the pieces, the last those behind
+        first = part == 0 ? 0 : row.head + from * Span<D>::kPer;
+        last = part == parts - 1 ? V : row.head + to * Span<D>::kPer;
+    }
+};
+
+template <class D, class Op>
+__global__ __launch_bounds__(256) void k_cat_part(Logits l, Op op, PartSums* to, int32_t parts) {
+    __shared__ Slots<256> slots;
     const int64_t n = blockIdx.x / parts;
     const int32_t part = blockIdx.x % parts;
+    const Span<D> row(row_of<D>(l, n), l.vocab);
+    if (op.ignored(n, l.vocab)) return;
+    const Piece p(row, l.vocab, part, parts);
+    uint4 held[2];
+    float m;
+    Sums sums;
+    row_sums<D, 256, 2, Op::ppo>(row, p.from, p.to, part == 0, scale_of(op.inv), held, slots, &m, &sums);
+    if (threadIdx.x == 0) to[blockIdx.x] = PartSums{m, sums};
+}
+
+// By one wave: the sums of a row from those of its parts (at most 64).
+template <bool U>
+__device__ __forceinline__ Sums join(const PartSums* from, int32_t parts, float c, float* m) {
+    const int lane = threadIdx.x & 63;
+    PartSums p{-INFINITY, Sums{0.0, 0.0}};
+    if (lane < parts) p = from[lane];
+    *m = wave_max((float)p.m);
+    // a part of nothing but -inf has sums 0 or NaN, which stay
+    if (p.m > -INFINITY) move_to<U>(p.sums, (p.m - (double)*m) * (double)c);
+    p.sums.s = wave_sum(p.sums.s);
+    if (U) p.sums.u = wave_sum(p.sums.u);
+    return p.sums;
+}
+
+template <class D, class Op, bool JOIN>
+__global__ __launch_bounds__(256) void k_cat_grad(Logits l, Op op, Out o, const PartSums* from, double* terms,
+                                                  const RowState* state, const float* gout, int32_t parts) {
+    constexpr int kThreads = 256;
+    __shared__ RowState share;
+    Teacher te(teacher_lds, Op::ppo ? 0 : op.k());
+    const int32_t blocks = JOIN && !o.grad ? 1 : parts;  // of a row
+    const int64_t n = blockIdx.x / blocks;
+    const int32_t part = blockIdx.x % blocks;
     const int tid = threadIdx.x;
     const auto* x = row_of<D>(l, n);
-    auto* g = static_cast<typename D::raw*>(grad) + n * grad_stride;
     const Span<D> row(x, l.vocab);
-    const RowState st = state[n];
+    const Piece p(row, l.vocab, part, parts);
+    RowState st;
+    if constexpr (JOIN) {
+        if (tid < 64) {
+            bool skip = op.ignored(n, l.vocab);
+            float m = -INFINITY, xa = 0.0f;
+            double lse = 0.0, Q = 0.0;
+            Sums sums{0.0, 0.0};
+            if (!skip) {
+                if constexpr (Op::ppo) xa = D::get(x[op.b.actions[n]]);
+                else Q = teacher_load<D>(op, n, l.vocab, x, te, &lse);
+                sums = join<Op::ppo>(from + n * parts, parts, scale_of(op.inv), &m);
+                skip = m == -INFINITY && sums.s == 0.0;
+            }
+            st = finish_row(op, o, n, l.rows, skip, m, sums, xa, te, lse, Q, part == 0, terms);
+            if (tid == 0) share = st;
+        }
+        if (!o.grad) return;
+        __syncthreads();
+        st = share;
+    } else {
+        st = state[n];
+    }
     const bool skip = st.logs == INFINITY;
+    auto* g = static_cast<typename D::raw*>(o.grad) + n * o.grad_stride;
     const double scale = gout ? (double)*gout : 1.0;
-    const int32_t per = (row.pieces + parts - 1) / parts;
-    const int32_t from = min(part * per, row.pieces), to = min(from + per, row.pieces);
-    // the first part also has the entries before the pieces, the last those behind
-    const int32_t first = part == 0 ? 0 : row.head + from * Span<D>::kPer;
-    const int32_t last = part == parts - 1 ? l.vocab : row.head + to * Span<D>::kPer;
     const Slope sl = op_slope(op, st, scale);
     const float each = (float)(scale * st.c);
     int64_t a = -1;
@@ -537,35 +618,37 @@ __global__ __launch_bounds__(THREADS) void k_cat_backward(Logits l, Op op, const
     if constexpr (Op::ppo) {
         if (!skip && tid == 0) {
             a = op.b.actions[n];
-            if (a >= first && a < last) va = slope_at<true>(sl, D::get(x[a])) + each;
+            if (a >= p.first && a < p.last) va = slope_at<true>(sl, D::get(x[a])) + each;
             else a = -1;
         }
     } else if (!skip) {
-        for (int j = tid; j < op.b.k; j += THREADS) {
-            const int64_t i = op.b.idx[n * op.b.k + j];
-            const bool in = i >= first && i < last;
-            te.idx[j] = in ? (int32_t)i : -1;
-            te.q[j] = in ? exp_64((double)op.b.logits[n * op.b.k + j] * op.inv - st.e) : 0.0;
-            te.v[j] = in ? D::get(x[i]) : 0.0f;
+        if constexpr (!JOIN) {
+            for (int j = tid; j < op.b.k; j += kThreads) {
+                const int64_t i = op.b.idx[n * op.b.k + j];
+                const bool in = i >= p.first && i < p.last;
+                te.idx[j] = in ? (int32_t)i : -1;
+                te.q[j] = in ? exp_64((double)op.b.logits[n * op.b.k + j] * op.inv - st.e) : 0.0;
+                te.v[j] = in ? D::get(x[i]) : 0.0f;
+            }
+            __syncthreads();
         }
-        __syncthreads();
-        named_slopes<THREADS>(te, op.b.k, sl, each);
+        named_slopes<kThreads>(te, op.b.k, p.first, p.last, sl, each);
     }
     const int mode = store_mode(g, x, l.rows * l.vocab * (int64_t)sizeof(typename D::raw));
     const int32_t e = tid < row.edges ? row.edge(tid) : -1;
-    const bool mine = e >= first && e < last;
+    const bool mine = e >= p.first && e < p.last;
     float xe = 0.0f;
     if (mine) xe = D::get(x[e]);
     __syncthreads();
-    put_pieces<D, Op::ppo, THREADS>(g, row, from, to, mode, sl, skip);
+    put_pieces<D, Op::ppo, kThreads>(g, row, p.from, p.to, mode, sl, skip);
     if (mine) g[e] = D::put(skip ? 0.0f : slope_at<Op::ppo>(sl, xe));
     if (skip) return;
     __syncthreads();
     if constexpr (Op::ppo) {
         if (a >= 0) g[a] = D::put(va);
     } else {
-        for (int j = tid; j < op.b.k; j += THREADS)
-            if (te.idx[j] >= 0) g[te.idx[j]] = D::put(te.v[j]);
+        for (int j = tid; j < op.b.k; j += kThreads)
+            if (te.idx[j] >= p.first && te.idx[j] < p.last) g[te.idx[j]] = D::put(te.v[j]);
     }
 }
 
@@ -908,11 +991,30 @@ void launch_row(const Logits& l, const Op& op, const Out& o, double* ws, hipStre
                        op, o, ws);
 }
 
+// How many blocks share a row: as many as bring the card 1024 blocks, with two
+// pieces for every thread.
+constexpr int kMostParts = 64;
+int64_t parts_of(int64_t rows, int32_t vocab, int32_t per) {
+    return std::max<int64_t>(1, std::min({1024 / rows, (int64_t)(vocab / per / 512), (int64_t)kMostParts}));
+}
+
+template <class D, class Op>
+void launch_parts(const Logits& l, const Op& op, const Out& o, double* ws, int64_t parts, hipStream_t st) {
+    PartSums* sums = reinterpret_cast<PartSums*>(ws + terms_bytes(l.rows) / sizeof(double));
+    const unsigned all = (unsigned)(l.rows * parts);
+    hipLaunchKernelGGL((k_cat_part<D, Op>), dim3(all), dim3(256), 0, st, l, op, sums, (int32_t)parts);
+    hipLaunchKernelGGL((k_cat_grad<D, Op, true>), dim3(o.grad ? all : (unsigned)l.rows), dim3(256), teacher_bytes(op), st, l,
+                       op, o, sums, ws, nullptr, nullptr, (int32_t)parts);
+}
+
 template <class D, class Op>
 int run_loss(const Logits& l, const Op& op, const Out& o, double* ws, hipStream_t st) {
     const int32_t pieces = l.vocab / Span<D>::kPer;
     int64_t parts = l.rows;
     if (l.vocab <= kShort) parts = launch_short<D, Op, false>(l, op, o, ws, nullptr, nullptr, st);
+    // (not where the gradient takes the logits' place: a block reads entries of other blocks' parts)
+    else if (const int64_t many = parts_of(l.rows, l.vocab, Span<D>::kPer); many > 1 && o.grad != l.x)
+        launch_parts<D>(l, op, o, ws, many, st);
     // Short rows leave most of a block idle between its barriers, long ones need many threads to be in
     // flight; what is held beyond a row's length is computed for nothing.  Measured, PPO with gradient, us:
     //   2048 x 65536 bf16:   64 threads x 4 pieces 178, 128 x 4 243, 256 x 8 477, 512 x 8 996
@@ -946,10 +1048,14 @@ int run_backward(const Logits& l, const Op& op, const double* state, const float
         launch_short<D, Op, true>(l, op, o, nullptr, reinterpret_cast<const RowState*>(state), gout, st);
         return launched();
     }
-    // 256 threads, eight pieces each
-    const int64_t parts = std::max<int64_t>(1, std::min<int64_t>(l.vocab / (2048 * Span<D>::kPer), INT32_MAX / l.rows));
-    hipLaunchKernelGGL((k_cat_backward<D, Op, 256>), dim3((unsigned)(l.rows * parts)), dim3(256), teacher_bytes(op), st, l, op,
-                       reinterpret_cast<const RowState*>(state), gout, grad, stride, (int32_t)parts);
+    // 256 threads, eight pieces each, fewer where there are few rows
+    const int64_t parts = std::max(parts_of(l.rows, l.vocab, Span<D>::kPer),
+                                   std::max<int64_t>(1, std::min<int64_t>(l.vocab / (2048 * Span<D>::kPer), INT32_MAX / l.rows)));
+    Out o{};
+    o.grad = grad;
+    o.grad_stride = stride;
+    hipLaunchKernelGGL((k_cat_grad<D, Op, false>), dim3((unsigned)(l.rows * parts)), dim3(256), teacher_bytes(op), st, l, op,
+                       o, nullptr, nullptr, reinterpret_cast<const RowState*>(state), gout, (int32_t)parts);
     return launched();
 }
 
@@ -992,7 +1098,8 @@ const char* workspace_fault(const rt_cat_logits* l, const void* ws, int64_t byte
 
 extern "C" int64_t rt_cat_loss_workspace_bytes(int64_t rows, int32_t vocab, int32_t dtype) {
     if (rows < 1 || rows > INT32_MAX || vocab < 1 || vocab > RT_CAT_MAX_VOCAB || bad_type(dtype)) return -1;
-    return terms_bytes(rows);
+    const int64_t parts = parts_of(rows, vocab, 16 / elem_size(dtype));
+    return terms_bytes(rows) + (parts > 1 ? rows * parts * (int64_t)sizeof(PartSums) : 0);
 }
 
 extern "C" int rt_cat_ppo(const rt_cat_logits* logits, const rt_cat_ppo_batch* batch, const rt_cat_ppo_hparams* hp,
