@@ -12,6 +12,7 @@
 // digit by digit from a histogram of the entries (top-k) or of their weights
 // (top-p) in LDS; then the running weight by index is searched segment by
 // segment.
+#include <algorithm>
 #include <string>
 
 #include "cat_rows.h"
@@ -346,17 +347,17 @@ struct Part {
 template <class D, class F>
 __device__ __forceinline__ void walk(const Span<D>& row, const Part<D>& p, F f) {
     const int lane = threadIdx.x & 63;
-    constexpr int kPer = Span<D>::kPer, kBatch = 4;
+    constexpr int kPer = Span<D>::kPer, kAhead = 4;
     const int32_t a = row.head + p.from * kPer, b = row.head + p.to * kPer;
     if (p.first + lane < a) f(D::get(row.x[p.first + lane]), p.first + lane);
     if (b + lane < p.last) f(D::get(row.x[b + lane]), b + lane);
-    for (int32_t i = p.from + lane; i < p.to; i += 64 * kBatch) {
-        uint4 r[kBatch];
+    for (int32_t i = p.from + lane; i < p.to; i += 64 * kAhead) {
+        uint4 r[kAhead];
 #pragma unroll
-        for (int k = 0; k < kBatch; ++k)
+        for (int k = 0; k < kAhead; ++k)
             if (i + 64 * k < p.to) r[k] = row.piece(i + 64 * k);
 #pragma unroll
-        for (int k = 0; k < kBatch; ++k) {
+        for (int k = 0; k < kAhead; ++k) {
             if (i + 64 * k >= p.to) break;
             const Unpack<D> x(r[k]);
 #pragma unroll
@@ -373,6 +374,8 @@ struct Binner {
     __device__ __forceinline__ int operator()(float x) const { return (int)fminf((m - x) * scale, (float)(kBins - 1)); }
 };
 
+constexpr float kMostT = 1e30f;  // above, numbers that the bins cannot tell apart weigh something
+
 // What is known of a row when its maximum is.
 struct Head {
     float m;
@@ -381,103 +384,20 @@ struct Head {
     __device__ Head(const Ask& ask, float m)
         : m(m), c(fmax(1.4426950408889634 / (double)ask.T, 1e-300)), theta(ask.least()), weigh{(double)m, c} {}
     __device__ __forceinline__ bool likely(float x) const { return !((double)x - (double)m < theta); }  // min-p keeps it
+    __device__ Binner binner() const { return Binner{m, (float)fmin(fmax(c * (kBins - 1) / 41.5, 1e-30), 3e38)}; }
 };
 
-// A row with top-k or top-p whose kept entries are too many for a list: the
-// cut from a histogram, by number or by weight, of the whole row; the entries
-// of the bin where it falls (top-k: up to there) are sorted.
-template <class D, int THREADS>
-__device__ void wide_row(const Args& A, int64_t n, const Ask& ask, const Head& h, Shared<THREADS>& s) {
-    if (ask.T > 1e30f) return slow_row<D, THREADS>(A, n, ask, h.m, s);
-    constexpr int kWaves = THREADS / 64;
-    const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
-    const int32_t V = A.vocab;
-    const Span<D> row(static_cast<const typename D::raw*>(A.x) + n * A.stride, V);
-    const Part<D> part(row, V, w, kWaves);
-    const Weigher weigh = h.weigh;
-    const Binner bin{h.m, (float)fmin(fmax(h.c * (kBins - 1) / 41.5, 1e-30), 3e38)};
-    uint64_t all = 0;
-    for (int i = tid; i < kBins; i += THREADS) s.hist[i] = 0;
-    __syncthreads();
-    walk(row, part, [&](float x, int32_t) {
-        const uint64_t v = weigh(x);
-        all += v;
-        if (v) atomicAdd(reinterpret_cast<unsigned long long*>(&s.hist[bin(x)]), (unsigned long long)(ask.K > 0 ? 1 : v));
-    });
-    all = block_sum<THREADS>(all, s.slots);
-
-    // Entries that weigh nothing are not in the histogram: they stand behind all others, and keeping them
-    // or not changes nothing.
-    uint64_t total = all, before, skipped;
-    if (ask.K > 0) {
-        total = 0;
-        for (int i = tid; i < kBins; i += THREADS) total += s.hist[i];
-        total = block_sum<THREADS>(total, s.slots);
-    }
-    const uint64_t want = ask.K > 0 ? min((uint64_t)ask.K, total) : ask.limit(all);
-    const int b = find_bin<THREADS, true>(s, want, &before);
-    if (tid == 0) s.many = 0;
-    __syncthreads();
-    walk(row, part, [&](float x, int32_t i) {
-        const int at = bin(x);
-        if ((at == b || (ask.K > 0 && at < b)) && weigh(x)) {
-            const int to = atomicAdd(&s.many, 1);
-            if (to < kList) s.list[to] = rank_of(x, i);
-        }
-    });
-    __syncthreads();
-    const int held = s.many;
-    if (held > kList) return slow_row<D, THREADS>(A, n, ask, h.m, s);
-    sort_list<THREADS>(s.list, held);
-    const auto value = [&](int i) { return weigh(of_key((uint32_t)(s.list[i] >> 32))); };
-    int keep;
-    if (ask.K > 0) {
-        uint64_t mass;
-        keep = (int)want;
-        scan_to<THREADS>(s, keep, value, UINT64_MAX, &mass);
-        if (ask.P < 1.0f) keep = min(keep, scan_to<THREADS>(s, keep, value, ask.limit(mass) - 1, &skipped) + 1);
-    } else {
-        keep = min(held, scan_to<THREADS>(s, held, value, want - before - 1, &skipped) + 1);
-    }
-    const uint64_t cut = s.list[keep - 1];  // the least rank that is kept
-    __syncthreads();
-    const auto kept = [&](float x, int32_t i) -> uint64_t {
-        return rank_of(x, i) < cut || !h.likely(x) ? 0 : weigh(x);
-    };
-    // the weight of what is kept, by waves: the first step of the search
-    uint64_t sum = 0, left = 0;
-    walk(row, part, [&](float x, int32_t i) { sum += kept(x, i); });
-    sum = wave_sum(sum);
-    if (lane == 0) s.slots[w] = sum;
-    __syncthreads();
-    for (int i = 0; i < kWaves; ++i) left += s.slots[i];
-    uint64_t target = ask.target(left);
-    int at = 0;
-    for (; at < kWaves - 1 && target >= s.slots[at]; ++at) target -= s.slots[at];
-    __syncthreads();
-    const Part<D> seg(row, V, at, kWaves);
-    const int32_t a = find_index<THREADS>(s, seg.first, seg.last - seg.first,
-                                          [&](int32_t i) { return kept(D::get(row.x[i]), i); }, target);
-    if (tid == 0) answer(A, n, a, ((double)D::get(row.x[a]) - (double)h.m) / (double)ask.T, all, left);
-}
-
-// The answer from a list of `held` entries that has all of the kept ones; false
-// where it has not (top-p needs more than the list weighs).
+// The answer from a list that has all that top-k keeps, and more.
 template <int THREADS>
-__device__ bool from_list(const Args& A, int64_t n, const Ask& ask, const Head& h, int held, uint64_t all,
-                          Shared<THREADS>& s) {
+__device__ void from_list(const Args& A, int64_t n, const Ask& ask, const Head& h, int held, Shared<THREADS>& s, uint64_t all) {
     sort_list<THREADS>(s.list, held);
     uint64_t mass, skipped;
     const auto high = [&](int i) { return of_key((uint32_t)(s.list[i] >> 32)); };
     const auto value = [&](int i) { return h.weigh(high(i)); };
-    int keep = ask.K > 0 ? min(ask.K, held) : held;
+    int keep = min(ask.K, held);
     scan_to<THREADS>(s, keep, value, UINT64_MAX, &mass);
-    if (ask.P < 1.0f) {
-        const uint64_t limit = ask.limit(ask.K > 0 ? mass : all);
-        if (limit > mass) return false;
-        // kept: those before which less than the limit lies
-        keep = min(keep, scan_to<THREADS>(s, keep, value, limit - 1, &skipped) + 1);
-    }
+    // kept by top-p: those before which less than the limit lies
+    if (ask.P < 1.0f) keep = min(keep, scan_to<THREADS>(s, keep, value, ask.limit(mass) - 1, &skipped) + 1);
     if (ask.Q > 0.0f)
         keep = max(1, scan_to<THREADS>(s, keep, [&](int i) { return (uint64_t)!h.likely(high(i)); }, 0, &skipped));
     scan_to<THREADS>(s, keep, value, UINT64_MAX, &mass);
@@ -490,21 +410,6 @@ __device__ bool from_list(const Args& A, int64_t n, const Ask& ask, const Head& 
         const uint64_t e = s.list[min(at, keep - 1)];
         answer(A, n, (int32_t)~(uint32_t)(e >> 32), ((double)of_key((uint32_t)e) - (double)h.m) / (double)ask.T, all, mass);
     }
-    return true;
-}
-
-// A value that surely has what is kept at or above it, if the kept are few: of
-// the maxima of `sets` disjoint parts of the row (as ranks, in s.list) the
-// K-th, since as many entries are not below it; without top-k the middle one.
-// 0: none.
-template <int THREADS>
-__device__ uint32_t floor_key(const Ask& ask, int sets, Shared<THREADS>& s) {
-    const int place = ask.K > 0 ? ask.K : sets / 2;
-    if (place > sets - sets / 4) return 0;  // the list would be too long
-    sort_list<THREADS>(s.list, sets);
-    const uint32_t key = (uint32_t)(s.list[place - 1] >> 32);
-    __syncthreads();
-    return key;
 }
 
 __device__ __forceinline__ void no_answer(const Args& A, int64_t n) {
@@ -522,77 +427,238 @@ __device__ void greedy(const Args& A, int64_t n, float m, int32_t lo, int32_t le
     }
 }
 
-// One block per row, two passes over it: the maxima, then the weight of all
-// and a list of the entries that may be kept.
-template <class D, int THREADS>
-__global__ __launch_bounds__(THREADS) void k_cat_sample(Args A) {
-    __shared__ Shared<THREADS> s;
-    constexpr int kWaves = THREADS / 64;
-    const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
-    const int64_t n = blockIdx.x;
-    const int32_t V = A.vocab;
-    const Span<D> row(static_cast<const typename D::raw*>(A.x) + n * A.stride, V);
-    const Part<D> part(row, V, w, kWaves);
-    const Ask ask(A.p, n, V);
+// ---- long rows, by parts ---------------------------------------------------
+// Up to 64 blocks share a row, one launch for each thing that all of it has to
+// be known for: the maximum; the weights, and a histogram of them where there
+// is a cut to find; the entries around the cut; the answer, by one block.
+constexpr int kParts = 64, kPartWaves = 4;
 
+struct RowSpace {
+    float top[kParts];                          // NaN: a NaN or +inf
+    uint64_t all[kParts * kPartWaves];          // the weight of each wave's part
+    uint64_t kept[kParts * kPartWaves];         // what of it is surely kept
+    uint64_t hist[kBins];
+    uint64_t list[kList];
+    int32_t many, pad[15];
+};
+
+struct Batch {
+    Args a;
+    RowSpace* space;  // of row `first`
+    int64_t first;
+    int32_t parts;
+};
+
+// The maximum of the row from those of its parts; NaN for a row without an answer.
+__device__ __forceinline__ float row_top(const RowSpace& r, int32_t parts) {
+    const int lane = threadIdx.x & 63;
+    const float v = lane < parts ? r.top[lane] : -INFINITY;
+    const float m = wave_max(v);
+    return __any(v != v) || m == -INFINITY ? NAN : m;
+}
+
+__device__ __forceinline__ bool cuts(const Ask& ask) { return ask.K > 0 || ask.P < 1.0f; }
+
+// Bin and sum before it where the cut falls, from the histogram in LDS.
+template <int THREADS>
+__device__ __forceinline__ int find_cut(const Ask& ask, uint64_t all, Shared<THREADS>& s, uint64_t* want, uint64_t* before) {
+    uint64_t total = all;
+    if (ask.K > 0) {
+        total = 0;
+        for (int i = threadIdx.x; i < kBins; i += THREADS) total += s.hist[i];
+        total = block_sum<THREADS>(total, s.slots);
+    }
+    // entries that weigh nothing are not in the histogram: they stand behind all others, and keeping
+    // them or not changes nothing
+    *want = ask.K > 0 ? min((uint64_t)ask.K, total) : ask.limit(all);
+    return find_bin<THREADS, true>(s, *want, before);
+}
+
+template <class D>
+__global__ __launch_bounds__(256) void k_cat_sample_top(Batch b) {
+    __shared__ float fs[4];
+    const int64_t r = blockIdx.x / b.parts, n = b.first + r;
+    const int32_t p = blockIdx.x % b.parts, V = b.a.vocab;
+    const int w = threadIdx.x >> 6;
+    const Span<D> row(static_cast<const typename D::raw*>(b.a.x) + n * b.a.stride, V);
+    const Part<D> part(row, V, p * kPartWaves + w, b.parts * kPartWaves);
+    RowSpace& to = b.space[r];
     float m = -INFINITY;
     int odd = 0;
     walk(row, part, [&](float x, int32_t) {
         m = fmaxf(m, x);
         odd |= !(x < INFINITY);
     });
-    s.list[tid] = (uint64_t)key_of(m) << 32;
-    m = block_max<THREADS>(m, s.fslots);
-    if (__syncthreads_or(odd) || m == -INFINITY) {
-        if (tid == 0) no_answer(A, n);
-        return;
+    m = block_max<256>(m, fs);
+    odd = __syncthreads_or(odd);
+    for (int i = p * 256 + threadIdx.x; i < kBins; i += b.parts * 256) to.hist[i] = 0;
+    if (threadIdx.x == 0) {
+        to.top[p] = odd ? NAN : m;
+        if (p == 0) to.many = 0;
     }
-    if (!(ask.T > 0.0f)) return greedy<D, THREADS>(A, n, m, 0, V, row, s);
+}
 
+template <class D>
+__global__ __launch_bounds__(256) void k_cat_sample_weigh(Batch b) {
+    __shared__ uint64_t hist[kBins];
+    const int64_t r = blockIdx.x / b.parts, n = b.first + r;
+    const int32_t p = blockIdx.x % b.parts, V = b.a.vocab;
+    const int tid = threadIdx.x, w = tid >> 6, seg = p * kPartWaves + w;
+    const Span<D> row(static_cast<const typename D::raw*>(b.a.x) + n * b.a.stride, V);
+    const Part<D> part(row, V, seg, b.parts * kPartWaves);
+    RowSpace& to = b.space[r];
+    const float m = row_top(to, b.parts);
+    const Ask ask(b.a.p, n, V);
+    if (m != m || !(ask.T > 0.0f)) return;
     const Head h(ask, m);
-    const bool some = ask.K > 0 || ask.P < 1.0f;
-    const uint32_t least = !some ? 0 : V <= kList ? 1 : floor_key<THREADS>(ask, THREADS, s);
-    if (some && !least) return wide_row<D, THREADS>(A, n, ask, h, s);
+    uint64_t all = 0, kept = 0;
+    if (cuts(ask)) {
+        const Binner bin = h.binner();
+        const bool count = ask.K > 0;
+        for (int i = tid; i < kBins; i += 256) hist[i] = 0;
+        __syncthreads();
+        walk(row, part, [&](float x, int32_t) {
+            const uint64_t v = h.weigh(x);
+            all += v;
+            if (v) atomicAdd(reinterpret_cast<unsigned long long*>(&hist[bin(x)]), (unsigned long long)(count ? 1 : v));
+        });
+        __syncthreads();
+        for (int i = tid; i < kBins; i += 256)
+            if (hist[i]) atomicAdd(reinterpret_cast<unsigned long long*>(&to.hist[i]), (unsigned long long)hist[i]);
+    } else {
+        walk(row, part, [&](float x, int32_t) {
+            const uint64_t v = h.weigh(x);
+            all += v;
+            kept += h.likely(x) ? v : 0;
+        });
+    }
+    all = wave_sum(all);
+    kept = wave_sum(kept);
+    if ((tid & 63) == 0) {
+        to.all[seg] = all;
+        to.kept[seg] = kept;
+    }
+}
+
+// Sum of n <= 256 numbers, by the whole block.
+template <int THREADS>
+__device__ __forceinline__ uint64_t sum_of(const uint64_t* v, int n, Shared<THREADS>& s) {
+    return block_sum<THREADS>((int)threadIdx.x < n ? v[threadIdx.x] : 0, s.slots);
+}
+
+template <class D>
+__global__ __launch_bounds__(256) void k_cat_sample_near(Batch b) {
+    __shared__ Shared<256> s;
+    const int64_t r = blockIdx.x / b.parts, n = b.first + r;
+    const int32_t p = blockIdx.x % b.parts, V = b.a.vocab;
+    const int tid = threadIdx.x, w = tid >> 6, seg = p * kPartWaves + w;
+    const Span<D> row(static_cast<const typename D::raw*>(b.a.x) + n * b.a.stride, V);
+    const Part<D> part(row, V, seg, b.parts * kPartWaves);
+    RowSpace& to = b.space[r];
+    const float m = row_top(to, b.parts);
+    const Ask ask(b.a.p, n, V);
+    if (m != m || !(ask.T > 0.0f) || !cuts(ask) || ask.T > kMostT) return;
+    const Head h(ask, m);
+    const Binner bin = h.binner();
+    for (int i = tid; i < kBins; i += 256) s.hist[i] = to.hist[i];
+    const uint64_t all = sum_of<256>(to.all, b.parts * kPartWaves, s);
+    uint64_t want, before, kept = 0;
+    const int at = find_cut<256>(ask, all, s, &want, &before);
+    if (ask.K > 0 && before + s.hist[at] > kList) return;
     if (tid == 0) s.many = 0;
     __syncthreads();
-    uint64_t all = 0, sum = 0;
-    if (some) {
-        const float floor = least > 1 ? of_key(least) : -INFINITY;
-        walk(row, part, [&](float x, int32_t i) {
-            all += h.weigh(x);
-            if (x >= floor) {
-                const int at = atomicAdd(&s.many, 1);
-                if (at < kList) s.list[at] = rank_of(x, i);
-            }
-        });
-        all = block_sum<THREADS>(all, s.slots);
-        if (s.many > kList || !from_list<THREADS>(A, n, ask, h, s.many, all, s)) wide_row<D, THREADS>(A, n, ask, h, s);
+    // top-k: all up to the bin of the cut; top-p: that bin, and the weight of those before it
+    walk(row, part, [&](float x, int32_t i) {
+        const int v = bin(x);
+        if (v > at) return;
+        if (v < at && ask.K <= 0) {
+            kept += h.likely(x) ? h.weigh(x) : 0;
+        } else if (h.weigh(x)) {
+            const int o = atomicAdd(&s.many, 1);
+            if (o < kList) s.list[o] = rank_of(x, i);
+        }
+    });
+    kept = wave_sum(kept);
+    if ((tid & 63) == 0) to.kept[seg] = kept;
+    __syncthreads();
+    const int many = min(s.many, kList);
+    if (tid == 0) s.where = atomicAdd(&to.many, s.many);
+    __syncthreads();
+    for (int i = tid; i < many; i += 256)
+        if (s.where + i < kList) to.list[s.where + i] = s.list[i];
+}
+
+// Which wave's part has an entry.
+template <class D>
+__device__ __forceinline__ int part_of(const Span<D>& row, int waves, int32_t i) {
+    const int32_t per = (row.pieces + waves - 1) / waves, piece = (i - row.head) / Span<D>::kPer;
+    return i < row.head ? 0 : piece >= row.pieces ? waves - 1 : piece / per;
+}
+
+template <class D>
+__global__ __launch_bounds__(1024) void k_cat_sample_answer(Batch b) {
+    constexpr int kThreads = 1024;
+    __shared__ Shared<kThreads> s;
+    __shared__ uint64_t segs[kParts * kPartWaves];
+    const int64_t n = b.first + blockIdx.x;
+    const int32_t V = b.a.vocab, waves = b.parts * kPartWaves;
+    const int tid = threadIdx.x;
+    const Span<D> row(static_cast<const typename D::raw*>(b.a.x) + n * b.a.stride, V);
+    const RowSpace& r = b.space[blockIdx.x];
+    const float m = row_top(r, b.parts);
+    if (m != m) {
+        if (tid == 0) no_answer(b.a, n);
         return;
     }
-    walk(row, part, [&](float x, int32_t) {
-        const uint64_t v = h.weigh(x);
-        all += v;
-        sum += h.likely(x) ? v : 0;
-    });
-    all = block_sum<THREADS>(all, s.slots);
-    sum = wave_sum(sum);
-    if (lane == 0) s.slots[w] = sum;
+    const Ask ask(b.a.p, n, V);
+    if (!(ask.T > 0.0f)) {
+        int p = 0;
+        while (r.top[p] != m) ++p;
+        const int32_t from = Part<D>(row, V, p * kPartWaves, waves).first;
+        const int32_t to = Part<D>(row, V, (p + 1) * kPartWaves - 1, waves).last;
+        return greedy<D, kThreads>(b.a, n, m, from, to - from, row, s);
+    }
+    const Head h(ask, m);
+    uint64_t cut = 0;  // the least rank that is kept
+    const uint64_t all = sum_of<kThreads>(r.all, waves, s);
+    for (int i = tid; i < waves; i += kThreads) segs[i] = r.kept[i];
+    if (cuts(ask)) {
+        if (ask.T > kMostT) return slow_row<D, kThreads>(b.a, n, ask, m, s);
+        for (int i = tid; i < kBins; i += kThreads) s.hist[i] = r.hist[i];
+        __syncthreads();
+        uint64_t want, before, skipped;
+        const int at = find_cut<kThreads>(ask, all, s, &want, &before);
+        const int many = r.many;
+        if ((ask.K > 0 && before + s.hist[at] > kList) || many > kList) return slow_row<D, kThreads>(b.a, n, ask, m, s);
+        for (int i = tid; i < many; i += kThreads) s.list[i] = r.list[i];
+        __syncthreads();
+        if (ask.K > 0) return from_list<kThreads>(b.a, n, ask, h, many, s, all);
+        sort_list<kThreads>(s.list, many);
+        const int last = scan_to<kThreads>(
+            s, many, [&](int i) { return h.weigh(of_key((uint32_t)(s.list[i] >> 32))); }, want - before - 1, &skipped);
+        cut = s.list[min(last, many - 1)];
+        for (int i = tid; i < many; i += kThreads) {
+            const uint64_t e = s.list[i];
+            const float x = of_key((uint32_t)(e >> 32));
+            if (e >= cut && h.likely(x))
+                atomicAdd(reinterpret_cast<unsigned long long*>(&segs[part_of(row, waves, (int32_t)~(uint32_t)e)]),
+                          (unsigned long long)h.weigh(x));
+        }
+    }
     __syncthreads();
-    uint64_t left = 0;
-    for (int i = 0; i < kWaves; ++i) left += s.slots[i];
+    const uint64_t left = sum_of<kThreads>(segs, waves, s);
     uint64_t target = ask.target(left);
     int at = 0;
-    for (; at < kWaves - 1 && target >= s.slots[at]; ++at) target -= s.slots[at];
-    __syncthreads();
-    const Part<D> seg(row, V, at, kWaves);
-    const int32_t a = find_index<THREADS>(
+    for (; at < waves - 1 && target >= segs[at]; ++at) target -= segs[at];
+    const Part<D> seg(row, V, at, waves);
+    const int32_t a = find_index<kThreads>(
         s, seg.first, seg.last - seg.first,
         [&](int32_t i) {
             const float x = D::get(row.x[i]);
-            return h.likely(x) ? h.weigh(x) : 0;
+            return rank_of(x, i) < cut || !h.likely(x) ? 0 : h.weigh(x);
         },
         target);
-    if (tid == 0) answer(A, n, a, ((double)D::get(row.x[a]) - (double)m) / (double)ask.T, all, left);
+    if (tid == 0) answer(b.a, n, a, ((double)D::get(row.x[a]) - (double)m) / (double)ask.T, all, left);
 }
 
 // ---- short rows ------------------------------------------------------------
@@ -680,14 +746,276 @@ __global__ __launch_bounds__(64) void k_cat_sample_tiny(Args A, int64_t rows) {
     answer(A, n, a, ((double)x[a] - (double)m) / (double)ask.T, all, left);
 }
 
+// ---- rows that are held ----------------------------------------------------
+// Up to 9216 entries: a team of one to sixteen waves has the row in registers.
+// Thread t has the entries [t per, (t + 1) per), so the order by index is that
+// of the threads; the row passes through LDS on its way there (per is odd: no
+// bank conflicts).  The cut is found between two keys, by halving their
+// distance and by the largest key that is left below the upper: a dozen steps
+// of E compares and a sum over the team.
+template <int THREADS>
+struct Team {
+    static constexpr int kWaves = THREADS / 64;
+    struct Slots { uint64_t v[2][kWaves]; };
+    Slots& s;
+    int turn;  // two sets in turn: one barrier for each exchange
+
+    __device__ explicit Team(Slots& s) : s(s), turn(0) {}
+    // v from every wave, combined
+    template <class T, class Op>
+    __device__ __forceinline__ T all(T v, Op op) {
+        v = lanes<64>(v, op);
+        if constexpr (kWaves > 1) {
+            uint64_t* slot = s.v[turn];
+            turn ^= 1;
+            if ((threadIdx.x & 63) == 0) slot[threadIdx.x >> 6] = (uint64_t)v;
+            __syncthreads();
+            v = (T)slot[0];
+#pragma unroll
+            for (int i = 1; i < kWaves; ++i) v = op(v, (T)slot[i]);
+        }
+        return v;
+    }
+    template <class T>
+    __device__ __forceinline__ T sum(T v) {
+        return all(v, [](T a, T b) { return a + b; });
+    }
+    __device__ __forceinline__ uint32_t top(uint32_t v) {
+        return all(v, [](uint32_t a, uint32_t b) { return max(a, b); });
+    }
+    // the sum of the threads before this one; `total` of all
+    __device__ __forceinline__ uint64_t before(uint64_t v, uint64_t* total) {
+        const int lane = threadIdx.x & 63;
+        uint64_t run = v;
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) {
+            const uint64_t q = __shfl_up(run, o);
+            if (lane >= o) run += q;
+        }
+        uint64_t all = __shfl(run, 63), at = run - v;
+        if constexpr (kWaves > 1) {
+            uint64_t* slot = s.v[turn];
+            turn ^= 1;
+            if (lane == 0) slot[threadIdx.x >> 6] = all;
+            __syncthreads();
+            all = 0;
+#pragma unroll
+            for (int i = 0; i < kWaves; ++i) {
+                if (i < (int)(threadIdx.x >> 6)) at += slot[i];
+                all += slot[i];
+            }
+        }
+        *total = all;
+        return at;
+    }
+};
+
+// The key at which the sum of value(e) over falling keys reaches `want` (1 <=
+// want <= the sum of all), and the sum above it.  S: the type of the sums.
+template <int E, class S, class T, class Value>
+__device__ __forceinline__ uint32_t held_key(T& team, const float (&x)[E], uint32_t least, uint32_t top, Value value, S want,
+                                             S* above) {
+    uint32_t lo = least, hi = top + 1;  // the sum of keys >= lo reaches `want`, that of keys >= hi does not
+    S over = 0;
+    const auto from = [&](uint32_t k) {
+        S s = 0;
+#pragma unroll
+        for (int e = 0; e < E; ++e) s += key_of(x[e]) >= k ? value(e) : (S)0;
+        return team.sum(s);
+    };
+    while (true) {
+        uint32_t k = 0;
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+            const uint32_t q = key_of(x[e]);
+            k = q < hi ? max(k, q) : k;
+        }
+        k = team.top(k);
+        S s = from(k);
+        if (s >= want) {
+            *above = over;
+            return k;
+        }
+        hi = k;
+        over = s;
+        // half way between the numbers (the numbers around 0 have most of the keys), or between the keys
+        uint32_t mid = key_of(0.5f * of_key(lo) + 0.5f * of_key(hi));
+        if (!(mid > lo && mid < hi)) mid = lo + (hi - lo) / 2;
+        s = from(mid);
+        if (s >= want) {
+            lo = mid;
+        } else {
+            hi = mid;
+            over = s;
+        }
+    }
+}
+
+template <class D, int THREADS, int E>
+__global__ __launch_bounds__(THREADS < 256 ? 256 : THREADS) void k_cat_sample_held(Args A, int64_t rows) {
+    constexpr int kRows = THREADS == 64 ? 4 : 1;  // of a block
+    extern __shared__ __align__(16) float staged[];
+    __shared__ typename Team<THREADS>::Slots slots;
+    Team<THREADS> team(slots);
+    const int t = threadIdx.x % THREADS;
+    const int64_t n = (int64_t)blockIdx.x * kRows + threadIdx.x / THREADS;
+    const int32_t V = A.vocab, per = ((V + THREADS - 1) / THREADS) | 1;
+    const bool in = n < rows;
+    float* mine = staged + threadIdx.x / THREADS * per * THREADS;
+    if (in) {
+        const auto* row = static_cast<const typename D::raw*>(A.x) + n * A.stride;
+#pragma unroll
+        for (int e = 0; e < E; ++e)
+            if (t + THREADS * e < V) mine[t + THREADS * e] = D::get(row[t + THREADS * e]);
+    }
+    __syncthreads();
+    if (!in) return;  // only of a block whose waves have a row each
+    float x[E];
+    uint32_t top = 0;
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+        const bool here = e < per && t * per + e < V;
+        x[e] = here ? mine[t * per + e] : -INFINITY;
+        top = max(top, x[e] < INFINITY ? key_of(x[e]) : UINT32_MAX);
+    }
+    top = team.top(top);
+    const float m = of_key(top);
+    if (top == UINT32_MAX || m == -INFINITY) {  // a NaN or +inf, or nothing
+        if (t == 0) no_answer(A, n);
+        return;
+    }
+    const Ask ask(A.p, n, V);
+    uint64_t total;
+    if (!(ask.T > 0.0f)) {
+        int32_t first = -1;
+#pragma unroll
+        for (int e = E - 1; e >= 0; --e) first = key_of(x[e]) == top ? t * per + e : first;
+        if (team.before(first >= 0, &total) == 0 && first >= 0) {
+            A.action[n] = first;
+            A.logprob[n] = A.kept[n] = 0.0f;
+        }
+        return;
+    }
+    const Head h(ask, m);
+    uint64_t wt[E], all = 0;
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+        wt[e] = h.weigh(x[e]);  // 0 where there is no entry
+        all += wt[e];
+        if (e & 1) __builtin_amdgcn_sched_barrier(0);  // two chains at a time: more only need registers
+    }
+    all = team.sum(all);
+    // What is not kept loses its weight.  Of the entries equal to the cut, and not lost yet, the first
+    // `ties` by index stay.
+    const auto drop = [&](uint32_t cut, uint64_t ties) {
+        uint32_t many = 0;
+#pragma unroll
+        for (int e = 0; e < E; ++e) many += key_of(x[e]) == cut && wt[e];
+        uint64_t at = team.before(many, &total);
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+            const uint32_t k = key_of(x[e]);
+            const bool tie = k == cut && wt[e];
+            if (k < cut || (tie && at >= ties)) wt[e] = 0;
+            at += tie;
+        }
+    };
+    uint64_t mass = all;
+    // no key below this has weight: 2^(40 - 41.5) < 1/2, and 2^-20 of the distance covers the rounding
+    const uint32_t least = key_of((float)((double)m - 41.5 * (1 + 0x1p-20) / h.c) - fabsf(m) * 0x1p-20f);
+    int32_t many = 0;
+    if (ask.K > 0) {
+#pragma unroll
+        for (int e = 0; e < E; ++e) many += wt[e] != 0;
+        many = team.sum(many);
+    }
+    if (ask.K > 0 && ask.K < many) {  // else top-k drops nothing that weighs
+        int32_t above;
+        const uint32_t cut = held_key<E, int32_t>(team, x, least, top, [&](int e) { return (int32_t)(wt[e] != 0); }, ask.K, &above);
+        drop(cut, (uint64_t)(ask.K - above));
+        mass = 0;
+#pragma unroll
+        for (int e = 0; e < E; ++e) mass += wt[e];
+        mass = team.sum(mass);
+    }
+    if (ask.P < 1.0f) {
+        uint64_t above;
+        const uint64_t want = ask.limit(mass);
+        const uint32_t cut = held_key<E, uint64_t>(team, x, least, top, [&](int e) { return wt[e]; }, want, &above);
+        const uint64_t each = h.weigh(of_key(cut));
+        drop(cut, (want - above + each - 1) / each);
+    }
+    uint64_t sum = 0, left;
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+        if (!h.likely(x[e])) wt[e] = 0;
+        sum += wt[e];
+    }
+    uint64_t at = team.before(sum, &left);
+    const uint64_t target = ask.target(left);
+    if (at <= target && target < at + sum) {
+        float xa = 0.0f;
+        int32_t a = -1;
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+            if (at <= target && target < at + wt[e]) {
+                a = t * per + e;
+                xa = x[e];
+            }
+            at += wt[e];
+        }
+        answer(A, n, a, ((double)xa - (double)m) / (double)ask.T, all, left);
+    }
+}
+
+constexpr int kHeld = 9216;
+
 template <class D>
-int run_sample(const Args& a, int64_t rows, hipStream_t st) {
-    if (a.vocab <= kTiny)
+void launch_held(const Args& a, int64_t rows, hipStream_t st) {
+    const auto go = [&](auto kernel, int threads) {
+        const int per = ((a.vocab + threads - 1) / threads) | 1, many = threads == 64 ? 4 : 1;
+        hipLaunchKernelGGL(kernel, dim3((unsigned)((rows + many - 1) / many)), dim3(threads * many),
+                           (size_t)per * threads * many * sizeof(float), st, a, rows);
+    };
+    const int32_t V = a.vocab;
+    if (V <= 64) go(k_cat_sample_held<D, 64, 1>, 64);
+    else if (V <= 64 * 3) go(k_cat_sample_held<D, 64, 3>, 64);
+    else if (V <= 64 * 5) go(k_cat_sample_held<D, 64, 5>, 64);
+    else if (V <= 64 * 9) go(k_cat_sample_held<D, 64, 9>, 64);
+    else if (V <= 256 * 5) go(k_cat_sample_held<D, 256, 5>, 256);
+    else if (V <= 256 * 9) go(k_cat_sample_held<D, 256, 9>, 256);
+    else if (V <= 512 * 9) go(k_cat_sample_held<D, 512, 9>, 512);
+    else go(k_cat_sample_held<D, 1024, 9>, 1024);
+}
+
+// Rows of one round: what their histograms and lists take is bounded, and they
+// fill the card.
+constexpr int64_t kBatch = 512;
+
+int64_t batch_of(int64_t rows) { return std::min(rows, kBatch); }
+
+template <class D>
+int run_sample(const Args& a, int64_t rows, void* space, hipStream_t st) {
+    if (a.vocab <= kTiny) {
         hipLaunchKernelGGL(k_cat_sample_tiny<D>, dim3((unsigned)((rows + 63) / 64)), dim3(64), 0, st, a, rows);
-    else if (a.vocab > 4096)
-        hipLaunchKernelGGL((k_cat_sample<D, 1024>), dim3((unsigned)rows), dim3(1024), 0, st, a);
-    else
-        hipLaunchKernelGGL((k_cat_sample<D, 256>), dim3((unsigned)rows), dim3(256), 0, st, a);
+        return launched();
+    }
+    if (a.vocab <= kHeld) {
+        launch_held<D>(a, rows, st);
+        return launched();
+    }
+    const bool cut = a.p.top_k || a.p.top_k_all > 0 || a.p.top_p || a.p.top_p_all < 1.0f;
+    const int64_t many = batch_of(rows), pieces = a.vocab / Span<D>::kPer;
+    // 2048 blocks of 256 threads, two pieces each at least
+    const int32_t parts = (int32_t)std::min<int64_t>({std::max<int64_t>(2048 / many, 1), pieces / 512, kParts});
+    for (int64_t first = 0; first < rows; first += many) {
+        const Batch b{a, static_cast<RowSpace*>(space), first, parts};
+        const unsigned here = (unsigned)std::min(many, rows - first), blocks = here * parts;
+        hipLaunchKernelGGL(k_cat_sample_top<D>, dim3(blocks), dim3(256), 0, st, b);
+        hipLaunchKernelGGL(k_cat_sample_weigh<D>, dim3(blocks), dim3(256), 0, st, b);
+        if (cut) hipLaunchKernelGGL(k_cat_sample_near<D>, dim3(blocks), dim3(256), 0, st, b);
+        hipLaunchKernelGGL(k_cat_sample_answer<D>, dim3(here), dim3(1024), 0, st, b);
+    }
     return launched();
 }
 
@@ -697,7 +1025,7 @@ int bad(const char* what) { return rt_internal_fail(RT_EINVAL, (std::string("rt_
 
 extern "C" int64_t rt_cat_sample_workspace_bytes(int64_t rows, int32_t vocab, int32_t dtype) {
     if (rows < 1 || rows > INT32_MAX || vocab < 1 || vocab > RT_CAT_MAX_VOCAB || bad_type(dtype)) return -1;
-    return 0;
+    return vocab <= kHeld ? 0 : batch_of(rows) * (int64_t)sizeof(RowSpace);
 }
 
 extern "C" int rt_cat_sample(const rt_cat_logits* logits, const rt_cat_sampling* params, int64_t* action_d,
@@ -711,7 +1039,7 @@ extern "C" int rt_cat_sample(const rt_cat_logits* logits, const rt_cat_sampling*
         return bad("workspace NULL, not 16-B aligned or too small");
     const Args a{logits->x, logits->row_stride, logits->vocab, *params, action_d, logprob_d, kept_logprob_d};
     const hipStream_t st = reinterpret_cast<hipStream_t>(stream);
-    if (logits->dtype == RT_DT_F32) return run_sample<F32>(a, logits->rows, st);
-    if (logits->dtype == RT_DT_BF16) return run_sample<BF16>(a, logits->rows, st);
-    return run_sample<F16>(a, logits->rows, st);
+    if (logits->dtype == RT_DT_F32) return run_sample<F32>(a, logits->rows, workspace_d, st);
+    if (logits->dtype == RT_DT_BF16) return run_sample<BF16>(a, logits->rows, workspace_d, st);
+    return run_sample<F16>(a, logits->rows, workspace_d, st);
 }
