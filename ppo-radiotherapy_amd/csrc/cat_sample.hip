@@ -49,12 +49,11 @@ struct Weigher {
 
 template <int THREADS>
 struct Shared {
-    uint64_t hist[kBins];  // also the list's second half of a sort by index
-    uint64_t list[kList];
+    uint64_t hist[kBins];
     uint64_t slots[THREADS / 64];
     float fslots[THREADS / 64];
     uint64_t found[2];
-    int32_t where, many;
+    int32_t where;
 };
 
 // The bin in which a running sum, from the highest bin down or (UP) from the
@@ -261,74 +260,6 @@ __device__ void slow_row(const Args& A, int64_t n, const Ask& ask, float m, Shar
 // An entry's place in the order, larger first: key, then index from below.
 __device__ __forceinline__ uint64_t rank_of(float x, int32_t i) { return (uint64_t)key_of(x) << 32 | (uint32_t)~i; }
 
-// Sorts list[0, n), n <= kList, largest first; what lies behind it is filled
-// with 0.  Returns after a barrier.
-template <int THREADS>
-__device__ void sort_list(uint64_t* list, int n) {
-    int size = 2;
-    while (size < n) size <<= 1;
-    for (int i = n + threadIdx.x; i < size; i += THREADS) list[i] = 0;
-    __syncthreads();
-    for (int k = 2; k <= size; k <<= 1) {
-        for (int j = k >> 1; j; j >>= 1) {
-            for (int p = threadIdx.x; p < size / 2; p += THREADS) {
-                const int i = 2 * p - (p & (j - 1)), o = i + j;
-                const uint64_t a = list[i], b = list[o];
-                if ((a < b) == ((i & k) == 0)) {
-                    list[i] = b;
-                    list[o] = a;
-                }
-            }
-            __syncthreads();
-        }
-    }
-}
-
-// Where the running sum of value(i), i < n <= kList, first exceeds `target`,
-// n if it never does; and the sum before that place.
-template <int THREADS, class Value>
-__device__ int scan_to(Shared<THREADS>& s, int n, Value value, uint64_t target, uint64_t* before) {
-    constexpr int kPer = kList / THREADS;
-    const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
-    uint64_t v[kPer], mine = 0;
-#pragma unroll
-    for (int i = 0; i < kPer; ++i) {
-        v[i] = tid * kPer + i < n ? value(tid * kPer + i) : 0;
-        mine += v[i];
-    }
-    uint64_t run = mine;
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-        const uint64_t q = __shfl_up(run, o);
-        if (lane >= o) run += q;
-    }
-    if (lane == 63) s.slots[w] = run;
-    if (tid == 0) s.where = n;
-    __syncthreads();
-    uint64_t at = run - mine, total = 0;
-    for (int i = 0; i < THREADS / 64; ++i) {
-        if (i < w) at += s.slots[i];
-        total += s.slots[i];
-    }
-    if (tid == 0) s.found[0] = total;
-    __syncthreads();
-    if (at <= target && target < at + mine) {
-#pragma unroll
-        for (int i = 0; i < kPer; ++i) {
-            if (at <= target && target < at + v[i]) {
-                s.where = tid * kPer + i;
-                s.found[0] = at;
-            }
-            at += v[i];
-        }
-    }
-    __syncthreads();
-    const int r = s.where;
-    *before = s.found[0];
-    __syncthreads();
-    return r;
-}
-
 // A wave's part of a row, in the order of the index: whole pieces, the first
 // wave also what lies before them, the last what lies behind.
 template <class D>
@@ -370,8 +301,8 @@ __device__ __forceinline__ void walk(const Span<D>& row, const Part<D>& p, F f) 
 // nothing (2^(40 - 41.5) < 1/2).  Each step of the arithmetic keeps the order,
 // so a bin's entries come before those of the next.
 struct Binner {
-    float m, scale;
-    __device__ __forceinline__ int operator()(float x) const { return (int)fminf((m - x) * scale, (float)(kBins - 1)); }
+    float m, scale, last;
+    __device__ __forceinline__ int operator()(float x) const { return (int)fminf((m - x) * scale, last); }
 };
 
 constexpr float kMostT = 1e30f;  // above, numbers that the bins cannot tell apart weigh something
@@ -384,33 +315,10 @@ struct Head {
     __device__ Head(const Ask& ask, float m)
         : m(m), c(fmax(1.4426950408889634 / (double)ask.T, 1e-300)), theta(ask.least()), weigh{(double)m, c} {}
     __device__ __forceinline__ bool likely(float x) const { return !((double)x - (double)m < theta); }  // min-p keeps it
-    __device__ Binner binner() const { return Binner{m, (float)fmin(fmax(c * (kBins - 1) / 41.5, 1e-30), 3e38)}; }
-};
-
-// The answer from a list that has all that top-k keeps, and more.
-template <int THREADS>
-__device__ void from_list(const Args& A, int64_t n, const Ask& ask, const Head& h, int held, Shared<THREADS>& s, uint64_t all) {
-    sort_list<THREADS>(s.list, held);
-    uint64_t mass, skipped;
-    const auto high = [&](int i) { return of_key((uint32_t)(s.list[i] >> 32)); };
-    const auto value = [&](int i) { return h.weigh(high(i)); };
-    int keep = min(ask.K, held);
-    scan_to<THREADS>(s, keep, value, UINT64_MAX, &mass);
-    // kept by top-p: those before which less than the limit lies
-    if (ask.P < 1.0f) keep = min(keep, scan_to<THREADS>(s, keep, value, ask.limit(mass) - 1, &skipped) + 1);
-    if (ask.Q > 0.0f)
-        keep = max(1, scan_to<THREADS>(s, keep, [&](int i) { return (uint64_t)!h.likely(high(i)); }, 0, &skipped));
-    scan_to<THREADS>(s, keep, value, UINT64_MAX, &mass);
-    // by index: a rank with its halves exchanged sorts that way
-    for (int i = threadIdx.x; i < keep; i += THREADS) s.list[i] = s.list[i] << 32 | s.list[i] >> 32;
-    __syncthreads();
-    sort_list<THREADS>(s.list, keep);
-    const int at = scan_to<THREADS>(s, keep, [&](int i) { return h.weigh(of_key((uint32_t)s.list[i])); }, ask.target(mass), &skipped);
-    if (threadIdx.x == 0) {
-        const uint64_t e = s.list[min(at, keep - 1)];
-        answer(A, n, (int32_t)~(uint32_t)(e >> 32), ((double)of_key((uint32_t)e) - (double)h.m) / (double)ask.T, all, mass);
+    __device__ Binner binner(int last = kBins - 1) const {
+        return Binner{m, (float)fmin(fmax(c * last / 41.5, 1e-30), 3e38), (float)last};
     }
-}
+};
 
 __device__ __forceinline__ void no_answer(const Args& A, int64_t n) {
     A.action[n] = -1;
@@ -425,6 +333,152 @@ __device__ void greedy(const Args& A, int64_t n, float m, int32_t lo, int32_t le
         A.action[n] = a;
         A.logprob[n] = A.kept[n] = 0.0f;
     }
+}
+
+// ---- the cut, among entries in registers -----------------------------------
+// A team of one to sixteen waves, and what they tell each other.
+template <int THREADS>
+struct Team {
+    static constexpr int kWaves = THREADS / 64;
+    struct Slots { uint64_t v[2][kWaves]; };
+    Slots& s;
+    int turn = 0;  // two sets in turn: one barrier for each exchange
+
+    __device__ explicit Team(Slots& s) : s(s) {}
+    // v from every wave, combined
+    template <class T, class Op>
+    __device__ __forceinline__ T all(T v, Op op) {
+        v = lanes<64>(v, op);
+        if constexpr (kWaves > 1) {
+            uint64_t* slot = s.v[turn];
+            turn ^= 1;
+            if ((threadIdx.x & 63) == 0) slot[threadIdx.x >> 6] = (uint64_t)v;
+            __syncthreads();
+            v = (T)slot[0];
+#pragma unroll
+            for (int i = 1; i < kWaves; ++i) v = op(v, (T)slot[i]);
+        }
+        return v;
+    }
+    template <class T>
+    __device__ __forceinline__ T sum(T v) {
+        return all(v, [](T a, T b) { return a + b; });
+    }
+    __device__ __forceinline__ uint32_t top(uint32_t v) {
+        return all(v, [](uint32_t a, uint32_t b) { return max(a, b); });
+    }
+    __device__ __forceinline__ void sync() {
+        if constexpr (kWaves > 1) __syncthreads();
+        else __builtin_amdgcn_wave_barrier();  // a wave's LDS accesses keep their order
+    }
+    // the sum of the threads before this one; `total` of all
+    __device__ __forceinline__ uint64_t before(uint64_t v, uint64_t* total) {
+        const int lane = threadIdx.x & 63;
+        uint64_t run = v;
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) {
+            const uint64_t q = __shfl_up(run, o);
+            if (lane >= o) run += q;
+        }
+        uint64_t all = __shfl(run, 63), at = run - v;
+        if constexpr (kWaves > 1) {
+            uint64_t* slot = s.v[turn];
+            turn ^= 1;
+            if (lane == 0) slot[threadIdx.x >> 6] = all;
+            __syncthreads();
+            all = 0;
+#pragma unroll
+            for (int i = 0; i < kWaves; ++i) {
+                if (i < (int)(threadIdx.x >> 6)) at += slot[i];
+                all += slot[i];
+            }
+        }
+        *total = all;
+        return at;
+    }
+};
+
+// The key at which the sum of value(e), over falling keys, reaches `want` (1 <=
+// want <= the sum of all), and the sum above it.  A histogram by bin(e) (larger
+// keys have no larger bin) says in which bin; there, the largest key that is
+// left, and then the middle of what is left, each with its sum: most bins have
+// an entry or two.  hist: BINS places of LDS.
+template <int BINS, int E, class K, class T, class Key, class Bin, class Value, class Middle>
+__device__ __forceinline__ K team_key(T& team, uint64_t* hist, Key key, Bin bin, Value value, uint64_t want, Middle middle,
+                                      uint64_t* above) {
+    constexpr int kThreads = T::kWaves * 64, kPer = BINS / kThreads;
+    const int t = threadIdx.x % kThreads;
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) hist[t + i * kThreads] = 0;
+    team.sync();
+#pragma unroll
+    for (int e = 0; e < E; ++e)
+        if (const uint64_t v = value(e))
+            atomicAdd(reinterpret_cast<unsigned long long*>(hist + bin(e)), (unsigned long long)v);
+    team.sync();
+    uint64_t mine = 0, total;
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) mine += hist[t * kPer + i];
+    uint64_t at = team.before(mine, &total);
+    uint32_t where = 0;
+    uint64_t over = 0;
+    if (at < want && want <= at + mine) {
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) {
+            const uint64_t v = hist[t * kPer + i];
+            if (at < want && want <= at + v) {
+                where = t * kPer + i;
+                over = at;
+            }
+            at += v;
+        }
+    }
+    where = team.top(where);
+    over = team.sum(over);
+    // the sum of keys >= lo reaches `want`, that of keys >= hi does not
+    K k = 0, lo = ~(K)0;
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+        const bool here = value(e) && (uint32_t)bin(e) == where;
+        k = here ? max(k, key(e)) : k;
+        lo = here ? min(lo, key(e)) : lo;
+    }
+    k = team.all(k, [](K a, K b) { return max(a, b); });
+    lo = team.all(lo, [](K a, K b) { return min(a, b); });
+    const auto from = [&](K least) {
+        uint64_t s = 0;
+#pragma unroll
+        for (int e = 0; e < E; ++e) s += key(e) >= least ? value(e) : 0;
+        return team.sum(s);
+    };
+    while (true) {
+        uint64_t sum = from(k);
+        if (sum >= want) {
+            *above = over;
+            return k;
+        }
+        K hi = k;
+        over = sum;
+        const K mid = middle(lo, hi);  // lo <= mid < hi
+        sum = from(mid);
+        if (sum >= want) {
+            lo = mid;
+        } else {
+            hi = mid;
+            over = sum;
+        }
+        k = 0;
+#pragma unroll
+        for (int e = 0; e < E; ++e) k = key(e) < hi ? max(k, key(e)) : k;
+        k = team.all(k, [](K a, K b) { return max(a, b); });
+    }
+}
+
+// The middle of two keys of numbers: half way between the numbers (those around
+// 0 have most of the keys), or between the keys.
+__device__ __forceinline__ uint32_t middle_key(uint32_t lo, uint32_t hi) {
+    const uint32_t mid = key_of(0.5f * of_key(lo) + 0.5f * of_key(hi));
+    return mid > lo && mid < hi ? mid : lo + (hi - lo) / 2;
 }
 
 // ---- long rows, by parts ---------------------------------------------------
@@ -565,8 +619,6 @@ __global__ __launch_bounds__(256) void k_cat_sample_near(Batch b) {
     uint64_t want, before, kept = 0;
     const int at = find_cut<256>(ask, all, s, &want, &before);
     if (ask.K > 0 && before + s.hist[at] > kList) return;
-    if (tid == 0) s.many = 0;
-    __syncthreads();
     // top-k: all up to the bin of the cut; top-p: that bin, and the weight of those before it
     walk(row, part, [&](float x, int32_t i) {
         const int v = bin(x);
@@ -574,18 +626,12 @@ __global__ __launch_bounds__(256) void k_cat_sample_near(Batch b) {
         if (v < at && ask.K <= 0) {
             kept += h.likely(x) ? h.weigh(x) : 0;
         } else if (h.weigh(x)) {
-            const int o = atomicAdd(&s.many, 1);
-            if (o < kList) s.list[o] = rank_of(x, i);
+            const int o = atomicAdd(&to.many, 1);
+            if (o < kList) to.list[o] = rank_of(x, i);
         }
     });
     kept = wave_sum(kept);
     if ((tid & 63) == 0) to.kept[seg] = kept;
-    __syncthreads();
-    const int many = min(s.many, kList);
-    if (tid == 0) s.where = atomicAdd(&to.many, s.many);
-    __syncthreads();
-    for (int i = tid; i < many; i += 256)
-        if (s.where + i < kList) to.list[s.where + i] = s.list[i];
 }
 
 // Which wave's part has an entry.
@@ -596,9 +642,10 @@ __device__ __forceinline__ int part_of(const Span<D>& row, int waves, int32_t i)
 }
 
 template <class D>
-__global__ __launch_bounds__(1024) void k_cat_sample_answer(Batch b) {
-    constexpr int kThreads = 1024;
+__global__ __launch_bounds__(512) void k_cat_sample_answer(Batch b) {
+    constexpr int kThreads = 512, kPer = kList / kThreads;
     __shared__ Shared<kThreads> s;
+    __shared__ Team<kThreads>::Slots slots;
     __shared__ uint64_t segs[kParts * kPartWaves];
     const int64_t n = b.first + blockIdx.x;
     const int32_t V = b.a.vocab, waves = b.parts * kPartWaves;
@@ -619,34 +666,84 @@ __global__ __launch_bounds__(1024) void k_cat_sample_answer(Batch b) {
         return greedy<D, kThreads>(b.a, n, m, from, to - from, row, s);
     }
     const Head h(ask, m);
+    Team<kThreads> team(slots);
     uint64_t cut = 0;  // the least rank that is kept
-    const uint64_t all = sum_of<kThreads>(r.all, waves, s);
-    for (int i = tid; i < waves; i += kThreads) segs[i] = r.kept[i];
+    const uint64_t all = team.sum(tid < waves ? r.all[tid] : 0);
+    if (tid < waves) segs[tid] = r.kept[tid];
     if (cuts(ask)) {
         if (ask.T > kMostT) return slow_row<D, kThreads>(b.a, n, ask, m, s);
         for (int i = tid; i < kBins; i += kThreads) s.hist[i] = r.hist[i];
         __syncthreads();
-        uint64_t want, before, skipped;
+        uint64_t want, before, above;
         const int at = find_cut<kThreads>(ask, all, s, &want, &before);
         const int many = r.many;
         if ((ask.K > 0 && before + s.hist[at] > kList) || many > kList) return slow_row<D, kThreads>(b.a, n, ask, m, s);
-        for (int i = tid; i < many; i += kThreads) s.list[i] = r.list[i];
-        __syncthreads();
-        if (ask.K > 0) return from_list<kThreads>(b.a, n, ask, h, many, s, all);
-        sort_list<kThreads>(s.list, many);
-        const int last = scan_to<kThreads>(
-            s, many, [&](int i) { return h.weigh(of_key((uint32_t)(s.list[i] >> 32))); }, want - before - 1, &skipped);
-        cut = s.list[min(last, many - 1)];
-        for (int i = tid; i < many; i += kThreads) {
-            const uint64_t e = s.list[i];
-            const float x = of_key((uint32_t)(e >> 32));
-            if (e >= cut && h.likely(x))
-                atomicAdd(reinterpret_cast<unsigned long long*>(&segs[part_of(row, waves, (int32_t)~(uint32_t)e)]),
-                          (unsigned long long)h.weigh(x));
+        uint64_t e[kPer], wt[kPer];  // ranks, no two alike; 0 and no weight where there is no entry
+        uint32_t top = 0, low = UINT32_MAX;
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) {
+            const int o = tid + i * kThreads;
+            e[i] = o < many ? r.list[o] : 0;
+            wt[i] = o < many ? h.weigh(of_key((uint32_t)(e[i] >> 32))) : 0;
+            if (o < many) {
+                top = max(top, (uint32_t)(e[i] >> 32));
+                low = min(low, (uint32_t)(e[i] >> 32));
+            }
         }
+        top = team.top(top);
+        low = team.all(low, [](uint32_t a, uint32_t b) { return min(a, b); });
+        const float first = of_key(top), reach = first - of_key(low);
+        const Binner fine{first, reach > 0.0f ? fminf((float)(kBins - 1) / reach, 3e38f) : 0.0f, (float)(kBins - 1)};
+        const auto key = [&](int i) { return e[i]; };
+        const auto place = [&](int i) { return fine(of_key((uint32_t)(e[i] >> 32))); };
+        const auto middle = [](uint64_t lo, uint64_t hi) { return lo + (hi - lo) / 2; };
+        const auto drop = [&] {
+#pragma unroll
+            for (int i = 0; i < kPer; ++i) wt[i] = e[i] < cut ? 0 : wt[i];
+        };
+        const auto weight = [&](int i) { return wt[i]; };
+        __syncthreads();  // s.hist is read above
+        if (ask.K > 0) {
+            cut = team_key<kBins, kPer, uint64_t>(team, s.hist, key, place, [&](int i) { return (uint64_t)(wt[i] != 0); }, want, middle, &above);
+            drop();
+            if (ask.P < 1.0f) {
+                uint64_t mass = 0;
+#pragma unroll
+                for (int i = 0; i < kPer; ++i) mass += wt[i];
+                mass = team.sum(mass);
+                cut = team_key<kBins, kPer, uint64_t>(team, s.hist, key, place, weight, ask.limit(mass), middle, &above);
+                drop();
+            }
+        } else {
+            cut = team_key<kBins, kPer, uint64_t>(team, s.hist, key, place, weight, want - before, middle, &above);
+            drop();
+        }
+        uint64_t left = 0;
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) {
+            if (!h.likely(of_key((uint32_t)(e[i] >> 32)))) wt[i] = 0;
+            left += wt[i];
+        }
+        if (ask.K > 0) {
+            // all that is kept is here: by index, a rank with its halves exchanged
+            left = team.sum(left);
+            const int shift = max(0, 21 - __clz((uint32_t)V));  // V >> shift < 2048
+            const uint64_t found = team_key<kBins, kPer, uint64_t>(
+                team, s.hist, [&](int i) { return e[i] << 32 | e[i] >> 32; },
+                [&](int i) { return (int)(~(uint32_t)e[i] >> shift); }, weight, ask.target(left) + 1, middle, &above);
+            if (tid == 0)
+                answer(b.a, n, (int32_t)~(uint32_t)(found >> 32),
+                       ((double)of_key((uint32_t)found) - (double)m) / (double)ask.T, all, left);
+            return;
+        }
+#pragma unroll
+        for (int i = 0; i < kPer; ++i)
+            if (wt[i])
+                atomicAdd(reinterpret_cast<unsigned long long*>(&segs[part_of(row, waves, (int32_t)~(uint32_t)e[i])]),
+                          (unsigned long long)wt[i]);
     }
     __syncthreads();
-    const uint64_t left = sum_of<kThreads>(segs, waves, s);
+    const uint64_t left = team.sum(tid < waves ? segs[tid] : 0);
     uint64_t target = ask.target(left);
     int at = 0;
     for (; at < waves - 1 && target >= segs[at]; ++at) target -= segs[at];
@@ -753,107 +850,11 @@ __global__ __launch_bounds__(64) void k_cat_sample_tiny(Args A, int64_t rows) {
 // bank conflicts).  The cut is found between two keys, by halving their
 // distance and by the largest key that is left below the upper: a dozen steps
 // of E compares and a sum over the team.
-template <int THREADS>
-struct Team {
-    static constexpr int kWaves = THREADS / 64;
-    struct Slots { uint64_t v[2][kWaves]; };
-    Slots& s;
-    int turn;  // two sets in turn: one barrier for each exchange
-
-    __device__ explicit Team(Slots& s) : s(s), turn(0) {}
-    // v from every wave, combined
-    template <class T, class Op>
-    __device__ __forceinline__ T all(T v, Op op) {
-        v = lanes<64>(v, op);
-        if constexpr (kWaves > 1) {
-            uint64_t* slot = s.v[turn];
-            turn ^= 1;
-            if ((threadIdx.x & 63) == 0) slot[threadIdx.x >> 6] = (uint64_t)v;
-            __syncthreads();
-            v = (T)slot[0];
-#pragma unroll
-            for (int i = 1; i < kWaves; ++i) v = op(v, (T)slot[i]);
-        }
-        return v;
-    }
-    template <class T>
-    __device__ __forceinline__ T sum(T v) {
-        return all(v, [](T a, T b) { return a + b; });
-    }
-    __device__ __forceinline__ uint32_t top(uint32_t v) {
-        return all(v, [](uint32_t a, uint32_t b) { return max(a, b); });
-    }
-    // the sum of the threads before this one; `total` of all
-    __device__ __forceinline__ uint64_t before(uint64_t v, uint64_t* total) {
-        const int lane = threadIdx.x & 63;
-        uint64_t run = v;
-#pragma unroll
-        for (int o = 1; o < 64; o <<= 1) {
-            const uint64_t q = __shfl_up(run, o);
-            if (lane >= o) run += q;
-        }
-        uint64_t all = __shfl(run, 63), at = run - v;
-        if constexpr (kWaves > 1) {
-            uint64_t* slot = s.v[turn];
-            turn ^= 1;
-            if (lane == 0) slot[threadIdx.x >> 6] = all;
-            __syncthreads();
-            all = 0;
-#pragma unroll
-            for (int i = 0; i < kWaves; ++i) {
-                if (i < (int)(threadIdx.x >> 6)) at += slot[i];
-                all += slot[i];
-            }
-        }
-        *total = all;
-        return at;
-    }
-};
-
-// The key at which the sum of value(e) over falling keys reaches `want` (1 <=
-// want <= the sum of all), and the sum above it.  S: the type of the sums.
-template <int E, class S, class T, class Value>
-__device__ __forceinline__ uint32_t held_key(T& team, const float (&x)[E], uint32_t least, uint32_t top, Value value, S want,
-                                             S* above) {
-    uint32_t lo = least, hi = top + 1;  // the sum of keys >= lo reaches `want`, that of keys >= hi does not
-    S over = 0;
-    const auto from = [&](uint32_t k) {
-        S s = 0;
-#pragma unroll
-        for (int e = 0; e < E; ++e) s += key_of(x[e]) >= k ? value(e) : (S)0;
-        return team.sum(s);
-    };
-    while (true) {
-        uint32_t k = 0;
-#pragma unroll
-        for (int e = 0; e < E; ++e) {
-            const uint32_t q = key_of(x[e]);
-            k = q < hi ? max(k, q) : k;
-        }
-        k = team.top(k);
-        S s = from(k);
-        if (s >= want) {
-            *above = over;
-            return k;
-        }
-        hi = k;
-        over = s;
-        // half way between the numbers (the numbers around 0 have most of the keys), or between the keys
-        uint32_t mid = key_of(0.5f * of_key(lo) + 0.5f * of_key(hi));
-        if (!(mid > lo && mid < hi)) mid = lo + (hi - lo) / 2;
-        s = from(mid);
-        if (s >= want) {
-            lo = mid;
-        } else {
-            hi = mid;
-            over = s;
-        }
-    }
-}
-
 template <class D, int THREADS, int E>
 __global__ __launch_bounds__(THREADS < 256 ? 256 : THREADS) void k_cat_sample_held(Args A, int64_t rows) {
     constexpr int kRows = THREADS == 64 ? 4 : 1;  // of a block
+    constexpr int kFine = THREADS == 64 ? 256 : THREADS == 256 ? 1024 : kBins;
+    __shared__ uint64_t hist[kRows][kFine];
     extern __shared__ __align__(16) float staged[];
     __shared__ typename Team<THREADS>::Slots slots;
     Team<THREADS> team(slots);
@@ -921,8 +922,10 @@ __global__ __launch_bounds__(THREADS < 256 ? 256 : THREADS) void k_cat_sample_he
         }
     };
     uint64_t mass = all;
-    // no key below this has weight: 2^(40 - 41.5) < 1/2, and 2^-20 of the distance covers the rounding
-    const uint32_t least = key_of((float)((double)m - 41.5 * (1 + 0x1p-20) / h.c) - fabsf(m) * 0x1p-20f);
+    const Binner bin = h.binner(kFine - 1);
+    const auto key = [&](int e) { return key_of(x[e]); };
+    const auto place = [&](int e) { return bin(x[e]); };
+    uint64_t* mine_hist = hist[threadIdx.x / THREADS];
     int32_t many = 0;
     if (ask.K > 0) {
 #pragma unroll
@@ -930,9 +933,10 @@ __global__ __launch_bounds__(THREADS < 256 ? 256 : THREADS) void k_cat_sample_he
         many = team.sum(many);
     }
     if (ask.K > 0 && ask.K < many) {  // else top-k drops nothing that weighs
-        int32_t above;
-        const uint32_t cut = held_key<E, int32_t>(team, x, least, top, [&](int e) { return (int32_t)(wt[e] != 0); }, ask.K, &above);
-        drop(cut, (uint64_t)(ask.K - above));
+        uint64_t above;
+        const uint32_t cut = team_key<kFine, E, uint32_t>(
+            team, mine_hist, key, place, [&](int e) { return (uint64_t)(wt[e] != 0); }, (uint64_t)ask.K, middle_key, &above);
+        drop(cut, (uint64_t)ask.K - above);
         mass = 0;
 #pragma unroll
         for (int e = 0; e < E; ++e) mass += wt[e];
@@ -941,7 +945,8 @@ __global__ __launch_bounds__(THREADS < 256 ? 256 : THREADS) void k_cat_sample_he
     if (ask.P < 1.0f) {
         uint64_t above;
         const uint64_t want = ask.limit(mass);
-        const uint32_t cut = held_key<E, uint64_t>(team, x, least, top, [&](int e) { return wt[e]; }, want, &above);
+        const uint32_t cut = team_key<kFine, E, uint32_t>(team, mine_hist, key, place, [&](int e) { return wt[e]; }, want,
+                                                          middle_key, &above);
         const uint64_t each = h.weigh(of_key(cut));
         drop(cut, (want - above + each - 1) / each);
     }
@@ -1014,7 +1019,7 @@ int run_sample(const Args& a, int64_t rows, void* space, hipStream_t st) {
         hipLaunchKernelGGL(k_cat_sample_top<D>, dim3(blocks), dim3(256), 0, st, b);
         hipLaunchKernelGGL(k_cat_sample_weigh<D>, dim3(blocks), dim3(256), 0, st, b);
         if (cut) hipLaunchKernelGGL(k_cat_sample_near<D>, dim3(blocks), dim3(256), 0, st, b);
-        hipLaunchKernelGGL(k_cat_sample_answer<D>, dim3(here), dim3(1024), 0, st, b);
+        hipLaunchKernelGGL(k_cat_sample_answer<D>, dim3(here), dim3(512), 0, st, b);
     }
     return launched();
 }
