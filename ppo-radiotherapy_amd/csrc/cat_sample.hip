@@ -198,7 +198,7 @@ __device__ __forceinline__ void answer(const Args& A, int64_t n, int32_t a, doub
 // entries than a list holds (many equal logits, a very large k) and for
 // temperatures past the histogram's range.
 template <class D, int THREADS>
-__device__ void slow_row(const Args& A, int64_t n, const Ask& ask, float m, Shared<THREADS>& s) {
+__device__ __forceinline__ void slow_row(const Args& A, int64_t n, const Ask& ask, float m, Shared<THREADS>& s) {
     constexpr bool kShort = sizeof(typename D::raw) == 2;
     const int32_t V = A.vocab;
     const auto* row = static_cast<const typename D::raw*>(A.x) + n * A.stride;
@@ -398,23 +398,43 @@ struct Team {
     }
 };
 
+// A thread's entries: E of them, in registers; or every `step`-th of a list, in
+// a loop that stays one (a kernel that runs once a row spends its time on
+// fetching code).
+template <int E>
+struct Held {
+    template <class F>
+    __device__ __forceinline__ void operator()(F f) const {
+#pragma unroll
+        for (int e = 0; e < E; ++e) f(e);
+    }
+};
+struct Listed {
+    int from, to, step;
+    template <class F>
+    __device__ __forceinline__ void operator()(F f) const {
+#pragma unroll 1
+        for (int i = from; i < to; i += step) f(i);
+    }
+};
+
 // The key at which the sum of value(e), over falling keys, reaches `want` (1 <=
 // want <= the sum of all), and the sum above it.  A histogram by bin(e) (larger
 // keys have no larger bin) says in which bin; there, the largest key that is
 // left, and then the middle of what is left, each with its sum: most bins have
 // an entry or two.  hist: BINS places of LDS.
-template <int BINS, int E, class K, class T, class Key, class Bin, class Value, class Middle>
-__device__ __forceinline__ K team_key(T& team, uint64_t* hist, Key key, Bin bin, Value value, uint64_t want, Middle middle,
+template <int BINS, class K, class T, class Each, class Key, class Bin, class Value, class Middle>
+__device__ __forceinline__ K team_key(T& team, uint64_t* hist, Each each, Key key, Bin bin, Value value, uint64_t want, Middle middle,
                                       uint64_t* above) {
     constexpr int kThreads = T::kWaves * 64, kPer = BINS / kThreads;
     const int t = threadIdx.x % kThreads;
 #pragma unroll
     for (int i = 0; i < kPer; ++i) hist[t + i * kThreads] = 0;
     team.sync();
-#pragma unroll
-    for (int e = 0; e < E; ++e)
+    each([&](int e) {
         if (const uint64_t v = value(e))
             atomicAdd(reinterpret_cast<unsigned long long*>(hist + bin(e)), (unsigned long long)v);
+    });
     team.sync();
     uint64_t mine = 0, total;
 #pragma unroll
@@ -437,18 +457,16 @@ __device__ __forceinline__ K team_key(T& team, uint64_t* hist, Key key, Bin bin,
     over = team.sum(over);
     // the sum of keys >= lo reaches `want`, that of keys >= hi does not
     K k = 0, lo = ~(K)0;
-#pragma unroll
-    for (int e = 0; e < E; ++e) {
+    each([&](int e) {
         const bool here = value(e) && (uint32_t)bin(e) == where;
         k = here ? max(k, key(e)) : k;
         lo = here ? min(lo, key(e)) : lo;
-    }
+    });
     k = team.all(k, [](K a, K b) { return max(a, b); });
     lo = team.all(lo, [](K a, K b) { return min(a, b); });
     const auto from = [&](K least) {
         uint64_t s = 0;
-#pragma unroll
-        for (int e = 0; e < E; ++e) s += key(e) >= least ? value(e) : 0;
+        each([&](int e) { s += key(e) >= least ? value(e) : 0; });
         return team.sum(s);
     };
     while (true) {
@@ -468,8 +486,7 @@ __device__ __forceinline__ K team_key(T& team, uint64_t* hist, Key key, Bin bin,
             over = sum;
         }
         k = 0;
-#pragma unroll
-        for (int e = 0; e < E; ++e) k = key(e) < hi ? max(k, key(e)) : k;
+        each([&](int e) { k = key(e) < hi ? max(k, key(e)) : k; });
         k = team.all(k, [](K a, K b) { return max(a, b); });
     }
 }
@@ -491,41 +508,102 @@ struct RowSpace {
     float top[kParts];                          // NaN: a NaN or +inf
     uint64_t all[kParts * kPartWaves];          // the weight of each wave's part
     uint64_t kept[kParts * kPartWaves];         // what of it is surely kept
-    uint64_t hist[kBins];
+    uint64_t coarse[kParts][64];                // the histogram of each part by 32 bins
     uint64_t list[kList];
     int32_t many, pad[15];
 };
+constexpr int kCoarse = kBins / 64;
 
 struct Batch {
     Args a;
     RowSpace* space;  // of row `first`
+    uint64_t* hist;   // [row][part][kBins]
     int64_t first;
     int32_t parts;
 };
 
 // The maximum of the row from those of its parts; NaN for a row without an answer.
-__device__ __forceinline__ float row_top(const RowSpace& r, int32_t parts) {
+__device__ __forceinline__ float part_top(const RowSpace& r, int32_t parts) {
     const int lane = threadIdx.x & 63;
-    const float v = lane < parts ? r.top[lane] : -INFINITY;
+    return lane < parts ? r.top[lane] : -INFINITY;
+}
+__device__ __forceinline__ float row_top(float v) {
     const float m = wave_max(v);
     return __any(v != v) || m == -INFINITY ? NAN : m;
 }
 
 __device__ __forceinline__ bool cuts(const Ask& ask) { return ask.K > 0 || ask.P < 1.0f; }
 
-// Bin and sum before it where the cut falls, from the histogram in LDS.
-template <int THREADS>
-__device__ __forceinline__ int find_cut(const Ask& ask, uint64_t all, Shared<THREADS>& s, uint64_t* want, uint64_t* before) {
-    uint64_t total = all;
-    if (ask.K > 0) {
-        total = 0;
-        for (int i = threadIdx.x; i < kBins; i += THREADS) total += s.hist[i];
-        total = block_sum<THREADS>(total, s.slots);
+// The lane at which the running sum of v reaches `want`, and the sum before it.
+__device__ __forceinline__ int lane_of(uint64_t v, uint64_t want, uint64_t* before) {
+    uint64_t run = v;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+        const uint64_t q = __shfl_up(run, o);
+        if ((int)(threadIdx.x & 63) >= o) run += q;
     }
-    // entries that weigh nothing are not in the histogram: they stand behind all others, and keeping
-    // them or not changes nothing
-    *want = ask.K > 0 ? min((uint64_t)ask.K, total) : ask.limit(all);
-    return find_bin<THREADS, true>(s, *want, before);
+    const int lane = __ffsll((long long)__ballot(run >= want)) - 1;
+    *before = __shfl(run - v, lane);
+    return lane;
+}
+
+// Where the cut falls: its bin, what is wanted, the sum before the bin and in
+// it.
+struct Near {
+    int bin;
+    uint64_t want, before, in;
+    // whether a list can hold what has to be in it
+    __device__ bool fits(const Ask& ask) const { return ask.K <= 0 || before + in <= kList; }
+};
+
+// By the whole block: 64 coarse bins, then the 32 of one, each the sum of all
+// parts (which write their own: adding them up in memory took longer).  Every
+// thread has a bin of every THREADS / 64-th part, or / 32-nd.
+template <int THREADS>
+struct NearRoom {
+    uint64_t sums[THREADS];
+    Near near;
+};
+
+template <int THREADS>
+__device__ __forceinline__ void find_near(const Ask& ask, const RowSpace& r, const uint64_t* hist, int32_t parts,
+                                          NearRoom<THREADS>& room) {
+    const int tid = threadIdx.x, lane = tid & 63;
+    Near n;
+    uint64_t v = 0, more;
+#pragma unroll 4
+    for (int p = tid / 64; p < parts; p += THREADS / 64) v += r.coarse[p][lane];
+    room.sums[tid] = v;
+    __syncthreads();
+    if (tid < 64) {
+        v = 0;
+#pragma unroll
+        for (int i = 0; i < THREADS / 64; ++i) v += room.sums[i * 64 + lane];
+        // entries that weigh nothing are not in the histogram: they stand behind all others, and keeping
+        // them or not changes nothing
+        n.want = ask.K > 0 ? min((uint64_t)ask.K, wave_sum(v)) : ask.limit(wave_sum(v));
+        n.bin = lane_of(v, n.want, &n.before) * kCoarse;
+        if (tid == 0) room.near = n;
+    }
+    __syncthreads();
+    n = room.near;
+    v = 0;
+#pragma unroll 4
+    for (int p = tid / kCoarse; p < parts; p += THREADS / kCoarse) v += hist[p * kBins + n.bin + tid % kCoarse];
+    room.sums[tid] = v;
+    __syncthreads();
+    if (tid < 64) {
+        v = 0;
+        if (lane < kCoarse)
+#pragma unroll
+            for (int i = 0; i < THREADS / kCoarse; ++i) v += room.sums[i * kCoarse + lane];
+        const int f = lane_of(v, n.want - n.before, &more);
+        n.bin += f;
+        n.before += more;
+        n.in = __shfl(v, f);
+        if (tid == 0) room.near = n;
+    }
+    __syncthreads();
 }
 
 template <class D>
@@ -545,7 +623,6 @@ __global__ __launch_bounds__(256) void k_cat_sample_top(Batch b) {
     });
     m = block_max<256>(m, fs);
     odd = __syncthreads_or(odd);
-    for (int i = p * 256 + threadIdx.x; i < kBins; i += b.parts * 256) to.hist[i] = 0;
     if (threadIdx.x == 0) {
         to.top[p] = odd ? NAN : m;
         if (p == 0) to.many = 0;
@@ -561,8 +638,9 @@ __global__ __launch_bounds__(256) void k_cat_sample_weigh(Batch b) {
     const Span<D> row(static_cast<const typename D::raw*>(b.a.x) + n * b.a.stride, V);
     const Part<D> part(row, V, seg, b.parts * kPartWaves);
     RowSpace& to = b.space[r];
-    const float m = row_top(to, b.parts);
+    const float v_top = part_top(to, b.parts);
     const Ask ask(b.a.p, n, V);
+    const float m = row_top(v_top);
     if (m != m || !(ask.T > 0.0f)) return;
     const Head h(ask, m);
     uint64_t all = 0, kept = 0;
@@ -577,8 +655,13 @@ __global__ __launch_bounds__(256) void k_cat_sample_weigh(Batch b) {
             if (v) atomicAdd(reinterpret_cast<unsigned long long*>(&hist[bin(x)]), (unsigned long long)(count ? 1 : v));
         });
         __syncthreads();
-        for (int i = tid; i < kBins; i += 256)
-            if (hist[i]) atomicAdd(reinterpret_cast<unsigned long long*>(&to.hist[i]), (unsigned long long)hist[i]);
+        uint64_t* own = b.hist + (r * b.parts + p) * (int64_t)kBins;
+#pragma unroll
+        for (int i = tid; i < kBins; i += 256) {
+            own[i] = hist[i];
+            const uint64_t sum = lanes_sum<kCoarse>(hist[i]);
+            if (i % kCoarse == 0) to.coarse[p][i / kCoarse] = sum;
+        }
     } else {
         walk(row, part, [&](float x, int32_t) {
             const uint64_t v = h.weigh(x);
@@ -594,70 +677,182 @@ __global__ __launch_bounds__(256) void k_cat_sample_weigh(Batch b) {
     }
 }
 
-// Sum of n <= 256 numbers, by the whole block.
-template <int THREADS>
-__device__ __forceinline__ uint64_t sum_of(const uint64_t* v, int n, Shared<THREADS>& s) {
-    return block_sum<THREADS>((int)threadIdx.x < n ? v[threadIdx.x] : 0, s.slots);
+// Sum of n <= 256 numbers, by each wave for itself.
+__device__ __forceinline__ uint64_t sum_of(const uint64_t* v, int n) {
+    uint64_t s = 0;
+    for (int i = threadIdx.x & 63; i < n; i += 64) s += v[i];
+    return wave_sum(s);
 }
 
 template <class D>
 __global__ __launch_bounds__(256) void k_cat_sample_near(Batch b) {
-    __shared__ Shared<256> s;
+    constexpr int kOwn = 512;
+    __shared__ NearRoom<256> room;
+    __shared__ int many, start_at;
+    __shared__ uint64_t own[kOwn];  // the block's entries, added to the row's list at once
     const int64_t r = blockIdx.x / b.parts, n = b.first + r;
     const int32_t p = blockIdx.x % b.parts, V = b.a.vocab;
     const int tid = threadIdx.x, w = tid >> 6, seg = p * kPartWaves + w;
     const Span<D> row(static_cast<const typename D::raw*>(b.a.x) + n * b.a.stride, V);
     const Part<D> part(row, V, seg, b.parts * kPartWaves);
     RowSpace& to = b.space[r];
-    const float m = row_top(to, b.parts);
+    const float v_top = part_top(to, b.parts);
     const Ask ask(b.a.p, n, V);
+    const float m = row_top(v_top);
     if (m != m || !(ask.T > 0.0f) || !cuts(ask) || ask.T > kMostT) return;
     const Head h(ask, m);
     const Binner bin = h.binner();
-    for (int i = tid; i < kBins; i += 256) s.hist[i] = to.hist[i];
-    const uint64_t all = sum_of<256>(to.all, b.parts * kPartWaves, s);
-    uint64_t want, before, kept = 0;
-    const int at = find_cut<256>(ask, all, s, &want, &before);
-    if (ask.K > 0 && before + s.hist[at] > kList) return;
-    // top-k: all up to the bin of the cut; top-p: that bin, and the weight of those before it
+    if (tid == 0) many = 0;
+    find_near<256>(ask, to, b.hist + r * b.parts * (int64_t)kBins, b.parts, room);
+    const Near& near = room.near;
+    if (!near.fits(ask)) return;
+    const int at = near.bin;
+    uint64_t kept = 0;
+    // top-k: all up to the bin of the cut.  top-p: that bin, and the weight of those before it from its
+    // coarse bin on (the rest is known by parts, unless min-p takes some of it)
+    const int start = ask.K > 0 || ask.Q > 0.0f ? 0 : at / kCoarse * kCoarse;
     walk(row, part, [&](float x, int32_t i) {
         const int v = bin(x);
-        if (v > at) return;
+        if (v > at || v < start) return;
         if (v < at && ask.K <= 0) {
             kept += h.likely(x) ? h.weigh(x) : 0;
         } else if (h.weigh(x)) {
-            const int o = atomicAdd(&to.many, 1);
-            if (o < kList) to.list[o] = rank_of(x, i);
+            const int o = atomicAdd(&many, 1);
+            if (o < kOwn) {
+                own[o] = rank_of(x, i);
+            } else {
+                const int l = atomicAdd(&to.many, 1);
+                if (l < kList) to.list[l] = rank_of(x, i);
+            }
         }
     });
     kept = wave_sum(kept);
     if ((tid & 63) == 0) to.kept[seg] = kept;
+    __syncthreads();
+    const int mine = min(many, kOwn);
+    if (tid == 0 && mine) start_at = atomicAdd(&to.many, mine);
+    __syncthreads();
+    for (int i = tid; i < mine; i += 256)
+        if (start_at + i < kList) to.list[start_at + i] = own[i];
 }
 
-// Which wave's part has an entry.
+// Which of the equal shares of a row has an entry.
 template <class D>
-__device__ __forceinline__ int part_of(const Span<D>& row, int waves, int32_t i) {
-    const int32_t per = (row.pieces + waves - 1) / waves, piece = (i - row.head) / Span<D>::kPer;
-    return i < row.head ? 0 : piece >= row.pieces ? waves - 1 : piece / per;
+__device__ __forceinline__ int share_of(const Span<D>& row, int shares, int32_t i) {
+    const int32_t per = (row.pieces + shares - 1) / shares, piece = (i - row.head) / Span<D>::kPer;
+    return i < row.head ? 0 : piece >= row.pieces ? shares - 1 : piece / per;
+}
+
+// What is known at the end: the least rank that is kept, by top-p, or the answer.
+struct Verdict {
+    uint64_t cut;
+    int32_t action;  // -1: still to be found
+    float x;
+    uint64_t left;
+};
+
+// What the block that answers has of a row.
+template <int THREADS>
+struct Room {
+    uint64_t hist[kBins];
+    uint64_t list[kList], weight[kList];  // ranks, and what of their weight is kept
+    uint64_t segs[kParts * kPartWaves];   // the weight of what is kept, by shares of the row
+    NearRoom<THREADS> near;
+    Verdict verdict;
+};
+
+// From the list, by a team: top-k rows whole, of top-p rows the cut, and the
+// weight of what the list has of the kept ones on to their shares of the row.
+template <class D, int THREADS, int BINS, class R>
+__device__ __forceinline__ Verdict settle(Team<THREADS> team, R& room, const Ask& ask, const Head& h, int many,
+                                          const Span<D>& row, int waves, int group, int32_t V) {
+    const Near& near = room.near.near;
+    const int t = threadIdx.x % THREADS;
+    const Listed each{t, many, THREADS};
+    const auto key = [&](int i) { return (uint32_t)(room.list[i] >> 32); };
+    const auto turned = [&](int i) { return (uint32_t)room.list[i]; };  // by index, the first ones highest
+    const auto weight = [&](int i) { return room.weight[i]; };
+    uint32_t top = 0, low = UINT32_MAX;
+    each([&](int i) {
+        room.weight[i] = h.weigh(of_key(key(i)));
+        top = max(top, key(i));
+        low = min(low, key(i));
+    });
+    top = team.top(top);
+    low = team.all(low, [](uint32_t a, uint32_t b) { return min(a, b); });
+    const float first = of_key(top), reach = first - of_key(low);
+    const Binner fine{first, reach > 0.0f ? fminf((float)(BINS - 1) / reach, 3e38f) : 0.0f, (float)(BINS - 1)};
+    const auto place = [&](int i) { return fine(of_key(key(i))); };
+    const int shift = max(0, 32 - __clz((uint32_t)V) - (31 - __clz(BINS)));  // V >> shift < BINS
+    const auto slot = [&](int i) { return (int)(~turned(i) >> shift); };
+    const auto middle = [](uint32_t lo, uint32_t hi) { return lo + (hi - lo) / 2; };
+    uint64_t above, cut = 0;
+    // Two rounds at most: by number, then by weight.  What is behind the cut loses its weight: smaller
+    // keys, and of the entries equal to it all but the first `ties`.
+#pragma unroll 1
+    for (int round = ask.K > 0 ? 0 : 1; round < (ask.P < 1.0f ? 2 : 1); ++round) {
+        uint64_t want = ask.K > 0 ? near.want : near.want - near.before;
+        if (round == 1 && ask.K > 0) {
+            uint64_t mass = 0;
+            each([&](int i) { mass += weight(i); });
+            want = ask.limit(team.sum(mass));
+        }
+        const auto value = [&](int i) { return round == 0 ? (uint64_t)(room.weight[i] != 0) : room.weight[i]; };
+        const uint32_t c = team_key<BINS, uint32_t>(team, room.hist, each, key, place, value, want, middle_key, &above);
+        const uint64_t one = round == 0 ? 1 : h.weigh(of_key(c)), ties = (want - above + one - 1) / one;
+        const auto tie = [&](int i) { return (uint64_t)(key(i) == c && room.weight[i]); };
+        uint64_t equal = 0;
+        each([&](int i) { equal += tie(i); });
+        uint32_t last = 0;
+        if (ties < team.sum(equal)) last = team_key<BINS, uint32_t>(team, room.hist, each, turned, slot, tie, ties, middle, &above);
+        each([&](int i) {
+            if (key(i) < c || (key(i) == c && turned(i) < last)) room.weight[i] = 0;
+        });
+        cut = (uint64_t)c << 32 | last;
+    }
+    uint64_t left = 0;
+    each([&](int i) {
+        if (!h.likely(of_key(key(i)))) room.weight[i] = 0;
+        left += weight(i);
+    });
+    if (ask.K > 0) {  // all that is kept is here
+        left = team.sum(left);
+        const uint32_t found = team_key<BINS, uint32_t>(team, room.hist, each, turned, slot, weight, ask.target(left) + 1, middle, &above);
+        uint32_t k = 0;
+        each([&](int i) { k = turned(i) == found && weight(i) ? key(i) : k; });
+        return Verdict{cut, (int32_t)~found, of_key(team.top(k)), left};
+    }
+    each([&](int i) {
+        if (const uint64_t w = weight(i))
+            atomicAdd(reinterpret_cast<unsigned long long*>(&room.segs[share_of(row, waves, (int32_t)~turned(i)) / group]),
+                      (unsigned long long)w);
+    });
+    return Verdict{cut, -1, 0.0f, 0};
 }
 
 template <class D>
 __global__ __launch_bounds__(512) void k_cat_sample_answer(Batch b) {
-    constexpr int kThreads = 512, kPer = kList / kThreads;
+    constexpr int kThreads = 512;
     __shared__ Shared<kThreads> s;
     __shared__ Team<kThreads>::Slots slots;
-    __shared__ uint64_t segs[kParts * kPartWaves];
+    __shared__ Team<64>::Slots one;
+    __shared__ Room<kThreads> room;
+    uint64_t* const segs = room.segs;
     const int64_t n = b.first + blockIdx.x;
     const int32_t V = b.a.vocab, waves = b.parts * kPartWaves;
     const int tid = threadIdx.x;
     const Span<D> row(static_cast<const typename D::raw*>(b.a.x) + n * b.a.stride, V);
     const RowSpace& r = b.space[blockIdx.x];
-    const float m = row_top(r, b.parts);
+    // one trip to memory for all of this
+    const float v_top = part_top(r, b.parts);
+    const Ask ask(b.a.p, n, V);
+    const uint64_t v_all = tid < waves ? r.all[tid] : 0, v_kept = tid < waves ? r.kept[tid] : 0;
+    const int many = r.many;
+    const float m = row_top(v_top);
     if (m != m) {
         if (tid == 0) no_answer(b.a, n);
         return;
     }
-    const Ask ask(b.a.p, n, V);
     if (!(ask.T > 0.0f)) {
         int p = 0;
         while (r.top[p] != m) ++p;
@@ -667,95 +862,92 @@ __global__ __launch_bounds__(512) void k_cat_sample_answer(Batch b) {
     }
     const Head h(ask, m);
     Team<kThreads> team(slots);
-    uint64_t cut = 0;  // the least rank that is kept
-    const uint64_t all = team.sum(tid < waves ? r.all[tid] : 0);
-    if (tid < waves) segs[tid] = r.kept[tid];
+    // top-p rows have the weight of what is kept by whole parts, others by each wave's
+    const int group = ask.K <= 0 && ask.P < 1.0f && !(ask.Q > 0.0f) ? kPartWaves : 1, shares = waves / group;
+    if (group == 1) {
+        if (tid < waves) segs[tid] = v_kept;
+    } else {
+        const uint64_t of_part = lanes_sum<kPartWaves>(v_kept);
+        if (tid < waves && tid % kPartWaves == 0) segs[tid / kPartWaves] = of_part;
+    }
+    const uint64_t all = team.sum(v_all);
+    Verdict v{0, -1, 0.0f, 0};
     if (cuts(ask)) {
-        if (ask.T > kMostT) return slow_row<D, kThreads>(b.a, n, ask, m, s);
-        for (int i = tid; i < kBins; i += kThreads) s.hist[i] = r.hist[i];
+        if (many <= kList)
+            for (int i = tid; i < many; i += kThreads) room.list[i] = r.list[i];
+        find_near<kThreads>(ask, r, b.hist + blockIdx.x * (int64_t)b.parts * kBins, b.parts, room.near);
+        const Near& near = room.near.near;
+        if (ask.T > kMostT || !near.fits(ask) || many > kList) return slow_row<D, kThreads>(b.a, n, ask, m, s);
         __syncthreads();
-        uint64_t want, before, above;
-        const int at = find_cut<kThreads>(ask, all, s, &want, &before);
-        const int many = r.many;
-        if ((ask.K > 0 && before + s.hist[at] > kList) || many > kList) return slow_row<D, kThreads>(b.a, n, ask, m, s);
-        uint64_t e[kPer], wt[kPer];  // ranks, no two alike; 0 and no weight where there is no entry
-        uint32_t top = 0, low = UINT32_MAX;
-#pragma unroll
-        for (int i = 0; i < kPer; ++i) {
-            const int o = tid + i * kThreads;
-            e[i] = o < many ? r.list[o] : 0;
-            wt[i] = o < many ? h.weigh(of_key((uint32_t)(e[i] >> 32))) : 0;
-            if (o < many) {
-                top = max(top, (uint32_t)(e[i] >> 32));
-                low = min(low, (uint32_t)(e[i] >> 32));
-            }
+        if (group > 1 && tid < b.parts) {
+            uint64_t known = 0;
+#pragma unroll 8
+            for (int i = 0; i < near.bin / kCoarse; ++i) known += r.coarse[tid][i];
+            segs[tid] += known;
         }
-        top = team.top(top);
-        low = team.all(low, [](uint32_t a, uint32_t b) { return min(a, b); });
-        const float first = of_key(top), reach = first - of_key(low);
-        const Binner fine{first, reach > 0.0f ? fminf((float)(kBins - 1) / reach, 3e38f) : 0.0f, (float)(kBins - 1)};
-        const auto key = [&](int i) { return e[i]; };
-        const auto place = [&](int i) { return fine(of_key((uint32_t)(e[i] >> 32))); };
-        const auto middle = [](uint64_t lo, uint64_t hi) { return lo + (hi - lo) / 2; };
-        const auto drop = [&] {
-#pragma unroll
-            for (int i = 0; i < kPer; ++i) wt[i] = e[i] < cut ? 0 : wt[i];
-        };
-        const auto weight = [&](int i) { return wt[i]; };
-        __syncthreads();  // s.hist is read above
-        if (ask.K > 0) {
-            cut = team_key<kBins, kPer, uint64_t>(team, s.hist, key, place, [&](int i) { return (uint64_t)(wt[i] != 0); }, want, middle, &above);
-            drop();
-            if (ask.P < 1.0f) {
-                uint64_t mass = 0;
-#pragma unroll
-                for (int i = 0; i < kPer; ++i) mass += wt[i];
-                mass = team.sum(mass);
-                cut = team_key<kBins, kPer, uint64_t>(team, s.hist, key, place, weight, ask.limit(mass), middle, &above);
-                drop();
+        __syncthreads();
+        if (many <= 512) {  // one wave is faster than the barriers of eight
+            if (tid < 64) {
+                v = settle<D, 64, 256>(Team<64>(one), room, ask, h, many, row, waves, group, V);
+                if (tid == 0) room.verdict = v;
             }
+            __syncthreads();
+            v = room.verdict;
         } else {
-            cut = team_key<kBins, kPer, uint64_t>(team, s.hist, key, place, weight, want - before, middle, &above);
-            drop();
+            v = settle<D, kThreads, kBins>(team, room, ask, h, many, row, waves, group, V);
         }
-        uint64_t left = 0;
-#pragma unroll
-        for (int i = 0; i < kPer; ++i) {
-            if (!h.likely(of_key((uint32_t)(e[i] >> 32)))) wt[i] = 0;
-            left += wt[i];
-        }
-        if (ask.K > 0) {
-            // all that is kept is here: by index, a rank with its halves exchanged
-            left = team.sum(left);
-            const int shift = max(0, 21 - __clz((uint32_t)V));  // V >> shift < 2048
-            const uint64_t found = team_key<kBins, kPer, uint64_t>(
-                team, s.hist, [&](int i) { return e[i] << 32 | e[i] >> 32; },
-                [&](int i) { return (int)(~(uint32_t)e[i] >> shift); }, weight, ask.target(left) + 1, middle, &above);
-            if (tid == 0)
-                answer(b.a, n, (int32_t)~(uint32_t)(found >> 32),
-                       ((double)of_key((uint32_t)found) - (double)m) / (double)ask.T, all, left);
-            return;
-        }
-#pragma unroll
-        for (int i = 0; i < kPer; ++i)
-            if (wt[i])
-                atomicAdd(reinterpret_cast<unsigned long long*>(&segs[part_of(row, waves, (int32_t)~(uint32_t)e[i])]),
-                          (unsigned long long)wt[i]);
+    }
+    if (v.action >= 0) {
+        if (tid == 0) answer(b.a, n, v.action, ((double)v.x - (double)m) / (double)ask.T, all, v.left);
+        return;
     }
     __syncthreads();
-    const uint64_t left = team.sum(tid < waves ? segs[tid] : 0);
+    const uint64_t left = sum_of(segs, shares);
     uint64_t target = ask.target(left);
     int at = 0;
-    for (; at < waves - 1 && target >= segs[at]; ++at) target -= segs[at];
-    const Part<D> seg(row, V, at, waves);
-    const int32_t a = find_index<kThreads>(
-        s, seg.first, seg.last - seg.first,
-        [&](int32_t i) {
-            const float x = D::get(row.x[i]);
-            return rank_of(x, i) < cut || !h.likely(x) ? 0 : h.weigh(x);
-        },
-        target);
-    if (tid == 0) answer(b.a, n, a, ((double)D::get(row.x[a]) - (double)m) / (double)ask.T, all, left);
+    for (; at < shares - 1 && target >= segs[at]; ++at) target -= segs[at];
+    // that share of the row, by waves, and one wave's of it in equal shares for the threads
+    const auto weight = [&](float x, int32_t i) -> uint64_t { return rank_of(x, i) < v.cut || !h.likely(x) ? 0 : h.weigh(x); };
+    const int32_t per_wave = (row.pieces + waves - 1) / waves, from_piece = min(at * group * per_wave, row.pieces);
+    Part<D> p(row, V, at * group, waves);
+    int32_t first = p.first, end = Part<D>(row, V, at * group + group - 1, waves).last;
+    uint64_t before, total;
+    if (end - first > 2 * kThreads) {
+        constexpr int kWaves = kThreads / 64;
+        const int w = tid >> 6;
+        const int32_t to_piece = min(from_piece + group * per_wave, row.pieces), per = (to_piece - from_piece + kWaves - 1) / kWaves;
+        const auto wave_part = [&](int k) {
+            Part<D> q = p;
+            q.from = min(from_piece + k * per, to_piece);
+            q.to = min(q.from + per, to_piece);
+            q.first = k == 0 ? first : row.head + q.from * Span<D>::kPer;
+            q.last = k == kWaves - 1 ? end : row.head + q.to * Span<D>::kPer;
+            return q;
+        };
+        uint64_t sum = 0;
+        walk(row, wave_part(w), [&](float x, int32_t i) { sum += weight(x, i); });
+        sum = wave_sum(sum);
+        if ((tid & 63) == 0) s.slots[w] = sum;
+        __syncthreads();
+        int k = 0;
+        for (; k < kWaves - 1 && target >= s.slots[k]; ++k) target -= s.slots[k];
+        const Part<D> q = wave_part(k);
+        first = q.first;
+        end = q.last;
+    }
+    const int32_t per = (end - first + kThreads - 1) / kThreads;
+    const int32_t from = min(first + tid * per, end), to = min(from + per, end);
+    uint64_t sum = 0;
+    for (int32_t i = from; i < to; ++i) sum += weight(D::get(row.x[i]), i);
+    before = team.before(sum, &total);
+    if (before <= target && target < before + sum) {
+        int32_t i = from;
+        for (; i < to - 1; ++i) {
+            before += weight(D::get(row.x[i]), i);
+            if (target < before) break;
+        }
+        answer(b.a, n, i, ((double)D::get(row.x[i]) - (double)m) / (double)ask.T, all, left);
+    }
 }
 
 // ---- short rows ------------------------------------------------------------
@@ -934,8 +1126,8 @@ __global__ __launch_bounds__(THREADS < 256 ? 256 : THREADS) void k_cat_sample_he
     }
     if (ask.K > 0 && ask.K < many) {  // else top-k drops nothing that weighs
         uint64_t above;
-        const uint32_t cut = team_key<kFine, E, uint32_t>(
-            team, mine_hist, key, place, [&](int e) { return (uint64_t)(wt[e] != 0); }, (uint64_t)ask.K, middle_key, &above);
+        const uint32_t cut = team_key<kFine, uint32_t>(
+            team, mine_hist, Held<E>{}, key, place, [&](int e) { return (uint64_t)(wt[e] != 0); }, (uint64_t)ask.K, middle_key, &above);
         drop(cut, (uint64_t)ask.K - above);
         mass = 0;
 #pragma unroll
@@ -945,7 +1137,7 @@ __global__ __launch_bounds__(THREADS < 256 ? 256 : THREADS) void k_cat_sample_he
     if (ask.P < 1.0f) {
         uint64_t above;
         const uint64_t want = ask.limit(mass);
-        const uint32_t cut = team_key<kFine, E, uint32_t>(team, mine_hist, key, place, [&](int e) { return wt[e]; }, want,
+        const uint32_t cut = team_key<kFine, uint32_t>(team, mine_hist, Held<E>{}, key, place, [&](int e) { return wt[e]; }, want,
                                                           middle_key, &above);
         const uint64_t each = h.weigh(of_key(cut));
         drop(cut, (want - above + each - 1) / each);
@@ -998,6 +1190,11 @@ void launch_held(const Args& a, int64_t rows, hipStream_t st) {
 constexpr int64_t kBatch = 512;
 
 int64_t batch_of(int64_t rows) { return std::min(rows, kBatch); }
+// 1536 blocks of 256 threads are on the card at once (six on a CU, by their registers: 2048 took 20 %
+// longer); two pieces for each thread at least
+int32_t parts_of(int64_t rows, int32_t vocab, int32_t per) {
+    return (int32_t)std::min<int64_t>({std::max<int64_t>(1536 / batch_of(rows), 1), vocab / per / 512, kParts});
+}
 
 template <class D>
 int run_sample(const Args& a, int64_t rows, void* space, hipStream_t st) {
@@ -1010,11 +1207,11 @@ int run_sample(const Args& a, int64_t rows, void* space, hipStream_t st) {
         return launched();
     }
     const bool cut = a.p.top_k || a.p.top_k_all > 0 || a.p.top_p || a.p.top_p_all < 1.0f;
-    const int64_t many = batch_of(rows), pieces = a.vocab / Span<D>::kPer;
-    // 2048 blocks of 256 threads, two pieces each at least
-    const int32_t parts = (int32_t)std::min<int64_t>({std::max<int64_t>(2048 / many, 1), pieces / 512, kParts});
+    const int64_t many = batch_of(rows);
+    const int32_t parts = parts_of(rows, a.vocab, Span<D>::kPer);
+    RowSpace* const rooms = static_cast<RowSpace*>(space);
     for (int64_t first = 0; first < rows; first += many) {
-        const Batch b{a, static_cast<RowSpace*>(space), first, parts};
+        const Batch b{a, rooms, reinterpret_cast<uint64_t*>(rooms + many), first, parts};
         const unsigned here = (unsigned)std::min(many, rows - first), blocks = here * parts;
         hipLaunchKernelGGL(k_cat_sample_top<D>, dim3(blocks), dim3(256), 0, st, b);
         hipLaunchKernelGGL(k_cat_sample_weigh<D>, dim3(blocks), dim3(256), 0, st, b);
@@ -1030,7 +1227,9 @@ int bad(const char* what) { return rt_internal_fail(RT_EINVAL, (std::string("rt_
 
 extern "C" int64_t rt_cat_sample_workspace_bytes(int64_t rows, int32_t vocab, int32_t dtype) {
     if (rows < 1 || rows > INT32_MAX || vocab < 1 || vocab > RT_CAT_MAX_VOCAB || bad_type(dtype)) return -1;
-    return vocab <= kHeld ? 0 : batch_of(rows) * (int64_t)sizeof(RowSpace);
+    if (vocab <= kHeld) return 0;
+    const int64_t hist = parts_of(rows, vocab, 16 / elem_size(dtype)) * kBins * (int64_t)sizeof(uint64_t);
+    return batch_of(rows) * ((int64_t)sizeof(RowSpace) + hist);
 }
 
 extern "C" int rt_cat_sample(const rt_cat_logits* logits, const rt_cat_sampling* params, int64_t* action_d,
