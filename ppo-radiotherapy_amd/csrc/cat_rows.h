@@ -66,28 +66,6 @@ __device__ __forceinline__ double log_64(double s) {
     return y * 0.6931471805599453 + d * (1.0 - d * (0.5 - d * 0.3333333333333333));
 }
 
-// Weights of a sampled row: 2^40 2^t as a whole number, t <= 0 (half to even,
-// by the rounding of the sum with 2^52, whose bits then hold it).
-constexpr double kUnit = 1099511627776.0;  // 2^40
-constexpr uint64_t kMagic = 0x4330000000000000ull;  // 2^52
-__device__ __forceinline__ uint64_t whole_bits(double t) {  // kMagic + the weight
-    t = fmax(t, -1100.0);
-    const double n = rint(t), f = t - n;
-    double p = 4.44553827187081e-10;
-    p = fma(p, f, 7.054911620801121e-09);
-    p = fma(p, f, 1.0178086009239696e-07);
-    p = fma(p, f, 1.3215486790144305e-06);
-    p = fma(p, f, 1.5252733804059838e-05);
-    p = fma(p, f, 0.00015403530393381606);
-    p = fma(p, f, 0.0013333558146428441);
-    p = fma(p, f, 0.009618129107628477);
-    p = fma(p, f, 0.055504108664821576);
-    p = fma(p, f, 0.2402265069591007);
-    p = fma(p, f, 0.6931471805599453);
-    p = fma(p, f, 1.0);
-    return __builtin_bit_cast(uint64_t, ldexp(p, (int)n + 40) + 4503599627370496.0);
-}
-
 // ---- reductions ------------------------------------------------------------
 // A value from the lane that the DPP control names: within 16 lanes an exchange
 // costs one VALU move and no trip through LDS.

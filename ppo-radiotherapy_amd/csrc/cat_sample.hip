@@ -14,6 +14,7 @@
 // segment.
 #include <algorithm>
 #include <string>
+#include <type_traits>
 
 #include "cat_rows.h"
 
@@ -22,7 +23,7 @@ namespace {
 using namespace rtcat;
 
 constexpr int kBins = 2048;  // of a histogram; 11 bits of a key
-constexpr int kList = 2048;  // entries that a block can sort
+constexpr int kList = 4096;  // entries around a cut that a block can have
 
 struct Args {
     const void* x;
@@ -42,9 +43,33 @@ __device__ __forceinline__ float of_key(uint32_t k) {
     return __uint_as_float(k & 0x80000000u ? k ^ 0x80000000u : ~k);
 }
 
+// 2^40 2^((x - m) c), c = log2(e) / T, as a whole number.  The product's whole
+// part n comes of its sum with 1.5 2^52 and is added to the exponent; 2^40 e^(f
+// ln 2), |f| <= 1/2, is the Taylor sum up to f^11 (within 7e-15 of it); the sum
+// with 2^52 rounds to a whole number, half to even, that its low bits hold.
+constexpr double kUnit = 1099511627776.0;  // 2^40
 struct Weigher {
-    double m, c;  // c = log2(e) / T
-    __device__ __forceinline__ uint64_t operator()(float x) const { return whole_bits(((double)x - m) * c) - kMagic; }
+    double m, c, least;  // least: of x - m, where nothing is left of the weight
+    __device__ Weigher(double m, double c) : m(m), c(c), least(-1000.0 / c) {}
+    __device__ __forceinline__ uint64_t operator()(float x) const {
+        const double kWhole = 6755399441055744.0;  // 1.5 2^52
+        const double d = fmax((double)x - m, least), t = fma(d, c, kWhole), f = fma(d, c, kWhole - t);
+        double p = kUnit * 4.44553827187081e-10;  // (ln 2)^11 / 11!, and so on down
+        p = fma(p, f, kUnit * 7.054911620801121e-09);
+        p = fma(p, f, kUnit * 1.0178086009239696e-07);
+        p = fma(p, f, kUnit * 1.3215486790144305e-06);
+        p = fma(p, f, kUnit * 1.5252733804059838e-05);
+        p = fma(p, f, kUnit * 0.00015403530393381606);
+        p = fma(p, f, kUnit * 0.0013333558146428441);
+        p = fma(p, f, kUnit * 0.009618129107628477);
+        p = fma(p, f, kUnit * 0.055504108664821576);
+        p = fma(p, f, kUnit * 0.2402265069591007);
+        p = fma(p, f, kUnit * 0.6931471805599453);
+        p = fma(p, f, kUnit);
+        const uint64_t n = (uint64_t)(uint32_t)__builtin_bit_cast(uint64_t, t) << 52;  // modulo 2^64, as the exponent is
+        const double w = __builtin_bit_cast(double, __builtin_bit_cast(uint64_t, p) + n);
+        return __builtin_bit_cast(uint64_t, w + 4503599627370496.0) - 0x4330000000000000ull;
+    }
 };
 
 template <int THREADS>
@@ -203,7 +228,7 @@ __device__ __forceinline__ void slow_row(const Args& A, int64_t n, const Ask& as
     const int32_t V = A.vocab;
     const auto* row = static_cast<const typename D::raw*>(A.x) + n * A.stride;
     const auto get = [&](int32_t i) { return D::get(row[i]); };
-    const Weigher weigh{(double)m, fmax(1.4426950408889634 / (double)ask.T, 1e-300)};
+    const Weigher weigh((double)m, fmax(1.4426950408889634 / (double)ask.T, 1e-300));
     uint64_t all = 0;
     for (int i = threadIdx.x; i < V; i += THREADS) all += weigh(get(i));
     all = block_sum<THREADS>(all, s.slots);
@@ -274,11 +299,16 @@ struct Part {
     }
 };
 
-// f(x, i) for every entry of a part; the lanes of one wave together.
-template <class D, class F>
-__device__ __forceinline__ void walk(const Span<D>& row, const Part<D>& p, F f) {
+// f(x, i) for every entry of a part; the lanes of one wave together, kAhead
+// pieces at a time.  `skip` says of a maximum whether all that is not above it
+// can be left out.
+struct Never {
+    __device__ __forceinline__ bool operator()(float) const { return false; }
+};
+template <int kAhead, class D, class F, class Skip = Never>
+__device__ __forceinline__ void walk(const Span<D>& row, const Part<D>& p, F f, Skip skip = Skip()) {
     const int lane = threadIdx.x & 63;
-    constexpr int kPer = Span<D>::kPer, kAhead = 4;
+    constexpr int kPer = Span<D>::kPer;
     const int32_t a = row.head + p.from * kPer, b = row.head + p.to * kPer;
     if (p.first + lane < a) f(D::get(row.x[p.first + lane]), p.first + lane);
     if (b + lane < p.last) f(D::get(row.x[b + lane]), b + lane);
@@ -291,6 +321,8 @@ __device__ __forceinline__ void walk(const Span<D>& row, const Part<D>& p, F f) 
         for (int k = 0; k < kAhead; ++k) {
             if (i + 64 * k >= p.to) break;
             const Unpack<D> x(r[k]);
+            if constexpr (!std::is_same_v<Skip, Never>)
+                if (!__any(!skip(x.max()))) continue;
 #pragma unroll
             for (int j = 0; j < kPer; ++j) f(x.v[j], row.head + (i + 64 * k) * kPer + j);
         }
@@ -313,8 +345,11 @@ struct Head {
     double c, theta;
     Weigher weigh;
     __device__ Head(const Ask& ask, float m)
-        : m(m), c(fmax(1.4426950408889634 / (double)ask.T, 1e-300)), theta(ask.least()), weigh{(double)m, c} {}
+        : m(m), c(fmax(1.4426950408889634 / (double)ask.T, 1e-300)), theta(ask.least()), weigh((double)m, c) {}
     __device__ __forceinline__ bool likely(float x) const { return !((double)x - (double)m < theta); }  // min-p keeps it
+    // entries in bins before this one are kept by min-p, those two or more behind it are not: the bin of
+    // the least logit, with one to spare for its rounding
+    __device__ int sure_bin(const Binner& bin) const { return theta == -INFINITY ? kBins : max(bin((float)((double)m + theta)) - 1, 0); }
     __device__ Binner binner(int last = kBins - 1) const {
         return Binner{m, (float)fmin(fmax(c * last / 41.5, 1e-30), 3e38), (float)last};
     }
@@ -617,7 +652,7 @@ __global__ __launch_bounds__(256) void k_cat_sample_top(Batch b) {
     RowSpace& to = b.space[r];
     float m = -INFINITY;
     int odd = 0;
-    walk(row, part, [&](float x, int32_t) {
+    walk<4>(row, part, [&](float x, int32_t) {
         m = fmaxf(m, x);
         odd |= !(x < INFINITY);
     });
@@ -631,7 +666,7 @@ __global__ __launch_bounds__(256) void k_cat_sample_top(Batch b) {
 
 template <class D>
 __global__ __launch_bounds__(256) void k_cat_sample_weigh(Batch b) {
-    __shared__ uint64_t hist[kBins];
+    __shared__ uint64_t hist[kBins + 64];  // behind the bins, a place for each lane's entries that weigh nothing
     const int64_t r = blockIdx.x / b.parts, n = b.first + r;
     const int32_t p = blockIdx.x % b.parts, V = b.a.vocab;
     const int tid = threadIdx.x, w = tid >> 6, seg = p * kPartWaves + w;
@@ -649,10 +684,11 @@ __global__ __launch_bounds__(256) void k_cat_sample_weigh(Batch b) {
         const bool count = ask.K > 0;
         for (int i = tid; i < kBins; i += 256) hist[i] = 0;
         __syncthreads();
-        walk(row, part, [&](float x, int32_t) {
+        walk<4>(row, part, [&](float x, int32_t) {
             const uint64_t v = h.weigh(x);
             all += v;
-            if (v) atomicAdd(reinterpret_cast<unsigned long long*>(&hist[bin(x)]), (unsigned long long)(count ? 1 : v));
+            const int at = v ? bin(x) : kBins + (tid & 63);
+            atomicAdd(reinterpret_cast<unsigned long long*>(&hist[at]), (unsigned long long)(count ? 1 : v));
         });
         __syncthreads();
         uint64_t* own = b.hist + (r * b.parts + p) * (int64_t)kBins;
@@ -663,7 +699,7 @@ __global__ __launch_bounds__(256) void k_cat_sample_weigh(Batch b) {
             if (i % kCoarse == 0) to.coarse[p][i / kCoarse] = sum;
         }
     } else {
-        walk(row, part, [&](float x, int32_t) {
+        walk<4>(row, part, [&](float x, int32_t) {
             const uint64_t v = h.weigh(x);
             all += v;
             kept += h.likely(x) ? v : 0;
@@ -708,10 +744,10 @@ __global__ __launch_bounds__(256) void k_cat_sample_near(Batch b) {
     if (!near.fits(ask)) return;
     const int at = near.bin;
     uint64_t kept = 0;
-    // top-k: all up to the bin of the cut.  top-p: that bin, and the weight of those before it from its
-    // coarse bin on (the rest is known by parts, unless min-p takes some of it)
-    const int start = ask.K > 0 || ask.Q > 0.0f ? 0 : at / kCoarse * kCoarse;
-    walk(row, part, [&](float x, int32_t i) {
+    // top-k: all up to the bin of the cut.  top-p: that bin, and the weight of those before it from the
+    // coarse bin on where top-p or min-p cuts (before, it is known by parts)
+    const int sure = h.sure_bin(bin), start = ask.K > 0 ? 0 : min(at, sure) / kCoarse * kCoarse;
+    walk<4>(row, part, [&](float x, int32_t i) {
         const int v = bin(x);
         if (v > at || v < start) return;
         if (v < at && ask.K <= 0) {
@@ -725,7 +761,7 @@ __global__ __launch_bounds__(256) void k_cat_sample_near(Batch b) {
                 if (l < kList) to.list[l] = rank_of(x, i);
             }
         }
-    });
+    }, [&](float x) { return bin(x) > min(at, ask.K > 0 ? kBins : sure + 2); });
     kept = wave_sum(kept);
     if ((tid & 63) == 0) to.kept[seg] = kept;
     __syncthreads();
@@ -863,7 +899,7 @@ __global__ __launch_bounds__(512) void k_cat_sample_answer(Batch b) {
     const Head h(ask, m);
     Team<kThreads> team(slots);
     // top-p rows have the weight of what is kept by whole parts, others by each wave's
-    const int group = ask.K <= 0 && ask.P < 1.0f && !(ask.Q > 0.0f) ? kPartWaves : 1, shares = waves / group;
+    const int group = ask.K <= 0 && ask.P < 1.0f ? kPartWaves : 1, shares = waves / group;
     if (group == 1) {
         if (tid < waves) segs[tid] = v_kept;
     } else {
@@ -877,16 +913,19 @@ __global__ __launch_bounds__(512) void k_cat_sample_answer(Batch b) {
             for (int i = tid; i < many; i += kThreads) room.list[i] = r.list[i];
         find_near<kThreads>(ask, r, b.hist + blockIdx.x * (int64_t)b.parts * kBins, b.parts, room.near);
         const Near& near = room.near.near;
+        const int sure = h.sure_bin(h.binner());
         if (ask.T > kMostT || !near.fits(ask) || many > kList) return slow_row<D, kThreads>(b.a, n, ask, m, s);
         __syncthreads();
         if (group > 1 && tid < b.parts) {
             uint64_t known = 0;
 #pragma unroll 8
-            for (int i = 0; i < near.bin / kCoarse; ++i) known += r.coarse[tid][i];
+            for (int i = 0; i < min(near.bin, sure) / kCoarse; ++i) known += r.coarse[tid][i];
             segs[tid] += known;
         }
         __syncthreads();
-        if (many <= 512) {  // one wave is faster than the barriers of eight
+        if (ask.K <= 0 && near.bin > sure + 2) {
+            // min-p cuts before top-p does
+        } else if (many <= 512) {  // one wave is faster than the barriers of eight
             if (tid < 64) {
                 v = settle<D, 64, 256>(Team<64>(one), room, ask, h, many, row, waves, group, V);
                 if (tid == 0) room.verdict = v;
@@ -925,7 +964,7 @@ __global__ __launch_bounds__(512) void k_cat_sample_answer(Batch b) {
             return q;
         };
         uint64_t sum = 0;
-        walk(row, wave_part(w), [&](float x, int32_t i) { sum += weight(x, i); });
+        walk<1>(row, wave_part(w), [&](float x, int32_t i) { sum += weight(x, i); });
         sum = wave_sum(sum);
         if ((tid & 63) == 0) s.slots[w] = sum;
         __syncthreads();
@@ -994,7 +1033,7 @@ __global__ __launch_bounds__(64) void k_cat_sample_tiny(Args A, int64_t rows) {
         A.logprob[n] = A.kept[n] = 0.0f;
         return;
     }
-    const Weigher weigh{(double)m, fmax(1.4426950408889634 / (double)ask.T, 1e-300)};
+    const Weigher weigh((double)m, fmax(1.4426950408889634 / (double)ask.T, 1e-300));
     uint64_t all = 0;
     for (int i = 0; i < V; ++i) {
         wt[i] = weigh(x[i]);
