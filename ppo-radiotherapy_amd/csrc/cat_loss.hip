@@ -108,14 +108,6 @@ __device__ __forceinline__ uint4 pack(const float* v) {
     return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
-// 16 bytes of entries that add nothing
-template <class D>
-__device__ __forceinline__ uint4 nothing() {
-    if constexpr (sizeof(typename D::raw) == 4) return make_uint4(0xff800000u, 0xff800000u, 0xff800000u, 0xff800000u);
-    const uint32_t two = (uint32_t)D::put(-INFINITY) * 0x10001u;
-    return make_uint4(two, two, two, two);
-}
-
 // ---- a row's sums ----------------------------------------------------------
 // In units of log 2: t = (x - m) c, c = log2(e) / T.  exp2 is the hardware's
 // (within one unit of the last place); up to eight terms are added in f32,

@@ -169,6 +169,14 @@ struct Unpack {
     }
 };
 
+// 16 bytes of entries that add nothing
+template <class D>
+__device__ __forceinline__ uint4 nothing() {
+    if constexpr (sizeof(typename D::raw) == 4) return make_uint4(0xff800000u, 0xff800000u, 0xff800000u, 0xff800000u);
+    const uint32_t two = (uint32_t)D::put(-INFINITY) * 0x10001u;
+    return make_uint4(two, two, two, two);
+}
+
 // ---- argument checks -------------------------------------------------------
 inline int elem_size(int32_t dtype) { return dtype == RT_DT_F32 ? 4 : 2; }
 inline bool bad_type(int32_t dtype) { return dtype != RT_DT_F32 && dtype != RT_DT_BF16 && dtype != RT_DT_F16; }

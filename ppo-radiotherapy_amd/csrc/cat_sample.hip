@@ -300,7 +300,7 @@ struct Part {
 };
 
 // f(x, i) for every entry of a part; the lanes of one wave together, kAhead
-// pieces at a time.  `skip` says of a maximum whether all that is not above it
+// pieces at a time, -inf where a lane has none.  `skip` says of a maximum whether all that is not above it
 // can be left out.
 struct Never {
     __device__ __forceinline__ bool operator()(float) const { return false; }
@@ -310,16 +310,15 @@ __device__ __forceinline__ void walk(const Span<D>& row, const Part<D>& p, F f, 
     const int lane = threadIdx.x & 63;
     constexpr int kPer = Span<D>::kPer;
     const int32_t a = row.head + p.from * kPer, b = row.head + p.to * kPer;
-    if (p.first + lane < a) f(D::get(row.x[p.first + lane]), p.first + lane);
-    if (b + lane < p.last) f(D::get(row.x[b + lane]), b + lane);
-    for (int32_t i = p.from + lane; i < p.to; i += 64 * kAhead) {
+    if (p.first < a) f(p.first + lane < a ? D::get(row.x[p.first + lane]) : -INFINITY, p.first + lane);
+    if (b < p.last) f(b + lane < p.last ? D::get(row.x[b + lane]) : -INFINITY, b + lane);
+    for (int32_t at = p.from; at < p.to; at += 64 * kAhead) {
+        const int32_t i = at + lane;
         uint4 r[kAhead];
 #pragma unroll
-        for (int k = 0; k < kAhead; ++k)
-            if (i + 64 * k < p.to) r[k] = row.piece(i + 64 * k);
+        for (int k = 0; k < kAhead; ++k) r[k] = i + 64 * k < p.to ? row.piece(i + 64 * k) : nothing<D>();
 #pragma unroll
         for (int k = 0; k < kAhead; ++k) {
-            if (i + 64 * k >= p.to) break;
             const Unpack<D> x(r[k]);
             if constexpr (!std::is_same_v<Skip, Never>)
                 if (!__any(!skip(x.max()))) continue;
@@ -335,6 +334,21 @@ __device__ __forceinline__ void walk(const Span<D>& row, const Part<D>& p, F f, 
 struct Binner {
     float m, scale, last;
     __device__ __forceinline__ int operator()(float x) const { return (int)fminf((m - x) * scale, last); }
+    // the least number whose bin is not behind b >= 0
+    __device__ uint32_t least_key(int b) const {
+        uint32_t lo = 0x00800000u, hi = key_of(m);  // from the lowest finite one
+        while (lo < hi) {
+            const uint32_t mid = lo + (hi - lo) / 2;
+            if ((*this)(of_key(mid)) <= b) hi = mid;
+            else lo = mid + 1;
+        }
+        return lo;
+    }
+    // the numbers of bins [from, to], which are not empty of numbers
+    __device__ void range(int from, int to, float* least, float* most) const {
+        *least = of_key(least_key(to));
+        *most = from > 0 ? of_key(least_key(from - 1) - 1) : m;
+    }
 };
 
 constexpr float kMostT = 1e30f;  // above, numbers that the bins cannot tell apart weigh something
@@ -504,7 +518,7 @@ __device__ __forceinline__ K team_key(T& team, uint64_t* hist, Each each, Key ke
         each([&](int e) { s += key(e) >= least ? value(e) : 0; });
         return team.sum(s);
     };
-    while (true) {
+    for (int step = 0; step < 64; ++step) {  // keys have 32 bits: halving alone ends sooner
         uint64_t sum = from(k);
         if (sum >= want) {
             *above = over;
@@ -524,6 +538,8 @@ __device__ __forceinline__ K team_key(T& team, uint64_t* hist, Each each, Key ke
         each([&](int e) { k = key(e) < hi ? max(k, key(e)) : k; });
         k = team.all(k, [](K a, K b) { return max(a, b); });
     }
+    *above = over;
+    return lo;
 }
 
 // The middle of two keys of numbers: half way between the numbers (those around
@@ -652,7 +668,7 @@ __global__ __launch_bounds__(256) void k_cat_sample_top(Batch b) {
     RowSpace& to = b.space[r];
     float m = -INFINITY;
     int odd = 0;
-    walk<4>(row, part, [&](float x, int32_t) {
+    walk<2>(row, part, [&](float x, int32_t) {
         m = fmaxf(m, x);
         odd |= !(x < INFINITY);
     });
@@ -684,7 +700,7 @@ __global__ __launch_bounds__(256) void k_cat_sample_weigh(Batch b) {
         const bool count = ask.K > 0;
         for (int i = tid; i < kBins; i += 256) hist[i] = 0;
         __syncthreads();
-        walk<4>(row, part, [&](float x, int32_t) {
+        walk<2>(row, part, [&](float x, int32_t) {
             const uint64_t v = h.weigh(x);
             all += v;
             const int at = v ? bin(x) : kBins + (tid & 63);
@@ -699,11 +715,16 @@ __global__ __launch_bounds__(256) void k_cat_sample_weigh(Batch b) {
             if (i % kCoarse == 0) to.coarse[p][i / kCoarse] = sum;
         }
     } else {
-        walk<4>(row, part, [&](float x, int32_t) {
-            const uint64_t v = h.weigh(x);
-            all += v;
-            kept += h.likely(x) ? v : 0;
-        });
+        if (h.theta == -INFINITY) {
+            walk<2>(row, part, [&](float x, int32_t) { all += h.weigh(x); });
+            kept = all;
+        } else {
+            walk<2>(row, part, [&](float x, int32_t) {
+                const uint64_t v = h.weigh(x);
+                all += v;
+                kept += h.likely(x) ? v : 0;
+            });
+        }
     }
     all = wave_sum(all);
     kept = wave_sum(kept);
@@ -722,10 +743,9 @@ __device__ __forceinline__ uint64_t sum_of(const uint64_t* v, int n) {
 
 template <class D>
 __global__ __launch_bounds__(256) void k_cat_sample_near(Batch b) {
-    constexpr int kOwn = 512;
+    constexpr int kOwn = 256;
     __shared__ NearRoom<256> room;
-    __shared__ int many, start_at;
-    __shared__ uint64_t own[kOwn];  // the block's entries, added to the row's list at once
+    __shared__ uint64_t own[kPartWaves][kOwn];  // a wave's entries, added to the row's list at once
     const int64_t r = blockIdx.x / b.parts, n = b.first + r;
     const int32_t p = blockIdx.x % b.parts, V = b.a.vocab;
     const int tid = threadIdx.x, w = tid >> 6, seg = p * kPartWaves + w;
@@ -738,38 +758,45 @@ __global__ __launch_bounds__(256) void k_cat_sample_near(Batch b) {
     if (m != m || !(ask.T > 0.0f) || !cuts(ask) || ask.T > kMostT) return;
     const Head h(ask, m);
     const Binner bin = h.binner();
-    if (tid == 0) many = 0;
+    int many = 0;
     find_near<256>(ask, to, b.hist + r * b.parts * (int64_t)kBins, b.parts, room);
     const Near& near = room.near;
     if (!near.fits(ask)) return;
     const int at = near.bin;
     uint64_t kept = 0;
-    // top-k: all up to the bin of the cut.  top-p: that bin, and the weight of those before it from the
-    // coarse bin on where top-p or min-p cuts (before, it is known by parts)
-    const int sure = h.sure_bin(bin), start = ask.K > 0 ? 0 : min(at, sure) / kCoarse * kCoarse;
-    walk<4>(row, part, [&](float x, int32_t i) {
-        const int v = bin(x);
-        if (v > at || v < start) return;
-        if (v < at && ask.K <= 0) {
-            kept += h.likely(x) ? h.weigh(x) : 0;
-        } else if (h.weigh(x)) {
-            const int o = atomicAdd(&many, 1);
+    // top-k: all up to the bin of the cut.  top-p: that bin; what stands before it is known by parts, but for
+    // the bins where min-p cuts.  Bins as ranges of numbers: most entries are neither
+    const int sure = h.sure_bin(bin);
+    const bool last_bins = at > kBins - 64;  // where the weights end
+    float low, high, low_p = INFINITY, high_p = -INFINITY;
+    bin.range(ask.K > 0 ? 0 : at, at, &low, &high);
+    if (ask.K <= 0 && min(sure + 2, at - 1) >= sure) bin.range(sure, min(sure + 2, at - 1), &low_p, &high_p);
+    walk<2>(row, part, [&](float x, int32_t i) {
+        const bool listed = x >= low && x <= high, split = x >= low_p && x <= high_p;
+        if (!__any(listed || split)) return;
+        // behind the entries of this wave: its lanes in turn
+        const bool add = listed && (!last_bins || h.weigh(x));
+        const uint64_t who = __ballot(add);
+        if (add) {
+            const int o = many + __popcll(who & ((1ull << (tid & 63)) - 1));
             if (o < kOwn) {
-                own[o] = rank_of(x, i);
+                own[w][o] = rank_of(x, i);
             } else {
                 const int l = atomicAdd(&to.many, 1);
                 if (l < kList) to.list[l] = rank_of(x, i);
             }
         }
-    }, [&](float x) { return bin(x) > min(at, ask.K > 0 ? kBins : sure + 2); });
+        many += __popcll(who);
+        if (split && h.likely(x)) kept += h.weigh(x);
+    }, [&](float x) { return x < fminf(low, low_p); });
     kept = wave_sum(kept);
     if ((tid & 63) == 0) to.kept[seg] = kept;
-    __syncthreads();
     const int mine = min(many, kOwn);
-    if (tid == 0 && mine) start_at = atomicAdd(&to.many, mine);
-    __syncthreads();
-    for (int i = tid; i < mine; i += 256)
-        if (start_at + i < kList) to.list[start_at + i] = own[i];
+    int first = 0;
+    if ((tid & 63) == 0 && mine) first = atomicAdd(&to.many, mine);
+    first = __shfl(first, 0);
+    for (int i = tid & 63; i < mine; i += 64)
+        if (first + i < kList) to.list[first + i] = own[w][i];
 }
 
 // Which of the equal shares of a row has an entry.
@@ -834,7 +861,9 @@ __device__ __forceinline__ Verdict settle(Team<THREADS> team, R& room, const Ask
             want = ask.limit(team.sum(mass));
         }
         const auto value = [&](int i) { return round == 0 ? (uint64_t)(room.weight[i] != 0) : room.weight[i]; };
-        const uint32_t c = team_key<BINS, uint32_t>(team, room.hist, each, key, place, value, want, middle_key, &above);
+        // (a bin of 16-bit logits often has one number, many times)
+        const uint32_t c = top == low ? (above = 0, top)
+                                      : team_key<BINS, uint32_t>(team, room.hist, each, key, place, value, want, middle_key, &above);
         const uint64_t one = round == 0 ? 1 : h.weigh(of_key(c)), ties = (want - above + one - 1) / one;
         const auto tie = [&](int i) { return (uint64_t)(key(i) == c && room.weight[i]); };
         uint64_t equal = 0;
@@ -891,7 +920,7 @@ __global__ __launch_bounds__(512) void k_cat_sample_answer(Batch b) {
     }
     if (!(ask.T > 0.0f)) {
         int p = 0;
-        while (r.top[p] != m) ++p;
+        while (p < b.parts - 1 && r.top[p] != m) ++p;
         const int32_t from = Part<D>(row, V, p * kPartWaves, waves).first;
         const int32_t to = Part<D>(row, V, (p + 1) * kPartWaves - 1, waves).last;
         return greedy<D, kThreads>(b.a, n, m, from, to - from, row, s);
@@ -916,16 +945,21 @@ __global__ __launch_bounds__(512) void k_cat_sample_answer(Batch b) {
         const int sure = h.sure_bin(h.binner());
         if (ask.T > kMostT || !near.fits(ask) || many > kList) return slow_row<D, kThreads>(b.a, n, ask, m, s);
         __syncthreads();
-        if (group > 1 && tid < b.parts) {
-            uint64_t known = 0;
-#pragma unroll 8
-            for (int i = 0; i < min(near.bin, sure) / kCoarse; ++i) known += r.coarse[tid][i];
-            segs[tid] += known;
+        if (group > 1) {  // the bins before both cuts, of each part: whole coarse ones, and the rest
+            const int end = min(near.bin, sure), coarse = end / kCoarse;
+            const int lane = tid & 63;
+            for (int p = tid >> 6; p < b.parts; p += kThreads / 64) {
+                const uint64_t* fine = b.hist + (blockIdx.x * (int64_t)b.parts + p) * kBins + coarse * kCoarse;
+                uint64_t known = lane < coarse ? r.coarse[p][lane] : 0;
+                if (lane < end % kCoarse) known += fine[lane];
+                known = wave_sum(known);
+                if (lane == 0) segs[p] += known;
+            }
         }
         __syncthreads();
         if (ask.K <= 0 && near.bin > sure + 2) {
             // min-p cuts before top-p does
-        } else if (many <= 512) {  // one wave is faster than the barriers of eight
+        } else if (many <= 128) {  // one wave is faster than the barriers of eight
             if (tid < 64) {
                 v = settle<D, 64, 256>(Team<64>(one), room, ask, h, many, row, waves, group, V);
                 if (tid == 0) room.verdict = v;
