@@ -68,16 +68,19 @@ class _Rows:
             raise ValueError("logits: expected a tensor on the GPU")
         self.x, self.device = logits, logits.device
         self.lead, self.vocab = shape[:-1], shape[-1]
-        self.n = math.prod(self.lead)
+        self.n = shape[0] if len(shape) == 2 else math.prod(self.lead)
         if self.vocab > _lib.CAT_MAX_VOCAB:
             raise ValueError(f"logits: {self.vocab} entries in a row, at most {_lib.CAT_MAX_VOCAB}")
         if self.n > 2**31 - 1:
             raise ValueError(f"logits: {self.n} rows, at most 2^31 - 1")
+        self.stride = self.vocab
+        if logits.is_contiguous():
+            return
         strides = logits.stride()
         if self.vocab > 1 and strides[-1] != 1:
             raise ValueError("logits: the entries of a row are not adjacent (stride 1)")
         # the leading dimensions, from the last: each as far apart as all rows before it together
-        self.stride, rows = self.vocab, 1
+        rows = 1
         for size, step in zip(reversed(self.lead), reversed(strides[:-1])):
             if size == 1 or self.n == 0:
                 continue
@@ -96,7 +99,7 @@ class _Rows:
             return None
         if not isinstance(t, torch.Tensor):
             raise TypeError(f"{name}: expected a tensor")
-        if t.shape != self.lead + tail:
+        if t.shape != (self.lead + tail if tail else self.lead):
             raise ValueError(f"{name}: shape {tuple(t.shape)}, expected {tuple(self.lead + tail)}")
         if t.device != self.device:
             raise ValueError(f"{name}: on {t.device}, the logits on {self.device}")
@@ -161,6 +164,18 @@ def _coef(v, name: str, low=None, positive=False) -> float:
     return v
 
 
+_SAMPLING_OFF = {"temperature": 1.0, "top_k": 0, "top_p": 1.0, "min_p": 0.0}
+
+
+@functools.lru_cache(maxsize=256)
+def _sampling(temperature, top_k, top_p, min_p):
+    """The parameters of all rows, checked."""
+    if not 0 <= top_k < 2**31 or int(top_k) != top_k:
+        raise ValueError(f"top_k: {top_k}")
+    return (_coef(temperature, "temperature", low=0.0), int(top_k), _coef(top_p, "top_p", low=0.0),
+            _coef(min_p, "min_p", low=0.0))
+
+
 def sample(logits, u, *, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0) -> Sample:
     """One action per row from uniform numbers u in [0, 1) (rt_cat_sample).
 
@@ -169,24 +184,19 @@ def sample(logits, u, *, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0) -> Samp
     Rows without a distribution (a NaN, +inf, nothing but -inf) get action -1
     and NaN."""
     r = _Rows(logits)
-    p = _lib.RtCatSampling()
-    hold = [r.per_row(u, "u")]
-    if hold[0] is None:
+    u = r.per_row(u, "u")
+    if u is None:
         raise TypeError("u: expected a tensor")
-    p.u = hold[0].data_ptr()
-    for name, v, dtype in (("temperature", temperature, torch.float32), ("top_k", top_k, torch.int32),
-                           ("top_p", top_p, torch.float32), ("min_p", min_p, torch.float32)):
+    params = {"temperature": temperature, "top_k": top_k, "top_p": top_p, "min_p": min_p}
+    rows = {}
+    for name, v in params.items():
         if isinstance(v, torch.Tensor):
-            if dtype == torch.int32 and v.dtype == torch.int64:
+            if name == "top_k" and v.dtype == torch.int64:
                 v = v.clamp(0, 2**31 - 1)
-            hold.append(r.per_row(v, name, dtype))
-            setattr(p, name, hold[-1].data_ptr())
-        elif dtype == torch.int32:
-            if int(v) != v or not 0 <= v < 2**31:
-                raise ValueError(f"top_k: {v}")
-            p.top_k_all = int(v)
-        else:
-            setattr(p, name + "_all", _coef(v, name, low=0.0))
+            rows[name] = r.per_row(v, name, torch.int32 if name == "top_k" else torch.float32)
+            params[name] = _SAMPLING_OFF[name]
+    p = _lib.RtCatSampling(u.data_ptr(), *((_lib.ptr(rows.get(k)) for k in params) if rows else (None,) * 4),
+                           *_sampling(*params.values()))
     out = Sample(r.empty(torch.int64), r.empty(), r.empty())
     if r.n == 0:
         return out
@@ -196,25 +206,26 @@ def sample(logits, u, *, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0) -> Samp
     return out
 
 
+@functools.lru_cache(maxsize=256)
+def _ppo_hparams(temperature, low, high, ent_coef, kl_coef):
+    return _lib.RtCatPpoHparams(_coef(temperature, "temperature", positive=True), _coef(low, "clip_coef", low=0.0),
+                                _coef(high, "clip_coef_high", low=0.0), _coef(ent_coef, "ent_coef"),
+                                _coef(kl_coef, "kl_coef"))
+
+
 class _Ppo:
     """The arguments of a PPO loss, checked and laid out."""
 
     def __init__(self, logits, actions, old_logprobs, advantages, weights, ref_logprobs, temperature, clip_coef,
                  clip_coef_high, ent_coef, kl_coef):
         r = self.r = _Rows(logits)
-        need = {"actions": (actions, torch.int64), "old_logprobs": (old_logprobs, torch.float32),
-                "advantages": (advantages, torch.float32)}
-        self.t = {}
-        for name, (t, dtype) in need.items():
-            self.t[name] = r.per_row(t, name, dtype)
-            if t is None:
-                raise TypeError(f"{name}: expected a tensor")
-        self.t["weights"] = r.per_row(weights, "weights")
-        self.t["ref_logprobs"] = r.per_row(ref_logprobs, "ref_logprobs")
-        low = _coef(clip_coef, "clip_coef", low=0.0)
-        high = low if clip_coef_high is None else _coef(clip_coef_high, "clip_coef_high", low=0.0)
-        self.hp = _lib.RtCatPpoHparams(_coef(temperature, "temperature", positive=True), low, high,
-                                       _coef(ent_coef, "ent_coef"), _coef(kl_coef, "kl_coef"))
+        if actions is None or old_logprobs is None or advantages is None:
+            raise TypeError("actions, old_logprobs, advantages: expected tensors")
+        self.actions = r.per_row(actions, "actions", torch.int64)
+        self.held = (r.per_row(old_logprobs, "old_logprobs"), r.per_row(advantages, "advantages"),
+                     r.per_row(weights, "weights"), r.per_row(ref_logprobs, "ref_logprobs"))
+        self.hp = _ppo_hparams(float(temperature), float(clip_coef),
+                               float(clip_coef if clip_coef_high is None else clip_coef_high), float(ent_coef), float(kl_coef))
         if self.hp.kl_coef != 0.0 and ref_logprobs is None:
             raise ValueError("kl_coef without ref_logprobs")
 
@@ -229,9 +240,7 @@ class _Ppo:
             res.stats.zero_()
             return res, state
         ws, n = _workspace("rt_cat_loss_workspace_bytes", r)
-        t = self.t
-        batch = _lib.RtCatPpoBatch(t["actions"].data_ptr(), t["old_logprobs"].data_ptr(), t["advantages"].data_ptr(),
-                                   _lib.ptr(t["weights"]), _lib.ptr(t["ref_logprobs"]))
+        batch = _lib.RtCatPpoBatch(self.actions.data_ptr(), *map(_lib.ptr, self.held))
         out = _lib.RtCatPpoOut(res.loss.data_ptr(), res.logprob.data_ptr(), res.entropy.data_ptr(),
                                res.stats.data_ptr(), _lib.ptr(grad), stride, _lib.ptr(state))
         r.call(_lib.load().rt_cat_ppo, "rt_cat_ppo", ctypes.byref(r.arg()), ctypes.byref(batch), ctypes.byref(self.hp),
@@ -239,18 +248,24 @@ class _Ppo:
         return res, state
 
 
+def _with_grad(fn, logits, op):
+    loss = fn.apply(logits, op)
+    return op.rest._replace(loss=loss)
+
+
 class _PpoFn(torch.autograd.Function):
+    """The loss alone: the other results go by `op`."""
+
     @staticmethod
     def forward(ctx, logits, op):
-        res, state = op.run(keep=True)
-        ctx.op = op
-        ctx.save_for_backward(logits, op.t["actions"], state)
-        ctx.mark_non_differentiable(*res[1:])
-        return tuple(res)
+        op.rest, state = op.run(keep=True)
+        ctx.temperature = op.hp.temperature
+        ctx.save_for_backward(logits, op.actions, state)
+        return op.rest.loss
 
     @staticmethod
     @torch.autograd.function.once_differentiable
-    def backward(ctx, gloss, *_):
+    def backward(ctx, gloss):
         logits, actions, state = ctx.saved_tensors
         r = _Rows(logits)
         grad, stride = r.grad_buffer(None)
@@ -258,7 +273,7 @@ class _PpoFn(torch.autograd.Function):
             return grad, None
         gloss = gloss.to(torch.float32).contiguous()
         r.call(_lib.load().rt_cat_ppo_backward, "rt_cat_ppo_backward", ctypes.byref(r.arg()), actions.data_ptr(),
-               ctx.op.hp.temperature, state.data_ptr(), gloss.data_ptr(), grad.data_ptr(), stride)
+               ctx.temperature, state.data_ptr(), gloss.data_ptr(), grad.data_ptr(), stride)
         return grad, None
 
 
@@ -274,7 +289,7 @@ def ppo_loss(logits, actions, old_logprobs, advantages, *, weights=None, ref_log
     op = _Ppo(logits, actions, old_logprobs, advantages, weights, ref_logprobs, temperature, clip_coef,
               clip_coef_high, ent_coef, kl_coef)
     if torch.is_grad_enabled() and logits.requires_grad:
-        return PpoLoss(*_PpoFn.apply(logits, op))
+        return _with_grad(_PpoFn, logits, op)
     return op.run()[0]
 
 
@@ -326,23 +341,23 @@ class _Distill:
 class _DistillFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, op):
-        res, state = op.run(keep=True)
-        ctx.op = op
-        ctx.save_for_backward(logits, op.idx, op.top, *(t for t in (op.lse, op.weights) if t is not None), state)
-        ctx.mark_non_differentiable(res.kl)
-        return tuple(res)
+        op.rest, state = op.run(keep=True)
+        ctx.k, ctx.temperature = op.k, op.temperature
+        ctx.save_for_backward(logits, op.idx, op.top, op.lse, op.weights, state)
+        return op.rest.loss
 
     @staticmethod
     @torch.autograd.function.once_differentiable
-    def backward(ctx, gloss, *_):
-        logits, *_, state = ctx.saved_tensors  # raises where one of them was changed in place
+    def backward(ctx, gloss):
+        logits, idx, top, lse, weights, state = ctx.saved_tensors  # raises where one of them was changed in place
         r = _Rows(logits)
         grad, stride = r.grad_buffer(None)
         if r.n == 0:
             return grad, None
         gloss = gloss.to(torch.float32).contiguous()
+        teacher = _lib.RtCatTeacher(idx.data_ptr(), top.data_ptr(), _lib.ptr(lse), _lib.ptr(weights), ctx.k, ctx.temperature)
         r.call(_lib.load().rt_cat_distill_backward, "rt_cat_distill_backward", ctypes.byref(r.arg()),
-               ctypes.byref(ctx.op.arg()), state.data_ptr(), gloss.data_ptr(), grad.data_ptr(), stride)
+               ctypes.byref(teacher), state.data_ptr(), gloss.data_ptr(), grad.data_ptr(), stride)
         return grad, None
 
 
@@ -356,7 +371,7 @@ def distill_loss(logits, teacher_idx, teacher_logits, *, weights=None, teacher_l
     weights: as ppo_loss.  Only `loss` is differentiable, by the logits."""
     op = _Distill(logits, teacher_idx, teacher_logits, weights, teacher_lse, temperature)
     if torch.is_grad_enabled() and logits.requires_grad:
-        return DistillLoss(*_DistillFn.apply(logits, op))
+        return _with_grad(_DistillFn, logits, op)
     return op.run()[0]
 
 
