@@ -364,8 +364,10 @@ struct Head {
     // entries in bins before this one are kept by min-p, those two or more behind it are not: the bin of
     // the least logit, with one to spare for its rounding
     __device__ int sure_bin(const Binner& bin) const { return theta == -INFINITY ? kBins : max(bin((float)((double)m + theta)) - 1, 0); }
-    __device__ Binner binner(int last = kBins - 1) const {
-        return Binner{m, (float)fmin(fmax(c * last / 41.5, 1e-30), 3e38), (float)last};
+    // Bins 0 to `last` over what weighs something, or over `reach` where that is less.
+    __device__ Binner binner(int last, float reach) const {
+        const double scale = fmax(c / 41.5, 1.0 / (double)reach);  // reach 0: infinite, as it is clamped
+        return Binner{m, (float)fmin(fmax(scale * last, 1e-30), 3e38), (float)last};
     }
 };
 
@@ -556,7 +558,7 @@ __device__ __forceinline__ uint32_t middle_key(uint32_t lo, uint32_t hi) {
 constexpr int kParts = 64, kPartWaves = 4;
 
 struct RowSpace {
-    float top[kParts];                          // NaN: a NaN or +inf
+    float top[kParts], low[kParts];             // largest (NaN: a NaN or +inf) and least finite logit
     uint64_t all[kParts * kPartWaves];          // the weight of each wave's part
     uint64_t kept[kParts * kPartWaves];         // what of it is surely kept
     uint64_t coarse[kParts][64];                // the histogram of each part by 32 bins
@@ -573,15 +575,18 @@ struct Batch {
     int32_t parts;
 };
 
-// The maximum of the row from those of its parts; NaN for a row without an answer.
-__device__ __forceinline__ float part_top(const RowSpace& r, int32_t parts) {
-    const int lane = threadIdx.x & 63;
-    return lane < parts ? r.top[lane] : -INFINITY;
-}
-__device__ __forceinline__ float row_top(float v) {
-    const float m = wave_max(v);
-    return __any(v != v) || m == -INFINITY ? NAN : m;
-}
+// The maximum of the row, and how far its least finite logit is below; from
+// those of its parts, by each wave.  NaN for a row without an answer.
+struct Extent {
+    float m, reach;
+    __device__ __forceinline__ Extent(const RowSpace& r, int32_t parts) {
+        const int lane = threadIdx.x & 63;
+        const float top = lane < parts ? r.top[lane] : -INFINITY, low = lane < parts ? r.low[lane] : INFINITY;
+        m = wave_max(top);
+        reach = m + wave_max(-low);
+        if (__any(top != top) || m == -INFINITY) m = NAN;
+    }
+};
 
 __device__ __forceinline__ bool cuts(const Ask& ask) { return ask.K > 0 || ask.P < 1.0f; }
 
@@ -666,16 +671,19 @@ __global__ __launch_bounds__(256) void k_cat_sample_top(Batch b) {
     const Span<D> row(static_cast<const typename D::raw*>(b.a.x) + n * b.a.stride, V);
     const Part<D> part(row, V, p * kPartWaves + w, b.parts * kPartWaves);
     RowSpace& to = b.space[r];
-    float m = -INFINITY;
+    float m = -INFINITY, low = INFINITY;
     int odd = 0;
     walk<2>(row, part, [&](float x, int32_t) {
         m = fmaxf(m, x);
+        low = fminf(low, x == -INFINITY ? INFINITY : x);
         odd |= !(x < INFINITY);
     });
     m = block_max<256>(m, fs);
+    low = -block_max<256>(-low, fs);
     odd = __syncthreads_or(odd);
     if (threadIdx.x == 0) {
         to.top[p] = odd ? NAN : m;
+        to.low[p] = low;
         if (p == 0) to.many = 0;
     }
 }
@@ -689,14 +697,14 @@ __global__ __launch_bounds__(256) void k_cat_sample_weigh(Batch b) {
     const Span<D> row(static_cast<const typename D::raw*>(b.a.x) + n * b.a.stride, V);
     const Part<D> part(row, V, seg, b.parts * kPartWaves);
     RowSpace& to = b.space[r];
-    const float v_top = part_top(to, b.parts);
+    const Extent extent(to, b.parts);
+    const float m = extent.m;
     const Ask ask(b.a.p, n, V);
-    const float m = row_top(v_top);
     if (m != m || !(ask.T > 0.0f)) return;
     const Head h(ask, m);
     uint64_t all = 0, kept = 0;
     if (cuts(ask)) {
-        const Binner bin = h.binner();
+        const Binner bin = h.binner(kBins - 1, extent.reach);
         const bool count = ask.K > 0;
         for (int i = tid; i < kBins; i += 256) hist[i] = 0;
         __syncthreads();
@@ -752,12 +760,12 @@ __global__ __launch_bounds__(256) void k_cat_sample_near(Batch b) {
     const Span<D> row(static_cast<const typename D::raw*>(b.a.x) + n * b.a.stride, V);
     const Part<D> part(row, V, seg, b.parts * kPartWaves);
     RowSpace& to = b.space[r];
-    const float v_top = part_top(to, b.parts);
+    const Extent extent(to, b.parts);
+    const float m = extent.m;
     const Ask ask(b.a.p, n, V);
-    const float m = row_top(v_top);
     if (m != m || !(ask.T > 0.0f) || !cuts(ask) || ask.T > kMostT) return;
     const Head h(ask, m);
-    const Binner bin = h.binner();
+    const Binner bin = h.binner(kBins - 1, extent.reach);
     int many = 0;
     find_near<256>(ask, to, b.hist + r * b.parts * (int64_t)kBins, b.parts, room);
     const Near& near = room.near;
@@ -827,7 +835,7 @@ struct Room {
 // From the list, by a team: top-k rows whole, of top-p rows the cut, and the
 // weight of what the list has of the kept ones on to their shares of the row.
 template <class D, int THREADS, int BINS, class R>
-__device__ __forceinline__ Verdict settle(Team<THREADS> team, R& room, const Ask& ask, const Head& h, int many,
+__device__ __forceinline__ Verdict settle(Team<THREADS>& team, R& room, const Ask& ask, const Head& h, int many,
                                           const Span<D>& row, int waves, int group, int32_t V) {
     const Near& near = room.near.near;
     const int t = threadIdx.x % THREADS;
@@ -909,11 +917,11 @@ __global__ __launch_bounds__(512) void k_cat_sample_answer(Batch b) {
     const Span<D> row(static_cast<const typename D::raw*>(b.a.x) + n * b.a.stride, V);
     const RowSpace& r = b.space[blockIdx.x];
     // one trip to memory for all of this
-    const float v_top = part_top(r, b.parts);
+    const Extent extent(r, b.parts);
+    const float m = extent.m;
     const Ask ask(b.a.p, n, V);
     const uint64_t v_all = tid < waves ? r.all[tid] : 0, v_kept = tid < waves ? r.kept[tid] : 0;
     const int many = r.many;
-    const float m = row_top(v_top);
     if (m != m) {
         if (tid == 0) no_answer(b.a, n);
         return;
@@ -942,7 +950,7 @@ __global__ __launch_bounds__(512) void k_cat_sample_answer(Batch b) {
             for (int i = tid; i < many; i += kThreads) room.list[i] = r.list[i];
         find_near<kThreads>(ask, r, b.hist + blockIdx.x * (int64_t)b.parts * kBins, b.parts, room.near);
         const Near& near = room.near.near;
-        const int sure = h.sure_bin(h.binner());
+        const int sure = h.sure_bin(h.binner(kBins - 1, extent.reach));
         if (ask.T > kMostT || !near.fits(ask) || many > kList) return slow_row<D, kThreads>(b.a, n, ask, m, s);
         __syncthreads();
         if (group > 1) {  // the bins before both cuts, of each part: whole coarse ones, and the rest
@@ -961,7 +969,8 @@ __global__ __launch_bounds__(512) void k_cat_sample_answer(Batch b) {
             // min-p cuts before top-p does
         } else if (many <= 128) {  // one wave is faster than the barriers of eight
             if (tid < 64) {
-                v = settle<D, 64, 256>(Team<64>(one), room, ask, h, many, row, waves, group, V);
+                Team<64> wave(one);
+                v = settle<D, 64, 256>(wave, room, ask, h, many, row, waves, group, V);
                 if (tid == 0) room.verdict = v;
             }
             __syncthreads();
@@ -1187,7 +1196,7 @@ __global__ __launch_bounds__(THREADS < 256 ? 256 : THREADS) void k_cat_sample_he
         }
     };
     uint64_t mass = all;
-    const Binner bin = h.binner(kFine - 1);
+    const Binner bin = h.binner(kFine - 1, INFINITY);
     const auto key = [&](int e) { return key_of(x[e]); };
     const auto place = [&](int e) { return bin(x[e]); };
     uint64_t* mine_hist = hist[threadIdx.x / THREADS];

@@ -90,7 +90,7 @@ def test_sample_ties_and_peaks(C, kind, v, dtype):
         check_sample(C, x, torch.rand(4, generator=gen(i), device="cuda"), par)
 
 
-@pytest.mark.parametrize("v", [11, 1000, 9000])
+@pytest.mark.parametrize("v", [11, 1000, 9000, 20000])
 def test_sample_extreme_numbers(C, v):
     """u at and beyond its ends; per-row parameters at and beyond theirs."""
     u = torch.tensor([0.0, 2.0 ** -24, 0.5, 1 - 2.0 ** -24, 1.0, 3.0, -1.0, NAN, INF], device="cuda")
