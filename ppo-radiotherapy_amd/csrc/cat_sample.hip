@@ -76,22 +76,19 @@ template <int THREADS>
 struct Shared {
     uint64_t hist[kBins];
     uint64_t slots[THREADS / 64];
-    float fslots[THREADS / 64];
     uint64_t found[2];
     int32_t where;
 };
 
-// The bin in which a running sum, from the highest bin down or (UP) from the
-// lowest up, reaches `want` (want >= 1 and <= the sum of all bins): the bin,
-// and the sum before it.
-template <int THREADS, bool UP = false>
+// The bin, from the highest down, in which a running sum reaches `want` (want
+// >= 1 and <= the sum of all bins): the bin, and the sum above it.
+template <int THREADS>
 __device__ int find_bin(Shared<THREADS>& s, uint64_t want, uint64_t* above) {
-    const auto place = [](int i) { return UP ? i : kBins - 1 - i; };
     constexpr int kPer = kBins / THREADS;
     const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
     uint64_t mine = 0;
 #pragma unroll
-    for (int i = 0; i < kPer; ++i) mine += s.hist[place(tid * kPer + i)];
+    for (int i = 0; i < kPer; ++i) mine += s.hist[kBins - 1 - (tid * kPer + i)];
     uint64_t run = mine;
 #pragma unroll
     for (int o = 1; o < 64; o <<= 1) {
@@ -104,7 +101,7 @@ __device__ int find_bin(Shared<THREADS>& s, uint64_t want, uint64_t* above) {
     for (int i = 0; i < w; ++i) before += s.slots[i];
     if (before < want && want <= before + mine) {
         for (int i = 0; i < kPer; ++i) {
-            const int b = place(tid * kPer + i);
+            const int b = kBins - 1 - (tid * kPer + i);
             const uint64_t h = s.hist[b];
             if (want <= before + h) {
                 s.where = b;
@@ -121,32 +118,86 @@ __device__ int find_bin(Shared<THREADS>& s, uint64_t want, uint64_t* above) {
     return b;
 }
 
+// A wave's part of a row, in the order of the index: whole pieces, the first
+// wave also what lies before them, the last what lies behind.
+template <class D>
+struct Part {
+    int32_t from, to, first, last;  // pieces; entries
+    __device__ Part(const Span<D>& row, int32_t V, int w, int waves) {
+        const int32_t per = (row.pieces + waves - 1) / waves;
+        from = min(w * per, row.pieces);
+        to = min(from + per, row.pieces);
+        first = w == 0 ? 0 : row.head + from * Span<D>::kPer;
+        last = w == waves - 1 ? V : row.head + to * Span<D>::kPer;
+    }
+};
+
+// f(x, i) for every entry of a part; the lanes of one wave together, kAhead
+// pieces at a time, -inf where a lane has none.  `skip` says of a maximum whether all that is not above it
+// can be left out.
+struct Never {
+    __device__ __forceinline__ bool operator()(float) const { return false; }
+};
+template <int kAhead, class D, class F, class Skip = Never>
+__device__ __forceinline__ void walk(const Span<D>& row, const Part<D>& p, F f, Skip skip = Skip()) {
+    const int lane = threadIdx.x & 63;
+    constexpr int kPer = Span<D>::kPer;
+    const int32_t a = row.head + p.from * kPer, b = row.head + p.to * kPer;
+    if (p.first < a) f(p.first + lane < a ? D::get(row.x[p.first + lane]) : -INFINITY, p.first + lane);
+    if (b < p.last) f(b + lane < p.last ? D::get(row.x[b + lane]) : -INFINITY, b + lane);
+    for (int32_t at = p.from; at < p.to; at += 64 * kAhead) {
+        const int32_t i = at + lane;
+        uint4 r[kAhead];
+#pragma unroll
+        for (int k = 0; k < kAhead; ++k) r[k] = i + 64 * k < p.to ? row.piece(i + 64 * k) : nothing<D>();
+#pragma unroll
+        for (int k = 0; k < kAhead; ++k) {
+            const Unpack<D> x(r[k]);
+            if constexpr (!std::is_same_v<Skip, Never>)
+                if (!__any(!skip(x.max()))) continue;
+#pragma unroll
+            for (int j = 0; j < kPer; ++j) f(x.v[j], row.head + (i + 64 * k) * kPer + j);
+        }
+    }
+}
+
 // The key at which the running sum of `weight` over falling keys reaches
-// `want`, and the sum above that key.  `weight` is 0 for entries that do not
-// take part.
-template <int THREADS, bool SHORT, class Get, class Weight>
-__device__ uint32_t find_key(Shared<THREADS>& s, int32_t V, Get get, Weight weight, uint64_t want, uint64_t* above) {
+// `want`, and the sum above that key, digit by digit.  `weight` is 0 for
+// entries that do not take part.
+template <class D, int THREADS, class Weight>
+__device__ __forceinline__ uint32_t find_key(Shared<THREADS>& s, const Span<D>& row, const Part<D>& part, Weight weight,
+                                             uint64_t want, uint64_t* above) {
+    constexpr bool kShort = sizeof(typename D::raw) == 2;
     uint32_t prefix = 0;
     uint64_t over = 0;
-    // 16-bit types fill the upper 21 bits of a key at most: the last digit follows from the sign
-    for (int level = 0; level < (SHORT ? 2 : 3); ++level) {
+    // 16-bit types fill the upper 22 bits of a key at most: the last digit follows from the sign
+#pragma unroll 1
+    for (int level = 0; level < (kShort ? 2 : 3); ++level) {
         const int shift = level == 0 ? 21 : level == 1 ? 10 : 0, bits = level == 2 ? 10 : 11;
         for (int i = threadIdx.x; i < kBins; i += THREADS) s.hist[i] = 0;
         __syncthreads();
-        for (int i = threadIdx.x; i < V; i += THREADS) {
-            const float x = get(i);
+        walk<1>(row, part, [&](float x, int32_t i) {
             const uint32_t k = key_of(x);
-            if (level && (k >> (shift + bits)) != prefix) continue;
-            const uint64_t w = weight(x, k);
-            if (w) atomicAdd(reinterpret_cast<unsigned long long*>(&s.hist[(k >> shift) & ((1u << bits) - 1)]), (unsigned long long)w);
-        }
+            const uint64_t w = level && (k >> (shift + bits)) != prefix ? 0 : weight(x, k, i);
+            const int b = (int)(k >> shift & ((1u << bits) - 1));
+            const uint64_t who = __ballot(w != 0);
+            if (!who) return;
+            // equal logits are what brings a row here: one addition where all lanes have one bin
+            if (__all(!w || b == __shfl(b, __ffsll((long long)who) - 1))) {
+                const uint64_t sum = wave_sum(w);
+                if (__ffsll((long long)who) - 1 == (int)(threadIdx.x & 63))
+                    atomicAdd(reinterpret_cast<unsigned long long*>(&s.hist[b]), (unsigned long long)sum);
+            } else if (w) {
+                atomicAdd(reinterpret_cast<unsigned long long*>(&s.hist[b]), (unsigned long long)w);
+            }
+        });
         __syncthreads();
         uint64_t a;
         const int b = find_bin<THREADS>(s, want - over, &a);
         over += a;
         prefix = prefix << bits | (uint32_t)b;
     }
-    if (SHORT) prefix = prefix << 10 | (prefix >> 21 ? 0u : 0x3ffu);
+    if (kShort) prefix = prefix << 10 | (prefix >> 21 ? 0u : 0x3ffu);
     *above = over;
     return prefix;
 }
@@ -224,35 +275,46 @@ __device__ __forceinline__ void answer(const Args& A, int64_t n, int32_t a, doub
 // temperatures past the histogram's range.
 template <class D, int THREADS>
 __device__ __forceinline__ void slow_row(const Args& A, int64_t n, const Ask& ask, float m, Shared<THREADS>& s) {
-    constexpr bool kShort = sizeof(typename D::raw) == 2;
     const int32_t V = A.vocab;
-    const auto* row = static_cast<const typename D::raw*>(A.x) + n * A.stride;
-    const auto get = [&](int32_t i) { return D::get(row[i]); };
+    const Span<D> row(static_cast<const typename D::raw*>(A.x) + n * A.stride, V);
+    const Part<D> part(row, V, threadIdx.x >> 6, THREADS / 64);
     const Weigher weigh((double)m, fmax(1.4426950408889634 / (double)ask.T, 1e-300));
-    uint64_t all = 0;
-    for (int i = threadIdx.x; i < V; i += THREADS) all += weigh(get(i));
-    all = block_sum<THREADS>(all, s.slots);
+    const auto sum = [&](auto f) {
+        uint64_t v = 0;
+        walk<1>(row, part, [&](float x, int32_t i) { v += f(x, i); });
+        return block_sum<THREADS>(v, s.slots);
+    };
+    // the entry at which the running sum of f, by index, first exceeds `target`: its wave's part, then there
+    const auto search = [&](auto f, uint64_t target) {
+        uint64_t v = 0;
+        walk<1>(row, part, [&](float x, int32_t i) { v += f(x, i); });
+        v = wave_sum(v);
+        if ((threadIdx.x & 63) == 0) s.slots[threadIdx.x >> 6] = v;
+        __syncthreads();
+        int w = 0;
+        for (; w < THREADS / 64 - 1 && target >= s.slots[w]; ++w) target -= s.slots[w];
+        __syncthreads();
+        const Part<D> p(row, V, w, THREADS / 64);
+        return find_index<THREADS>(s, p.first, p.last - p.first, [&](int32_t i) { return f(D::get(row.x[i]), i); }, target);
+    };
+    const uint64_t all = sum([&](float x, int32_t) { return weigh(x); });
 
     // the least key that is kept, and how many of the entries equal to it
     uint32_t cut = 0;
-    uint64_t ties = UINT64_MAX, mass = all;
+    uint64_t ties = UINT64_MAX, mass = all, above;
     if (ask.K > 0) {
-        uint64_t above;
-        cut = find_key<THREADS, kShort>(s, V, get, [](float, uint32_t) { return (uint64_t)1; }, (uint64_t)ask.K, &above);
+            cut = find_key<D, THREADS>(s, row, part, [&](float x, uint32_t, int32_t) { return (uint64_t)(x > -INFINITY); },
+                                   min((uint64_t)ask.K, sum([](float x, int32_t) { return (uint64_t)(x > -INFINITY); })), &above);
         ties = (uint64_t)ask.K - above;
-        mass = 0;
-        if (ask.P < 1.0f) {
-            for (int i = threadIdx.x; i < V; i += THREADS)
-                if (key_of(get(i)) > cut) mass += weigh(get(i));
-            mass = block_sum<THREADS>(mass, s.slots) + ties * weigh(of_key(cut));
-        }
+        if (ask.P < 1.0f)
+            mass = sum([&](float x, int32_t) { return key_of(x) > cut ? weigh(x) : 0; }) +
+                   min(ties, sum([&](float x, int32_t) { return (uint64_t)(key_of(x) == cut); })) * weigh(of_key(cut));
     }
     if (ask.P < 1.0f) {
         const uint64_t want = ask.limit(mass);
         const uint32_t from = cut;
-        uint64_t above;
-        const uint32_t k = find_key<THREADS, kShort>(
-            s, V, get, [&](float x, uint32_t key) { return key >= from ? weigh(x) : 0; }, want, &above);
+        const uint32_t k = find_key<D, THREADS>(
+            s, row, part, [&](float x, uint32_t key, int32_t) { return key >= from ? weigh(x) : 0; }, want, &above);
         const uint64_t w = weigh(of_key(k));
         const uint64_t need = (want - above + w - 1) / w;
         if (k > cut || need < ties) ties = need;
@@ -261,72 +323,19 @@ __device__ __forceinline__ void slow_row(const Args& A, int64_t n, const Ask& as
     const double theta = ask.least();
     // entries equal to the cut: the last index that is kept
     int32_t last = V;
-    if (ties != UINT64_MAX) {
-        uint64_t equal = 0;
-        for (int i = threadIdx.x; i < V; i += THREADS) equal += key_of(get(i)) == cut;
-        equal = block_sum<THREADS>(equal, s.slots);
-        if (ties < equal)
-            last = find_index<THREADS>(s, 0, V, [&](int32_t i) { return (uint64_t)(key_of(get(i)) == cut); }, ties - 1);
-    }
-    const auto kept = [&](int32_t i) -> uint64_t {
-        const float x = get(i);
+    if (ties != UINT64_MAX && ties < sum([&](float x, int32_t) { return (uint64_t)(key_of(x) == cut); }))
+        last = search([&](float x, int32_t) { return (uint64_t)(key_of(x) == cut); }, ties - 1);
+    const auto kept = [&](float x, int32_t i) -> uint64_t {
         const uint32_t k = key_of(x);
-        if (k < cut || (k == cut && i > last) || (double)x - (double)m < theta) return 0;
-        return weigh(x);
+        return k < cut || (k == cut && i > last) || (double)x - (double)m < theta ? 0 : weigh(x);
     };
-    uint64_t left = 0;
-    for (int i = threadIdx.x; i < V; i += THREADS) left += kept(i);
-    left = block_sum<THREADS>(left, s.slots);
-    const int32_t a = find_index<THREADS>(s, 0, V, kept, ask.target(left));
-    if (threadIdx.x == 0) answer(A, n, a, ((double)get(a) - (double)m) / (double)ask.T, all, left);
+    const uint64_t left = sum(kept);
+    const int32_t a = search(kept, ask.target(left));
+    if (threadIdx.x == 0) answer(A, n, a, ((double)D::get(row.x[a]) - (double)m) / (double)ask.T, all, left);
 }
 
-// ---- one block per row -----------------------------------------------------
 // An entry's place in the order, larger first: key, then index from below.
 __device__ __forceinline__ uint64_t rank_of(float x, int32_t i) { return (uint64_t)key_of(x) << 32 | (uint32_t)~i; }
-
-// A wave's part of a row, in the order of the index: whole pieces, the first
-// wave also what lies before them, the last what lies behind.
-template <class D>
-struct Part {
-    int32_t from, to, first, last;  // pieces; entries
-    __device__ Part(const Span<D>& row, int32_t V, int w, int waves) {
-        const int32_t per = (row.pieces + waves - 1) / waves;
-        from = min(w * per, row.pieces);
-        to = min(from + per, row.pieces);
-        first = w == 0 ? 0 : row.head + from * Span<D>::kPer;
-        last = w == waves - 1 ? V : row.head + to * Span<D>::kPer;
-    }
-};
-
-// f(x, i) for every entry of a part; the lanes of one wave together, kAhead
-// pieces at a time, -inf where a lane has none.  `skip` says of a maximum whether all that is not above it
-// can be left out.
-struct Never {
-    __device__ __forceinline__ bool operator()(float) const { return false; }
-};
-template <int kAhead, class D, class F, class Skip = Never>
-__device__ __forceinline__ void walk(const Span<D>& row, const Part<D>& p, F f, Skip skip = Skip()) {
-    const int lane = threadIdx.x & 63;
-    constexpr int kPer = Span<D>::kPer;
-    const int32_t a = row.head + p.from * kPer, b = row.head + p.to * kPer;
-    if (p.first < a) f(p.first + lane < a ? D::get(row.x[p.first + lane]) : -INFINITY, p.first + lane);
-    if (b < p.last) f(b + lane < p.last ? D::get(row.x[b + lane]) : -INFINITY, b + lane);
-    for (int32_t at = p.from; at < p.to; at += 64 * kAhead) {
-        const int32_t i = at + lane;
-        uint4 r[kAhead];
-#pragma unroll
-        for (int k = 0; k < kAhead; ++k) r[k] = i + 64 * k < p.to ? row.piece(i + 64 * k) : nothing<D>();
-#pragma unroll
-        for (int k = 0; k < kAhead; ++k) {
-            const Unpack<D> x(r[k]);
-            if constexpr (!std::is_same_v<Skip, Never>)
-                if (!__any(!skip(x.max()))) continue;
-#pragma unroll
-            for (int j = 0; j < kPer; ++j) f(x.v[j], row.head + (i + 64 * k) * kPer + j);
-        }
-    }
-}
 
 // Bins of falling logits, by t = (m - x) / (T ln 2): the last holds what weighs
 // nothing (2^(40 - 41.5) < 1/2).  Each step of the arithmetic keeps the order,
