@@ -343,13 +343,18 @@ __device__ __forceinline__ uint64_t rank_of(float x, int32_t i) { return (uint64
 struct Binner {
     float m, scale, last;
     __device__ __forceinline__ int operator()(float x) const { return (int)fminf((m - x) * scale, last); }
-    // the least number whose bin is not behind b >= 0
+    // the least number whose bin is not behind b >= 0, by a wave: 64 keys at a time
     __device__ uint32_t least_key(int b) const {
         uint32_t lo = 0x00800000u, hi = key_of(m);  // from the lowest finite one
         while (lo < hi) {
-            const uint32_t mid = lo + (hi - lo) / 2;
-            if ((*this)(of_key(mid)) <= b) hi = mid;
-            else lo = mid + 1;
+            const uint32_t step = (hi - lo) / 64 + 1;
+            const uint32_t k = min((uint64_t)hi, lo + (uint64_t)step * (threadIdx.x & 63));
+            const uint64_t reached = __ballot((*this)(of_key(k)) <= b);
+            const int first = reached ? __ffsll((long long)reached) - 1 : 64;
+            const uint32_t below = lo + step * (uint32_t)(first - 1);
+            if (first == 0) return lo;
+            if (first < 64) hi = (uint32_t)min((uint64_t)hi, (uint64_t)below + step);
+            lo = below + 1;
         }
         return lo;
     }
