@@ -461,7 +461,8 @@ template <class D, class Op, int THREADS, int HELD>
 __global__ __launch_bounds__(THREADS) void k_cat_row(Logits l, Op op, Out o, double* terms) {
     __shared__ Slots<THREADS> slots;
     Teacher te(teacher_lds, Op::ppo ? 0 : op.k());
-    const int64_t n = blockIdx.x;
+    const int64_t n = block_index();
+    if (n >= l.rows) return;
     const int tid = threadIdx.x;
     const auto* x = row_of<D>(l, n);
     const Span<D> row(x, l.vocab);
@@ -571,9 +572,10 @@ __global__ __launch_bounds__(256) void k_cat_grad(Logits l, Op op, Out o, const 
     constexpr int kThreads = 256;
     __shared__ RowState share;
     Teacher te(teacher_lds, Op::ppo ? 0 : op.k());
-    const int32_t blocks = JOIN && !o.grad ? 1 : parts;  // of a row
-    const int64_t n = blockIdx.x / blocks;
-    const int32_t part = blockIdx.x % blocks;
+    const uint32_t blocks = JOIN && !o.grad ? 1 : parts, block = (uint32_t)block_index();  // of a row; rows parts < 2^31
+    const int64_t n = block / blocks;
+    const int32_t part = (int32_t)(block % blocks);
+    if (n >= l.rows) return;
     const int tid = threadIdx.x;
     const auto* x = row_of<D>(l, n);
     const Span<D> row(x, l.vocab);
@@ -655,7 +657,7 @@ __device__ __forceinline__ void block_terms(const double* term, double* ds, doub
 #pragma unroll
     for (int k = 0; k < TERMS; ++k) {
         const double r = block_sum<256>(term[k], ds);
-        if (threadIdx.x == 0) to[(int64_t)blockIdx.x * TERMS + k] = r;
+        if (threadIdx.x == 0) to[block_index() * TERMS + k] = r;
     }
 }
 
@@ -666,7 +668,8 @@ __global__ __launch_bounds__(256) void k_cat_short(Logits l, Op op, Out o, doubl
                                                    const float* gout) {
     __shared__ double ds[4];
     const int t = threadIdx.x % G;
-    const int64_t n = (int64_t)blockIdx.x * (256 / G) + threadIdx.x / G;
+    const int64_t n0 = block_index() * (256 / G), n = n0 + threadIdx.x / G;
+    if (n0 >= l.rows) return;
     const bool in = n < l.rows;
     const int32_t V = l.vocab;
     const auto* x = row_of<D>(l, in ? n : 0);
@@ -801,7 +804,8 @@ __global__ __launch_bounds__(256) void k_cat_tiny(Logits l, Op op, Out o, double
     __shared__ float tile[256 * (kTiny + 1)];
     const int tid = threadIdx.x;
     const int32_t V = l.vocab, pitch = V | 1;
-    const int64_t n0 = (int64_t)blockIdx.x * 256, n = n0 + tid;
+    const int64_t n0 = block_index() * 256, n = n0 + tid;
+    if (n0 >= l.rows) return;
     const int32_t here = (int32_t)min((int64_t)256, l.rows - n0);
     const float per = 1.0f / (float)V;  // (i + 1/2) / V is 1/64 or more away from a whole number
     for (int32_t i = tid; i < here * V; i += 256) {
@@ -914,7 +918,7 @@ int64_t launch_short(const Logits& l, const Op& op, const Out& o, double* ws, co
                      hipStream_t st) {
     const auto go = [&](auto kernel, int per_block) {
         const int64_t blocks = (l.rows + per_block - 1) / per_block;
-        hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(256), 0, st, l, op, o, ws, state, gout);
+        hipLaunchKernelGGL(kernel, grid_of(blocks), dim3(256), 0, st, l, op, o, ws, state, gout);
         return blocks;
     };
     const int32_t V = l.vocab;
@@ -979,8 +983,8 @@ size_t teacher_bytes(const Distill& op) { return Teacher::bytes(op.b.k); }
 
 template <class D, class Op, int THREADS, int HELD>
 void launch_row(const Logits& l, const Op& op, const Out& o, double* ws, hipStream_t st) {
-    hipLaunchKernelGGL((k_cat_row<D, Op, THREADS, HELD>), dim3((unsigned)l.rows), dim3(THREADS), teacher_bytes(op), st, l,
-                       op, o, ws);
+    hipLaunchKernelGGL((k_cat_row<D, Op, THREADS, HELD>), grid_of(l.rows), dim3(THREADS), teacher_bytes(op), st, l, op, o,
+                       ws);
 }
 
 // How many blocks share a row: as many as bring the card 1024 blocks, with two
@@ -1046,8 +1050,8 @@ int run_backward(const Logits& l, const Op& op, const double* state, const float
     Out o{};
     o.grad = grad;
     o.grad_stride = stride;
-    hipLaunchKernelGGL((k_cat_grad<D, Op, false>), dim3((unsigned)(l.rows * parts)), dim3(256), teacher_bytes(op), st, l, op,
-                       o, nullptr, nullptr, reinterpret_cast<const RowState*>(state), gout, (int32_t)parts);
+    hipLaunchKernelGGL((k_cat_grad<D, Op, false>), grid_of(l.rows * parts), dim3(256), teacher_bytes(op), st, l, op, o,
+                       nullptr, nullptr, reinterpret_cast<const RowState*>(state), gout, (int32_t)parts);
     return launched();
 }
 
@@ -1066,6 +1070,7 @@ int bad(const char* who, const char* what) {
 const char* grad_fault(const rt_cat_logits* l, const void* grad, int64_t stride) {
     const int64_t es = elem_size(l->dtype);
     if (stride < l->vocab) return "gradient rows overlap (stride < vocab)";
+    if (stride > INT64_MAX / 16 / l->rows) return "gradient stride out of range";
     if ((uintptr_t)grad % es) return "gradient not aligned to its element";
     if (grad == l->x) return stride == l->row_stride || l->rows == 1 ? nullptr : "in-place gradient with another stride";
     const uintptr_t x0 = (uintptr_t)l->x, x1 = x0 + ((l->rows - 1) * l->row_stride + l->vocab) * es;
@@ -1155,6 +1160,7 @@ extern "C" int rt_cat_distill_backward(const rt_cat_logits* logits, const rt_cat
     if (!row_state_d || !grad_d) return bad(me, "NULL argument");
     if (const char* f = grad_fault(logits, grad_d, grad_stride)) return bad(me, f);
     const Logits l{logits->x, logits->rows, logits->row_stride, logits->vocab};
-    return pick_backward(logits->dtype, l, Distill{*teacher, teacher->temperature, 1.0 / teacher->temperature}, row_state_d, grad_loss_d, grad_d,
-                         grad_stride, reinterpret_cast<hipStream_t>(stream));
+    const Distill op{*teacher, teacher->temperature, 1.0 / teacher->temperature};
+    return pick_backward(logits->dtype, l, op, row_state_d, grad_loss_d, grad_d, grad_stride,
+                         reinterpret_cast<hipStream_t>(stream));
 }

@@ -177,6 +177,16 @@ __device__ __forceinline__ uint4 nothing() {
     return make_uint4(two, two, two, two);
 }
 
+// ---- launches --------------------------------------------------------------
+// A dimension of a launch has less than 2^32 threads: past 2^20 blocks the grid
+// has a second one, and block_index() may then be behind the last block.
+inline dim3 grid_of(int64_t blocks) {
+    constexpr int64_t kMost = 1 << 20;
+    if (blocks <= kMost) return dim3((unsigned)blocks);
+    return dim3((unsigned)kMost, (unsigned)((blocks + kMost - 1) / kMost));
+}
+__device__ __forceinline__ int64_t block_index() { return (int64_t)blockIdx.y << 20 | blockIdx.x; }
+
 // ---- argument checks -------------------------------------------------------
 inline int elem_size(int32_t dtype) { return dtype == RT_DT_F32 ? 4 : 2; }
 inline bool bad_type(int32_t dtype) { return dtype != RT_DT_F32 && dtype != RT_DT_BF16 && dtype != RT_DT_F16; }
@@ -187,6 +197,7 @@ inline const char* logits_fault(const rt_cat_logits* l) {
     if (l->rows < 1 || l->rows > INT32_MAX) return "rows out of range";
     if (l->vocab < 1 || l->vocab > RT_CAT_MAX_VOCAB) return "vocab out of range";
     if (l->row_stride < 0) return "negative row stride";
+    if (l->row_stride > INT64_MAX / 16 / l->rows) return "row stride out of range";
     if ((uintptr_t)l->x % elem_size(l->dtype)) return "logits not aligned to their element";
     return nullptr;
 }

@@ -400,6 +400,14 @@ __device__ void greedy(const Args& A, int64_t n, float m, int32_t lo, int32_t le
     }
 }
 
+// Between a wave's accesses to LDS that other lanes of it made: they keep their
+// order in the hardware, the compiler has to keep it too.
+__device__ __forceinline__ void wave_sync() {
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+
 // ---- the cut, among entries in registers -----------------------------------
 // A team of one to sixteen waves, and what they tell each other.
 template <int THREADS>
@@ -434,7 +442,7 @@ struct Team {
     }
     __device__ __forceinline__ void sync() {
         if constexpr (kWaves > 1) __syncthreads();
-        else __builtin_amdgcn_wave_barrier();  // a wave's LDS accesses keep their order
+        else wave_sync();
     }
     // the sum of the threads before this one; `total` of all
     __device__ __forceinline__ uint64_t before(uint64_t v, uint64_t* total) {
@@ -813,6 +821,7 @@ __global__ __launch_bounds__(256) void k_cat_sample_near(Batch b) {
     }, [&](float x) { return x < fminf(low, low_p); });
     kept = wave_sum(kept);
     if ((tid & 63) == 0) to.kept[seg] = kept;
+    wave_sync();
     const int mine = min(many, kOwn);
     int first = 0;
     if ((tid & 63) == 0 && mine) first = atomicAdd(&to.many, mine);
@@ -1147,7 +1156,7 @@ __global__ __launch_bounds__(THREADS < 256 ? 256 : THREADS) void k_cat_sample_he
     __shared__ typename Team<THREADS>::Slots slots;
     Team<THREADS> team(slots);
     const int t = threadIdx.x % THREADS;
-    const int64_t n = (int64_t)blockIdx.x * kRows + threadIdx.x / THREADS;
+    const int64_t n = block_index() * kRows + threadIdx.x / THREADS;
     const int32_t V = A.vocab, per = ((V + THREADS - 1) / THREADS) | 1;
     const bool in = n < rows;
     float* mine = staged + threadIdx.x / THREADS * per * THREADS;
@@ -1158,7 +1167,7 @@ __global__ __launch_bounds__(THREADS < 256 ? 256 : THREADS) void k_cat_sample_he
             if (t + THREADS * e < V) mine[t + THREADS * e] = D::get(row[t + THREADS * e]);
     }
     __syncthreads();
-    if (!in) return;  // only of a block whose waves have a row each
+    if (!in) return;  // a wave of a block whose waves have a row each, or all of a block
     float x[E];
     uint32_t top = 0;
 #pragma unroll
@@ -1267,7 +1276,7 @@ template <class D>
 void launch_held(const Args& a, int64_t rows, hipStream_t st) {
     const auto go = [&](auto kernel, int threads) {
         const int per = ((a.vocab + threads - 1) / threads) | 1, many = threads == 64 ? 4 : 1;
-        hipLaunchKernelGGL(kernel, dim3((unsigned)((rows + many - 1) / many)), dim3(threads * many),
+        hipLaunchKernelGGL(kernel, grid_of((rows + many - 1) / many), dim3(threads * many),
                            (size_t)per * threads * many * sizeof(float), st, a, rows);
     };
     const int32_t V = a.vocab;

@@ -42,7 +42,7 @@ WS = (1 << 20, 1 << 16)  # address, bytes
 
 @pytest.mark.parametrize("l,word", [
     (_logits(x=None), b"NULL"), (_logits(rows=0), b"rows"), (_logits(rows=2 ** 31), b"rows"), (_logits(vocab=0), b"vocab"),
-    (_logits(vocab=_lib.CAT_MAX_VOCAB + 1), b"vocab"), (_logits(dtype=3), b"type"), (_logits(stride=-1), b"stride"),
+    (_logits(vocab=_lib.CAT_MAX_VOCAB + 1), b"vocab"), (_logits(dtype=3), b"type"), (_logits(stride=-1), b"stride"), (_logits(stride=2 ** 58), b"stride"),
     (_logits(x=4098), b"aligned"), (_logits(x=4097, dtype=_lib.DT_BF16), b"aligned")])
 def test_bad_logits_are_refused(l, word):
     L = _lib.load()
