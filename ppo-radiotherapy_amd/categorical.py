@@ -13,10 +13,11 @@ logits: a discretised beam action ([..., bins]) or a token ([..., vocab]).
 Logits are float32, bfloat16 or float16 on the GPU, entries of a row adjacent
 (stride 1), leading dimensions any that collapse to evenly spaced rows; -inf
 marks an entry that cannot be taken.  Everything is enqueued on the current
-stream of the logits' device, nothing synchronises, and all of it can be
-captured in a graph (in a training graph prefer the `_grad` forms: they need no
-autograd).  The definitions stand in include/rtenv.h; wrong arguments raise
-ValueError or TypeError before anything is launched.
+stream of the logits' device, nothing synchronises, and all but the autograd
+forms can be captured in a graph (there take the `_grad` forms, and
+`logits.backward(grad)` for what lies before).  The definitions stand in
+include/rtenv.h; wrong arguments raise ValueError or TypeError before anything
+is launched.
 """
 from __future__ import annotations
 
@@ -130,6 +131,8 @@ class _Rows:
         o = _Rows(out)
         if self.n > 1 and o.stride < self.vocab:
             raise ValueError("out: rows overlap")
+        if not out.is_inference():
+            torch.autograd.graph.increment_version(out)  # as an operation in place: autograd's check sees it
         return out, max(o.stride, self.vocab)
 
     def call(self, fn, what: str, *args):
@@ -249,6 +252,10 @@ class _Ppo:
 
 
 def _with_grad(fn, logits, op):
+    # A captured backward pass ends the process where an eager graph of the same leaves is alive (their
+    # nodes keep its stream): nothing here can tell.
+    if torch.cuda.is_current_stream_capturing():
+        raise RuntimeError("logits require grad while a graph is captured: take the _grad form")
     loss = fn.apply(logits, op)
     return op.rest._replace(loss=loss)
 

@@ -515,6 +515,60 @@ def test_changed_inputs_are_noticed(C):
         r.loss.backward()
 
 
+def test_gradient_in_place_is_noticed(C):
+    """Logits that another graph has saved, written over with their gradient."""
+    h = torch.randn(3, 20, device="cuda")
+    w = torch.ones(3, 20, device="cuda", requires_grad=True)
+    z = (w * h).sum()
+    a, old, adv, _, _ = ppo_inputs(3, 20, 62, h)
+    C.ppo_loss_grad(h, a, old, adv, out=h)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        z.backward()
+
+
+def test_autograd_is_refused_in_a_capture(C):
+    x = torch.randn(3, 20, device="cuda", requires_grad=True)
+    a, old, adv, _, _ = ppo_inputs(3, 20, 63, x.detach())
+    idx, top, _ = teacher_inputs(3, 20, 4, 63)
+    C.ppo_loss_grad(x.detach(), a, old, adv)
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        with pytest.raises(RuntimeError, match="captured"):
+            C.ppo_loss(x, a, old, adv)
+        with pytest.raises(RuntimeError, match="captured"):
+            C.distill_loss(x, idx, top)
+        r, grad = C.ppo_loss_grad(x.detach(), a, old, adv)
+    g.replay()
+    want, wgrad = C.ppo_loss_grad(x.detach(), a, old, adv)
+    assert torch.equal(grad, wgrad) and torch.equal(r.loss, want.loss)
+
+
+@pytest.mark.parametrize("v,n,n_loss", [(33, 2 ** 26 + 5, 2 ** 28 + 3), (577, 2 ** 24 + 3, 2 ** 26 + 5), (1025, 2 ** 24 + 3, 2 ** 26 + 5)])
+def test_more_rows_than_one_launch_dimension_has(C, v, n, n_loss):
+    """2^32 threads and more; one row of logits for all (stride 0), so that every row's result is known."""
+    row = rows(1, v, torch.bfloat16, 71)
+    x = row.expand(n, v)
+    u = torch.zeros(n, device="cuda")
+    few = torch.tensor([0.1, 0.5, 0.93], device="cuda")
+    u[-3:] = few
+    got, want = C.sample(x, u, top_p=0.9), C.sample(row.expand(3, v), few, top_p=0.9)
+    zero = C.sample(row, u[:1], top_p=0.9)
+    for p, q, z in zip(got, want, zero):
+        assert torch.equal(p[-3:], q) and bool((p[:-3] == z).all())
+    del got, u
+    n = n_loss
+    x = row.expand(n, v)
+    a = torch.full((n,), -1, device="cuda")
+    a[-2:] = torch.tensor([0, v - 1], device="cuda")
+    f = torch.zeros(n, device="cuda")
+    f[-2:] = torch.tensor([1.0, -2.0], device="cuda")
+    r = C.ppo_loss(x, a, f, f, weights=torch.ones(1, device="cuda").expand(n))
+    s = C.ppo_loss(x[-2:], a[-2:], f[-2:], f[-2:], weights=torch.ones(2, device="cuda"))
+    assert torch.equal(r.logprob[-2:], s.logprob) and not r.logprob[:-2].any()
+    assert torch.equal(r.loss, s.loss) and torch.equal(r.stats, s.stats)
+
+
 def test_refusals(C):
     x = torch.randn(4, 10, device="cuda")
     v = torch.zeros(4, device="cuda")
@@ -582,12 +636,9 @@ def test_policy_iteration_together(C):
     gW = obs.reshape(T * N, D).double().t() @ want["grad"][0]
     room = obs.reshape(T * N, D).double().abs().t() @ (want["grad"][1] + want["grad"][0].abs() * 2.0 ** -20)
     assert ((W.grad.double() - gW).abs() <= room).all()
-    before = float(want["loss"][0])
     with torch.no_grad():
         W -= 0.5 * W.grad
         x = obs.reshape(T * N, D).mm(W)
-        after = float(C.ppo_loss(x, s.action.reshape(-1), s.logprob.reshape(-1), adv.reshape(-1), temperature=1.1, ent_coef=0.01).loss)
-    assert after < before
     top, idx = x.topk(6, dim=1)
     student = torch.zeros(T * N, V, device="cuda")
     r, grad = C.distill_loss_grad(student, idx, top, temperature=1.0)
