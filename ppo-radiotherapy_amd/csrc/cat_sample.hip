@@ -1055,6 +1055,455 @@ __global__ __launch_bounds__(512) void k_cat_sample_answer(Batch b) {
     }
 }
 
+// ---- long rows of bf16, by counts ------------------------------------------
+// A bf16 row has few different numbers, so how often each one occurs says all
+// about it: one pass counts them, before the maximum is known, with integers
+// alone; weights are worked out once for each number and not for each entry
+// (the 20 f64 operations of a weight for each of 256 x 131072 entries took
+// 47 us, a pass that counts reads them at HBM's pace).  The cut comes exactly
+// from the counts, ties included; what is left is to find an index in one part
+// of the row, with the weights by number in LDS.
+//
+// A place for each number with 2^-36 < |x| < 2^12, largest first, 0 in the
+// middle.  -inf is not counted.  Rows with others that weigh something go the
+// slow way.
+constexpr int kSigned = 48 * 128, kPlaces = 2 * kSigned, kZero = kSigned - 1;
+constexpr uint32_t kLowBits = (127 - 36) << 23;  // of the lowest magnitude; as its positive number's place is 0's
+enum { kOdd = 1, kAbove = 2, kBelow = 4, kBetween = 8 };  // NaN or +inf; past the places
+
+// The place of x, or -1 and what is the matter with it.
+__device__ __forceinline__ int place_of(float x, uint32_t* flags) {
+    const uint32_t b = __float_as_uint(x), t = (b & 0x7fffffffu) - kLowBits;
+    if (t < (uint32_t)kSigned << 16 && b != kLowBits) return kSigned + ((int)(t >> 16) ^ ~((int32_t)b >> 31));
+    if (x == 0.0f) return kZero;
+    if (x != -INFINITY) *flags |= !(x < INFINITY) ? kOdd : x >= 4096.0f ? kAbove : x <= -4096.0f ? kBelow : kBetween;
+    return -1;
+}
+__device__ __forceinline__ float number_at(int place) {
+    if (place == kZero) return 0.0f;
+    const int s = place < kSigned ? -1 : 0;
+    return __uint_as_float((kLowBits + ((uint32_t)((place - kSigned) ^ s) << 16)) | (s ? 0u : 0x80000000u));
+}
+
+constexpr int kBinade = 128, kBinades = kPlaces / kBinade;
+constexpr int kMostCounts = 32, kCountWaves = 8, kPickWaves = 16;
+
+struct Counts {
+    Args a;
+    uint32_t* many;  // [row of the batch][part][kPlaces / 2]: two counts, a part has less than 2^16 entries
+    uint4* has;      // [row][part]: a bit for each binade that has entries (only those are in `many`); the flags
+    int64_t first;
+    int32_t parts;
+};
+
+// 48 KB of LDS: three blocks of eight waves on a CU.
+__global__ __launch_bounds__(512) void k_cat_sample_count(Counts b) {
+    __shared__ __align__(16) uint32_t many[kPlaces];
+    __shared__ uint32_t has[4];
+    const int64_t r = blockIdx.x / b.parts, n = b.first + r;
+    const int32_t p = blockIdx.x % b.parts, V = b.a.vocab;
+    const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
+    const Span<BF16> row(static_cast<const uint16_t*>(b.a.x) + n * b.a.stride, V);
+    const Part<BF16> part(row, V, p * kCountWaves + w, b.parts * kCountWaves);
+    for (int i = tid; i < kPlaces / 4; i += 512) reinterpret_cast<uint4*>(many)[i] = make_uint4(0, 0, 0, 0);
+    if (tid < 4) has[tid] = 0;
+    __syncthreads();
+    uint32_t flags = 0;
+    walk<4>(row, part, [&](float x, int32_t) {
+        const int at = place_of(x, &flags);
+        if (at >= 0) atomicAdd(&many[at], 1u);
+    });
+    if (flags) atomicOr(&has[3], flags);
+    __syncthreads();
+    uint32_t* to = b.many + blockIdx.x * (int64_t)(kPlaces / 2);
+    for (int i = w; i < kBinades; i += kCountWaves) {
+        const uint2 c = reinterpret_cast<const uint2*>(many + i * kBinade)[lane];
+        if (!__any(c.x | c.y)) continue;
+        to[i * (kBinade / 2) + lane] = c.x | c.y << 16;
+        if (lane == 0) atomicOr(&has[i / 32], 1u << i % 32);
+    }
+    __syncthreads();
+    if (tid == 0) b.has[blockIdx.x] = make_uint4(has[0], has[1], has[2], has[3]);
+}
+
+// A row with numbers that have no place: the key, and then the index, of each
+// cut by halving, a pass over the row for every step (1 ms for 131072 entries).
+// In little code and few registers: it stands in a kernel that has better to do.
+template <class T>
+__device__ __forceinline__ void other_row(const Args& A, int64_t n, const Ask& ask, T& team) {
+    const int32_t V = A.vocab;
+    const uint16_t* const x = static_cast<const uint16_t*>(A.x) + n * A.stride;
+    const auto key = [](float v) { return key_of(v) >> 16; };
+    uint32_t top = 0;
+    for (int32_t i = threadIdx.x; i < V; i += T::kWaves * 64) top = max(top, key_of(BF16::get(x[i])));
+    const float m = of_key(team.top(top));
+    const bool greedily = !(ask.T > 0.0f);
+    const Head h(ask, m);
+    // over the entries before `end`, of those with a larger key than `least`, or that one and an index up to `last`:
+    // how many they are, or what they weigh
+    const auto pass = [&](uint32_t least, int32_t last, int32_t end, bool by_number, double theta) {
+        uint64_t v = 0;
+#pragma unroll 4
+        for (int32_t i = threadIdx.x; i < end; i += T::kWaves * 64) {
+            const float f = BF16::get(x[i]);
+            const uint32_t k = key(f);
+            const bool in = k > least || (k == least && i <= last);
+            v += !in || (double)f - (double)m < theta ? 0 : by_number ? (uint64_t)(f > -INFINITY) : h.weigh(f);
+        }
+        return team.sum(v);
+    };
+    uint32_t cut = 0;
+    int32_t last = V - 1;
+    uint64_t all = 0, left = 0;
+    if (greedily) {
+        cut = key(m);
+    } else {
+        all = left = pass(0, last, V, false, -INFINITY);
+#pragma unroll 1
+        for (int round = 0; round < 2; ++round) {  // top-k, top-p
+            const bool by_number = round == 0;
+            if (by_number ? ask.K <= 0 : !(ask.P < 1.0f)) continue;
+            const uint64_t want = by_number ? min((uint64_t)ask.K, pass(0, last, V, true, -INFINITY)) : ask.limit(left);
+            uint32_t c = 0;
+#pragma unroll 1
+            for (uint32_t bit = 0x8000; bit; bit >>= 1)
+                if ((c | bit) <= cut || pass(c | bit, V, V, by_number, -INFINITY) >= want) c |= bit;
+            int32_t lo = 0, hi = c == cut ? last : V - 1;
+#pragma unroll 1
+            while (lo < hi) {
+                const int32_t mid = (lo + hi) / 2;
+                if (pass(c, mid, V, by_number, -INFINITY) >= want) hi = mid;
+                else lo = mid + 1;
+            }
+            cut = c;
+            last = lo;
+            left = pass(cut, last, V, false, -INFINITY);
+        }
+        left = pass(cut, last, V, false, h.theta);
+    }
+    const uint64_t target = greedily ? 0 : ask.target(left);
+    int32_t lo = 0, hi = V - 1;
+#pragma unroll 1
+    while (lo < hi) {
+        const int32_t mid = (lo + hi) / 2;
+        if (pass(cut, last, mid + 1, greedily, greedily ? -INFINITY : h.theta) > target) hi = mid;
+        else lo = mid + 1;
+    }
+    if (threadIdx.x) return;
+    if (greedily) {
+        A.action[n] = lo;
+        A.logprob[n] = A.kept[n] = 0.0f;
+    } else {
+        answer(A, n, lo, ((double)BF16::get(x[lo]) - (double)m) / (double)ask.T, all, left);
+    }
+}
+
+// One block for a row.  The binades in turn for the waves: those that have
+// entries are next to one another.
+__global__ __launch_bounds__(1024) void k_cat_sample_pick(Counts b) {
+    constexpr int kThreads = 64 * kPickWaves, kOwn = kBinades / kPickWaves, kAhead = 8;
+    static_assert(kOwn * kPickWaves == kBinades && kPickWaves == 16, "two binades of a wave in each word of a mask");
+    __shared__ struct {
+        uint64_t weight[kPlaces];  // of a number; and how many there are.  Not set where a binade has none
+        uint32_t many[kPlaces];
+    } room;
+    __shared__ Team<kThreads>::Slots slots;
+    __shared__ uint64_t mass_of[kBinades], sums[kPickWaves][kMostCounts];
+    __shared__ uint32_t many_of[kBinades], ties_of[kPickWaves];
+    const int64_t n = b.first + blockIdx.x;
+    const int32_t V = b.a.vocab, parts = b.parts;
+    const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const Span<BF16> row(static_cast<const uint16_t*>(b.a.x) + n * b.a.stride, V);
+    const uint32_t* const counts = b.many + (int64_t)blockIdx.x * parts * (kPlaces / 2) + lane;
+    const Ask ask(b.a.p, n, V);
+    const uint4 has = lane < parts ? b.has[blockIdx.x * parts + lane] : make_uint4(0, 0, 0, 0);
+    const uint32_t has_word[4] = {has.x, has.y, has.z, has.w};
+    const auto any_of = [](uint32_t v) { return lanes<64>(v, [](uint32_t a, uint32_t b) { return a | b; }); };
+    const auto binade = [&](int i) { return w + kPickWaves * i; };  // the wave's i-th
+    uint32_t held[kAhead][kOwn];  // of kAhead parts, in one trip to memory; all that there are, mostly
+    const auto load = [&](int from) {
+#pragma unroll
+        for (int j = 0; j < kAhead; ++j) {
+#pragma unroll
+            for (int i = 0; i < kOwn; ++i) held[j][i] = 0;
+            if (from + j < parts)
+#pragma unroll
+                for (int i = 0; i < kOwn; ++i) {
+                    const uint32_t bits = __builtin_amdgcn_readlane(has_word[i / 2], from + j);
+                    if (bits >> (w + kPickWaves * (i & 1)) & 1)
+                        held[j][i] = counts[(from + j) * (kPlaces / 2) + binade(i) * (kBinade / 2)];
+                }
+        }
+    };
+    uint32_t first = kPlaces;
+    {
+        uint2 many[kOwn] = {};
+#pragma unroll 1
+        for (int from = 0; from < parts; from += kAhead) {
+            load(from);
+#pragma unroll
+            for (int j = 0; j < kAhead; ++j)
+#pragma unroll
+                for (int i = 0; i < kOwn; ++i) many[i].x += held[j][i] & 0xffff, many[i].y += held[j][i] >> 16;
+        }
+#pragma unroll
+        for (int i = kOwn - 1; i >= 0; --i) {
+            const int at = binade(i) * kBinade + 2 * lane;
+            reinterpret_cast<uint2*>(room.many)[at / 2] = many[i];
+            first = many[i].x ? at : many[i].y ? at + 1 : first;
+        }
+    }
+    const uint32_t flags = any_of(has.w);
+    if (flags & kOdd) {
+        if (tid == 0) no_answer(b.a, n);
+        return;
+    }
+    Team<kThreads> team(slots);
+    first = team.all(first, [](uint32_t a, uint32_t b) { return min(a, b); });
+    if (first == kPlaces && !flags) {
+        if (tid == 0) no_answer(b.a, n);
+        return;
+    }
+    const bool greedily = !(ask.T > 0.0f);
+    float m = first < kPlaces ? number_at(first) : 0.0f;
+    if (flags) {
+        const Weigher weigh((double)m, fmax(1.4426950408889634 / (double)(greedily ? 1.0f : ask.T), 1e-300));
+        if (first == kPlaces || flags & kAbove || (flags & kBetween && (m <= 0.0f || weigh(0x1p-36f))) ||
+            (flags & kBelow && weigh(-4096.0f)))
+            return other_row(b.a, n, ask, team);
+    }
+    const Head h(ask, m);
+    uint32_t mine = 0;  // a bit for each of the wave's binades that have entries
+#pragma unroll
+    for (int i = 0; i < kOwn; ++i) mine |= (any_of(has_word[i / 2]) >> (w + kPickWaves * (i & 1)) & 1) << i;
+    mine = __builtin_amdgcn_readfirstlane(mine);
+#pragma unroll 1
+    for (int i = 0; i < kOwn; ++i) {
+        uint64_t mass = 0;
+        uint32_t many = 0;
+        if (mine >> i & 1) {
+            const int at = binade(i) * kBinade + 2 * lane;
+            const uint2 c = reinterpret_cast<const uint2*>(room.many)[at / 2];
+            uint64_t v0 = at == (int)first, v1 = at + 1 == (int)first;
+            if (!greedily) {
+                v0 = h.weigh(number_at(at));
+                v1 = h.weigh(number_at(at + 1));
+            }
+            room.weight[at] = v0;
+            room.weight[at + 1] = v1;
+            mass = wave_sum(c.x * v0 + c.y * v1);
+            many = wave_sum((v0 ? c.x : 0) + (v1 ? c.y : 0));
+        }
+        if (lane == 0) {
+            mass_of[binade(i)] = mass;
+            many_of[binade(i)] = many;
+        }
+    }
+    __syncthreads();
+    // The cut, by every wave for itself.
+    const auto pair = [&](int i, bool by_number, uint64_t* low) {  // of places i, i + 1
+        const uint2 c = reinterpret_cast<const uint2*>(room.many)[i / 2];
+        const uint64_t v0 = room.weight[i], v1 = room.weight[i + 1];
+        *low = c.x * (by_number ? (uint64_t)(v0 != 0) : v0);
+        return *low + c.y * (by_number ? (uint64_t)(v1 != 0) : v1);
+    };
+    // the place at which the running sum reaches `want`, and how much of that place is wanted
+    const auto find = [&](uint64_t want, bool by_number, uint64_t* need) {
+        uint64_t v = 0, low = 0, before, more;
+        if (lane < kBinades / 2) {
+            low = by_number ? many_of[2 * lane] : mass_of[2 * lane];
+            v = low + (by_number ? many_of[2 * lane + 1] : mass_of[2 * lane + 1]);
+        }
+        int at = lane_of(v, want, &before);
+        low = __shfl(low, at);
+        const bool odd = want > before + low;
+        want -= before + (odd ? low : 0);
+        const int base = (2 * at + odd) * kBinade;
+        v = pair(base + 2 * lane, by_number, &low);
+        at = lane_of(v, want, &more);
+        want -= more;
+        low = __shfl(low, at);
+        const bool second = want > low;
+        *need = want - (second ? low : 0);
+        return base + 2 * at + second;
+    };
+    const auto mass_before = [&](int place) {
+        uint64_t v = 0, low;
+        if (lane < kBinades / 2) v = (2 * lane < place / kBinade ? mass_of[2 * lane] : 0) + (2 * lane + 1 < place / kBinade ? mass_of[2 * lane + 1] : 0);
+        const int at = place / kBinade * kBinade + 2 * lane;
+        if (at < place) {  // (the binade of a place that was found has entries)
+            const uint64_t both = pair(at, false, &low);
+            v += at + 1 < place ? both : low;
+        }
+        return wave_sum(v);
+    };
+    const uint64_t all = wave_sum(lane < kBinades / 2 ? mass_of[2 * lane] + mass_of[2 * lane + 1] : 0);
+    // Kept are the places before `cut`, and of its entries the first `ties` by index.
+    int cut = kPlaces;
+    uint64_t ties = 0, left = all, need;
+    if (!greedily) {
+        if (ask.K > 0) {
+            const uint64_t many = wave_sum(lane < kBinades / 2 ? many_of[2 * lane] + many_of[2 * lane + 1] : 0);
+            if ((uint64_t)ask.K < many) {
+                cut = find(ask.K, true, &ties);
+                left = mass_before(cut) + ties * room.weight[cut];
+            }
+        }
+        if (ask.P < 1.0f) {
+            cut = find(ask.limit(left), false, &need);
+            const uint64_t one = room.weight[cut];
+            ties = (need + one - 1) / one;
+            left = mass_before(cut) + ties * one;
+        }
+        if (h.theta > -INFINITY) {  // a place that has entries and is the last that min-p keeps, or the one behind it
+            int lo = 0, step = kPlaces / 64;  // lo is kept
+            for (; step > 0; step = step == 1 ? 0 : max(step / 64, 1)) {
+                const int at = lo + step * (lane + 1);
+                const uint64_t gone = __ballot(at >= kPlaces || !h.likely(number_at(at)));
+                lo += step * (gone ? __ffsll((long long)gone) - 1 : 64);
+            }
+            const int end = lo + 1;
+            if (end <= cut) {
+                cut = end;
+                ties = 0;
+                left = 0;
+            }
+        }
+    }
+    // What is kept of each part: before the cut by each wave's binades, of the ties by a lane for each part.
+    uint32_t tied = 0;
+    if (ties && lane < parts && ((cut < 4096 ? has.x : cut < 8192 ? has.y : has.z) >> cut / kBinade % 32 & 1))
+        tied = b.many[((int64_t)blockIdx.x * parts + lane) * (kPlaces / 2) + cut / 2] >> (cut & 1 ? 16 : 0) & 0xffff;
+#pragma unroll 1
+    for (int from = 0; from < parts; from += kAhead) {
+        if (parts > kAhead) load(from);
+        uint64_t s[kAhead] = {};
+#pragma unroll
+        for (int i = 0; i < kOwn; ++i) {
+            const int at = binade(i) * kBinade + 2 * lane;
+            if (!(mine >> i & 1) || binade(i) * kBinade >= cut) continue;
+            const uint64_t v0 = at < cut ? room.weight[at] : 0, v1 = at + 1 < cut ? room.weight[at + 1] : 0;
+#pragma unroll
+            for (int j = 0; j < kAhead; ++j)
+                if (from + j < parts) s[j] += (held[j][i] & 0xffff) * v0 + (held[j][i] >> 16) * v1;
+        }
+#pragma unroll
+        for (int j = 0; j < kAhead; ++j) {
+            if (from + j >= parts) break;
+            const uint64_t sum = __any(s[j] != 0) ? wave_sum(s[j]) : 0;
+            if (lane == 0) sums[w][from + j] = sum;
+        }
+    }
+    __syncthreads();
+    uint64_t v = 0, target, before;
+    uint32_t rest = 0;
+    if (lane < parts)
+#pragma unroll
+        for (int i = 0; i < kPickWaves; ++i) v += sums[i][lane];
+    if (ties) {
+        uint32_t run = tied;
+#pragma unroll
+        for (int o = 1; o < kMostCounts; o <<= 1) {
+            const uint32_t q = __shfl_up(run, o);
+            if (lane >= o) run += q;
+        }
+        run -= tied;
+        rest = run < ties ? (uint32_t)ties - run : 0;  // of part `lane`, those that are kept
+        v += min(rest, tied) * room.weight[cut];
+    }
+    left = wave_sum(v);
+    target = greedily ? 0 : ask.target(left);
+    const int p = lane_of(v, target + 1, &before);
+    target -= before;
+    rest = __shfl(rest, p);
+    // In that part, by waves and then by threads: the weight of what is not a tie, and the ties, of which the
+    // first `rest` count (where some but not all of them do)
+    if (ties && rest >= __shfl(tied, p)) {
+        ++cut;
+        rest = 0;
+    }
+    const uint64_t tie_weight = rest ? room.weight[cut] : 0;
+    float least = number_at(cut - (rest ? 0 : 1));  // that counts
+    if (flags & kBetween) least = fmaxf(least, 0x1p-36f);  // they weigh nothing, and have no place
+    const auto add = [&](float x, uint64_t& s, uint32_t& t) {
+        if (!(x >= least)) return;
+        const uint32_t q = __float_as_uint(x + 0.0f);  // -0 as +0
+        const int at = kSigned + ((int)((max(q & 0x7fffffffu, kLowBits) - kLowBits) >> 16) ^ ~((int32_t)q >> 31));
+        if (at == cut) ++t;
+        else s += room.weight[at];
+    };
+    const auto weight = [&](uint64_t s, uint32_t t) { return s + min(t, rest) * tie_weight; };
+    const int32_t per_wave = (row.pieces + parts * kCountWaves - 1) / (parts * kCountWaves);
+    const int32_t from_piece = min(p * kCountWaves * per_wave, row.pieces), to_piece = min(from_piece + kCountWaves * per_wave, row.pieces);
+    const int32_t per = (to_piece - from_piece + kPickWaves - 1) / kPickWaves;
+    const auto wave_part = [&](int k) {
+        Part<BF16> q(row, V, 0, 1);
+        q.from = min(from_piece + k * per, to_piece);
+        q.to = min(q.from + per, to_piece);
+        q.first = p == 0 && k == 0 ? 0 : row.head + q.from * Span<BF16>::kPer;
+        q.last = p == parts - 1 && k == kPickWaves - 1 ? V : row.head + q.to * Span<BF16>::kPer;
+        return q;
+    };
+    uint64_t s = 0;
+    uint32_t t = 0;
+    {
+        const Part<BF16> q = wave_part(w);
+        constexpr int kBatch = 6;
+        const int32_t a = row.head + q.from * Span<BF16>::kPer, z = row.head + q.to * Span<BF16>::kPer;
+        if (q.first + lane < a) add(BF16::get(row.x[q.first + lane]), s, t);
+        if (z + lane < q.last) add(BF16::get(row.x[z + lane]), s, t);
+        for (int32_t at = q.from; at < q.to; at += 64 * kBatch) {
+            uint4 r[kBatch];
+#pragma unroll
+            for (int k = 0; k < kBatch; ++k) r[k] = at + 64 * k + lane < q.to ? row.piece(at + 64 * k + lane) : nothing<BF16>();
+#pragma unroll
+            for (int k = 0; k < kBatch; ++k) {
+                if (at + 64 * k >= q.to) break;
+                const Unpack<BF16> x(r[k]);
+#pragma unroll
+                for (int j = 0; j < Span<BF16>::kPer; ++j) add(x.v[j], s, t);
+            }
+        }
+    }
+    s = wave_sum(s);
+    if (rest) t = wave_sum(t);
+    __syncthreads();
+    if (lane == 0) {
+        sums[w][0] = s;
+        ties_of[w] = t;
+    }
+    __syncthreads();
+    s = 0;
+    t = 0;
+    int k = 0;
+    for (; k < kPickWaves - 1 && weight(s + sums[k][0], t + ties_of[k]) <= target; ++k) {
+        s += sums[k][0];
+        t += ties_of[k];
+    }
+    const Part<BF16> q = wave_part(k);
+    const int32_t each = (q.last - q.first + kThreads - 1) / kThreads;
+    const int32_t from = min(q.first + tid * each, q.last), to = min(from + each, q.last);
+    uint64_t own = 0;
+    uint32_t own_ties = 0;
+    for (int32_t i = from; i < to; ++i) add(BF16::get(row.x[i]), own, own_ties);
+    uint64_t total;
+    s += team.before(own, &total);
+    if (rest) t += (uint32_t)team.before(own_ties, &total);
+    if (weight(s, t) <= target && target < weight(s + own, t + own_ties)) {
+        int32_t i = from;
+        for (; i < to - 1; ++i) {
+            add(BF16::get(row.x[i]), s, t);
+            if (target < weight(s, t)) break;
+        }
+        if (greedily) {
+            b.a.action[n] = i;
+            b.a.logprob[n] = b.a.kept[n] = 0.0f;
+        } else {
+            answer(b.a, n, i, ((double)BF16::get(row.x[i]) - (double)m) / (double)ask.T, all, left);
+        }
+    }
+}
+
 // ---- short rows ------------------------------------------------------------
 // Up to 32 entries: one lane per row, the block's rows in LDS (an odd number of
 // words apart: no two lanes on one bank).  The order is not sorted: an entry's
@@ -1301,16 +1750,27 @@ int32_t parts_of(int64_t rows, int32_t vocab, int32_t per) {
     return (int32_t)std::min<int64_t>({std::max<int64_t>(1536 / batch_of(rows), 1), vocab / per / 512, kParts});
 }
 
+// 768 blocks of 512 threads are on the card at once; two pieces for each thread at least, and counts in 16 bits
+int32_t counts_of(int64_t rows, int32_t vocab) {
+    const int64_t most = std::min(vocab / 8192, 8), least = (vocab + 57343) / 57344;
+    return (int32_t)std::max(least, std::min(768 / batch_of(rows), most));
+}
+
+int run_counts(const Args& a, int64_t rows, void* space, hipStream_t st) {
+    const int64_t many = batch_of(rows);
+    const int32_t parts = counts_of(rows, a.vocab);
+    uint32_t* const counts = static_cast<uint32_t*>(space);
+    for (int64_t first = 0; first < rows; first += many) {
+        const Counts b{a, counts, reinterpret_cast<uint4*>(counts + many * parts * (kPlaces / 2)), first, parts};
+        const unsigned here = (unsigned)std::min(many, rows - first);
+        hipLaunchKernelGGL(k_cat_sample_count, dim3(here * parts), dim3(512), 0, st, b);
+        hipLaunchKernelGGL(k_cat_sample_pick, dim3(here), dim3(64 * kPickWaves), 0, st, b);
+    }
+    return launched();
+}
+
 template <class D>
-int run_sample(const Args& a, int64_t rows, void* space, hipStream_t st) {
-    if (a.vocab <= kTiny) {
-        hipLaunchKernelGGL(k_cat_sample_tiny<D>, dim3((unsigned)((rows + 63) / 64)), dim3(64), 0, st, a, rows);
-        return launched();
-    }
-    if (a.vocab <= kHeld) {
-        launch_held<D>(a, rows, st);
-        return launched();
-    }
+int run_parts(const Args& a, int64_t rows, void* space, hipStream_t st) {
     const bool cut = a.p.top_k || a.p.top_k_all > 0 || a.p.top_p || a.p.top_p_all < 1.0f;
     const int64_t many = batch_of(rows);
     const int32_t parts = parts_of(rows, a.vocab, Span<D>::kPer);
@@ -1326,6 +1786,20 @@ int run_sample(const Args& a, int64_t rows, void* space, hipStream_t st) {
     return launched();
 }
 
+template <class D>
+int run_sample(const Args& a, int64_t rows, void* space, hipStream_t st) {
+    if (a.vocab <= kTiny) {
+        hipLaunchKernelGGL(k_cat_sample_tiny<D>, dim3((unsigned)((rows + 63) / 64)), dim3(64), 0, st, a, rows);
+        return launched();
+    }
+    if (a.vocab <= kHeld) {
+        launch_held<D>(a, rows, st);
+        return launched();
+    }
+    if constexpr (std::is_same_v<D, BF16>) return run_counts(a, rows, space, st);
+    else return run_parts<D>(a, rows, space, st);
+}
+
 int bad(const char* what) { return rt_internal_fail(RT_EINVAL, (std::string("rt_cat_sample: ") + what).c_str()); }
 
 }  // namespace
@@ -1333,6 +1807,8 @@ int bad(const char* what) { return rt_internal_fail(RT_EINVAL, (std::string("rt_
 extern "C" int64_t rt_cat_sample_workspace_bytes(int64_t rows, int32_t vocab, int32_t dtype) {
     if (rows < 1 || rows > INT32_MAX || vocab < 1 || vocab > RT_CAT_MAX_VOCAB || bad_type(dtype)) return -1;
     if (vocab <= kHeld) return 0;
+    if (dtype == RT_DT_BF16)
+        return batch_of(rows) * counts_of(rows, vocab) * (kPlaces / 2 * (int64_t)sizeof(uint32_t) + (int64_t)sizeof(uint4));
     const int64_t hist = parts_of(rows, vocab, 16 / elem_size(dtype)) * kBins * (int64_t)sizeof(uint64_t);
     return batch_of(rows) * ((int64_t)sizeof(RowSpace) + hist);
 }

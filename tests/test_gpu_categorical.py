@@ -133,6 +133,36 @@ def test_sample_special_rows(C, dtype, v):
         check_sample(C, x, u, par)
 
 
+@pytest.mark.parametrize("v", [9217, 70000, 200003])
+def test_sample_bf16_of_every_magnitude(C, v):
+    """Numbers from the least to the largest that bf16 has, those that weigh something and those that do not."""
+    x = rows(13, v, torch.bfloat16, 15, pad=3, off=1)
+    odd = torch.randperm(v, generator=gen(16), device="cuda")[:400]
+    bits = lambda lo, hi: torch.randint(lo, hi, (400,), generator=gen(17), device="cuda").short().view(torch.bfloat16)  # noqa: E731
+    x[0, odd] = bits(1, 128)                  # subnormal
+    x[1] *= 2.0 ** -20
+    x[2] *= 2.0 ** -40                        # next to one another, all weigh the same or nearly
+    x[3, odd] = bits(0x4580, 0x4680)          # 2^12 and more
+    x[4, odd] = -bits(0x4580, 0x7f80)
+    x[5] = -(x[5].abs() * 2.0 ** 13)          # nothing above -2^12
+    x[5] = x[5].clamp(max=-5000.0)
+    x[6] = -x[6].abs() - 5.0                  # all negative, tiny ones on top
+    x[6, odd] = -bits(1, 0x2d80)
+    x[7, odd] = bits(1, 0x2d80)               # tiny ones where they weigh nothing
+    x[7, odd[0]] = 100.0
+    x[8] = -INF
+    x[8, odd] = bits(0, 0x7f80)
+    x[9] = -INF
+    x[9, odd] = bits(1, 0x2d80)
+    x[10] = -INF
+    x[10, odd] = -bits(0x4580, 0x7f80)
+    x[11, odd] = bits(0x2d80, 0x2e00)         # the borders of 2^-36
+    x[12, odd] = bits(0x4570, 0x4580)         # and of 2^12
+    u = torch.rand(13, generator=gen(18), device="cuda")
+    for par in (*FILTERS.values(), {"temperature": 3000.0}, {"temperature": 1e32, "top_p": 0.5}, {"temperature": 1e-3, "top_k": 40}):
+        check_sample(C, x, u, par)
+
+
 def test_sample_large_batches(C):
     """More rows than a grid holds at once, wide rows of every filter side by side, and one long row."""
     g = gen(4)
