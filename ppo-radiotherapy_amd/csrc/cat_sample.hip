@@ -8,10 +8,13 @@
 //
 // The three filters are prefixes of one order (falling logits, equal ones by
 // index), so their intersection is the shortest of them: a least key, and
-// where entries equal to it are cut apart, a last index.  The key is found
-// digit by digit from a histogram of the entries (top-k) or of their weights
-// (top-p) in LDS; then the running weight by index is searched segment by
-// segment.
+// where entries equal to it are cut apart, a last index.
+//
+// By the row's length: a lane has a row of up to 32 entries; a team of 64 to
+// 1024 threads holds one of up to 9216 in registers; a longer one is shared by
+// blocks.  There bf16 rows go by counts of each number (two launches, one pass
+// over the row and a second one over a part of it), f32 and f16 rows by bins
+// (four launches, three passes).
 #include <algorithm>
 #include <string>
 #include <type_traits>
@@ -133,8 +136,8 @@ struct Part {
 };
 
 // f(x, i) for every entry of a part; the lanes of one wave together, kAhead
-// pieces at a time, -inf where a lane has none.  `skip` says of a maximum whether all that is not above it
-// can be left out.
+// pieces at a time, -inf where a lane has none.  `skip` says of a maximum
+// whether all that is not above it can be left out.
 struct Never {
     __device__ __forceinline__ bool operator()(float) const { return false; }
 };
@@ -270,9 +273,11 @@ __device__ __forceinline__ void answer(const Args& A, int64_t n, int32_t a, doub
 }
 
 // ---- any row, slowly -------------------------------------------------------
-// Digit by digit over the whole row: for rows whose cut falls among more
-// entries than a list holds (many equal logits, a very large k) and for
-// temperatures past the histogram's range.
+// By one block, the key digit by digit from a histogram over the whole row: for
+// f32 and f16 rows whose cut falls among more entries than a list holds (many
+// equal logits, a very large k) and for temperatures past the bins' range.
+// 780 us for a row of 131072 equal f32 logits under top-k and top-p, where the
+// entries add to one place of LDS.
 template <class D, int THREADS>
 __device__ __forceinline__ void slow_row(const Args& A, int64_t n, const Ask& ask, float m, Shared<THREADS>& s) {
     const int32_t V = A.vocab;
@@ -303,7 +308,7 @@ __device__ __forceinline__ void slow_row(const Args& A, int64_t n, const Ask& as
     uint32_t cut = 0;
     uint64_t ties = UINT64_MAX, mass = all, above;
     if (ask.K > 0) {
-            cut = find_key<D, THREADS>(s, row, part, [&](float x, uint32_t, int32_t) { return (uint64_t)(x > -INFINITY); },
+        cut = find_key<D, THREADS>(s, row, part, [&](float x, uint32_t, int32_t) { return (uint64_t)(x > -INFINITY); },
                                    min((uint64_t)ask.K, sum([](float x, int32_t) { return (uint64_t)(x > -INFINITY); })), &above);
         ties = (uint64_t)ask.K - above;
         if (ask.P < 1.0f)
@@ -573,10 +578,13 @@ __device__ __forceinline__ uint32_t middle_key(uint32_t lo, uint32_t hi) {
     return mid > lo && mid < hi ? mid : lo + (hi - lo) / 2;
 }
 
-// ---- long rows, by parts ---------------------------------------------------
+// ---- long rows of f32 and f16, by parts ------------------------------------
 // Up to 64 blocks share a row, one launch for each thing that all of it has to
 // be known for: the maximum; the weights, and a histogram of them where there
 // is a cut to find; the entries around the cut; the answer, by one block.
+// 63 x 50021 f32, top-p: 5 + 16 + 14 + 17 us, 50 together (12.6 MB: 2.5 us of
+// HBM).  The weights are bound by f64 arithmetic and LDS additions, the others
+// by the trips to memory and barriers that follow one another.
 constexpr int kParts = 64, kPartWaves = 4;
 
 struct RowSpace {
@@ -1065,8 +1073,14 @@ __global__ __launch_bounds__(512) void k_cat_sample_answer(Batch b) {
 // of the row, with the weights by number in LDS.
 //
 // A place for each number with 2^-36 < |x| < 2^12, largest first, 0 in the
-// middle.  -inf is not counted.  Rows with others that weigh something go the
-// slow way.
+// middle.  -inf is not counted.  Rows with other numbers that weigh something
+// go the slow way.
+//
+// 256 x 131072, filters of all kinds: 21 us for the counts (67 MB: 3.2 TB/s),
+// 23 us for the rest by one block a row, 8 of them in the search of a part, the
+// others in loads and barriers that follow one another.  One row of 131072: 7
+// and 19 us.  Fewer parts make the search longer, more of them the counts: at
+// 256 rows six in place of three took 47 us in all, not 43.
 constexpr int kSigned = 48 * 128, kPlaces = 2 * kSigned, kZero = kSigned - 1;
 constexpr uint32_t kLowBits = (127 - 36) << 23;  // of the lowest magnitude; as its positive number's place is 0's
 enum { kOdd = 1, kAbove = 2, kBelow = 4, kBetween = 8 };  // NaN or +inf; past the places
@@ -1127,8 +1141,10 @@ __global__ __launch_bounds__(512) void k_cat_sample_count(Counts b) {
 }
 
 // A row with numbers that have no place: the key, and then the index, of each
-// cut by halving, a pass over the row for every step (1 ms for 131072 entries).
-// In little code and few registers: it stands in a kernel that has better to do.
+// cut by halving, a pass over the row for every step (131072 entries: 0.2 ms
+// without a cut, 0.9 with one, 1.6 with two).  In little code and few
+// registers: it stands in the kernel that every row goes through, and with
+// slow_row() there that one spilled (20 us more for each call).
 template <class T>
 __device__ __forceinline__ void other_row(const Args& A, int64_t n, const Ask& ask, T& team) {
     const int32_t V = A.vocab;
@@ -1199,7 +1215,9 @@ __device__ __forceinline__ void other_row(const Args& A, int64_t n, const Ask& a
 }
 
 // One block for a row.  The binades in turn for the waves: those that have
-// entries are next to one another.
+// entries are next to one another.  The counts stay in registers for the second
+// use, of up to eight parts; loops over a wave's binades that are not unrolled,
+// and cuts found by every wave for itself, where a barrier would cost more.
 __global__ __launch_bounds__(1024) void k_cat_sample_pick(Counts b) {
     constexpr int kThreads = 64 * kPickWaves, kOwn = kBinades / kPickWaves, kAhead = 8;
     static_assert(kOwn * kPickWaves == kBinades && kPickWaves == 16, "two binades of a wave in each word of a mask");
@@ -1508,6 +1526,7 @@ __global__ __launch_bounds__(1024) void k_cat_sample_pick(Counts b) {
 // Up to 32 entries: one lane per row, the block's rows in LDS (an odd number of
 // words apart: no two lanes on one bank).  The order is not sorted: an entry's
 // place in it is how many stand before it, and what is kept is a 32-bit mask.
+// 24576 x 11 f32: 8 us, a launch and one chain of f64 weights.
 constexpr int kTiny = 32;
 
 template <class D>
@@ -1590,12 +1609,13 @@ __global__ __launch_bounds__(64) void k_cat_sample_tiny(Args A, int64_t rows) {
 }
 
 // ---- rows that are held ----------------------------------------------------
-// Up to 9216 entries: a team of one to sixteen waves has the row in registers.
-// Thread t has the entries [t per, (t + 1) per), so the order by index is that
-// of the threads; the row passes through LDS on its way there (per is odd: no
-// bank conflicts).  The cut is found between two keys, by halving their
-// distance and by the largest key that is left below the upper: a dozen steps
-// of E compares and a sum over the team.
+// Up to 9216 entries: a team of one to sixteen waves has the row in registers,
+// nine entries a thread at most (with 17 the weights spill).  Thread t has the
+// entries [t per, (t + 1) per), so the order by index is that of the threads;
+// the row passes through LDS on its way there (per is odd: no bank conflicts).
+// The cut is found by team_key; each exchange is one barrier.  Bound by f64
+// arithmetic and those barriers: 4096 x 2048 f32 32 us without a filter, 64
+// with top-p (33.5 MB: 7 us of HBM); 65536 x 64 49 and 86.
 template <class D, int THREADS, int E>
 __global__ __launch_bounds__(THREADS < 256 ? 256 : THREADS) void k_cat_sample_held(Args A, int64_t rows) {
     constexpr int kRows = THREADS == 64 ? 4 : 1;  // of a block
