@@ -522,8 +522,8 @@ __global__ __launch_bounds__(THREADS) void k_cat_row(Logits l, Op op, Out o, dou
 // Few long rows leave most of the card idle at one block each, so several have
 // a part of a row: its sums first, then, each block from all parts' sums, the
 // part's gradient.  The backward pass is the second step alone, from the state.
-// 8 x 131072 bf16: 4 + 5 us, each a launch and two trips to memory; by one block
-// a row 39 together.  Backward, 1023 x 32003 f32: 39 us for 262 MB, 6.7 TB/s (the
+// 8 x 131072 bf16: 4 + 5 us, each a launch and two trips to memory, the whole
+// call 28 (39 by one block a row).  Backward, 1023 x 32003 f32: 39 us for 262 MB, 6.7 TB/s (the
 // logits lie in cache from the forward pass).
 struct PartSums {
     double m;
