@@ -48,17 +48,22 @@ struct Ppo {
         const int64_t a = b.actions[n];
         return a < 0 || a >= V || (b.weights && b.weights[n] == 0.0f);
     }
+    // What a row has beside its logits, asked for before their sums are known.
+    struct Given { float w, adv, old, ref; };
+    __device__ Given given(int64_t n) const {
+        return Given{b.weights ? b.weights[n] : 0.0f, b.advantages[n], b.old_logprobs[n], b.ref_logprobs ? b.ref_logprobs[n] : 0.0f};
+    }
     // From the row's log-probability of its action and its entropy: the state, and the weighted terms.
-    __device__ RowState finish(int64_t n, int64_t rows, double m, double logs, double lp, double h, double* term) const {
-        const double w = b.weights ? (double)b.weights[n] : 1.0 / (double)rows;
-        const double A = b.advantages[n], lr = lp - (double)b.old_logprobs[n], r = exp_64(lr);
+    __device__ RowState finish(const Given& g, int64_t rows, double m, double logs, double lp, double h, double* term) const {
+        const double w = b.weights ? (double)g.w : 1.0 / (double)rows;
+        const double A = g.adv, lr = lp - (double)g.old, r = exp_64(lr);
         const double lo = 1.0 - low, hi = 1.0 + high;
         const double rc = r < lo ? lo : r > hi ? hi : r;
         const double one = -A * r, two = -A * rc;
         const double pg = one >= two ? one : two > one ? two : one + two;  // the larger, NaN if one is
         double c = one >= two ? one : two > one ? 0.0 : pg, kl = 0.0;
         if (b.ref_logprobs) {
-            const double away = (double)b.ref_logprobs[n] - lp, q = exp_64(away);
+            const double away = (double)g.ref - lp, q = exp_64(away);
             kl = q - away - 1.0;
             if (klc != 0.0) c += klc * (1.0 - q);
         }
@@ -87,9 +92,9 @@ struct Distill {
 
     __device__ bool ignored(int64_t n, int32_t) const { return b.weights && b.weights[n] == 0.0f; }
     __device__ int32_t k() const { return b.k; }
-    __device__ double weight(int64_t n, int64_t rows) const {
-        return b.weights ? (double)b.weights[n] : 1.0 / (double)rows;
-    }
+    struct Given { float w; };
+    __device__ Given given(int64_t n) const { return Given{b.weights ? b.weights[n] : 0.0f}; }
+    __device__ double weight(const Given& g, int64_t rows) const { return b.weights ? (double)g.w : 1.0 / (double)rows; }
 };
 
 template <class D>
@@ -380,11 +385,11 @@ __device__ double teacher_load(const Distill& op, int64_t n, int32_t V, const ty
 
 // ---- from the sums to the loss ---------------------------------------------
 // By one wave: the row's state, its outputs, its terms of the sums over rows.
-__device__ __forceinline__ RowState ppo_row(const Ppo& op, const Out& o, int64_t n, int64_t rows, float m, double S,
-                                            double U, float xa, bool write, double* term) {
+__device__ __forceinline__ RowState ppo_row(const Ppo& op, const Out& o, const Ppo::Given& given, int64_t n, int64_t rows,
+                                            float m, double S, double U, float xa, bool write, double* term) {
     const double logs = log_64(S), lp = ((double)xa - (double)m) * op.inv - logs;
     const double h = logs - 0.6931471805599453 * (U / S);
-    const RowState st = op.finish(n, rows, m, logs, lp, h, term);
+    const RowState st = op.finish(given, rows, m, logs, lp, h, term);
     if (write) {
         o.logprob[n] = (float)lp;
         o.entropy[n] = (float)h;
@@ -392,8 +397,8 @@ __device__ __forceinline__ RowState ppo_row(const Ppo& op, const Out& o, int64_t
     return st;
 }
 
-__device__ __forceinline__ RowState distill_row(const Distill& op, const Out& o, int64_t n, int64_t rows, float m, double S,
-                                                const Teacher& te, double lse, double Q, bool write, double* term) {
+__device__ __forceinline__ RowState distill_row(const Distill& op, const Out& o, const Distill::Given& given, int64_t n,
+                                                int64_t rows, float m, double S, const Teacher& te, double lse, double Q, bool write, double* term) {
     const int lane = threadIdx.x & 63;
     const double logs = log_64(S), inv = op.inv;
     double kl = 0.0;
@@ -402,7 +407,7 @@ __device__ __forceinline__ RowState distill_row(const Distill& op, const Out& o,
         if (te.idx[j] >= 0 && q != 0.0) kl += q * (te.lq[j] - (((double)te.v[j] - (double)m) * inv - logs));
     }
     kl = wave_sum(kl);
-    const double w = op.weight(n, rows);
+    const double w = op.weight(given, rows);
     if (write) o.kl[n] = (float)kl;
     term[0] = w * kl;
     // E is 0 throughout: its place keeps the teacher's normaliser for the backward pass
@@ -410,7 +415,7 @@ __device__ __forceinline__ RowState distill_row(const Distill& op, const Out& o,
 }
 
 template <class Op>
-__device__ __forceinline__ RowState finish_row(const Op& op, const Out& o, int64_t n, int64_t rows, bool skip, float m,
+__device__ __forceinline__ RowState finish_row(const Op& op, const Out& o, const typename Op::Given& given, int64_t n, int64_t rows, bool skip, float m,
                                                const Sums& sums, float xa, const Teacher& te, double lse, double Q,
                                                bool write, double* terms) {
     const int tid = threadIdx.x;
@@ -418,10 +423,10 @@ __device__ __forceinline__ RowState finish_row(const Op& op, const Out& o, int64
     double term[Op::terms] = {};
     write = write && tid == 0;
     if constexpr (Op::ppo) {
-        if (!skip) st = ppo_row(op, o, n, rows, m, sums.s, sums.u, xa, write, term);
+        if (!skip) st = ppo_row(op, o, given, n, rows, m, sums.s, sums.u, xa, write, term);
         else if (write) o.logprob[n] = o.entropy[n] = 0.0f;
     } else {
-        if (!skip) st = distill_row(op, o, n, rows, m, sums.s, te, lse, Q, write, term);
+        if (!skip) st = distill_row(op, o, given, n, rows, m, sums.s, te, lse, Q, write, term);
         else if (write) o.kl[n] = 0.0f;
     }
     if (write) {
@@ -473,6 +478,7 @@ __global__ __launch_bounds__(THREADS) void k_cat_row(Logits l, Op op, Out o, dou
     float m = -INFINITY, xa = 0.0f;
     Sums sums{0.0, 0.0};
     bool skip = op.ignored(n, l.vocab);
+    const auto given = op.given(n);
     double lse = 0.0, Q = 0.0;
     if (!skip) {
         if constexpr (Op::ppo) xa = D::get(x[op.b.actions[n]]);
@@ -481,7 +487,7 @@ __global__ __launch_bounds__(THREADS) void k_cat_row(Logits l, Op op, Out o, dou
         skip = m == -INFINITY && sums.s == 0.0;
     }
     if (tid < 64) {
-        const RowState st = finish_row(op, o, n, l.rows, skip, m, sums, xa, te, lse, Q, true, terms);
+        const RowState st = finish_row(op, o, given, n, l.rows, skip, m, sums, xa, te, lse, Q, true, terms);
         if (tid == 0) slots.state = st;
     }
     if (!o.grad) return;
@@ -590,6 +596,7 @@ __global__ __launch_bounds__(256) void k_cat_grad(Logits l, Op op, Out o, const 
     if constexpr (JOIN) {
         if (tid < 64) {
             bool skip = op.ignored(n, l.vocab);
+            const auto given = op.given(n);
             float m = -INFINITY, xa = 0.0f;
             double lse = 0.0, Q = 0.0;
             Sums sums{0.0, 0.0};
@@ -599,7 +606,7 @@ __global__ __launch_bounds__(256) void k_cat_grad(Logits l, Op op, Out o, const 
                 sums = join<Op::ppo>(from + n * parts, parts, scale_of(op.inv), &m);
                 skip = m == -INFINITY && sums.s == 0.0;
             }
-            st = finish_row(op, o, n, l.rows, skip, m, sums, xa, te, lse, Q, part == 0, terms);
+            st = finish_row(op, o, given, n, l.rows, skip, m, sums, xa, te, lse, Q, part == 0, terms);
             if (tid == 0) share = st;
         }
         if (!o.grad) return;
@@ -660,12 +667,15 @@ __global__ __launch_bounds__(256) void k_cat_grad(Logits l, Op op, Out o, const 
 
 // The sums of a block's rows, in a fixed order.
 template <int TERMS>
-__device__ __forceinline__ void block_terms(const double* term, double* ds, double* to) {
+__device__ __forceinline__ void block_terms(const double* term, double (*ds)[TERMS], double* to) {
 #pragma unroll
     for (int k = 0; k < TERMS; ++k) {
-        const double r = block_sum<256>(term[k], ds);
-        if (threadIdx.x == 0) to[block_index() * TERMS + k] = r;
+        const double r = wave_sum(term[k]);
+        if ((threadIdx.x & 63) == 0) ds[threadIdx.x >> 6][k] = r;
     }
+    __syncthreads();
+    const int k = threadIdx.x;
+    if (k < TERMS) to[block_index() * TERMS + k] = ds[0][k] + ds[1][k] + ds[2][k] + ds[3][k];
 }
 
 // G lanes per row, E entries each, in registers.  GIVEN: the backward pass,
@@ -673,7 +683,7 @@ __device__ __forceinline__ void block_terms(const double* term, double* ds, doub
 template <class D, class Op, int G, int E, bool GIVEN>
 __global__ __launch_bounds__(256) void k_cat_short(Logits l, Op op, Out o, double* terms, const RowState* state,
                                                    const float* gout) {
-    __shared__ double ds[4];
+    __shared__ double ds[4][Op::terms];
     const int t = threadIdx.x % G;
     const int64_t n0 = block_index() * (256 / G), n = n0 + threadIdx.x / G;
     if (n0 >= l.rows) return;
@@ -683,17 +693,31 @@ __global__ __launch_bounds__(256) void k_cat_short(Logits l, Op op, Out o, doubl
     double term[Op::terms] = {};
     RowState st{0.0, INFINITY, 0.0, 0.0, 0.0};
     bool skip = !in || (GIVEN ? false : op.ignored(n, V));
+    typename Op::Given given{};
+    if (!GIVEN && in) given = op.given(n);
     if (GIVEN && in) {
         st = state[n];
         skip = st.logs == INFINITY;
+    }
+    // the lane's first entry of the teacher's, asked for before the logits are waited for
+    struct { int32_t i; float t, x; } first{-1, 0.0f, 0.0f};
+    const int64_t at = Op::ppo || !in ? 0 : n * op.k();
+    if constexpr (!Op::ppo) {
+        if (!skip && t < op.b.k) {
+            const int64_t i = op.b.idx[at + t];
+            first.t = op.b.logits[at + t];
+            if (i >= 0 && i < V) first.i = (int32_t)i;
+        }
     }
     float v[E], m = -INFINITY;
 #pragma unroll
     for (int e = 0; e < E; ++e) {
         const int32_t i = t + G * e;
         v[e] = !skip && i < V ? D::get(x[i]) : -INFINITY;
-        m = fmaxf(m, v[e]);
     }
+    if (!Op::ppo && !GIVEN && first.i >= 0) first.x = D::get(x[first.i]);
+#pragma unroll
+    for (int e = 0; e < E; ++e) m = fmaxf(m, v[e]);
     if constexpr (!GIVEN) {
         const double c = 1.4426950408889634 * op.inv;
         m = lanes_max<G>(m);
@@ -710,39 +734,38 @@ __global__ __launch_bounds__(256) void k_cat_short(Logits l, Op op, Out o, doubl
         skip = skip || S == 0.0;
         if constexpr (Op::ppo) {
             if (!skip) {
-                st = ppo_row(op, o, n, l.rows, m, S, U, D::get(x[op.b.actions[n]]), t == 0, term);
+                st = ppo_row(op, o, given, n, l.rows, m, S, U, D::get(x[op.b.actions[n]]), t == 0, term);
             } else if (in && t == 0) {
                 o.logprob[n] = o.entropy[n] = 0.0f;
             }
         } else {
             double kl = 0.0, Q = 0.0, lse = 0.0;
-            const double logs = log_64(S), w = skip ? 0.0 : op.weight(n, l.rows);
-            const int64_t at = in ? n * op.b.k : 0;
+            const double logs = log_64(S), w = skip ? 0.0 : op.weight(given, l.rows);
+            // f(the teacher's logit, the student's) for the lane's entries
+            const auto entries = [&](auto f) {
+                if (first.i >= 0) f(first.t, first.x);
+                for (int j = t + G; j < op.b.k; j += G) {
+                    const int64_t i = op.b.idx[at + j];
+                    if (i >= 0 && i < V) f(op.b.logits[at + j], D::get(x[i]));
+                }
+            };
             if (op.b.lse) {
                 if (!skip) lse = op.b.lse[n];
             } else {
                 float tm = -INFINITY;
-                for (int j = t; j < op.b.k; j += G) {
-                    const int64_t i = op.b.idx[at + j];
-                    if (i >= 0 && i < V) tm = fmaxf(tm, op.b.logits[at + j]);
-                }
+                entries([&](float tl, float) { tm = fmaxf(tm, tl); });
                 tm = lanes_max<G>(tm);
                 if (tm == -INFINITY) tm = 0.0f;
-                for (int j = t; j < op.b.k; j += G) {
-                    const int64_t i = op.b.idx[at + j];
-                    if (i >= 0 && i < V) lse += exp2_64(((double)op.b.logits[at + j] - (double)tm) * c);
-                }
+                entries([&](float tl, float) { lse += exp2_64(((double)tl - (double)tm) * c); });
                 lse = lanes_sum<G>(lse);
                 lse = lse == 0.0 ? 0.0 : (double)tm * op.inv + log_64(lse);
             }
             if (!skip) {
-                for (int j = t; j < op.b.k; j += G) {
-                    const int64_t i = op.b.idx[at + j];
-                    if (i < 0 || i >= V) continue;
-                    const double lq = (double)op.b.logits[at + j] * op.inv - lse, q = exp_64(lq);
-                    if (q != 0.0) kl += q * (lq - (((double)D::get(x[i]) - (double)m) * op.inv - logs));
+                entries([&](float tl, float xl) {
+                    const double lq = (double)tl * op.inv - lse, q = exp_64(lq);
+                    if (q != 0.0) kl += q * (lq - (((double)xl - (double)m) * op.inv - logs));
                     Q += q;
-                }
+                });
             }
             kl = lanes_sum<G>(kl);
             Q = lanes_sum<G>(Q);
@@ -765,17 +788,16 @@ __global__ __launch_bounds__(256) void k_cat_short(Logits l, Op op, Out o, doubl
     float named[E] = {};
     if constexpr (!Op::ppo) {
         // the teacher's entries in turn, each met by the lane that has its place
-        const int64_t at = n * op.b.k;
         for (int j0 = 0; j0 < op.b.k; j0 += G) {
-            int32_t idx = -1;
-            float q = 0.0f;
-            if (!skip && j0 + t < op.b.k) {
+            int32_t idx = j0 ? -1 : first.i;
+            float tl = first.t;
+            if (j0 && !skip && j0 + t < op.b.k) {
                 const int64_t i = op.b.idx[at + j0 + t];
-                if (i >= 0 && i < V) {
-                    idx = (int32_t)i;
-                    q = (float)exp_64((double)op.b.logits[at + j0 + t] * op.inv - st.e);
-                }
+                tl = op.b.logits[at + j0 + t];
+                if (i >= 0 && i < V) idx = (int32_t)i;
             }
+            const float q = skip || idx < 0 ? 0.0f : (float)exp_64((double)tl * op.inv - st.e);
+            if (skip) idx = -1;
             const int many = min(G, op.b.k - j0);
             for (int j = 0; j < many; ++j) {
                 const int32_t bi = __shfl(idx, j, G);
@@ -808,28 +830,26 @@ constexpr int kTiny = 32;
 template <class D, class Op, bool GIVEN>
 __global__ __launch_bounds__(256) void k_cat_tiny(Logits l, Op op, Out o, double* terms, const RowState* state,
                                                   const float* gout) {
-    __shared__ double ds[4];
+    __shared__ double ds[4][Op::terms];
     __shared__ float tile[256 * (kTiny + 1)];
     const int tid = threadIdx.x;
     const int32_t V = l.vocab, pitch = V | 1;
     const int64_t n0 = block_index() * 256, n = n0 + tid;
     if (n0 >= l.rows) return;
     const int32_t here = (int32_t)min((int64_t)256, l.rows - n0);
-    const float per = 1.0f / (float)V;  // (i + 1/2) / V is 1/64 or more away from a whole number
-    for (int32_t i = tid; i < here * V; i += 256) {
-        const int32_t r = (int32_t)(((float)i + 0.5f) * per), c = i - r * V;
-        tile[r * pitch + c] = D::get(row_of<D>(l, n0 + r)[c]);
-    }
-    __syncthreads();
     const bool in = tid < here;
-    float* x = tile + tid * pitch;
-    double term[Op::terms] = {};
     RowState st{0.0, INFINITY, 0.0, 0.0, 0.0};
     bool skip = !in || (GIVEN ? false : op.ignored(n, V));
+    typename Op::Given given{};
+    if (!GIVEN && in) given = op.given(n);
     if (GIVEN && in) {
         st = state[n];
         skip = st.logs == INFINITY;
     }
+    load_tile<D, 256>(tile, row_of<D>(l, n0), l.stride, here, V);
+    __syncthreads();
+    float* x = tile + tid * pitch;
+    double term[Op::terms] = {};
     if constexpr (!GIVEN) {
         if (!skip) {
             const double c = 1.4426950408889634 * op.inv;
@@ -845,9 +865,9 @@ __global__ __launch_bounds__(256) void k_cat_tiny(Logits l, Op op, Out o, double
             skip = S == 0.0;
             if (!skip) {
                 if constexpr (Op::ppo) {
-                    st = ppo_row(op, o, n, l.rows, m, S, U, x[op.b.actions[n]], true, term);
+                    st = ppo_row(op, o, given, n, l.rows, m, S, U, x[op.b.actions[n]], true, term);
                 } else {
-                    const double logs = log_64(S), w = op.weight(n, l.rows);
+                    const double logs = log_64(S), w = op.weight(given, l.rows);
                     const int64_t at = n * op.b.k;
                     double lse = 0.0, kl = 0.0, Q = 0.0;
                     if (op.b.lse) {
@@ -906,8 +926,9 @@ __global__ __launch_bounds__(256) void k_cat_tiny(Logits l, Op op, Out o, double
         }
     }
     __syncthreads();
+    const float per = 1.0f / (float)V;
     for (int32_t i = tid; i < here * V; i += 256) {
-        const int32_t r = (int32_t)(((float)i + 0.5f) * per), c = i - r * V;
+        const int32_t r = (int32_t)(((float)i + 0.5f) * per), c = i - r * V;  // as load_tile's
         static_cast<typename D::raw*>(o.grad)[(n0 + r) * o.grad_stride + c] = D::put(tile[r * pitch + c]);
     }
 }

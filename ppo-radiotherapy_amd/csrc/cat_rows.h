@@ -169,6 +169,27 @@ struct Unpack {
     }
 };
 
+// Rows of V <= 32 entries into LDS, V | 1 words apart; eight trips to memory at
+// once (one by one they were most of what such a row took).
+template <class D, int THREADS>
+__device__ __forceinline__ void load_tile(float* tile, const typename D::raw* x, int64_t stride, int32_t rows, int32_t V) {
+    constexpr int kAhead = 8;
+    const float per = 1.0f / (float)V;  // (i + 1/2) / V is 1/64 or more away from a whole number
+    for (int32_t from = threadIdx.x; from < rows * V; from += kAhead * THREADS) {
+        typename D::raw v[kAhead];
+        int32_t at[kAhead];
+#pragma unroll
+        for (int k = 0; k < kAhead; ++k) {
+            const int32_t i = from + k * THREADS, r = (int32_t)(((float)i + 0.5f) * per), c = i - r * V;
+            at[k] = r * (V | 1) + c;
+            if (i < rows * V) v[k] = x[r * stride + c];
+        }
+#pragma unroll
+        for (int k = 0; k < kAhead; ++k)
+            if (from + k * THREADS < rows * V) tile[at[k]] = D::get(v[k]);
+    }
+}
+
 // 16 bytes of entries that add nothing
 template <class D>
 __device__ __forceinline__ uint4 nothing() {

@@ -1142,16 +1142,17 @@ __global__ __launch_bounds__(512) void k_cat_sample_count(Counts b) {
 
 // A row with numbers that have no place: the key, and then the index, of each
 // cut by halving, a pass over the row for every step (131072 entries: 0.2 ms
-// without a cut, 0.9 with one, 1.6 with two).  In little code and few
+// without a cut, 1.2 with one, 2.1 with two).  In little code and few
 // registers: it stands in the kernel that every row goes through, and with
 // slow_row() there that one spilled (20 us more for each call).
 template <class T>
 __device__ __forceinline__ void other_row(const Args& A, int64_t n, const Ask& ask, T& team) {
+    constexpr int kThreads = T::kWaves * 64;
     const int32_t V = A.vocab;
     const uint16_t* const x = static_cast<const uint16_t*>(A.x) + n * A.stride;
     const auto key = [](float v) { return key_of(v) >> 16; };
     uint32_t top = 0;
-    for (int32_t i = threadIdx.x; i < V; i += T::kWaves * 64) top = max(top, key_of(BF16::get(x[i])));
+    for (int32_t i = threadIdx.x; i < V; i += kThreads) top = max(top, key_of(BF16::get(x[i])));
     const float m = of_key(team.top(top));
     const bool greedily = !(ask.T > 0.0f);
     const Head h(ask, m);
@@ -1159,12 +1160,19 @@ __device__ __forceinline__ void other_row(const Args& A, int64_t n, const Ask& a
     // how many they are, or what they weigh
     const auto pass = [&](uint32_t least, int32_t last, int32_t end, bool by_number, double theta) {
         uint64_t v = 0;
-#pragma unroll 4
-        for (int32_t i = threadIdx.x; i < end; i += T::kWaves * 64) {
-            const float f = BF16::get(x[i]);
-            const uint32_t k = key(f);
-            const bool in = k > least || (k == least && i <= last);
-            v += !in || (double)f - (double)m < theta ? 0 : by_number ? (uint64_t)(f > -INFINITY) : h.weigh(f);
+#pragma unroll 1
+        for (int32_t i = threadIdx.x; i < end; i += 4 * kThreads) {
+            uint64_t four = 0xff80ff80ff80ff80ull;  // -inf
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                if (i + j * kThreads < end) four ^= (uint64_t)(x[i + j * kThreads] ^ 0xff80) << 16 * j;
+#pragma unroll 1
+            for (int j = 0; j < 4; ++j, four >>= 16) {
+                const float f = BF16::get((uint16_t)four);
+                const uint32_t k = key(f);
+                const bool in = k > least || (k == least && i + j * kThreads <= last);
+                v += !in || (double)f - (double)m < theta ? 0 : by_number ? (uint64_t)(f > -INFINITY) : h.weigh(f);
+            }
         }
         return team.sum(v);
     };
@@ -1537,11 +1545,7 @@ __global__ __launch_bounds__(64) void k_cat_sample_tiny(Args A, int64_t rows) {
     const int32_t V = A.vocab, pitch = V | 1;
     const int64_t n0 = (int64_t)blockIdx.x * 64, n = n0 + tid;
     const int32_t here = (int32_t)min((int64_t)64, rows - n0);
-    const float per = 1.0f / (float)V;  // (i + 1/2) / V is 1/64 or more away from a whole number
-    for (int32_t i = tid; i < here * V; i += 64) {
-        const int32_t r = (int32_t)(((float)i + 0.5f) * per), c = i - r * V;
-        tile[r * pitch + c] = D::get(static_cast<const typename D::raw*>(A.x)[(n0 + r) * A.stride + c]);
-    }
+    load_tile<D, 64>(tile, static_cast<const typename D::raw*>(A.x) + n0 * A.stride, A.stride, here, V);
     __syncthreads();
     if (tid >= here) return;
     const float* x = tile + tid * pitch;
