@@ -1769,9 +1769,10 @@ constexpr int64_t kBatch = 512;
 
 int64_t batch_of(int64_t rows) { return std::min(rows, kBatch); }
 // 1536 blocks of 256 threads are on the card at once (six on a CU, by their registers: 2048 took 20 %
-// longer); two pieces for each thread at least
-int32_t parts_of(int64_t rows, int32_t vocab, int32_t per) {
-    return (int32_t)std::min<int64_t>({std::max<int64_t>(1536 / batch_of(rows), 1), vocab / per / 512, kParts});
+// longer); 16 entries for each thread at least (63 x 50021 f32, top-p: 44 us, with eight 52: every part has a
+// histogram to write and to read)
+int32_t parts_of(int64_t rows, int32_t vocab) {
+    return (int32_t)std::min<int64_t>({std::max<int64_t>(1536 / batch_of(rows), 1), vocab / 4096, kParts});
 }
 
 // 768 blocks of 512 threads are on the card at once; two pieces for each thread at least, and counts in 16 bits
@@ -1797,7 +1798,7 @@ template <class D>
 int run_parts(const Args& a, int64_t rows, void* space, hipStream_t st) {
     const bool cut = a.p.top_k || a.p.top_k_all > 0 || a.p.top_p || a.p.top_p_all < 1.0f;
     const int64_t many = batch_of(rows);
-    const int32_t parts = parts_of(rows, a.vocab, Span<D>::kPer);
+    const int32_t parts = parts_of(rows, a.vocab);
     RowSpace* const rooms = static_cast<RowSpace*>(space);
     for (int64_t first = 0; first < rows; first += many) {
         const Batch b{a, rooms, reinterpret_cast<uint64_t*>(rooms + many), first, parts};
@@ -1833,7 +1834,7 @@ extern "C" int64_t rt_cat_sample_workspace_bytes(int64_t rows, int32_t vocab, in
     if (vocab <= kHeld) return 0;
     if (dtype == RT_DT_BF16)
         return batch_of(rows) * counts_of(rows, vocab) * (kPlaces / 2 * (int64_t)sizeof(uint32_t) + (int64_t)sizeof(uint4));
-    const int64_t hist = parts_of(rows, vocab, 16 / elem_size(dtype)) * kBins * (int64_t)sizeof(uint64_t);
+    const int64_t hist = parts_of(rows, vocab) * kBins * (int64_t)sizeof(uint64_t);
     return batch_of(rows) * ((int64_t)sizeof(RowSpace) + hist);
 }
 

@@ -163,6 +163,14 @@ def test_sample_bf16_of_every_magnitude(C, v):
         check_sample(C, x, u, par)
 
 
+@pytest.mark.parametrize("v", [57343, 57345, 114688, 2 ** 20])
+def test_sample_more_equal_logits_than_16_bits_count(C, v):
+    for i, par in enumerate(FILTERS.values()):
+        x = rows(2, v, torch.bfloat16, 19, off=i % 2, kind="flat")
+        x[1, v // 3:] = -2.0
+        check_sample(C, x, torch.rand(2, generator=gen(20 + i), device="cuda"), par)
+
+
 def test_sample_large_batches(C):
     """More rows than a grid holds at once, wide rows of every filter side by side, and one long row."""
     g = gen(4)
