@@ -251,6 +251,29 @@ class _Ppo:
         return res, state
 
 
+class _Final(torch.autograd.Function):
+    """A gradient by `logits` that is not differentiated: trying to raises."""
+
+    @staticmethod
+    def forward(ctx, grad, logits):
+        return grad
+
+    @staticmethod
+    def backward(ctx, g):
+        raise RuntimeError("ppo_loss and distill_loss are differentiated once only")
+
+
+def _once(backward):
+    def run(ctx, gloss):
+        if not torch.is_grad_enabled():  # no graph of the gradient is asked for
+            return backward(ctx, gloss), None
+        with torch.no_grad():
+            grad = backward(ctx, gloss)
+        return _Final.apply(grad, ctx.saved_tensors[0]), None
+
+    return staticmethod(run)
+
+
 def _with_grad(fn, logits, op):
     # A captured backward pass ends the process where an eager graph of the same leaves is alive (their
     # nodes keep its stream): nothing here can tell.
@@ -270,18 +293,18 @@ class _PpoFn(torch.autograd.Function):
         ctx.save_for_backward(logits, op.actions, state)
         return op.rest.loss
 
-    @staticmethod
-    @torch.autograd.function.once_differentiable
+    @_once
     def backward(ctx, gloss):
         logits, actions, state = ctx.saved_tensors
         r = _Rows(logits)
         grad, stride = r.grad_buffer(None)
         if r.n == 0:
-            return grad, None
-        gloss = gloss.to(torch.float32).contiguous()
+            return grad
+        if gloss.dtype != torch.float32:
+            gloss = gloss.float()
         r.call(_lib.load().rt_cat_ppo_backward, "rt_cat_ppo_backward", ctypes.byref(r.arg()), actions.data_ptr(),
                ctx.temperature, state.data_ptr(), gloss.data_ptr(), grad.data_ptr(), stride)
-        return grad, None
+        return grad
 
 
 def ppo_loss(logits, actions, old_logprobs, advantages, *, weights=None, ref_logprobs=None, temperature=1.0,
@@ -353,19 +376,19 @@ class _DistillFn(torch.autograd.Function):
         ctx.save_for_backward(logits, op.idx, op.top, op.lse, op.weights, state)
         return op.rest.loss
 
-    @staticmethod
-    @torch.autograd.function.once_differentiable
+    @_once
     def backward(ctx, gloss):
         logits, idx, top, lse, weights, state = ctx.saved_tensors  # raises where one of them was changed in place
         r = _Rows(logits)
         grad, stride = r.grad_buffer(None)
         if r.n == 0:
-            return grad, None
-        gloss = gloss.to(torch.float32).contiguous()
+            return grad
+        if gloss.dtype != torch.float32:
+            gloss = gloss.float()
         teacher = _lib.RtCatTeacher(idx.data_ptr(), top.data_ptr(), _lib.ptr(lse), _lib.ptr(weights), ctx.k, ctx.temperature)
         r.call(_lib.load().rt_cat_distill_backward, "rt_cat_distill_backward", ctypes.byref(r.arg()),
                ctypes.byref(teacher), state.data_ptr(), gloss.data_ptr(), grad.data_ptr(), stride)
-        return grad, None
+        return grad
 
 
 def distill_loss(logits, teacher_idx, teacher_logits, *, weights=None, teacher_lse=None, temperature=1.0) -> DistillLoss:

@@ -553,6 +553,20 @@ def test_changed_inputs_are_noticed(C):
         r.loss.backward()
 
 
+def test_second_derivatives_are_refused(C):
+    x = torch.randn(3, 20, device="cuda", requires_grad=True)
+    a, old, adv, _, _ = ppo_inputs(3, 20, 64, x.detach())
+    idx, top, _ = teacher_inputs(3, 20, 4, 64)
+    for loss in (lambda: C.ppo_loss(x, a, old, adv).loss, lambda: C.distill_loss(x, idx, top).loss):
+        plain, = torch.autograd.grad(loss(), x)
+        g, = torch.autograd.grad(loss(), x, create_graph=True)
+        assert torch.equal(g, plain)
+        with pytest.raises(RuntimeError, match="once only"):
+            torch.autograd.grad(g.sum(), x)
+        with pytest.raises(RuntimeError, match="once only"):
+            (g.square().sum() + x.sum()).backward()
+
+
 def test_gradient_in_place_is_noticed(C):
     """Logits that another graph has saved, written over with their gradient."""
     h = torch.randn(3, 20, device="cuda")
