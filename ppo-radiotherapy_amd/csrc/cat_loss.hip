@@ -663,7 +663,7 @@ __global__ __launch_bounds__(256) void k_cat_grad(Logits l, Op op, Out o, const 
 // Up to 1024 entries: many rows, so more of them lie next to the border of the
 // clip, and the memory they need is small beside the arithmetic of a row: the
 // sums are in f64 throughout.  Bound by that arithmetic: 32768 x 64 f32 with 8
-// of a teacher's entries 16 us (17 MB: 4 us).
+// of a teacher's entries 15 us (17 MB: 4 us).
 
 // The sums of a block's rows, in a fixed order.
 template <int TERMS>

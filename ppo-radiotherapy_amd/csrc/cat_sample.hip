@@ -582,7 +582,7 @@ __device__ __forceinline__ uint32_t middle_key(uint32_t lo, uint32_t hi) {
 // Up to 64 blocks share a row, one launch for each thing that all of it has to
 // be known for: the maximum; the weights, and a histogram of them where there
 // is a cut to find; the entries around the cut; the answer, by one block.
-// 63 x 50021 f32, top-p: 5 + 16 + 14 + 17 us, 50 together (12.6 MB: 2.5 us of
+// 63 x 50021 f32, top-p: 5 + 13 + 11 + 15 us, 43 together (12.6 MB: 2.5 us of
 // HBM).  The weights are bound by f64 arithmetic and LDS additions, the others
 // by the trips to memory and barriers that follow one another.
 constexpr int kParts = 64, kPartWaves = 4;
@@ -1076,7 +1076,7 @@ __global__ __launch_bounds__(512) void k_cat_sample_answer(Batch b) {
 // middle.  -inf is not counted.  Rows with other numbers that weigh something
 // go the slow way.
 //
-// 256 x 131072, filters of all kinds: 21 us for the counts (67 MB: 3.2 TB/s),
+// 256 x 131072, filters of all kinds: 22 us for the counts (67 MB: 3 TB/s),
 // 23 us for the rest by one block a row, 8 of them in the search of a part, the
 // others in loads and barriers that follow one another.  One row of 131072: 7
 // and 19 us.  Fewer parts make the search longer, more of them the counts: at
