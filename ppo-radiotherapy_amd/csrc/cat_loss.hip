@@ -398,7 +398,8 @@ __device__ __forceinline__ RowState ppo_row(const Ppo& op, const Out& o, const P
 }
 
 __device__ __forceinline__ RowState distill_row(const Distill& op, const Out& o, const Distill::Given& given, int64_t n,
-                                                int64_t rows, float m, double S, const Teacher& te, double lse, double Q, bool write, double* term) {
+                                                int64_t rows, float m, double S, const Teacher& te, double lse, double Q,
+                                                bool write, double* term) {
     const int lane = threadIdx.x & 63;
     const double logs = log_64(S), inv = op.inv;
     double kl = 0.0;
@@ -415,7 +416,8 @@ __device__ __forceinline__ RowState distill_row(const Distill& op, const Out& o,
 }
 
 template <class Op>
-__device__ __forceinline__ RowState finish_row(const Op& op, const Out& o, const typename Op::Given& given, int64_t n, int64_t rows, bool skip, float m,
+__device__ __forceinline__ RowState finish_row(const Op& op, const Out& o, const typename Op::Given& given, int64_t n,
+                                               int64_t rows, bool skip, float m,
                                                const Sums& sums, float xa, const Teacher& te, double lse, double Q,
                                                bool write, double* terms) {
     const int tid = threadIdx.x;

@@ -1355,8 +1355,9 @@ __global__ __launch_bounds__(1024) void k_cat_sample_pick(Counts b) {
     };
     const auto mass_before = [&](int place) {
         uint64_t v = 0, low;
-        if (lane < kBinades / 2) v = (2 * lane < place / kBinade ? mass_of[2 * lane] : 0) + (2 * lane + 1 < place / kBinade ? mass_of[2 * lane + 1] : 0);
-        const int at = place / kBinade * kBinade + 2 * lane;
+        const int whole = place / kBinade, at = whole * kBinade + 2 * lane;
+        if (lane < kBinades / 2)
+            v = (2 * lane < whole ? mass_of[2 * lane] : 0) + (2 * lane + 1 < whole ? mass_of[2 * lane + 1] : 0);
         if (at < place) {  // (the binade of a place that was found has entries)
             const uint64_t both = pair(at, false, &low);
             v += at + 1 < place ? both : low;
