@@ -500,7 +500,12 @@ struct Listed {
 // want <= the sum of all), and the sum above it.  A histogram by bin(e) (larger
 // keys have no larger bin) says in which bin; there, the largest key that is
 // left, and then the middle of what is left, each with its sum: most bins have
-// an entry or two.  hist: BINS places of LDS.
+// an entry or two.  The first kMiddles middles are those of `middle`, which
+// suits the bin; numbers next to 0 can be more than a hundred halvings apart,
+// but any two keys are 32, so from then on the keys are halved, and the search
+// ends in kMiddles + 33 steps.  hist: BINS places of LDS.
+constexpr int kMiddles = 16;
+
 template <int BINS, class K, class T, class Each, class Key, class Bin, class Value, class Middle>
 __device__ __forceinline__ K team_key(T& team, uint64_t* hist, Each each, Key key, Bin bin, Value value, uint64_t want, Middle middle,
                                       uint64_t* above) {
@@ -547,7 +552,7 @@ __device__ __forceinline__ K team_key(T& team, uint64_t* hist, Each each, Key ke
         each([&](int e) { s += key(e) >= least ? value(e) : 0; });
         return team.sum(s);
     };
-    for (int step = 0; step < 64; ++step) {  // keys have 32 bits: halving alone ends sooner
+    for (int step = 0; step < kMiddles + 33; ++step) {
         uint64_t sum = from(k);
         if (sum >= want) {
             *above = over;
@@ -555,7 +560,8 @@ __device__ __forceinline__ K team_key(T& team, uint64_t* hist, Each each, Key ke
         }
         K hi = k;
         over = sum;
-        const K mid = middle(lo, hi);  // lo <= mid < hi
+        K mid = middle(lo, hi);
+        if (step >= kMiddles || mid <= lo || mid >= hi) mid = lo + (hi - lo) / 2;  // lo <= mid < hi
         sum = from(mid);
         if (sum >= want) {
             lo = mid;
@@ -567,15 +573,14 @@ __device__ __forceinline__ K team_key(T& team, uint64_t* hist, Each each, Key ke
         each([&](int e) { k = key(e) < hi ? max(k, key(e)) : k; });
         k = team.all(k, [](K a, K b) { return max(a, b); });
     }
-    *above = over;
+    *above = over;  // (not reached)
     return lo;
 }
 
-// The middle of two keys of numbers: half way between the numbers (those around
-// 0 have most of the keys), or between the keys.
+// The key half way between the numbers of two keys (those around 0 have most of
+// the keys).
 __device__ __forceinline__ uint32_t middle_key(uint32_t lo, uint32_t hi) {
-    const uint32_t mid = key_of(0.5f * of_key(lo) + 0.5f * of_key(hi));
-    return mid > lo && mid < hi ? mid : lo + (hi - lo) / 2;
+    return key_of(0.5f * of_key(lo) + 0.5f * of_key(hi));
 }
 
 // ---- long rows of f32 and f16, by parts ------------------------------------

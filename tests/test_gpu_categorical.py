@@ -200,6 +200,36 @@ def test_sample_frequencies(C):
     assert ((count[top.indices] - p * n).abs() <= 1.0).all()
 
 
+def small_numbers(kind, n, v, seed):
+    """Rows whose numbers next to 0 spread over many binades."""
+    g = gen(seed)
+    if kind == "logsigmoid":    # half of them within 1e-6 of 0
+        return torch.nn.functional.logsigmoid(30 * torch.randn(n, v, generator=g, device="cuda"))
+    if kind == "powers":        # a binade each, and zeros behind them
+        x = torch.zeros(n, v, device="cuda")
+        many = min(v, 150)
+        x[:, :many] = 2.0 ** (27 - torch.arange(many, device="cuda", dtype=torch.float64)).float()
+        return torch.gather(x, 1, torch.rand(n, v, generator=g, device="cuda").argsort(1))
+    x = 10.0 ** -(3 + 35 * torch.rand(n, v, generator=g, device="cuda", dtype=torch.float64))
+    if kind == "both":
+        x *= torch.where(torch.rand(n, v, generator=g, device="cuda") < 0.5, -1.0, 1.0)
+    else:
+        x = -x
+    return x.float()
+
+
+@pytest.mark.parametrize("kind", ["logsigmoid", "below", "both", "powers"])
+@pytest.mark.parametrize("v", [40, 300, 2000, 9000, 20000])
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_sample_cut_among_small_numbers(C, kind, v, dtype):
+    """The cut between numbers that one bin holds and that are tens of binades apart."""
+    x = small_numbers(kind, 4, v, v).to(dtype)
+    t = 1e10 if kind == "powers" else 1.0
+    for i, par in enumerate(({"top_k": 7}, {"top_k": 100}, {"top_k": 129}, {"top_k": 140}, {"top_k": 400}, {"top_k": 1500},
+                             {"top_p": 0.613}, {"top_p": 0.03}, {"top_k": 300, "top_p": 0.37})):
+        check_sample(C, x, torch.rand(4, generator=gen(i), device="cuda"), par | {"temperature": t})
+
+
 # ---- losses ---------------------------------------------------------------
 def ppo_inputs(n, v, seed, logits):
     g = gen(seed)
