@@ -1077,9 +1077,9 @@ __global__ __launch_bounds__(512) void k_cat_sample_answer(Batch b) {
 // from the counts, ties included; what is left is to find an index in one part
 // of the row, with the weights by number in LDS.
 //
-// A place for each number with 2^-36 < |x| < 2^12, largest first, 0 in the
-// middle.  -inf is not counted.  Rows with other numbers that weigh something
-// go the slow way.
+// A place for each number with 2^-36 < |x| < 2^12 and for -2^-36, largest
+// first, 0 in the middle.  -inf is not counted.  Rows with other numbers that
+// weigh something go the slow way.
 //
 // 256 x 131072, filters of all kinds: 22 us for the counts (67 MB: 3 TB/s),
 // 23 us for the rest by one block a row, 8 of them in the search of a part, the
@@ -1456,7 +1456,9 @@ __global__ __launch_bounds__(1024) void k_cat_sample_pick(Counts b) {
     }
     const uint64_t tie_weight = rest ? room.weight[cut] : 0;
     float least = number_at(cut - (rest ? 0 : 1));  // that counts
-    if (flags & kBetween) least = fmaxf(least, 0x1p-36f);  // they weigh nothing, and have no place
+    // Numbers up to 2^-36 that weigh nothing have no place (nor has 2^-36, whose place is 0's and may not be
+    // set): from the next one on
+    if (flags & kBetween) least = fmaxf(least, 0x1.02p-36f);
     const auto add = [&](float x, uint64_t& s, uint32_t& t) {
         if (!(x >= least)) return;
         const uint32_t q = __float_as_uint(x + 0.0f);  // -0 as +0

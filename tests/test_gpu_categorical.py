@@ -230,6 +230,21 @@ def test_sample_cut_among_small_numbers(C, kind, v, dtype):
         check_sample(C, x, torch.rand(4, generator=gen(i), device="cuda"), par | {"temperature": t})
 
 
+@pytest.mark.parametrize("v", [9300, 70001])
+def test_sample_bf16_at_the_border_of_the_places(C, v):
+    """2^-36, which has no place of its own and weighs nothing, and is the only number near 0, in rows after others of
+    zeros."""
+    n = 600 if v < 10000 else 520
+    x = torch.zeros(n, v, dtype=torch.bfloat16, device="cuda")
+    x[512:] = 2.0 ** -36
+    x[512:, v // 2] = 100.0
+    x[512:, v - 3] = 99.5
+    x[515, 7:] = 100.0
+    u = torch.rand(n, generator=gen(n), device="cuda")
+    for par in ({}, {"temperature": 0.0}, {"temperature": 2.0, "min_p": 1e-30}, {"top_k": v - 1}):
+        check_sample(C, x, u, par)
+
+
 # ---- losses ---------------------------------------------------------------
 def ppo_inputs(n, v, seed, logits):
     g = gen(seed)
