@@ -375,7 +375,7 @@ __device__ double teacher_load(const Distill& op, int64_t n, int32_t V, const ty
     }
     double Q = 0.0;
     for (int j = lane; j < op.b.k; j += 64) {
-        const double lq = te.idx[j] < 0 ? -INFINITY : te.lq[j] * inv - *lse, q = exp2_64(lq * 1.4426950408889634);
+        const double lq = te.idx[j] < 0 ? -INFINITY : te.lq[j] * inv - *lse, q = exp_64(lq);
         te.lq[j] = lq;
         te.q[j] = q;
         Q += q;

@@ -36,11 +36,13 @@ struct F16 {
 };
 
 // ---- 2^t in 64 bits --------------------------------------------------------
-// t <= 0 or NaN.  t = n + f, |f| <= 1/2; the Taylor sum of exp(f ln 2) up to
-// f^11 leaves (ln 2 / 2)^12 / 12! < 7e-15.
+// t <= 1100 (where 2^t is infinite) or NaN.  t = n + f, |f| <= 1/2, n from the
+// sum with 1.5 2^52, whose low word holds it (a NaN's is any number); the Taylor
+// sum of exp(f ln 2) up to f^11 leaves (ln 2 / 2)^12 / 12! < 7e-15.
 __device__ __forceinline__ double exp2_64(double t) {
+    const double kWhole = 6755399441055744.0;  // 1.5 2^52
     t = t < -1100.0 ? -1100.0 : t;
-    const double n = rint(t), f = t - n;
+    const double sum = t + kWhole, f = t - (sum - kWhole);
     double p = 4.44553827187081e-10;  // (ln 2)^11 / 11!, and so on down
     p = fma(p, f, 7.054911620801121e-09);
     p = fma(p, f, 1.0178086009239696e-07);
@@ -53,10 +55,14 @@ __device__ __forceinline__ double exp2_64(double t) {
     p = fma(p, f, 0.2402265069591007);
     p = fma(p, f, 0.6931471805599453);
     p = fma(p, f, 1.0);
-    return ldexp(p, (int)n);
+    return ldexp(p, (int)(uint32_t)__builtin_bit_cast(uint64_t, sum));
 }
 
-__device__ __forceinline__ double exp_64(double x) { return exp2_64(x * 1.4426950408889634); }
+// e^x of any x: infinite past the doubles, and for +inf
+__device__ __forceinline__ double exp_64(double x) {
+    const double t = x * 1.4426950408889634;
+    return exp2_64(t > 1100.0 ? 1100.0 : t);
+}
 
 // log s, s >= 1 or NaN: the hardware's log2 (within 2^-22), corrected by what
 // it leaves, d < 2^-20: log(1 + d) up to d^3 is exact to 2^-80.

@@ -641,6 +641,35 @@ def test_autograd_is_refused_in_a_capture(C):
     assert torch.equal(grad, wgrad) and torch.equal(r.loss, want.loss)
 
 
+@pytest.mark.parametrize("v", [11, 300, 2000, 60000])
+def test_ppo_impossible_before(C, v):
+    """An action that the old policy ruled out, or nearly: the ratio is infinite, the clipped side finite."""
+    x = rows(4, v, torch.float32, 81)
+    a, old, adv, w, _ = ppo_inputs(4, v, 81, x)
+    adv = adv.abs() + 0.5
+    old[1], old[2] = -INF, -1e30
+    want = P.ppo(x, a, old, adv, w, low=0.2, high=0.3)
+    rest = P.ppo(x[::3], a[::3], old[::3], adv[::3], w[::3], low=0.2, high=0.3)
+    clipped = -(w[1:3] * adv[1:3]).double().sum() * 1.3
+    for r, g in (C.ppo_loss_grad(x, a, old, adv, weights=w, clip_coef=0.2, clip_coef_high=0.3), (None, None)):
+        if r is None:
+            leaf = x.detach().requires_grad_()
+            r = C.ppo_loss(leaf, a, old, adv, weights=w, clip_coef=0.2, clip_coef_high=0.3)
+            g, = torch.autograd.grad(r.loss, leaf)
+        near(r._asdict(), want, ("logprob", "entropy"))
+        assert r.stats[3] == -INF and r.stats[4].isnan()  # sums of -inf, and of inf - inf, by their definition
+        assert abs(float(r.loss.detach() - rest["loss"][0] - clipped)) <= float(rest["loss"][1]) + 2.0 ** -22 * float(clipped.abs())
+        assert not g[1:3].any()
+        near({"grad": g[::3]}, rest, ("grad",))
+    r, g = C.ppo_loss_grad(x, a, old, -adv, weights=w)  # the other side is not clipped
+    assert r.loss == INF and not g[::3].isnan().any()
+    r = C.ppo_loss(x, a, old.clamp(max=0).abs() * INF, adv.nan_to_num(), weights=w)  # certain before: the ratio is 0
+    assert r.loss == 0.0
+    idx = torch.tensor([[0], [1]], device="cuda")  # a teacher's normaliser of nothing
+    r = C.distill_loss(x[:2], idx, torch.zeros(2, 1, device="cuda"), teacher_lse=torch.tensor([0.0, -INF], device="cuda"))
+    assert r.kl[0].isfinite() and r.kl[1] == INF
+
+
 @pytest.mark.parametrize("v,n,n_loss", [(33, 2 ** 26 + 5, 2 ** 28 + 3), (577, 2 ** 24 + 3, 2 ** 26 + 5), (1025, 2 ** 24 + 3, 2 ** 26 + 5)])
 def test_more_rows_than_one_launch_dimension_has(C, v, n, n_loss):
     """2^32 threads and more; one row of logits for all (stride 0), so that every row's result is known."""
