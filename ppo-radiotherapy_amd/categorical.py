@@ -4,11 +4,11 @@ The Gaussian agent's rollout and update steps (rt_policy_sample, rt_ppo_grad;
 train.py:143-149, 197-246) for a policy that picks one entry of a row of
 logits: a discretised beam action ([..., bins]) or a token ([..., vocab]).
 
-    a = sample(logits, u, temperature=0.8, top_k=50, top_p=0.9)    # rollout
-    out = ppo_loss(logits, a.action, a.logprob, adv)               # update, autograd
+    a = sample(logits, u, temperature=0.8, top_k=50, top_p=0.9)                   # rollout
+    out = ppo_loss(logits, a.action, a.logprob, adv, temperature=0.8)             # update, autograd
     out.loss.backward()
-    out, grad = ppo_loss_grad(logits, a.action, a.logprob, adv)    # the same in one pass over the logits
-    out = distill_loss(logits, idx, top_logits, temperature=2.0)   # from a teacher's top logits
+    out, grad = ppo_loss_grad(logits, a.action, a.logprob, adv, temperature=0.8)  # the same in one pass over the logits
+    out = distill_loss(logits, idx, top_logits, temperature=2.0)                  # from a teacher's top logits
 
 Logits are float32, bfloat16 or float16 on the GPU, entries of a row adjacent
 (stride 1), leading dimensions any that collapse to evenly spaced rows; -inf
@@ -313,9 +313,10 @@ def ppo_loss(logits, actions, old_logprobs, advantages, *, weights=None, ref_log
     sum over rows of the surrogate, - ent_coef * entropy, + kl_coef * the KL
     estimate against ref_logprobs.
 
-    weights: one per row, None: 1 / rows each.  A row with weight 0 or an
-    action outside the vocabulary is ignored.  Only `loss` is differentiable,
-    and only with respect to the logits."""
+    temperature: the one that old_logprobs (and ref_logprobs) were taken at, as
+    sample's logprob.  weights: one per row, None: 1 / rows each.  A row with
+    weight 0 or an action outside the vocabulary is ignored.  Only `loss` is
+    differentiable, and only with respect to the logits."""
     op = _Ppo(logits, actions, old_logprobs, advantages, weights, ref_logprobs, temperature, clip_coef,
               clip_coef_high, ent_coef, kl_coef)
     if torch.is_grad_enabled() and logits.requires_grad:

@@ -731,6 +731,29 @@ def test_refusals(C):
         C.ppo_loss_grad(wide[:, :10], i, v, v, out=wide[:, 5:15])
 
 
+def test_documented_use(C):
+    """README's and the module's own lines: of an unmoved policy the ratio is 1 throughout."""
+    import os
+    import re
+
+    with open(os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "README.md")) as f:
+        readme = re.search(r"```python\nfrom ppo_radiotherapy_amd import categorical\n(.*?)```", f.read(), re.S).group(1)
+    module = "\n".join(re.findall(r"^    (\S.*)$", C.__doc__, re.M))
+    for text in (readme, module):
+        logits = rows(64, 50, torch.float32, 91).requires_grad_()
+        lines = {"categorical": C, "logits": logits, "u": torch.rand(64, generator=gen(92), device="cuda"), "adv": torch.ones(64, device="cuda")}
+        lines |= {k: getattr(C, k) for k in ("sample", "ppo_loss", "ppo_loss_grad", "distill_loss")}
+        lines["top_logits"], lines["idx"] = lines["teacher_logits"], lines["teacher_idx"] = rows(64, 50, torch.float32, 93).topk(5)
+        seen = []
+        for line in text.splitlines():
+            exec(line, lines)
+            if "ppo_loss" in line:
+                seen.append(lines["out"].stats)
+        assert len(seen) >= 2
+        for s in seen:
+            assert s[5] == 0 and abs(float(s[3])) <= 2.0 ** -19 and abs(float(s[4])) <= 2.0 ** -30
+
+
 def test_policy_iteration_together(C):
     """The operators as one iteration uses them: sample a rollout, GAE, a PPO update of a linear policy through
     autograd, then its distillation into another; each step against the definitions in 64 bits."""
