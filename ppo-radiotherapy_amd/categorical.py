@@ -27,6 +27,7 @@ import math
 from typing import NamedTuple
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 
@@ -274,6 +275,12 @@ def _once(backward):
     return staticmethod(run)
 
 
+def _differentiated(logits) -> bool:
+    if forward_ad.unpack_dual(logits).tangent is not None:
+        raise RuntimeError("ppo_loss and distill_loss have no forward mode: the logits' tangent would be lost")
+    return torch.is_grad_enabled() and logits.requires_grad
+
+
 def _with_grad(fn, logits, op):
     # A captured backward pass ends the process where an eager graph of the same leaves is alive (their
     # nodes keep its stream): nothing here can tell.
@@ -319,7 +326,7 @@ def ppo_loss(logits, actions, old_logprobs, advantages, *, weights=None, ref_log
     differentiable, and only with respect to the logits."""
     op = _Ppo(logits, actions, old_logprobs, advantages, weights, ref_logprobs, temperature, clip_coef,
               clip_coef_high, ent_coef, kl_coef)
-    if torch.is_grad_enabled() and logits.requires_grad:
+    if _differentiated(logits):
         return _with_grad(_PpoFn, logits, op)
     return op.run()[0]
 
@@ -401,7 +408,7 @@ def distill_loss(logits, teacher_idx, teacher_logits, *, weights=None, teacher_l
     vocabulary; without it its probabilities are normalised over the k.
     weights: as ppo_loss.  Only `loss` is differentiable, by the logits."""
     op = _Distill(logits, teacher_idx, teacher_logits, weights, teacher_lse, temperature)
-    if torch.is_grad_enabled() and logits.requires_grad:
+    if _differentiated(logits):
         return _with_grad(_DistillFn, logits, op)
     return op.run()[0]
 

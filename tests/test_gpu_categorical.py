@@ -754,6 +754,23 @@ def test_documented_use(C):
             assert s[5] == 0 and abs(float(s[3])) <= 2.0 ** -19 and abs(float(s[4])) <= 2.0 ** -30
 
 
+def test_forward_mode_is_refused(C):
+    """A tangent of the logits would be lost: nothing carries it on."""
+    from torch.autograd import forward_ad
+
+    x = torch.randn(3, 20, device="cuda")
+    a, old, adv, _, _ = ppo_inputs(3, 20, 65, x)
+    idx, top, _ = teacher_inputs(3, 20, 4, 65)
+    want = C.ppo_loss(x, a, old, adv).loss
+    with forward_ad.dual_level():
+        dual = forward_ad.make_dual(x, torch.ones_like(x))
+        for call in (lambda y: C.ppo_loss(y, a, old, adv), lambda y: C.distill_loss(y, idx, top)):
+            for y in (dual, dual.bfloat16()):
+                with pytest.raises(RuntimeError, match="forward"):
+                    call(y)
+        assert torch.equal(C.ppo_loss(x, a, old, adv).loss, want)  # no tangent, nothing lost
+
+
 def test_policy_iteration_together(C):
     """The operators as one iteration uses them: sample a rollout, GAE, a PPO update of a linear policy through
     autograd, then its distillation into another; each step against the definitions in 64 bits."""
