@@ -264,8 +264,21 @@ class _Final(torch.autograd.Function):
         raise RuntimeError("ppo_loss and distill_loss are differentiated once only")
 
 
+def _no_capture(device):
+    # A captured backward pass ends the process where an eager graph of the same leaves is alive (their
+    # nodes keep its stream): nothing here can tell.
+    if torch.cuda.current_device() == device.index:
+        capturing = torch.cuda.is_current_stream_capturing()
+    else:
+        with torch.cuda.device(device):
+            capturing = torch.cuda.is_current_stream_capturing()
+    if capturing:
+        raise RuntimeError("logits require grad while a graph is captured: take the _grad form")
+
+
 def _once(backward):
     def run(ctx, gloss):
+        _no_capture(gloss.device)
         if not torch.is_grad_enabled():  # no graph of the gradient is asked for
             return backward(ctx, gloss), None
         with torch.no_grad():
@@ -282,10 +295,7 @@ def _differentiated(logits) -> bool:
 
 
 def _with_grad(fn, logits, op):
-    # A captured backward pass ends the process where an eager graph of the same leaves is alive (their
-    # nodes keep its stream): nothing here can tell.
-    if torch.cuda.is_current_stream_capturing():
-        raise RuntimeError("logits require grad while a graph is captured: take the _grad form")
+    _no_capture(logits.device)
     loss = fn.apply(logits, op)
     return op.rest._replace(loss=loss)
 

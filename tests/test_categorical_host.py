@@ -5,6 +5,7 @@ import ctypes
 import math
 import os
 import subprocess
+import types
 
 import numpy as np
 import pytest
@@ -126,6 +127,45 @@ def test_python_refuses_host_tensors():
         categorical.ppo_loss([1.0], v, v, v)
     with pytest.raises(ValueError, match="no entries"):
         categorical.distill_loss(torch.zeros(2, 0), v, v)
+
+
+def test_captures_are_looked_for_on_the_logits_device(monkeypatch):
+    """The stream that counts is that of the logits' device, in the forward and in the backward pass."""
+    class On:  # of torch.cuda.device
+        now = 0
+
+        def __init__(self, device):
+            self.index = device.index
+
+        def __enter__(self):
+            self.before, On.now = On.now, self.index
+
+        def __exit__(self, *_):
+            On.now = self.before
+
+    monkeypatch.setattr(torch.cuda, "device", On)
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: On.now)
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: On.now == 1)
+
+    class Fn:
+        @staticmethod
+        def apply(logits, op):
+            raise LookupError
+
+    class Op:
+        rest = None
+
+    away, here = (types.SimpleNamespace(device=torch.device("cuda", k)) for k in (1, 0))
+    with pytest.raises(RuntimeError, match="captured"):
+        categorical._with_grad(Fn, away, Op)
+    with pytest.raises(LookupError):
+        categorical._with_grad(Fn, here, Op)
+    backward = categorical._once(lambda ctx, gloss: "gradient").__func__
+    with pytest.raises(RuntimeError, match="captured"):
+        backward(None, away)
+    with torch.no_grad():
+        assert backward(None, here) == ("gradient", None)
+    assert On.now == 0
 
 
 def test_oracle_sampling_by_hand():
