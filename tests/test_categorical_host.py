@@ -108,6 +108,53 @@ def test_every_refusal_says_why():
         assert L.rt_cat_ppo(l, b, hp, O, *WS, None) == -1 and word in L.rt_last_error()
 
 
+def test_every_refusal_names_its_argument():
+    """What each refusal says, read right behind its call."""
+    L = _lib.load()
+    l = _logits()
+    B, H, O = _lib.RtCatPpoBatch, _lib.RtCatPpoHparams, _lib.RtCatPpoOut
+    T, D, S = _lib.RtCatTeacher, _lib.RtCatDistillOut, _lib.RtCatSampling
+    batch, hp, out, s = B(4096, 4096, 4096), H(1.0, 0.2, 0.2), O(4096, 4096, 4096, 4096), S(u=4096)
+    te, dout = T(4096, 4096, None, None, 2, 1.0), D(4096, 4096)
+    far = 1 << 22  # a gradient that is nowhere near the logits
+    ppo = lambda b=batch, h=hp, o=out, ws=WS: L.rt_cat_ppo(l, b, h, o, *ws, None)  # noqa: E731
+    dis = lambda t=te, o=dout, ws=WS: L.rt_cat_distill(l, t, o, *ws, None)  # noqa: E731
+    long = _logits(stride=9217, vocab=9217)
+    calls = [
+        (lambda: ppo(b=None), "NULL batch"), (lambda: ppo(b=B(None, 4096, 4096)), "NULL batch"),
+        (lambda: ppo(b=B(4096, None, 4096)), "NULL batch"), (lambda: ppo(b=B(4096, 4096, None)), "NULL batch"),
+        (lambda: ppo(h=None), "temperature"), (lambda: ppo(h=H(math.nan, 0.2, 0.2)), "temperature"),
+        (lambda: ppo(h=H(math.inf, 0.2, 0.2)), "temperature"), (lambda: ppo(h=H(1.0, 0.2, math.nan)), "clip"),
+        (lambda: ppo(h=H(1.0, 0.2, 0.2, math.inf)), "not finite"), (lambda: ppo(h=H(1.0, 0.2, 0.2, 0.0, math.nan)), "not finite"),
+        (lambda: ppo(h=H(1.0, 0.2, 0.2, 0.0, 0.1)), "ref_logprobs"),
+        *((lambda k=k: ppo(o=O(*(None if i == k else 4096 for i in range(4)))), "NULL output") for k in range(4)),
+        (lambda: ppo(o=O(4096, 4096, 4096, 4096, far, 9)), "rows overlap"), (lambda: ppo(o=O(4096, 4096, 4096, 4096, far, 2 ** 58)), "stride"),
+        (lambda: ppo(o=O(4096, 4096, 4096, 4096, far + 2, 10)), "aligned"), (lambda: ppo(o=O(4096, 4096, 4096, 4096, 4096, 11)), "in-place"),
+        (lambda: ppo(o=O(4096, 4096, 4096, 4096, 4096 + 40, 10)), "overlaps"), (lambda: ppo(ws=(None, 0)), "workspace NULL"),
+        (lambda: ppo(ws=(1 << 20, 8)), "too small"), (lambda: ppo(ws=((1 << 20) + 8, 1 << 16)), "aligned"),
+        (lambda: L.rt_cat_ppo_backward(l, None, 1.0, 4096, None, far, 10, None), "NULL argument"),
+        (lambda: L.rt_cat_ppo_backward(l, 4096, 1.0, None, None, far, 10, None), "NULL argument"),
+        (lambda: L.rt_cat_ppo_backward(l, 4096, 1.0, 4096, None, None, 10, None), "NULL argument"),
+        (lambda: L.rt_cat_ppo_backward(l, 4096, -1.0, 4096, None, far, 10, None), "temperature"),
+        (lambda: L.rt_cat_ppo_backward(l, 4096, 1.0, 4096, None, far, 9, None), "rows overlap"),
+        (lambda: L.rt_cat_sample(l, None, 4096, 4096, 4096, *WS, None), "NULL parameters"),
+        (lambda: L.rt_cat_sample(l, S(), 4096, 4096, 4096, *WS, None), "NULL parameters"),
+        *((lambda k=k: L.rt_cat_sample(l, s, *(None if i == k else 4096 for i in range(3)), *WS, None), "NULL output") for k in range(3)),
+        *((lambda w=w: L.rt_cat_sample(long, s, 4096, 4096, 4096, *w, None), "workspace") for w in ((None, 1 << 30), (1 << 20, 8), ((1 << 20) + 8, 1 << 30))),
+        (lambda: dis(t=None), "teacher"), (lambda: dis(t=T(4096, None, None, None, 2, 1.0)), "teacher"),
+        (lambda: dis(t=T(4096, 4096, None, None, 0, 1.0)), "entries"), (lambda: dis(t=T(4096, 4096, None, None, _lib.CAT_MAX_TOP + 1, 1.0)), "entries"),
+        (lambda: dis(t=T(4096, 4096, None, None, 2, 0.0)), "temperature"), (lambda: dis(o=D(4096, None)), "NULL output"),
+        (lambda: dis(o=D(None, 4096)), "NULL output"), (lambda: dis(o=D(4096, 4096, far, 9)), "rows overlap"), (lambda: dis(ws=(None, 0)), "workspace"),
+        (lambda: L.rt_cat_distill_backward(l, te, None, None, far, 10, None), "NULL argument"),
+        (lambda: L.rt_cat_distill_backward(l, te, 4096, None, None, 10, None), "NULL argument"),
+        (lambda: L.rt_cat_distill_backward(l, T(), 4096, None, far, 10, None), "teacher"),
+        (lambda: L.rt_cat_distill_backward(l, te, 4096, None, 4096 + 40, 10, None), "overlaps"),
+    ]
+    for k, (call, word) in enumerate(calls):
+        assert call() == -1, k
+        assert word in L.rt_last_error().decode(), (k, word)
+
+
 def test_workspace_sizes():
     L = _lib.load()
     for f in (L.rt_cat_sample_workspace_bytes, L.rt_cat_loss_workspace_bytes):
