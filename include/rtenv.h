@@ -595,7 +595,8 @@ typedef struct rt_cat_ppo_out {
     float* entropy;                /* [rows] of softmax(x / T), ignored rows 0 */
     float* stats;                  /* [6] weighted sums: pg_loss, kl, entropy, old_approx_kl, approx_kl, clipfrac */
     void* grad;                    /* d loss / d logits in the logits' type, or NULL (loss alone).
-                                      May be the logits themselves (same address and stride) */
+                                      May be the logits themselves (same address and stride), or lie
+                                      between their rows (same stride, no element of both) */
     int64_t grad_stride;           /* elements, >= vocab */
     double* row_state;             /* [rows][RT_CAT_ROW_STATE] for rt_cat_ppo_backward, or NULL */
 } rt_cat_ppo_out;

@@ -345,7 +345,8 @@ def ppo_loss_grad(logits, actions, old_logprobs, advantages, *, weights=None, re
                   clip_coef=0.2, clip_coef_high=None, ent_coef=0.0, kl_coef=0.0, out=None):
     """(ppo_loss, its gradient by the logits) in one call, outside autograd.
 
-    out: where the gradient goes; the logits themselves may be given."""
+    out: where the gradient goes: memory apart from the logits, other columns of
+    their buffer, or the logits themselves."""
     op = _Ppo(logits, actions, old_logprobs, advantages, weights, ref_logprobs, temperature, clip_coef,
               clip_coef_high, ent_coef, kl_coef)
     grad, stride = op.r.grad_buffer(out)

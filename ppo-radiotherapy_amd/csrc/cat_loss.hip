@@ -1106,7 +1106,10 @@ const char* grad_fault(const rt_cat_logits* l, const void* grad, int64_t stride)
     if (grad == l->x) return stride == l->row_stride || l->rows == 1 ? nullptr : "in-place gradient with another stride";
     const uintptr_t x0 = (uintptr_t)l->x, x1 = x0 + ((l->rows - 1) * l->row_stride + l->vocab) * es;
     const uintptr_t g0 = (uintptr_t)grad, g1 = g0 + ((l->rows - 1) * stride + l->vocab) * es;
-    return g0 < x1 && x0 < g1 ? "gradient overlaps the logits" : nullptr;
+    if (g0 >= x1 || x0 >= g1) return nullptr;
+    // rows of one buffer, the gradient's between the logits': how far behind a row of the logits one starts
+    const int64_t step = stride * es, row = l->vocab * es, apart = (int64_t)(g0 - x0) % step, behind = apart < 0 ? apart + step : apart;
+    return stride == l->row_stride && behind >= row && behind + row <= step ? nullptr : "gradient overlaps the logits";
 }
 
 bool finite_pos(float v) { return v > 0.0f && std::isfinite(v); }

@@ -670,6 +670,36 @@ def test_ppo_impossible_before(C, v):
     assert r.kl[0].isfinite() and r.kl[1] == INF
 
 
+@pytest.mark.parametrize("v", [11, 300, 5000, 60000])
+def test_gradient_between_the_rows(C, v):
+    """Logits and gradient as columns of one buffer, that share no element."""
+    a, old, adv, w, _ = ppo_inputs(5, v, 95, torch.zeros(5, v, device="cuda"))
+    idx, top, _ = teacher_inputs(5, v, 4, 95)
+    for dtype in DTYPES:
+        for gap, first in ((0, False), (3, True)):
+            wide = torch.full((5, 2 * v + 2 * gap), 5.0, dtype=dtype, device="cuda")
+            left, right = wide[:, :v], wide[:, v + gap:2 * v + gap]
+            x, out = (right, left) if first else (left, right)
+            x.copy_(rows(5, v, dtype, 96))
+            y = x.clone()
+            r, g = C.ppo_loss_grad(x, a, old, adv, weights=w, out=out)
+            assert g is out and torch.equal(x, y) and (wide[:, v:v + gap] == 5).all() and (wide[:, 2 * v + gap:] == 5).all()
+            near(r._asdict() | {"grad": out}, P.ppo(y, a, old, adv, w), ("loss", "logprob", "entropy", "stats", "grad"))
+            r, g = C.distill_loss_grad(x, idx, top, weights=w, out=out)
+            assert torch.equal(x, y)
+            near(r._asdict() | {"grad": out}, P.distill(y, idx, top, w), ("loss", "kl", "grad"))
+    from ppo_radiotherapy_amd._lib import RtError
+
+    wide = torch.randn(5, 2 * v, device="cuda")
+    for at in (1, v - 1):
+        with pytest.raises(RtError, match="overlaps"):
+            C.ppo_loss_grad(wide[:, :v], a, old, adv, out=wide[:, at:at + v])
+    flat = torch.randn(10 * v, device="cuda")
+    for x, out in ((flat.as_strided((5, v), (2 * v, 1)), flat[5 * v:].view(5, v)), (flat[:5 * v].view(5, v), flat[4 * v:9 * v].view(5, v))):
+        with pytest.raises(RtError, match="overlaps"):
+            C.ppo_loss_grad(x, a, old, adv, out=out)
+
+
 @pytest.mark.parametrize("v,n,n_loss", [(33, 2 ** 26 + 5, 2 ** 28 + 3), (577, 2 ** 24 + 3, 2 ** 26 + 5), (1025, 2 ** 24 + 3, 2 ** 26 + 5)])
 def test_more_rows_than_one_launch_dimension_has(C, v, n, n_loss):
     """2^32 threads and more; one row of logits for all (stride 0), so that every row's result is known."""
