@@ -16,8 +16,9 @@ marks an entry that cannot be taken.  Everything is enqueued on the current
 stream of the logits' device, nothing synchronises, and all but the autograd
 forms can be captured in a graph (there take the `_grad` forms, and
 `logits.backward(grad)` for what lies before).  The definitions stand in
-include/rtenv.h; wrong arguments raise ValueError or TypeError before anything
-is launched.
+include/rtenv.h; wrong arguments raise ValueError or TypeError, those that the
+library itself refuses (a gradient that overlaps the logits) RtError, before
+anything is launched.
 """
 from __future__ import annotations
 
@@ -162,10 +163,12 @@ def _workspace(name: str, r: _Rows):
 
 
 def _coef(v, name: str, low=None, positive=False) -> float:
-    v = float(v)
-    if not math.isfinite(v) or (low is not None and v < low) or (positive and v <= 0):
-        raise ValueError(f"{name}: {v}")
-    return v
+    """v as the kernels get it, in 32 bits."""
+    x = float(v)
+    f = ctypes.c_float(x).value
+    if not math.isfinite(f) or (low is not None and x < low) or (positive and f <= 0):
+        raise ValueError(f"{name}: {x}")
+    return f
 
 
 _SAMPLING_OFF = {"temperature": 1.0, "top_k": 0, "top_p": 1.0, "min_p": 0.0}

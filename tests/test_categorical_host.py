@@ -215,6 +215,22 @@ def test_captures_are_looked_for_on_the_logits_device(monkeypatch):
     assert On.now == 0
 
 
+def test_scalars_are_checked_as_the_kernels_get_them():
+    """In 32 bits: what rounds to 0 or to infinity there is refused with the arguments."""
+    ppo = categorical._ppo_hparams
+    for args in ((1e-60, 0.2, 0.2, 0.0, 0.0), (1e39, 0.2, 0.2, 0.0, 0.0), (1.0, 1e39, 0.2, 0.0, 0.0), (1.0, 0.2, 1e300, 0.0, 0.0),
+                 (1.0, 0.2, 0.2, -1e39, 0.0), (1.0, 0.2, 0.2, 0.0, 1e39)):
+        with pytest.raises(ValueError):
+            ppo(*args)
+    for args in ((1e39, 0, 1.0, 0.0), (1.0, 0, 1e39, 0.0), (1.0, 0, 1.0, 1e39), (-1e-60, 0, 1.0, 0.0)):
+        with pytest.raises(ValueError):
+            categorical._sampling(*args)
+    with pytest.raises(ValueError, match="temperature"):
+        categorical._coef(1e-60, "temperature", positive=True)
+    assert categorical._sampling(1e-60, 3, 0.1, 0.0) == (0.0, 3, ctypes.c_float(0.1).value, 0.0)
+    assert ppo(1e-45, 0.2, 0.2, 0.0, 0.0).temperature > 0
+
+
 def test_oracle_sampling_by_hand():
     x = np.log(np.array([0.1, 0.4, 0.2, 0.3]))
     row = lambda u, **kw: P.sample_row(x, u, **kw)[0]  # noqa: E731
