@@ -641,6 +641,7 @@ typedef struct rt_cat_distill_out {
  * [idx_j = v]).  Ignored rows and rows without a finite logit as rt_cat_ppo. */
 int rt_cat_distill(const rt_cat_logits* logits, const rt_cat_teacher* teacher, const rt_cat_distill_out* out,
                    void* workspace_d, int64_t workspace_bytes, void* stream);
+/* From the row_state, as rt_cat_ppo_backward; of the teacher it reads idx, logits, k and temperature. */
 int rt_cat_distill_backward(const rt_cat_logits* logits, const rt_cat_teacher* teacher, const double* row_state_d,
                             const float* grad_loss_d, void* grad_d, int64_t grad_stride, void* stream);
 

@@ -395,19 +395,19 @@ class _DistillFn(torch.autograd.Function):
     def forward(ctx, logits, op):
         op.rest, state = op.run(keep=True)
         ctx.k, ctx.temperature = op.k, op.temperature
-        ctx.save_for_backward(logits, op.idx, op.top, op.lse, op.weights, state)
+        ctx.save_for_backward(logits, op.idx, op.top, state)  # (weights and lse are in the state)
         return op.rest.loss
 
     @_once
     def backward(ctx, gloss):
-        logits, idx, top, lse, weights, state = ctx.saved_tensors  # raises where one of them was changed in place
+        logits, idx, top, state = ctx.saved_tensors  # raises where one of them was changed in place
         r = _Rows(logits)
         grad, stride = r.grad_buffer(None)
         if r.n == 0:
             return grad
         if gloss.dtype != torch.float32:
             gloss = gloss.float()
-        teacher = _lib.RtCatTeacher(idx.data_ptr(), top.data_ptr(), _lib.ptr(lse), _lib.ptr(weights), ctx.k, ctx.temperature)
+        teacher = _lib.RtCatTeacher(idx.data_ptr(), top.data_ptr(), None, None, ctx.k, ctx.temperature)
         r.call(_lib.load().rt_cat_distill_backward, "rt_cat_distill_backward", ctypes.byref(r.arg()),
                ctypes.byref(teacher), state.data_ptr(), gloss.data_ptr(), grad.data_ptr(), stride)
         return grad

@@ -801,6 +801,29 @@ def test_forward_mode_is_refused(C):
         assert torch.equal(C.ppo_loss(x, a, old, adv).loss, want)  # no tangent, nothing lost
 
 
+def test_what_the_backward_pass_does_not_read_may_change(C):
+    """Weights and normalisers are in the row state: their buffers may be filled anew before the backward pass."""
+    for v in (20, 3000):
+        x = torch.randn(3, v, device="cuda", requires_grad=True)
+        a, old, adv, w, ref = ppo_inputs(3, v, 66, x.detach())
+        idx, top, _ = teacher_inputs(3, v, 4, 66)
+        lse = torch.logsumexp(top, 1) + 0.1
+        for loss, inputs in ((lambda: C.ppo_loss(x, a, old, adv, weights=w, ref_logprobs=ref, kl_coef=0.1).loss, (w, old, adv, ref)),
+                             (lambda: C.distill_loss(x, idx, top, weights=w, teacher_lse=lse).loss, (w, lse))):
+            want, = torch.autograd.grad(loss(), x)
+            later, kept = loss(), [t.clone() for t in inputs]
+            for t in inputs:
+                t.fill_(5.0)
+            got, = torch.autograd.grad(later, x)
+            assert torch.equal(got, want)
+            for t, k in zip(inputs, kept):
+                t.copy_(k)
+        later = C.distill_loss(x, idx, top, weights=w).loss
+        top.add_(1.0)  # what it does read is noticed
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            later.backward()
+
+
 def test_policy_iteration_together(C):
     """The operators as one iteration uses them: sample a rollout, GAE, a PPO update of a linear policy through
     autograd, then its distillation into another; each step against the definitions in 64 bits."""
