@@ -115,10 +115,12 @@ __device__ __forceinline__ uint4 pack(const float* v) {
 
 // ---- a row's sums ----------------------------------------------------------
 // In units of log 2: t = (x - m) c, c = log2(e) / T.  exp2 is the hardware's
-// (within one unit of the last place); up to eight terms are added in f32,
-// those sums in f64.  c is rounded to f32 (2^-25 of t) and so is t (2^-24):
-// together they move log S by less than 2^-23 of the row's entropy, less than
-// the f32 outputs resolve.
+// (within one unit of the last place, 0 below 2^-126); up to eight terms are
+// added in f32, those sums in f64.  c is rounded to f32 (2^-25 of t), and so are
+// x - m, of f32 logits, and t (2^-24 each): together they move log S by less than
+// 1.25 2^-23 of the row's entropy, and exp2 moves it by 2^-23 at most: about what
+// the f32 outputs resolve.  In f64 (20 operations an entry) each pass over 4096 x
+// 131072 would take 270 us of arithmetic, where memory takes 215.
 struct Sums {
     double s, u;  // sum 2^t and sum t 2^t
 };
@@ -262,7 +264,13 @@ __device__ __forceinline__ void row_sums(const Span<D>& row, int32_t from, int32
 }
 
 // ---- a row's gradient ------------------------------------------------------
-// scale p (E lp + F) = 2^t (a t + b), f32; rounded once to the logits' type.
+// scale p (E lp + F) = 2^t (a t + b); rounded once to the logits' type.  In f32
+// with the hardware's exp2, also for short rows whose sums are in f64: an entry is
+// off by |t| 2^-22 of its size and a few roundings; against 64 bits all outputs are
+// 4.4e-8 and 5.7e-8 off (196608 x 11, 32768 x 64), with f64 throughout 2.5e-8 and
+// 3.2e-8.
+// What a term C or -C q leaves at a named entry is rounded at the size of C.
+// Below 2^-126 of the scale a gradient is 0.
 struct Slope {
     float m, c, a, b;
 };
@@ -664,8 +672,9 @@ __global__ __launch_bounds__(256) void k_cat_grad(Logits l, Op op, Out o, const 
 // ---- short rows ------------------------------------------------------------
 // Up to 1024 entries: many rows, so more of them lie next to the border of the
 // clip, and the memory they need is small beside the arithmetic of a row: the
-// sums are in f64 throughout.  Bound by that arithmetic: 32768 x 64 f32 with 8
-// of a teacher's entries 15 us (17 MB: 4 us).
+// sums are in f64 throughout.  Bound by the issue of vector instructions: 32768 x
+// 64 f32 with 8 of a teacher's entries 15.5 us (17 MB: 4 us), 827 of them a wave
+// of four rows, 0.94 a cycle and CU.
 
 // The sums of a block's rows, in a fixed order.
 template <int TERMS>
@@ -789,7 +798,8 @@ __global__ __launch_bounds__(256) void k_cat_short(Logits l, Op op, Out o, doubl
     const double scale = gout ? (double)*gout : 1.0;
     float named[E] = {};
     if constexpr (!Op::ppo) {
-        // the teacher's entries in turn, each met by the lane that has its place
+        // the teacher's entries in turn, each met by the lane that has its place (q of one entry that is named
+        // again and again is added in f32: 1024 times, 24 2^-24 off)
         for (int j0 = 0; j0 < op.b.k; j0 += G) {
             int32_t idx = j0 ? -1 : first.i;
             float tl = first.t;
@@ -826,7 +836,8 @@ __global__ __launch_bounds__(256) void k_cat_short(Logits l, Op op, Out o, doubl
 // exp, divisions) is done once and not by every lane that has a part of it.
 // The block's rows pass through LDS (rows an odd number of words apart: no two
 // lanes on one bank), where the accesses to memory are those of one long row.
-// 196608 x 11 f32, PPO with gradient: 14 us for 23 MB.
+// 196608 x 11 f32, PPO with gradient: 14 us for 23 MB, 0.64 vector instructions a
+// cycle and CU: twelve waves on it, each a chain of f64 steps.
 constexpr int kTiny = 32;
 
 template <class D, class Op, bool GIVEN>
@@ -1043,11 +1054,12 @@ int run_loss(const Logits& l, const Op& op, const Out& o, double* ws, hipStream_
     else if (const int64_t many = parts_of(l.rows, l.vocab, Span<D>::kPer); many > 1 && o.grad != l.x)
         launch_parts<D>(l, op, o, ws, many, st);
     // Short rows leave most of a block idle between its barriers, long ones need many threads to be in
-    // flight; what is held beyond a row's length is computed for nothing.  Measured, PPO with gradient, us:
-    //   2048 x 65536 bf16:   64 threads x 4 pieces 178, 128 x 4 243, 256 x 8 477, 512 x 8 996
-    //   8192 x 16384 bf16:   64 x 8 133, 128 x 8 130, 256 x 8 163, 512 x 8 306
-    //   32000 x 8000 bf16:   64 x 8 285, 128 x 8 239, 256 x 8 218, 512 x 8 258
-    //   131072 x 2048 bf16:  64 x 8 338, 128 x 8 313, 256 x 8 284, 512 x 8 258, 1024 x 8 286
+    // flight; what is held beyond a row's length is computed for nothing.  Measured, PPO with gradient, us
+    // (rows x entries; threads x pieces):
+    //   65536 x 2048 bf16:   64 x 4 178, 128 x 4 243, 256 x 8 477, 512 x 8 996
+    //   16384 x 8192 bf16:   64 x 8 133, 128 x 8 130, 256 x 8 163, 512 x 8 306
+    //   8000 x 32000 bf16:   64 x 8 285, 128 x 8 239, 256 x 8 218, 512 x 8 258
+    //   2048 x 131072 bf16:  64 x 8 338, 128 x 8 313, 256 x 8 284, 512 x 8 258, 1024 x 8 286
     else if (pieces <= 64 * 4) launch_row<D, Op, 64, 4>(l, op, o, ws, st);
     else if (pieces <= 64 * 8) launch_row<D, Op, 64, 8>(l, op, o, ws, st);
     else if (!o.grad) launch_row<D, Op, 256, 0>(l, op, o, ws, st);

@@ -64,8 +64,10 @@ __device__ __forceinline__ double exp_64(double x) {
     return exp2_64(t > 1100.0 ? 1100.0 : t);
 }
 
-// log s, s >= 1 or NaN: the hardware's log2 (within 2^-22), corrected by what
-// it leaves, d < 2^-20: log(1 + d) up to d^3 is exact to 2^-80.
+// log s, 1 <= s <= 2^20 or NaN: the hardware's log2, corrected by what it
+// leaves.  Floats below 20 are 2^-19 apart, the instruction is within one of
+// them, and s was rounded to f32 before: d < 2^-18, and log(1 + d) up to d^3
+// leaves d^4 / 4 < 2^-74.
 __device__ __forceinline__ double log_64(double s) {
     const double y = (double)__builtin_amdgcn_logf((float)s);
     const double d = s * exp2_64(-y) - 1.0;

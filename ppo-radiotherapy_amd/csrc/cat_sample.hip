@@ -587,7 +587,7 @@ __device__ __forceinline__ uint32_t middle_key(uint32_t lo, uint32_t hi) {
 // Up to 64 blocks share a row, one launch for each thing that all of it has to
 // be known for: the maximum; the weights, and a histogram of them where there
 // is a cut to find; the entries around the cut; the answer, by one block.
-// 63 x 50021 f32, top-p: 5 + 13 + 11 + 15 us, 43 together (12.6 MB: 2.5 us of
+// 63 x 50021 f32, top-p: 5 + 13 + 11 + 15 us, 43 together (f16 46; 12.6 MB: 2.5 us of
 // HBM).  The weights are bound by f64 arithmetic and LDS additions, the others
 // by the trips to memory and barriers that follow one another.
 constexpr int kParts = 64, kPartWaves = 4;
@@ -1625,9 +1625,13 @@ __global__ __launch_bounds__(64) void k_cat_sample_tiny(Args A, int64_t rows) {
 // nine entries a thread at most (with 17 the weights spill).  Thread t has the
 // entries [t per, (t + 1) per), so the order by index is that of the threads;
 // the row passes through LDS on its way there (per is odd: no bank conflicts).
-// The cut is found by team_key; each exchange is one barrier.  Bound by f64
-// arithmetic and those barriers: 4096 x 2048 f32 32 us without a filter, 64
-// with top-p (33.5 MB: 7 us of HBM); 65536 x 64 49 and 86.
+// The cut is found by team_key; each exchange is one barrier.  65536 x 64 f32:
+// 50 us without a filter, 85 with top-p (17 MB: 3.6 us of HBM), bound by the issue
+// of vector instructions, 460 and 862 a wave and row: 1.05 and 1.14 a cycle and
+// CU, waves waiting for their turn more than half of their time.  A weight is some
+// 30 of them, the rest are exchanges of 64 bits between 64 lanes that have an entry
+// each.  4096 x 2048: 30 and 63 us (33.5 MB: 6.7), 0.60 and 0.74 a cycle, the rest
+// barriers and dependent steps.
 template <class D, int THREADS, int E>
 __global__ __launch_bounds__(THREADS < 256 ? 256 : THREADS) void k_cat_sample_held(Args A, int64_t rows) {
     constexpr int kRows = THREADS == 64 ? 4 : 1;  // of a block
